@@ -403,7 +403,7 @@ def _gefen():
 def _own_adamw(s):
     opt = s["opt"]
     opt.step()
-    moments = [opt.moments(p) for p in s["params"]]
+    moments = opt.moments(s["params"])
     out = {"p": [p.detach() for p in s["params"]], "m": [m for m, _ in moments], "v": [v for _, v in moments]}
     if s["case"]["clip"]:
         out["norm"] = opt.grad_norm
