@@ -13,11 +13,12 @@ except PackageNotFoundError:
     __version__ = "0.0.0+unknown"
 
 from gefen import kernels
+from gefen.adamw import AdamW
 from gefen.gefen import Gefen
 from gefen.kernels import period_variance as _period_variance  # noqa: F401 (registers its custom op)
 from gefen.gefen_muon import GefenMuon
 from gefen.hybrid import GefenMuonHybrid
 from gefen.params import DEFAULT_BACKUP_SUBSTRINGS, is_muon_param, split_params_for_muon, validate_split
 
-__all__ = ["Gefen", "GefenMuon", "GefenMuonHybrid", "split_params_for_muon", "validate_split", "is_muon_param",
+__all__ = ["AdamW", "Gefen", "GefenMuon", "GefenMuonHybrid", "split_params_for_muon", "validate_split", "is_muon_param",
            "DEFAULT_BACKUP_SUBSTRINGS", "kernels", "__version__"]

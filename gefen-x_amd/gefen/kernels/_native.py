@@ -82,6 +82,21 @@ class MuonItem(ctypes.Structure):
     ]
 
 
+class AdamWDesc(ctypes.Structure):
+    """Mirror of ``gefenx_adamw_desc`` (include/gefenx.h)."""
+
+    _fields_ = [
+        ("p", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+        ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq_scale", ctypes.c_void_p),
+        ("numel", ctypes.c_int64), ("key", ctypes.c_uint64),
+        ("step_size", ctypes.c_float), ("wd_factor", ctypes.c_float),
+        ("beta1", ctypes.c_float), ("alpha1", ctypes.c_float), ("beta2", ctypes.c_float), ("alpha2", ctypes.c_float),
+        ("inv_sqrt_bc2", ctypes.c_float), ("eps", ctypes.c_float),
+        ("dtype", ctypes.c_int32), ("bits", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -138,6 +153,10 @@ SIGNATURES = {
     "gefenx_muon_apply_batch": (_I, [_P, _I, _I, _P, _P, _I64, _I64, _D, _D, _D, _D, _P, _P]),
     "gefenx_muon_cautious_count_batch": (_I, [_P, _I, _I, _P, _P, _I64, _I64, _P, _P]),
     "gefenx_gemm_nt_bf16": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _F, _F, _P]),
+    "gefenx_adamw_step": (_I, [_P, _I, _P, _P]),
+    "gefenx_adamw_norm_workspace_bytes": (_SZ, [_P, _I]),
+    "gefenx_adamw_norm": (_I, [_P, _I, _D, _P, _P, _SZ, _P]),
+    "gefenx_adamw_moments": (_I, [_P, _I, _P]),
     "gefenx_profile_enable": (_I, [_I]),
     "gefenx_profile_read": (_I, [_I, _P, _P, _P, _P]),
     "gefenx_profile_reset": (_I, []),

@@ -494,6 +494,61 @@ int gefenx_gemm_nt_bf16(const void* A, const void* B, const void* C, void* D, in
                         int64_t N, int64_t K, float alpha, float beta, void* stream);
 
 /* ------------------------------------------------------------------------
+ * AdamW over many tensors, the exponential averages in fp32 or in 8 bits.  No
+ * counterpart in the reference, which leaves AdamW to torch
+ * (hybrid.py:546-560).  Per element, in fp32, each operation rounded:
+ *   g' = coef * g,  m <- m * beta1 + g' * alpha1,  v <- v * beta2 + g'^2 * alpha2
+ *   p  <- D(p * wd_factor - step_size * m / (sqrt(v) * inv_sqrt_bc2 + eps))
+ * bits == 32: exp_avg, exp_avg_sq are fp32 [numel], the scales NULL.
+ * bits == 8: codes of one byte, and fp32 scales [ceil(numel / 256)] of blocks
+ * of 256 elements:
+ *   exp_avg     E4M3 of m / scale, nearest even; scale = max(max|m| * RN(1/448), 2^-126)
+ *   exp_avg_sq  0 for v == 0, else the code c in 1..255 of x = v / scale,
+ *               scale = max(max v, 2^-126): c stands for the float whose bits
+ *               are (c + 761) << 20 (3 mantissa bits, 1 down to 2^-32), and is
+ *               ((bits(x) + 16 r) >> 20) - 761 clamped to 1..255, with r the 16
+ *               random bits of element i: bits 16 (i % 4) .. of the SplitMix64
+ *               finalizer of key + 0x9E3779B97F4A7C15 * (i / 4 + 1).
+ *   A block with an inf or NaN gets the scale NaN.
+ * Elements are taken in storage order: p, grad and the averages are each numel
+ * contiguous elements, at any alignment of their type.
+ * ---------------------------------------------------------------------- */
+typedef struct gefenx_adamw_desc {
+    void* p;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int64_t numel;
+    uint64_t key;        /* bits == 8: of this tensor's random bits in this step */
+    float step_size;     /* lr / (1 - beta1^t) */
+    float wd_factor;     /* 1 - lr * weight_decay */
+    float beta1, alpha1; /* alpha: 1 - beta, rounded from double */
+    float beta2, alpha2;
+    float inv_sqrt_bc2;  /* 1 / sqrt(1 - beta2^t) */
+    float eps;
+    int32_t dtype;       /* gefenx_dtype of p and grad */
+    int32_t bits;        /* 8 or 32 */
+} gefenx_adamw_desc;
+
+/* Step every tensor of descs[n] (read during the call).  grad_coef: NULL, or a
+ * device float that the gradients are multiplied by (gefenx_adamw_norm's). */
+int gefenx_adamw_step(const gefenx_adamw_desc* descs, int n, const float* grad_coef, void* stream);
+
+/* The 2-norm of all gradients together and the factor that clips them:
+ * norm_out (device float[2]) = {norm, min(1, max_norm / (norm + 1e-6))}; sums
+ * in float64 in a fixed order.  Reads grad, numel and dtype alone.  workspace:
+ * gefenx_adamw_norm_workspace_bytes(descs, n) bytes (any contents). */
+size_t gefenx_adamw_norm_workspace_bytes(const gefenx_adamw_desc* descs, int n);
+int gefenx_adamw_norm(const gefenx_adamw_desc* descs, int n, double max_norm, float* norm_out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The values that 8-bit averages stand for: fp32 [numel] of exp_avg to p, of
+ * exp_avg_sq to grad (which this call writes); dtype GEFENX_F32, bits 8. */
+int gefenx_adamw_moments(const gefenx_adamw_desc* descs, int n, void* stream);
+
+/* ------------------------------------------------------------------------
  * Kernel timing.  When enabled, every update-kernel launch is bracketed by
  * HIP events on its own stream and tagged with its kind and algorithmic
  * bytes (compulsory traffic of the step it belongs to); gefenx_profile_read
