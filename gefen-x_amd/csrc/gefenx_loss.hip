@@ -1,0 +1,593 @@
+// gefenx_loss.hip -- losses over the logits of a language model, and the gradient of the logits.
+//
+// With l_t = x_t[y_t] - logsumexp(x_t) the log-probability of row t's label,
+//   preference:  r_i = beta sum_t (l_t - ref_t),  h_j = r_j - r_{B+j},
+//                loss = mean_j -(1-e) log s(h_j) - e log s(-h_j)
+//   policy:      q = exp(l - old), loss = sum_t w_t (-min(q A, clip(q) A) + c (e^d - d - 1)),  d = ref - l
+// and either way d loss / d x_tv = k_t ([v = y_t] - softmax(x_t)_v): a pass over the logits for the row
+// statistics, a few numbers per row and sequence, and a pass that writes the gradient.  Both passes are
+// bound by memory; rows without a label are not read.
+#include <hip/hip_runtime.h>
+
+#include "gefenx.h"
+#include "gefenx_device.h"
+#include "gefenx_internal.h"
+
+namespace gx {
+namespace {
+
+constexpr int kT = 256;               // threads of a row workgroup
+constexpr int kPass = kT * 8;         // logits of one pass of it
+constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
+constexpr int kSeqT = 1024;           // threads of a sequence workgroup
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eRest = (float)(1.44269504088896340736 - (double)kLog2e);
+
+struct Rows {
+    const void* x;
+    const int64_t* labels;
+    const int32_t* cu;
+    int64_t rows, per_batch, batch_stride, row_stride;
+    int64_t vocab, ignore;
+    int32_t n_seq, splits;
+    int64_t split_chunks;  // chunks of 8 logits of a split
+};
+
+__device__ __forceinline__ int64_t row_offset(const Rows& q, int64_t r) {
+    const int64_t b = r / q.per_batch;
+    return b * q.batch_stride + (r - b * q.per_batch) * q.row_stride;
+}
+
+// The sequence of row r, -1: none.
+__device__ __forceinline__ int seq_of(const Rows& q, int64_t r) {
+    if (!q.cu) return (int)(r / q.per_batch);
+    int lo = 0, hi = q.n_seq;  // the last i with cu[i] <= r
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sload(q.cu + mid) <= r) lo = mid; else hi = mid - 1;
+    }
+    return lo < q.n_seq && sload(q.cu + lo) <= r ? lo : -1;
+}
+
+// Eight logits; beyond `left` of them -inf, which adds nothing to any sum.
+template <int DT>
+__device__ __forceinline__ void load_logits(const typename Elem<DT>::T* base, int64_t left, Raw8<DT>& r) {
+    if (left >= 8) {
+        load_raw8_any<DT>(base, r);
+        return;
+    }
+    if constexpr (DT == F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r.f[k] = k < left ? *gbl(base + k) : -__builtin_inff();
+    } else {
+        constexpr uint32_t kNegInf = DT == BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = 2 * k < left ? (uint32_t)*gbl(base + 2 * k) : kNegInf;
+            const uint32_t hi = 2 * k + 1 < left ? (uint32_t)*gbl(base + 2 * k + 1) : kNegInf;
+            r.w[k] = lo | (hi << 16);
+        }
+    }
+}
+
+// The constant's rounding would lean every sum one way, and a sequence adds up thousands of them: its
+// rest goes into the product too.
+__device__ __forceinline__ float exp_(float x) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eRest, x * kLog2e));
+}
+
+// A running maximum and the sum of exp(x - maximum).  The maximum of nothing is -inf, and -inf logits
+// add 0; NaN and +inf logits make the sum NaN.
+struct Soft {
+    float m = -__builtin_inff(), s = 0.0f;
+    __device__ __forceinline__ void rebase(float m2) {
+        if (m2 > m) {
+            s = s * exp_(m - m2);
+            m = m2;
+        }
+    }
+    __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.0f : m; }
+    __device__ __forceinline__ void join(float m2, float s2) {
+        const float top = m2 > m ? m2 : m;
+        const float b = top == -__builtin_inff() ? 0.0f : top;
+        s = s * exp_(m - b) + s2 * exp_(m2 - b);
+        m = top;
+    }
+};
+
+template <int DT, int N>
+__device__ __forceinline__ void add_chunks(Soft& a, const Raw8<DT> (&r)[N]) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, raw_elem<DT>(r[c], k));
+    a.rebase(top);
+    const float b = a.base();
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a.s += exp_(raw_elem<DT>(r[c], k) - b);
+}
+
+__device__ __forceinline__ void wave_join(Soft& a) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(a.m, off, 64), s2 = __shfl_xor(a.s, off, 64);
+        a.join(m2, s2);
+    }
+}
+
+// ------------------------------------------------------------ row statistics
+// part[row][split] = {maximum, sum of exp(x - maximum)} of a split of a row.
+template <int DT>
+__global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restrict__ part) {
+    using T = typename Elem<DT>::T;
+    __shared__ float2 waves[kT / 64];
+    const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
+    const int64_t label = sload(q.labels + r);
+    if (label == q.ignore) return;
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const int64_t chunks = (q.vocab + 7) / 8;
+    int64_t c = split * q.split_chunks, end = c + q.split_chunks;
+    if (end > chunks) end = chunks;
+    const int64_t whole = end * 8 <= q.vocab ? end : end - 1;
+    Soft a;
+    for (c += threadIdx.x; c + 3 * kT < whole; c += 4 * kT) {
+        Raw8<DT> v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_raw8_any<DT>(x + (c + i * kT) * 8, v[i]);
+        add_chunks<DT, 4>(a, v);
+    }
+    for (; c < end; c += kT) {
+        Raw8<DT> v[1];
+        load_logits<DT>(x + c * 8, q.vocab - c * 8, v[0]);
+        add_chunks<DT, 1>(a, v);
+    }
+    wave_join(a);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(a.m, a.s);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < kT / 64; ++w) a.join(waves[w].x, waves[w].y);
+        part[blockIdx.x] = make_float2(a.m, a.s);
+    }
+}
+
+// ------------------------------------------------------------ tokens and sequences
+struct Token {           // what the sequence kernels read and write per row
+    const float* ref;    // may be null (policy without a KL term, preference without a reference)
+    const float* old;
+    const float* adv;    // per row or per sequence
+    float* logps;
+    float2* stats;       // {maximum, sum}
+    float* k;            // d loss / d logp of a row but for its sequence's weight; may be null
+    int32_t adv_per_row;
+    float lo, hi, kl_coef;
+};
+
+struct SeqSums {         // per sequence, in float64
+    double a, kl, clipped, n;
+};
+
+enum { kLogps = 0, kPreference = 1, kPolicy = 2 };
+
+// Row r's statistics from its splits, by a group of `lanes` (a power of two, up to 64).
+__device__ __forceinline__ Soft join_splits(const Rows& q, const float2* part, int64_t r, int lane, int lanes) {
+    Soft a;
+    for (int i = lane; i < q.splits; i += lanes) {
+        const float2 p = part[r * q.splits + i];
+        a.join(p.x, p.y);
+    }
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(a.m, off, 64), s2 = __shfl_xor(a.s, off, 64);
+        a.join(m2, s2);
+    }
+    return a;
+}
+
+template <int DT>
+__device__ __forceinline__ double token_logp(const Rows& q, int64_t r, int64_t label, const Soft& a) {
+    using T = typename Elem<DT>::T;
+    if (label < 0 || label >= q.vocab) return __longlong_as_double(0x7ff8000000000000ll);  // no such logit
+    const float x = to_f32<DT>(*gbl((const T*)q.x + row_offset(q, r) + label));
+    return ((double)x - (double)a.m) - log((double)a.s);
+}
+
+// One workgroup per sequence (kLogps: per kSeqT / lanes rows), a group of lanes per row.
+template <int DT, int MODE>
+__global__ __launch_bounds__(kSeqT) void k_tokens(const Rows q, const Token t, const float2* __restrict__ part, int lanes,
+                                                  SeqSums* __restrict__ sums) {
+    __shared__ SeqSums waves[kSeqT / 64];
+    const int group = threadIdx.x / lanes, lane = threadIdx.x % lanes, groups = kSeqT / lanes;
+    int64_t begin, end;
+    if (MODE == kLogps) {
+        begin = (int64_t)blockIdx.x * groups;
+        end = begin + groups;
+    } else if (q.cu) {
+        begin = sload(q.cu + blockIdx.x);
+        end = sload(q.cu + blockIdx.x + 1);
+    } else {
+        begin = (int64_t)blockIdx.x * q.per_batch;
+        end = begin + q.per_batch;
+    }
+    begin = begin < 0 ? 0 : begin;
+    end = end > q.rows ? q.rows : end;
+    if (MODE != kLogps && q.cu) {  // rows before the first sequence and after the last belong to none
+        const int64_t first = blockIdx.x == 0 ? (begin < q.rows ? begin : q.rows) : 0;
+        for (int64_t r = threadIdx.x; r < first; r += kSeqT) t.logps[r] = 0.0f;
+        if (blockIdx.x + 1 == gridDim.x)
+            for (int64_t r = (end > 0 ? end : 0) + threadIdx.x; r < q.rows; r += kSeqT) t.logps[r] = 0.0f;
+    }
+    SeqSums own = {0.0, 0.0, 0.0, 0.0};
+    for (int64_t r = begin + group; r < end; r += groups) {
+        const int64_t label = *gbl(q.labels + r);
+        float logp = 0.0f, k = 0.0f;
+        Soft a;
+        if (label != q.ignore) {
+            a = join_splits(q, part, r, lane, lanes);
+            const double exact = token_logp<DT>(q, r, label, a);
+            logp = (float)exact;
+            if (MODE == kPreference && lane == 0) {
+                own.a += exact - (t.ref ? (double)*gbl(t.ref + r) : 0.0);
+                own.n += 1.0;
+            }
+            if (MODE == kPolicy && lane == 0) {
+                const float adv = *gbl(t.adv + (t.adv_per_row ? r : (int64_t)blockIdx.x));
+                const float ratio = expf(logp - *gbl(t.old + r));
+                const float bound = __builtin_fminf(__builtin_fmaxf(ratio, t.lo), t.hi);
+                const float plain = ratio * adv, clip = bound * adv;
+                const bool clipped = clip < plain;
+                float each = clipped ? -clip : -plain;
+                k = clipped ? 0.0f : -plain;
+                if (t.ref) {
+                    const float d = *gbl(t.ref + r) - logp;
+                    const float e = expm1f(d);
+                    each += t.kl_coef * (e - d);
+                    k -= t.kl_coef * e;
+                    own.kl += (double)(e - d);
+                }
+                own.a += (double)each;
+                own.clipped += clipped ? 1.0 : 0.0;
+                own.n += 1.0;
+            }
+        }
+        if (lane == 0) {
+            t.logps[r] = logp;
+            t.stats[r] = make_float2(a.m, a.s);
+            if (MODE == kPolicy) t.k[r] = k;
+        }
+    }
+    if (MODE == kLogps) return;
+    own.a = wave_sum_d(own.a);
+    own.kl = wave_sum_d(own.kl);
+    own.clipped = wave_sum_d(own.clipped);
+    own.n = wave_sum_d(own.n);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = own;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kSeqT / 64; ++w) {
+            own.a += waves[w].a;
+            own.kl += waves[w].kl;
+            own.clipped += waves[w].clipped;
+            own.n += waves[w].n;
+        }
+        sums[blockIdx.x] = own;
+    }
+}
+
+__device__ __forceinline__ double block_sum(double v, double* waves) {
+    v = wave_sum_d(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double total = 0.0;
+    for (int w = 0; w < kT / 64; ++w) total += waves[w];
+    return total;
+}
+
+// Rewards of either side, and weights per sequence, the chosen ones first.
+__global__ __launch_bounds__(kT) void k_preference(const SeqSums* __restrict__ sums, int n_seq, double beta, double smoothing,
+                                                   int average, float* __restrict__ loss_out, float* __restrict__ chosen,
+                                                   float* __restrict__ rejected, float* __restrict__ weights) {
+    __shared__ double waves[kT / 64];
+    const int pairs = n_seq / 2;
+    double loss = 0.0;
+    for (int j = threadIdx.x; j < pairs; j += kT) {
+        const SeqSums c = sums[j], r = sums[pairs + j];
+        const double wc = beta / (average && c.n > 0.0 ? c.n : 1.0), wr = beta / (average && r.n > 0.0 ? r.n : 1.0);
+        const double h = c.a * wc - r.a * wr;
+        // log s(h) = min(h, 0) - log(1 + e^-|h|)
+        const double tail = log1p(exp(-fabs(h)));
+        loss += (1.0 - smoothing) * (tail - fmin(h, 0.0)) + smoothing * (tail + fmax(h, 0.0));
+        const double k = (1.0 / (1.0 + exp(-h)) - (1.0 - smoothing)) / pairs;
+        chosen[j] = (float)(c.a * wc);
+        rejected[j] = (float)(r.a * wr);
+        weights[j] = (float)(k * wc);
+        weights[pairs + j] = (float)(-k * wr);
+    }
+    const double total = block_sum(loss, waves);
+    if (threadIdx.x == 0) *loss_out = (float)(total / pairs);
+}
+
+// Loss, mean KL, share of clipped tokens; weights per sequence.
+__global__ __launch_bounds__(kT) void k_policy(const SeqSums* __restrict__ sums, int n_seq, int by_sequence,
+                                               float* __restrict__ loss_out, float* __restrict__ kl_out,
+                                               float* __restrict__ clipped_out, float* __restrict__ weights) {
+    __shared__ double waves[kT / 64];
+    double n = 0.0, seqs = 0.0, kl = 0.0, clipped = 0.0;
+    for (int i = threadIdx.x; i < n_seq; i += kT) {
+        n += sums[i].n;
+        seqs += sums[i].n > 0.0 ? 1.0 : 0.0;
+        kl += sums[i].kl;
+        clipped += sums[i].clipped;
+    }
+    n = block_sum(n, waves);
+    seqs = block_sum(seqs, waves);
+    kl = block_sum(kl, waves);
+    clipped = block_sum(clipped, waves);
+    const double tokens = n > 0.0 ? n : 1.0;
+    double loss = 0.0;
+    for (int i = threadIdx.x; i < n_seq; i += kT) {
+        const double w = sums[i].n > 0.0 ? (by_sequence ? 1.0 / (sums[i].n * seqs) : 1.0 / tokens) : 0.0;
+        loss += sums[i].a * w;
+        weights[i] = (float)w;
+    }
+    loss = block_sum(loss, waves);
+    if (threadIdx.x == 0) {
+        *loss_out = (float)loss;
+        *kl_out = (float)(kl / tokens);
+        *clipped_out = (float)(clipped / tokens);
+    }
+}
+
+// ------------------------------------------------------------ gradient
+// grad[r][v] = k_r ([v = y_r] - exp(x - max) / sum); k_r = k[r] * weights[sequence] * scale.
+template <int DT>
+__global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* __restrict__ stats, const float* __restrict__ k,
+                                                    const float* __restrict__ weights, const float* __restrict__ scale_dev,
+                                                    float scale, void* __restrict__ grad) {
+    using T = typename Elem<DT>::T;
+    const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
+    const int64_t label = sload(q.labels + r);
+    float coef = 0.0f;
+    if (label != q.ignore) {
+        coef = scale_dev ? sload(scale_dev) * scale : scale;
+        if (k) coef *= sload(k + r);
+        if (weights) {
+            const int s = seq_of(q, r);
+            coef = s >= 0 ? coef * sload(weights + s) : 0.0f;
+        }
+        if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+    }
+    T* out = (T*)grad + r * q.vocab;
+    const int64_t chunks = (q.vocab + 7) / 8;
+    int64_t c = split * q.split_chunks, end = c + q.split_chunks;
+    if (end > chunks) end = chunks;
+    const int64_t whole = end * 8 <= q.vocab ? end : end - 1;
+    c += threadIdx.x;
+    if (coef == 0.0f) {
+        const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (; c < whole; c += kT) store8_any<DT>(out + c * 8, zeros);
+        if (c < end)
+            for (int64_t v = c * 8; v < q.vocab; ++v) out[v] = from_f32<DT>(0.0f);
+        return;
+    }
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const float2 st = make_float2(sload(&stats[r].x), sload(&stats[r].y));
+    const float each = -coef / st.y;
+    const auto chunk = [&](const Raw8<DT>& v, int64_t at, float g[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = each * exp_(raw_elem<DT>(v, i) - st.x);
+        const uint64_t here = (uint64_t)(label - at);
+        if (here < 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] += here == (uint64_t)i ? coef : 0.0f;
+        }
+    };
+    for (; c + 3 * kT < whole; c += 4 * kT) {
+        Raw8<DT> v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_raw8_any<DT>(x + (c + i * kT) * 8, v[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float g[8];
+            chunk(v[i], (c + i * kT) * 8, g);
+            store8_any<DT>(out + (c + i * kT) * 8, g);
+        }
+    }
+    for (; c < end; c += kT) {
+        Raw8<DT> v;
+        float g[8];
+        const int64_t left = q.vocab - c * 8;
+        load_logits<DT>(x + c * 8, left, v);
+        chunk(v, c * 8, g);
+        if (left >= 8) {
+            store8_any<DT>(out + c * 8, g);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) out[c * 8 + i] = from_f32<DT>(g[i]);
+        }
+    }
+}
+
+// ------------------------------------------------------------ host side
+int launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GEFENX_OK : set_error(GEFENX_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+// Row workgroups: one per row, or enough to fill the chip where the rows are few, each of a pass or more.
+int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q) {
+    if (!l) return set_error(GEFENX_EINVAL, "%s: null descriptor", what);
+    if (l->dtype != GEFENX_F32 && l->dtype != GEFENX_F16 && l->dtype != GEFENX_BF16)
+        return set_error(GEFENX_EDTYPE, "%s: unsupported dtype %d", what, l->dtype);
+    if (l->rows < 0 || l->vocab < 1 || l->rows > 0x7fffffff || l->vocab > 0x7fffffff || l->rows_per_batch < 1)
+        return set_error(GEFENX_EINVAL, "%s: bad sizes (rows=%lld of %lld, vocab=%lld)", what, (long long)l->rows,
+                         (long long)l->rows_per_batch, (long long)l->vocab);
+    if (l->rows > 0 && (!l->logits || !l->labels)) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    if (sequences && (l->n_seq < 1 || (!l->cu_seqlens && l->rows != 0 && l->rows != l->n_seq * l->rows_per_batch)))
+        return set_error(GEFENX_EINVAL, "%s: bad sequences (%d over %lld rows)", what, l->n_seq, (long long)l->rows);
+    q.x = l->logits;
+    q.labels = l->labels;
+    q.cu = l->cu_seqlens;
+    q.rows = l->rows;
+    q.per_batch = l->rows_per_batch;
+    q.batch_stride = l->batch_stride;
+    q.row_stride = l->row_stride;
+    q.vocab = l->vocab;
+    q.ignore = l->ignore_index;
+    q.n_seq = l->n_seq;
+    const int64_t chunks = (l->vocab + 7) / 8, passes = (l->vocab + kPass - 1) / kPass;
+    int64_t splits = l->rows > 0 ? (kWantedWgs + l->rows - 1) / l->rows : 1;
+    splits = splits < 1 ? 1 : (splits > passes ? passes : splits);
+    q.split_chunks = (chunks + splits - 1) / splits;
+    q.splits = (int32_t)((chunks + q.split_chunks - 1) / q.split_chunks);
+    return GEFENX_OK;
+}
+
+size_t align16(size_t n) { return (n + 15) & ~size_t(15); }
+size_t part_bytes(const Rows& q) { return align16(sizeof(float2) * (size_t)q.rows * (size_t)q.splits); }
+size_t ws_bytes(const Rows& q) { return part_bytes(q) + sizeof(SeqSums) * (size_t)(q.n_seq > 0 ? q.n_seq : 0) + 16; }
+
+template <class F>
+int by_dtype(int dtype, F&& f) {
+    switch (dtype) {
+        case GEFENX_F32: return f(std::integral_constant<int, F32>());
+        case GEFENX_F16: return f(std::integral_constant<int, F16>());
+        default: return f(std::integral_constant<int, BF16>());
+    }
+}
+
+int run_stats(const char* what, const Rows& q, int dtype, float2* part, hipStream_t s) {
+    if (q.rows == 0) return GEFENX_OK;
+    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
+    return by_dtype(dtype, [&](auto dt) {
+        k_row_stats<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, part);
+        return launched(what);
+    });
+}
+
+template <int MODE>
+int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const float2* part, SeqSums* sums, hipStream_t s) {
+    int lanes = 1;
+    while (lanes < q.splits && lanes < 64) lanes *= 2;
+    const int64_t wgs = MODE == kLogps ? (q.rows * lanes + kSeqT - 1) / kSeqT : q.n_seq;
+    if (wgs == 0) return GEFENX_OK;
+    return by_dtype(dtype, [&](auto dt) {
+        k_tokens<decltype(dt)::value, MODE><<<(uint32_t)wgs, kSeqT, 0, s>>>(q, t, part, lanes, sums);
+        return launched(what);
+    });
+}
+
+int need(const char* what, const Rows& q, const void* ws, size_t bytes) {
+    if (!ws || bytes < ws_bytes(q))
+        return set_error(GEFENX_EINVAL, "%s: workspace of %zu bytes, %zu needed", what, bytes, ws_bytes(q));
+    return GEFENX_OK;
+}
+
+}  // namespace
+}  // namespace gx
+
+using namespace gx;
+
+extern "C" {
+
+size_t gefenx_loss_workspace_bytes(const gefenx_logits* logits) {
+    Rows q;
+    return make_rows("gefenx_loss_workspace_bytes", logits, false, q) == GEFENX_OK ? ws_bytes(q) : 0;
+}
+
+int gefenx_token_logps(const gefenx_logits* logits, float* logps, float* stats, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    const char* what = "gefenx_token_logps";
+    Rows q;
+    int rc = make_rows(what, logits, false, q);
+    if (rc == GEFENX_OK) rc = need(what, q, workspace, workspace_bytes);
+    if (rc != GEFENX_OK) return rc;
+    if (q.rows > 0 && (!logps || !stats)) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float2* part = static_cast<float2*>(workspace);
+    Token t = {};
+    t.logps = logps;
+    t.stats = reinterpret_cast<float2*>(stats);
+    rc = run_stats(what, q, logits->dtype, part, s);
+    return rc == GEFENX_OK ? run_tokens<kLogps>(what, q, logits->dtype, t, part, nullptr, s) : rc;
+}
+
+int gefenx_preference_loss(const gefenx_logits* logits, const float* ref_logps, double beta, double label_smoothing, int average,
+                           float* loss, float* chosen_rewards, float* rejected_rewards, float* logps, float* stats,
+                           float* weights, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "gefenx_preference_loss";
+    Rows q;
+    int rc = make_rows(what, logits, true, q);
+    if (rc == GEFENX_OK) rc = need(what, q, workspace, workspace_bytes);
+    if (rc != GEFENX_OK) return rc;
+    if (q.n_seq % 2) return set_error(GEFENX_EINVAL, "%s: %d sequences are no pairs", what, q.n_seq);
+    if (!loss || !chosen_rewards || !rejected_rewards || !weights || (q.rows > 0 && (!logps || !stats)))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float2* part = static_cast<float2*>(workspace);
+    SeqSums* sums = reinterpret_cast<SeqSums*>(static_cast<char*>(workspace) + part_bytes(q));
+    Token t = {};
+    t.ref = ref_logps;
+    t.logps = logps;
+    t.stats = reinterpret_cast<float2*>(stats);
+    rc = run_stats(what, q, logits->dtype, part, s);
+    if (rc == GEFENX_OK) rc = run_tokens<kPreference>(what, q, logits->dtype, t, part, sums, s);
+    if (rc != GEFENX_OK) return rc;
+    k_preference<<<1, kT, 0, s>>>(sums, q.n_seq, beta, label_smoothing, average, loss, chosen_rewards, rejected_rewards, weights);
+    return launched(what);
+}
+
+int gefenx_policy_loss(const gefenx_logits* logits, const float* old_logps, const float* advantages, int advantages_per_row,
+                       const float* ref_logps, double clip_low, double clip_high, double kl_coef, int by_sequence,
+                       float* loss, float* kl, float* clip_fraction, float* logps, float* stats, float* k, float* weights,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "gefenx_policy_loss";
+    Rows q;
+    int rc = make_rows(what, logits, true, q);
+    if (rc == GEFENX_OK) rc = need(what, q, workspace, workspace_bytes);
+    if (rc != GEFENX_OK) return rc;
+    if (!loss || !kl || !clip_fraction || !weights || !advantages || (q.rows > 0 && (!logps || !stats || !k || !old_logps)))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float2* part = static_cast<float2*>(workspace);
+    SeqSums* sums = reinterpret_cast<SeqSums*>(static_cast<char*>(workspace) + part_bytes(q));
+    Token t = {};
+    t.ref = ref_logps;
+    t.old = old_logps;
+    t.adv = advantages;
+    t.adv_per_row = advantages_per_row;
+    t.logps = logps;
+    t.stats = reinterpret_cast<float2*>(stats);
+    t.k = k;
+    t.lo = (float)(1.0 - clip_low);
+    t.hi = (float)(1.0 + clip_high);
+    t.kl_coef = (float)kl_coef;
+    rc = run_stats(what, q, logits->dtype, part, s);
+    if (rc == GEFENX_OK) rc = run_tokens<kPolicy>(what, q, logits->dtype, t, part, sums, s);
+    if (rc != GEFENX_OK) return rc;
+    k_policy<<<1, kT, 0, s>>>(sums, q.n_seq, by_sequence, loss, kl, clip_fraction, weights);
+    return launched(what);
+}
+
+int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const float* k, const float* weights,
+                       const float* scale_dev, double scale, void* grad, void* stream) {
+    const char* what = "gefenx_logits_grad";
+    Rows q;
+    int rc = make_rows(what, logits, weights != nullptr, q);
+    if (rc != GEFENX_OK) return rc;
+    if (q.rows == 0) return GEFENX_OK;
+    if (!stats || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return by_dtype(logits->dtype, [&](auto dt) {
+        k_logits_grad<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(
+            q, reinterpret_cast<const float2*>(stats), k, weights, scale_dev, (float)scale, grad);
+        return launched(what);
+    });
+}
+
+}  // extern "C"

@@ -18,7 +18,10 @@ from gefen.gefen import Gefen
 from gefen.kernels import period_variance as _period_variance  # noqa: F401 (registers its custom op)
 from gefen.gefen_muon import GefenMuon
 from gefen.hybrid import GefenMuonHybrid
+from gefen.losses import (PolicyLoss, PreferenceLoss, policy_loss, policy_loss_and_grad, preference_loss,
+                          preference_loss_and_grad, token_logps)
 from gefen.params import DEFAULT_BACKUP_SUBSTRINGS, is_muon_param, split_params_for_muon, validate_split
 
 __all__ = ["AdamW", "Gefen", "GefenMuon", "GefenMuonHybrid", "split_params_for_muon", "validate_split", "is_muon_param",
-           "DEFAULT_BACKUP_SUBSTRINGS", "kernels", "__version__"]
+           "PolicyLoss", "PreferenceLoss", "policy_loss", "policy_loss_and_grad", "preference_loss",
+           "preference_loss_and_grad", "token_logps", "DEFAULT_BACKUP_SUBSTRINGS", "kernels", "__version__"]

@@ -97,6 +97,18 @@ class AdamWDesc(ctypes.Structure):
     ]
 
 
+class Logits(ctypes.Structure):
+    """Mirror of ``gefenx_logits`` (include/gefenx.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("labels", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+        ("rows", ctypes.c_int64), ("rows_per_batch", ctypes.c_int64),
+        ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("vocab", ctypes.c_int64), ("ignore_index", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("n_seq", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -157,6 +169,11 @@ SIGNATURES = {
     "gefenx_adamw_norm_workspace_bytes": (_SZ, [_P, _I]),
     "gefenx_adamw_norm": (_I, [_P, _I, _D, _P, _P, _SZ, _P]),
     "gefenx_adamw_moments": (_I, [_P, _I, _P]),
+    "gefenx_loss_workspace_bytes": (_SZ, [_P]),
+    "gefenx_token_logps": (_I, [_P, _P, _P, _P, _SZ, _P]),
+    "gefenx_preference_loss": (_I, [_P, _P, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gefenx_policy_loss": (_I, [_P, _P, _P, _I, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gefenx_logits_grad": (_I, [_P, _P, _P, _P, _P, _D, _P, _P]),
     "gefenx_profile_enable": (_I, [_I]),
     "gefenx_profile_read": (_I, [_I, _P, _P, _P, _P]),
     "gefenx_profile_reset": (_I, []),

@@ -1,0 +1,302 @@
+"""Losses over the logits of a language model, and their gradient, on the MI355X.
+
+What a fine-tuning loop computes before the optimizer steps: the
+log-probability of each label, the preference loss over pairs of answers
+(paired log ratios against a reference) and the clipped policy loss with a KL
+term.  The reference has no losses.  Each reads the logits in their own type,
+without a copy in fp32 and without their softmax in memory, and writes their
+gradient once; rows whose label is ``ignore_index`` are not read and get a zero
+gradient.
+
+Logits are [..., vocab] (last dimension of stride 1; up to two leading
+dimensions of any strides are read in place) in fp32, fp16 or bf16; labels are
+int64 of the leading shape, and ``logits[..., t, :]`` predicts ``labels[..., t]``
+(shift the labels, not the logits).  Per-token inputs have the labels' shape,
+are constants (no gradient flows into them) and are taken in fp32.  Sequences are
+the rows of logits [N, S, vocab], or, with ``cu_seqlens`` (int32 [N + 1] on the
+device), lie one after another in [T, vocab].  Sums over tokens are in float64.
+
+The plain calls are differentiable in the logits.  The ``*_and_grad`` calls return
+the gradient with the loss, for a training loop that feeds it to
+``logits.backward(grad)``; ``grad_scale`` (a number or a device scalar, such as a
+GradScaler's) multiplies it before it is rounded to the logits' type.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from gefen.gefen import _on_device
+from gefen.kernels import _native
+from gefen.kernels.automatic_gefen_fused import _dtype_code
+
+_DTYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))
+
+
+class PreferenceLoss(NamedTuple):
+    """loss (0-dim), beta times the log ratio of each chosen and rejected
+    sequence [N / 2], the labels' log-probabilities (0 where ignored)."""
+    loss: torch.Tensor
+    chosen_rewards: torch.Tensor
+    rejected_rewards: torch.Tensor
+    logps: torch.Tensor
+
+
+class PolicyLoss(NamedTuple):
+    """loss, mean KL estimate and share of clipped tokens (0-dim), the labels'
+    log-probabilities (0 where ignored)."""
+    loss: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+    logps: torch.Tensor
+
+
+class _Call:
+    """The logits of one call, checked, and the descriptor that the kernels read them by."""
+
+    def __init__(self, logits, labels, ignore_index, cu_seqlens=None, sequences=True):
+        if not isinstance(logits, torch.Tensor) or not isinstance(labels, torch.Tensor):
+            raise TypeError("logits and labels must be tensors")
+        if logits.device.type != "cuda":
+            raise ValueError("Expected logits on a HIP device, got {}".format(logits.device))
+        if logits.dtype not in _DTYPES:
+            raise NotImplementedError("logits of {} are not implemented (fp32, fp16, bf16)".format(logits.dtype))
+        if logits.dim() < 1 or logits.shape[-1] < 1:
+            raise ValueError("logits need a vocabulary dimension, got shape {}".format(tuple(logits.shape)))
+        if labels.dtype != torch.int64 or labels.shape != logits.shape[:-1] or labels.device != logits.device:
+            raise ValueError("labels must be int64 of shape {} on {}, got {} of shape {} on {}".format(
+                tuple(logits.shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
+        self.device, self.shape, self.vocab = logits.device, logits.shape, logits.shape[-1]
+        self.n_seq, self.cu = 0, None
+        if cu_seqlens is not None:
+            if logits.dim() != 2:
+                raise ValueError("with cu_seqlens logits are [tokens, vocab], got shape {}".format(tuple(logits.shape)))
+            if (not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2
+                    or cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.device != logits.device):
+                raise ValueError("cu_seqlens must be int32 or int64 [sequences + 1] on {}".format(logits.device))
+            self.cu = cu_seqlens.to(torch.int32).contiguous()
+            self.n_seq = cu_seqlens.numel() - 1
+        elif sequences:
+            if logits.dim() != 3 or logits.shape[0] < 1:
+                raise ValueError("logits are [sequences, tokens, vocab], or [tokens, vocab] with cu_seqlens, got shape "
+                                 "{}".format(tuple(logits.shape)))
+            self.n_seq = logits.shape[0]
+        x = logits.detach()
+        if x.dim() > 3 or (x.stride(-1) != 1 and x.shape[-1] > 1):
+            x = x.contiguous()
+        x = x.reshape(-1, self.vocab) if x.dim() > 3 else x
+        x = x[(None,) * (3 - x.dim())]  # [batches, rows of a batch, vocab]
+        self.logits, self.labels = x, labels.detach().contiguous()
+        self.rows = self.labels.numel()
+        self.desc = _native.Logits(
+            logits=x.data_ptr(), labels=self.labels.data_ptr(), cu_seqlens=None if self.cu is None else self.cu.data_ptr(),
+            rows=self.rows, rows_per_batch=max(1, x.shape[1]), batch_stride=x.stride(0), row_stride=x.stride(1),
+            vocab=self.vocab, ignore_index=int(ignore_index), dtype=_dtype_code(x.dtype), n_seq=self.n_seq)
+        self.ref = ctypes.byref(self.desc)
+        self.stream = torch.cuda.current_stream(self.device).cuda_stream
+
+    def per_token(self, t, name):
+        """A per-token input as the kernels read it, or None."""
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor) or t.shape != self.labels.shape or t.device != self.device \
+                or not t.is_floating_point():
+            raise ValueError("{} must be a floating tensor of the labels' shape {} on {}, got {}".format(
+                name, tuple(self.labels.shape), self.device,
+                "{} of shape {} on {}".format(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor)
+                else type(t).__name__))
+        return t.detach().to(torch.float32).contiguous()
+
+    def empty(self, *shape):
+        return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+    def workspace(self):
+        n = int(_native.load().gefenx_loss_workspace_bytes(self.ref))
+        return torch.empty(max(n, 16), dtype=torch.uint8, device=self.device), n
+
+    def grad(self, stats, k, weights, scale):
+        """The gradient of the logits, contiguous in their shape."""
+        out = torch.empty(self.shape, dtype=self.logits.dtype, device=self.device)
+        factor, scale_dev = 1.0, None
+        if isinstance(scale, torch.Tensor):
+            if scale.numel() != 1 or scale.device != self.device:
+                raise ValueError("grad_scale must be a number or one value on {}".format(self.device))
+            scale_dev = scale.detach().to(torch.float32)
+        else:
+            factor = float(scale)
+        with _on_device(self.device):
+            _native.check(_native.load().gefenx_logits_grad(
+                self.ref, _ptr(stats), _ptr(k), _ptr(weights), _ptr(scale_dev), factor, _ptr(out), self.stream),
+                "logits gradient")
+        return out
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _probability(value, name, most):
+    value = float(value)
+    if not 0.0 <= value < most:
+        raise ValueError("{} must be in [0, {}) but is: {!r}".format(name, most, value))
+    return value
+
+
+def _finite(value, name):
+    value = float(value)
+    if not abs(value) < float("inf"):
+        raise ValueError("{} must be finite but is: {!r}".format(name, value))
+    return value
+
+
+# ------------------------------------------------------------ forward passes
+
+def _logps_forward(call):
+    logps, stats = call.empty(*call.labels.shape), call.empty(call.rows, 2)
+    ws, n = call.workspace()
+    with _on_device(call.device):
+        _native.check(_native.load().gefenx_token_logps(call.ref, _ptr(logps), _ptr(stats), _ptr(ws), n, call.stream),
+                      "token_logps")
+    return logps, stats
+
+
+def _preference_forward(call, ref_logps, beta, smoothing, average):
+    if call.n_seq % 2:
+        raise ValueError("preference_loss needs pairs: the chosen sequences, then as many rejected ones, got {}".format(
+            call.n_seq))
+    ref = call.per_token(ref_logps, "ref_logps")
+    beta, smoothing = _finite(beta, "beta"), _probability(smoothing, "label_smoothing", 0.5)
+    pairs = call.n_seq // 2
+    loss, chosen, rejected, weights = call.empty(), call.empty(pairs), call.empty(pairs), call.empty(call.n_seq)
+    logps, stats = call.empty(*call.labels.shape), call.empty(call.rows, 2)
+    ws, n = call.workspace()
+    with _on_device(call.device):
+        _native.check(_native.load().gefenx_preference_loss(
+            call.ref, _ptr(ref), beta, smoothing, 1 if average else 0, _ptr(loss), _ptr(chosen), _ptr(rejected),
+            _ptr(logps), _ptr(stats), _ptr(weights), _ptr(ws), n, call.stream), "preference_loss")
+    return PreferenceLoss(loss, chosen, rejected, logps), stats, weights
+
+
+def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction):
+    old, ref = call.per_token(old_logps, "old_logps"), call.per_token(ref_logps, "ref_logps")
+    if old is None:
+        raise ValueError("policy_loss needs old_logps")
+    if reduction not in ("token", "sequence"):
+        raise ValueError("reduction must be 'token' or 'sequence' but is: {!r}".format(reduction))
+    clip_low, clip_high = _probability(clip_low, "clip_low", 1.0), float(clip_high)
+    if not clip_high >= 0.0:
+        raise ValueError("clip_high must not be negative but is: {!r}".format(clip_high))
+    kl_coef = _finite(kl_coef, "kl_coef")
+    if kl_coef and ref is None:
+        raise ValueError("kl_coef={} needs ref_logps".format(kl_coef))
+    if (isinstance(advantages, torch.Tensor) and advantages.shape == (call.n_seq,) != call.labels.shape
+            and advantages.device == call.device and advantages.is_floating_point()):
+        adv, per_row = advantages.detach().to(torch.float32).contiguous(), 0
+    else:
+        adv, per_row = call.per_token(advantages, "advantages (one per token or one per sequence)"), 1
+        if adv is None:
+            raise ValueError("policy_loss needs advantages")
+    loss, kl, clipped, weights = call.empty(), call.empty(), call.empty(), call.empty(call.n_seq)
+    logps, stats, k = call.empty(*call.labels.shape), call.empty(call.rows, 2), call.empty(call.rows)
+    ws, n = call.workspace()
+    with _on_device(call.device):
+        _native.check(_native.load().gefenx_policy_loss(
+            call.ref, _ptr(old), _ptr(adv), per_row, _ptr(ref), clip_low, clip_high, kl_coef,
+            1 if reduction == "sequence" else 0, _ptr(loss), _ptr(kl), _ptr(clipped), _ptr(logps), _ptr(stats), _ptr(k),
+            _ptr(weights), _ptr(ws), n, call.stream), "policy_loss")
+    return PolicyLoss(loss, kl, clipped, logps), stats, k, weights
+
+
+# ------------------------------------------------------------ autograd
+
+class _TokenLogps(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ignore_index):
+        logps, stats = _logps_forward(_Call(logits, labels, ignore_index, sequences=False))
+        ctx.ignore_index = ignore_index
+        ctx.save_for_backward(logits, labels, stats)
+        return logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, labels, stats = ctx.saved_tensors
+        call = _Call(logits, labels, ctx.ignore_index, sequences=False)
+        return call.grad(stats, call.per_token(grad, "gradient"), None, 1.0), None, None
+
+
+class _SequenceLoss(torch.autograd.Function):
+    """Both sequence losses: `forward_of` returns the outputs and what the gradient needs."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, cu_seqlens, ignore_index, forward_of):
+        call = _Call(logits, labels, ignore_index, cu_seqlens)
+        out, stats, k, weights = forward_of(call)
+        ctx.ignore_index = ignore_index
+        ctx.save_for_backward(logits, labels, cu_seqlens, stats, k, weights)
+        ctx.mark_non_differentiable(*out[1:])
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, *unused):
+        if grad is None:
+            return None, None, None, None, None
+        logits, labels, cu_seqlens, stats, k, weights = ctx.saved_tensors
+        return _Call(logits, labels, ctx.ignore_index, cu_seqlens).grad(stats, k, weights, grad), None, None, None, None
+
+
+def token_logps(logits, labels, *, ignore_index=-100):
+    """log softmax(logits)[label] of every row, fp32 in the labels' shape (0
+    where ignored); differentiable in the logits."""
+    return _TokenLogps.apply(logits, labels, ignore_index)
+
+
+def preference_loss(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0, average=False,
+                    ignore_index=-100):
+    """Preference loss of pairs of sequences, the chosen ones first:
+
+        reward = beta * sum over the sequence's labels of (logp - ref_logp)
+        h = reward of the chosen - reward of the rejected
+        loss = mean of -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)
+
+    average: rewards are divided by the sequence's number of labels (a sequence
+    without any has reward 0).  ref_logps: the reference model's token_logps;
+    None: zeros."""
+    def forward_of(call):
+        out, stats, weights = _preference_forward(call, ref_logps, beta, label_smoothing, average)
+        return out, stats, None, weights
+    return PreferenceLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of))
+
+
+def preference_loss_and_grad(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0,
+                             average=False, ignore_index=-100, grad_scale=1.0):
+    """(preference_loss(...), gradient of the loss times grad_scale in the logits)."""
+    call = _Call(logits, labels, ignore_index, cu_seqlens)
+    out, stats, weights = _preference_forward(call, ref_logps, beta, label_smoothing, average)
+    return out, call.grad(stats, None, weights, grad_scale)
+
+
+def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, reduction="token", ignore_index=-100):
+    """Clipped policy loss with a KL term; per labelled token, with q = exp(logp - old_logp), d = ref_logp - logp:
+
+        -min(q A, clamp(q, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(d) - d - 1)
+
+    reduction: "token", the mean over all labelled tokens, or "sequence", the mean over the sequences that have
+    any of their mean; 0 without any.  advantages: one per token, or one per sequence [N]."""
+    def forward_of(call):
+        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)
+    return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of))
+
+
+def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2,
+                         clip_high=0.2, kl_coef=0.0, reduction="token", ignore_index=-100, grad_scale=1.0):
+    """(policy_loss(...), gradient of the loss times grad_scale in the logits)."""
+    call = _Call(logits, labels, ignore_index, cu_seqlens)
+    out, stats, k, weights = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)
+    return out, call.grad(stats, k, weights, grad_scale)

@@ -549,6 +549,69 @@ int gefenx_adamw_norm(const gefenx_adamw_desc* descs, int n, double max_norm, fl
 int gefenx_adamw_moments(const gefenx_adamw_desc* descs, int n, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Losses over the logits of a language model, and the gradient of the logits.
+ * No counterpart in the reference.  Row r of the logits (vocab elements, the
+ * last dimension of stride 1) predicts labels[r]; a row whose label is
+ * ignore_index takes no part (it is not read, and its gradient is 0), any other
+ * label outside [0, vocab) makes the results that it takes part in NaN.  With
+ * l = x[label] - logsumexp(x) in fp32, all sums over rows in float64.
+ * Sequences: cu_seqlens NULL: each batch of rows_per_batch rows is one
+ * (rows == n_seq * rows_per_batch); else a device int32[n_seq + 1], sequence i
+ * has rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1.
+ * ---------------------------------------------------------------------- */
+typedef struct gefenx_logits {
+    const void* logits;
+    const int64_t* labels;     /* device int64 [rows] */
+    const int32_t* cu_seqlens;
+    int64_t rows, rows_per_batch;
+    int64_t batch_stride, row_stride; /* elements: row r starts at (r / rows_per_batch)
+                                       * * batch_stride + (r % rows_per_batch) * row_stride */
+    int64_t vocab;
+    int64_t ignore_index;
+    int32_t dtype;             /* gefenx_dtype of the logits and their gradient */
+    int32_t n_seq;             /* 0 where sequences do not matter */
+} gefenx_logits;
+
+/* Bytes of device scratch (any contents) for the calls below. */
+size_t gefenx_loss_workspace_bytes(const gefenx_logits* logits);
+
+/* logps[r] = l (0 where ignored); stats[r] = {max x, sum exp(x - max)}, fp32[2],
+ * for gefenx_logits_grad. */
+int gefenx_token_logps(const gefenx_logits* logits, float* logps, float* stats, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Preference loss of n_seq / 2 pairs, the chosen sequences first:
+ *   reward_i = beta * sum_t (l_t - ref_t) (average: / the sequence's labels; 0 without any)
+ *   loss = mean_j -(1 - s) log sigmoid(h_j) - s log sigmoid(-h_j),  h_j = reward_j - reward_{n_seq/2 + j}
+ * ref_logps: fp32 [rows] or NULL (zeros).  Written: loss[1], the rewards of
+ * either side [n_seq / 2], logps[rows], and stats / weights[n_seq] for
+ * gefenx_logits_grad. */
+int gefenx_preference_loss(const gefenx_logits* logits, const float* ref_logps, double beta,
+                           double label_smoothing, int average, float* loss, float* chosen_rewards,
+                           float* rejected_rewards, float* logps, float* stats, float* weights, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Clipped policy loss: with q = exp(l - old), d = ref - l,
+ *   each = -min(q A, clamp(q, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)
+ *   loss = mean over the labelled rows, or (by_sequence) mean over the sequences that have
+ *   labelled rows of the mean over these; 0 without any.
+ * advantages: fp32 [rows] (advantages_per_row) or [n_seq]; ref_logps NULL: no KL
+ * term.  Written: loss[1], kl[1] (mean over the labelled rows), clip_fraction[1]
+ * (share of them whose minimum is the clamped term), logps[rows], and stats /
+ * k[rows] / weights[n_seq] for gefenx_logits_grad. */
+int gefenx_policy_loss(const gefenx_logits* logits, const float* old_logps, const float* advantages,
+                       int advantages_per_row, const float* ref_logps, double clip_low, double clip_high,
+                       double kl_coef, int by_sequence, float* loss, float* kl, float* clip_fraction,
+                       float* logps, float* stats, float* k, float* weights, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* grad[r][v] = c_r ([v == label] - softmax(x_r)[v]) in the logits' dtype, [rows,
+ * vocab] contiguous, with c_r = k[r] (NULL: 1) * weights[sequence of r] (NULL: 1)
+ * * *scale_dev (NULL: 1) * scale, rounded once. */
+int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const float* k, const float* weights,
+                       const float* scale_dev, double scale, void* grad, void* stream);
+
+/* ------------------------------------------------------------------------
  * Kernel timing.  When enabled, every update-kernel launch is bracketed by
  * HIP events on its own stream and tagged with its kind and algorithmic
  * bytes (compulsory traffic of the step it belongs to); gefenx_profile_read

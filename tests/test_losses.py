@@ -1,0 +1,39 @@
+"""Argument checks of the losses that need no GPU."""
+import pytest
+import torch
+
+import gefen
+
+
+def test_host_logits_are_refused():
+    logits, labels = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.long)
+    with pytest.raises(ValueError, match="HIP device"):
+        gefen.token_logps(logits, labels)
+    with pytest.raises(ValueError, match="HIP device"):
+        gefen.preference_loss(logits, labels)
+    with pytest.raises(ValueError, match="HIP device"):
+        gefen.policy_loss_and_grad(logits, labels, torch.zeros(2, 3), torch.zeros(2))
+
+
+def test_other_things_than_tensors_are_refused():
+    with pytest.raises(TypeError):
+        gefen.token_logps([[1.0]], torch.zeros(1, dtype=torch.long))
+
+
+def test_bad_descriptors_are_refused_on_the_host():
+    import ctypes
+    from gefen.kernels import _native
+    lib = _native.load()
+    good = dict(logits=64, labels=64, rows=4, rows_per_batch=2, batch_stride=10, row_stride=5, vocab=5, dtype=0, n_seq=2)
+    assert lib.gefenx_loss_workspace_bytes(ctypes.byref(_native.Logits(**good))) > 0
+    for change in ({"dtype": 3}, {"vocab": 0}, {"rows": -1}, {"rows_per_batch": 0}, {"labels": None}, {"rows": 1 << 31}):
+        d = _native.Logits(**{**good, **change})
+        assert lib.gefenx_loss_workspace_bytes(ctypes.byref(d)) == 0, change
+        assert lib.gefenx_token_logps(ctypes.byref(d), 64, 64, 64, 1 << 20, None) == (-2 if "dtype" in change else -1), change
+    odd = _native.Logits(**{**good, "rows": 6, "n_seq": 3})
+    assert lib.gefenx_preference_loss(ctypes.byref(odd), None, 0.1, 0.0, 0, 64, 64, 64, 64, 64, 64, 64, 1 << 20, None) == -1
+    none = _native.Logits(**{**good, "n_seq": 0})
+    assert lib.gefenx_preference_loss(ctypes.byref(none), None, 0.1, 0.0, 0, 64, 64, 64, 64, 64, 64, 64, 1 << 20, None) == -1
+    small = _native.Logits(**good)
+    assert lib.gefenx_token_logps(ctypes.byref(small), 64, 64, 64, 8, None) == -1
+    assert "workspace" in _native.last_error()
