@@ -39,7 +39,7 @@ struct Batch {
     Item it[kItems];
     int32_t end[kItems];  // workgroups up to and including tensor i
     int32_t n;
-    int32_t iters;        // a workgroup's chunks per lane (8-bit moments: pairs of chunks)
+    int32_t iters;        // gradient norm: passes of a workgroup
 };
 static_assert(sizeof(Batch) <= 4080, "kernel arguments");
 
@@ -54,56 +54,81 @@ __device__ __forceinline__ int find_item(const Batch& b, int w, int& local) {
     return lo;
 }
 
-// ------------------------------------------------------------ chunks of 8
-// Whole chunks by vector accesses of any alignment, the last one of a tensor by elements.
+// ------------------------------------------------------------ runs of elements
+// A lane moves W consecutive elements at a time: 16 bytes of the widest stream beside it, so that a
+// wave's accesses to that stream leave no gaps (two 16-byte pieces of 8 fp32 elements a lane took the
+// fp32 step of 218M bf16 elements from 793 to 883 us).  Whole runs by vector accesses of any
+// alignment, a tensor's last one by elements.
 
-template <int DT>
-__device__ __forceinline__ void load_chunk(const typename Elem<DT>::T* base, int64_t left, Raw8<DT>& r) {
-    if (left >= 8) {
-        load_raw8_any<DT>(base, r);
-        return;
-    }
-    if constexpr (DT == F32) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r.f[k] = k < left ? *gbl(base + k) : 0.0f;
+template <class T, int W> struct Run { T e[W]; };
+
+template <class T, int W>
+__device__ __forceinline__ Run<T, W> load_run(const T* base, int64_t left) {
+    typedef uint32_t V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
+    static_assert(W * sizeof(T) >= 8, "vectors of two words and more");
+    Run<T, W> r;
+    if (left >= W) {
+        const auto v = __builtin_nontemporal_load(GX_GLOBAL_AS(const V, base));
+        __builtin_memcpy(&r, &v, sizeof(r));
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = 2 * k < left ? *gbl(base + 2 * k) : 0, hi = 2 * k + 1 < left ? *gbl(base + 2 * k + 1) : 0;
-            r.w[k] = lo | (hi << 16);
+        for (int k = 0; k < W; ++k) r.e[k] = k < left ? *gbl(base + k) : T(0);
+    }
+    return r;
+}
+
+template <class T, int W>
+__device__ __forceinline__ void store_run(T* base, int64_t left, const Run<T, W>& r) {
+    typedef uint32_t V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
+    if (left >= W) {
+        V v;
+        __builtin_memcpy(&v, &r, sizeof(r));
+        __builtin_nontemporal_store(v, GX_GLOBAL_AS(V, base));
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+            if (k < left) *gbl(base + k) = r.e[k];
+    }
+}
+
+// Four codes to a word.
+__device__ __forceinline__ uint32_t load_codes4(const uint8_t* base, int64_t left) {
+    typedef uint32_t V __attribute__((aligned(1)));
+    if (left >= 4) return __builtin_nontemporal_load(GX_GLOBAL_AS(const V, base));
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        if (k < left) w |= (uint32_t)*gbl(base + k) << (8 * k);
+    return w;
+}
+
+template <int W>
+__device__ __forceinline__ void load_codes(const uint8_t* base, int64_t left, uint32_t (&c)[W / 4]) {
+    if (W == 8 && left >= 8) {
+        const RawIdx8 v = load_raw_idx8_any(base);
+        c[0] = v.lo;
+        c[W / 4 - 1] = v.hi;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) c[i] = load_codes4(base + 4 * i, left - 4 * i);
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void store_codes(uint8_t* base, int64_t left, const uint32_t (&c)[W / 4]) {
+    if (left >= W) {
+        if constexpr (W == 8) {
+            const u32x2 a = {c[0], c[1]};
+            __builtin_nontemporal_store(a, GX_GLOBAL_AS(u32x2_a1, base));
+        } else {
+            typedef uint32_t V __attribute__((aligned(1)));
+            __builtin_nontemporal_store(c[0], GX_GLOBAL_AS(V, base));
         }
-    }
-}
-
-template <int DT>
-__device__ __forceinline__ void store_chunk(typename Elem<DT>::T* base, int64_t left, const float v[8]) {
-    if (left >= 8) {
-        store8_any<DT>(base, v);
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k < left) *gbl(base + k) = from_f32<DT>(v[k]);
-}
-
-__device__ __forceinline__ RawIdx8 load_codes(const uint8_t* base, int64_t left) {
-    if (left >= 8) return load_raw_idx8_any(base);
-    uint32_t w[2] = {0u, 0u};
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k < left) w[k >> 2] |= (uint32_t)*gbl(base + k) << (8 * (k & 3));
-    return RawIdx8{w[0], w[1]};
-}
-
-__device__ __forceinline__ void store_codes(uint8_t* base, int64_t left, const uint32_t w[2]) {
-    if (left >= 8) {
-        const u32x2 a = {w[0], w[1]};
-        __builtin_nontemporal_store(a, GX_GLOBAL_AS(u32x2_a1, base));
-        return;
+        for (int k = 0; k < W; ++k)
+            if (k < left) *gbl(base + k) = (uint8_t)(c[k >> 2] >> (8 * (k & 3)));
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (k < left) *gbl(base + k) = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
 }
 
 // The moments round after each operation, as the formula written in torch does, so 8-bit codes follow
@@ -112,38 +137,43 @@ __device__ __forceinline__ void advance(const Item& t, float g, float& m, float&
     m = m * t.b1 + g * t.a1;
     v = v * t.b2 + g * g * t.a2;
 }
+// FAST: the hardware's square root and reciprocal, 1 unit each, as good as the exact ones before p
+// rounds.  That square root takes v below 2^-126 for 0, which eps has to drown: sqrt(2^-126) / sqrt(bc2)
+// is under 2^-24 eps for eps >= kFastEps and 1 / sqrt(bc2) up to 2^6.
+constexpr float kFastEps = 1e-10f;
+template <bool FAST>
 __device__ __forceinline__ float stepped(const Item& t, float p, float m, float v) {
-    const float d = __builtin_fmaf(__builtin_sqrtf(v), t.rbc2, t.eps);
-    return __builtin_fmaf(-t.step, m / d, p * t.wdf);
+    if constexpr (FAST) {
+        const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v), t.rbc2, t.eps);
+        return __builtin_fmaf(-t.step, m * __builtin_amdgcn_rcpf(d), p * t.wdf);
+    } else {
+        const float d = __builtin_fmaf(__builtin_sqrtf(v), t.rbc2, t.eps);
+        return __builtin_fmaf(-t.step, m / d, p * t.wdf);
+    }
 }
 
 // ------------------------------------------------------------ fp32 moments
+constexpr int kW32 = 4;  // elements of a lane
 template <int DT>
 __global__ __launch_bounds__(kT) void k_adamw(const Batch b, const float* __restrict__ coef) {
     using T = typename Elem<DT>::T;
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
     const float c = coef ? sload(coef) : 1.0f;
-    for (int it = 0; it < b.iters; ++it) {
-        const int64_t at = (((int64_t)local * b.iters + it) * kT + threadIdx.x) * 8;
-        const int64_t left = t.n - at;
-        if (left <= 0) return;
-        Raw8<DT> g, p;
-        Raw8<F32> m, v;
-        load_chunk<DT>((const T*)t.g + at, left, g);
-        load_chunk<F32>((const float*)t.m + at, left, m);
-        load_chunk<F32>((const float*)t.v + at, left, v);
-        load_chunk<DT>((const T*)t.p + at, left, p);
-        float q[8];
+    const int64_t at = ((int64_t)local * kT + threadIdx.x) * kW32;
+    const int64_t left = t.n - at;
+    if (left <= 0) return;
+    const auto g = load_run<T, kW32>((const T*)t.g + at, left);
+    auto m = load_run<float, kW32>((const float*)t.m + at, left), v = load_run<float, kW32>((const float*)t.v + at, left);
+    auto p = load_run<T, kW32>((const T*)t.p + at, left);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            advance(t, raw_elem<DT>(g, k) * c, m.f[k], v.f[k]);
-            q[k] = stepped(t, raw_elem<DT>(p, k), m.f[k], v.f[k]);
-        }
-        store_chunk<F32>((float*)t.m + at, left, m.f);
-        store_chunk<F32>((float*)t.v + at, left, v.f);
-        store_chunk<DT>((T*)t.p + at, left, q);
+    for (int k = 0; k < kW32; ++k) {
+        advance(t, to_f32<DT>(g.e[k]) * c, m.e[k], v.e[k]);
+        p.e[k] = from_f32<DT>(stepped<false>(t, to_f32<DT>(p.e[k]), m.e[k], v.e[k]));
     }
+    store_run<float, kW32>((float*)t.m + at, left, m);
+    store_run<float, kW32>((float*)t.v + at, left, v);
+    store_run<T, kW32>((T*)t.p + at, left, p);
 }
 
 // ------------------------------------------------------------ 8-bit moments
@@ -160,50 +190,40 @@ __device__ __forceinline__ uint64_t mix64(uint64_t z) {
     return z ^ (z >> 31);
 }
 
-__device__ __forceinline__ void decode_m(const RawIdx8& c, float scale, float m[8]) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.lo, true);
-    const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.hi, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.hi, true);
-    m[0] = a.x * scale; m[1] = a.y * scale; m[2] = b.x * scale; m[3] = b.y * scale;
-    m[4] = d.x * scale; m[5] = d.y * scale; m[6] = e.x * scale; m[7] = e.y * scale;
+__device__ __forceinline__ void decode_m(uint32_t c, float scale, float* m) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+    m[0] = a[0] * scale; m[1] = a[1] * scale; m[2] = b[0] * scale; m[3] = b[1] * scale;
 }
 
-__device__ __forceinline__ void decode_v(const RawIdx8& c, float scale, float v[8]) {
+__device__ __forceinline__ void decode_v(uint32_t c, float scale, float* v) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t x = raw_idx(c, k);
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t x = (c >> (8 * k)) & 0xffu;
         v[k] = (x ? __uint_as_float((x + kCode0) << 20) : 0.0f) * scale;
     }
 }
 
-__device__ __forceinline__ void encode_m(const float m[8], float inv, uint32_t w[2]) {
-    float x[8];
+__device__ __forceinline__ uint32_t encode_m(const float* m, float inv) {
+    float x[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = __builtin_amdgcn_fmed3f(m[k] * inv, -448.0f, 448.0f);
-    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4], x[5], 0, false);
-    w[0] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
-    w[1] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[6], x[7], hi, true);
+    for (int k = 0; k < 4; ++k) x[k] = __builtin_amdgcn_fmed3f(m[k] * inv, -448.0f, 448.0f);
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
 }
 
-// at: the chunk's first element, a multiple of 8: two draws of four elements each
-__device__ __forceinline__ void encode_v(const float v[8], float inv, uint64_t key, int64_t at, uint32_t w[2]) {
-    constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ULL;
-    const uint64_t z0 = key + kGolden * ((uint64_t)(at >> 2) + 1);
+// at: the first element of the four, a multiple of 4: one draw
+__device__ __forceinline__ uint32_t encode_v(const float* v, float inv, uint64_t key, int64_t at) {
+    const uint64_t z = mix64(key + 0x9E3779B97F4A7C15ULL * ((uint64_t)(at >> 2) + 1));
+    const uint32_t r[2] = {(uint32_t)z, (uint32_t)(z >> 32)};
+    uint32_t packed = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint64_t z = mix64(h ? z0 + kGolden : z0);
-        const uint32_t r[2] = {(uint32_t)z, (uint32_t)(z >> 32)};
-        uint32_t packed = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t dither = (k & 1 ? r[k >> 1] >> 12 : r[k >> 1] << 4) & 0xffff0u;
-            const float x = v[4 * h + k];
-            int c = (int)((__float_as_uint(x * inv) + dither) >> 20) - kCode0;
-            c = c < 1 ? 1 : (c > 255 ? 255 : c);
-            packed |= (uint32_t)(x == 0.0f ? 0 : c) << (8 * k);
-        }
-        w[h] = packed;
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t dither = (k & 1 ? r[k >> 1] >> 12 : r[k >> 1] << 4) & 0xffff0u;
+        int c = (int)((__float_as_uint(v[k] * inv) + dither) >> 20) - kCode0;
+        c = c < 1 ? 1 : (c > 255 ? 255 : c);
+        packed |= (uint32_t)(v[k] == 0.0f ? 0 : c) << (8 * k);
     }
+    return packed;
 }
 
 // Largest value of a block's 16 lanes, in each of them (bits of non-negative floats, NaN above inf).
@@ -220,63 +240,68 @@ __device__ __forceinline__ float block_scale(float amax) {
     return amax <= 3.402823466e38f ? (amax > kTiny ? amax : kTiny) : __uint_as_float(0x7fc00000u);
 }
 
-template <int DT>
+// A block of 256 elements by 16 lanes, each with N runs of W of them: the moments stay in registers
+// between the block's maxima and its codes.
+template <int DT, bool FAST>
 __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __restrict__ coef) {
     using T = typename Elem<DT>::T;
+    constexpr int W = 16 / sizeof(T), N = kBlock8 / (kGroup * W);
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
     const float c = coef ? sload(coef) : 1.0f;
-    const int lane = threadIdx.x & (kGroup - 1), group = threadIdx.x / kGroup;
-    for (int it = 0; it < b.iters; ++it) {
-        const int64_t blk = ((int64_t)local * b.iters + it) * (kT / kGroup) + group;
-        const int64_t at0 = blk * kBlock8 + lane * 8;
-        // the 16 lanes of a block leave together or stay together: what they exchange is among themselves
-        if (blk * kBlock8 >= t.n) return;
-        Raw8<DT> g[2], p[2];
-        RawIdx8 mc[2], vc[2];
-        const float ms = *gbl(t.ms + blk), vs = *gbl(t.vs + blk);
+    const int lane = threadIdx.x & (kGroup - 1);
+    const int64_t blk = (int64_t)local * (kT / kGroup) + threadIdx.x / kGroup;
+    // the 16 lanes of a block leave together or stay together: what they exchange is among themselves
+    if (blk * kBlock8 >= t.n) return;
+    const int64_t at0 = blk * kBlock8 + lane * W;
+    Run<T, W> g[N], p[N];
+    uint32_t mc[N][W / 4], vc[N][W / 4];
+    const float ms = *gbl(t.ms + blk), vs = *gbl(t.vs + blk);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t at = at0 + h * (kBlock8 / 2), left = t.n - at;
-            load_chunk<DT>((const T*)t.g + at, left, g[h]);
-            mc[h] = load_codes((const uint8_t*)t.m + at, left);
-            vc[h] = load_codes((const uint8_t*)t.v + at, left);
-            load_chunk<DT>((const T*)t.p + at, left, p[h]);
-        }
-        float m[2][8], v[2][8];
-        uint32_t mx = 0, vx = 0;
+    for (int h = 0; h < N; ++h) {
+        const int64_t at = at0 + h * kGroup * W, left = t.n - at;
+        g[h] = load_run<T, W>((const T*)t.g + at, left);
+        load_codes<W>((const uint8_t*)t.m + at, left, mc[h]);
+        load_codes<W>((const uint8_t*)t.v + at, left, vc[h]);
+        p[h] = load_run<T, W>((const T*)t.p + at, left);
+    }
+    float m[N][W], v[N][W];
+    uint32_t mx = 0, vx = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t at = at0 + h * (kBlock8 / 2), left = t.n - at;
-            decode_m(mc[h], ms, m[h]);
-            decode_v(vc[h], vs, v[h]);
-            float q[8];
+    for (int h = 0; h < N; ++h) {
+        const int64_t at = at0 + h * kGroup * W, left = t.n - at;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                advance(t, raw_elem<DT>(g[h], k) * c, m[h][k], v[h][k]);
-                q[k] = stepped(t, raw_elem<DT>(p[h], k), m[h][k], v[h][k]);
-                const uint32_t mb = __float_as_uint(m[h][k]) & 0x7fffffffu, vb = __float_as_uint(v[h][k]) & 0x7fffffffu;
-                mx = mb > mx ? mb : mx;
-                vx = vb > vx ? vb : vx;
-            }
-            if (left > 0) store_chunk<DT>((T*)t.p + at, left, q);
+        for (int i = 0; i < W / 4; ++i) {
+            decode_m(mc[h][i], ms, m[h] + 4 * i);
+            decode_v(vc[h][i], vs, v[h] + 4 * i);
         }
-        const float mscale = block_scale(__uint_as_float(group16_max(mx)) * (1.0f / 448.0f));
-        const float vscale = block_scale(__uint_as_float(group16_max(vx)));
-        const float minv = 1.0f / mscale, vinv = 1.0f / vscale;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t at = at0 + h * (kBlock8 / 2), left = t.n - at;
-            uint32_t w[2];
-            encode_m(m[h], minv, w);
-            if (left > 0) store_codes((uint8_t*)t.m + at, left, w);
-            encode_v(v[h], vinv, t.key, at, w);
-            if (left > 0) store_codes((uint8_t*)t.v + at, left, w);
+        for (int k = 0; k < W; ++k) {
+            advance(t, to_f32<DT>(g[h].e[k]) * c, m[h][k], v[h][k]);
+            p[h].e[k] = from_f32<DT>(stepped<FAST>(t, to_f32<DT>(p[h].e[k]), m[h][k], v[h][k]));
+            const uint32_t mb = __float_as_uint(m[h][k]) & 0x7fffffffu, vb = __float_as_uint(v[h][k]) & 0x7fffffffu;
+            mx = mb > mx ? mb : mx;
+            vx = vb > vx ? vb : vx;
         }
-        if (lane == 0) {
-            *gbl(t.ms + blk) = mscale;
-            *gbl(t.vs + blk) = vscale;
+        store_run<T, W>((T*)t.p + at, left, p[h]);
+    }
+    const float mscale = block_scale(__uint_as_float(group16_max(mx)) * (1.0f / 448.0f));
+    const float vscale = block_scale(__uint_as_float(group16_max(vx)));
+    const float minv = 1.0f / mscale, vinv = 1.0f / vscale;
+#pragma unroll
+    for (int h = 0; h < N; ++h) {
+        const int64_t at = at0 + h * kGroup * W, left = t.n - at;
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            mc[h][i] = encode_m(m[h] + 4 * i, minv);
+            vc[h][i] = encode_v(v[h] + 4 * i, vinv, t.key, at + 4 * i);
         }
+        store_codes<W>((uint8_t*)t.m + at, left, mc[h]);
+        store_codes<W>((uint8_t*)t.v + at, left, vc[h]);
+    }
+    if (lane == 0) {
+        *gbl(t.ms + blk) = mscale;
+        *gbl(t.vs + blk) = vscale;
     }
 }
 
@@ -284,18 +309,16 @@ __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __res
 __global__ __launch_bounds__(kT) void k_adamw8_values(const Batch b) {
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
-    for (int it = 0; it < b.iters; ++it) {
-        const int64_t at = (((int64_t)local * b.iters + it) * kT + threadIdx.x) * 8;
-        const int64_t left = t.n - at;
-        if (left <= 0) return;
-        const RawIdx8 mc = load_codes((const uint8_t*)t.m + at, left), vc = load_codes((const uint8_t*)t.v + at, left);
-        const int64_t blk = at / kBlock8;
-        float x[8];
-        decode_m(mc, *gbl(t.ms + blk), x);
-        store_chunk<F32>((float*)t.p + at, left, x);
-        decode_v(vc, *gbl(t.vs + blk), x);
-        store_chunk<F32>((float*)const_cast<void*>(t.g) + at, left, x);
-    }
+    const int64_t at = ((int64_t)local * kT + threadIdx.x) * 4;
+    const int64_t left = t.n - at;
+    if (left <= 0) return;
+    const uint32_t mc = load_codes4((const uint8_t*)t.m + at, left), vc = load_codes4((const uint8_t*)t.v + at, left);
+    const int64_t blk = at / kBlock8;
+    Run<float, 4> x;
+    decode_m(mc, *gbl(t.ms + blk), x.e);
+    store_run<float, 4>((float*)t.p + at, left, x);
+    decode_v(vc, *gbl(t.vs + blk), x.e);
+    store_run<float, 4>((float*)const_cast<void*>(t.g) + at, left, x);
 }
 
 // ------------------------------------------------------------ gradient norm
@@ -311,11 +334,10 @@ __global__ __launch_bounds__(kT) void k_grad_sumsq(const Batch b, double* __rest
         const int64_t at = (((int64_t)local * b.iters + it) * kT + threadIdx.x) * 8;
         const int64_t left = t.n - at;
         if (left <= 0) break;
-        Raw8<DT> g;
-        load_chunk<DT>((const T*)t.g + at, left, g);
+        const auto g = load_run<T, 8>((const T*)t.g + at, left);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const double x = (double)raw_elem<DT>(g, k);
+            const double x = (double)to_f32<DT>(g.e[k]);
             s = __builtin_fma(x, x, s);
         }
     }
@@ -375,15 +397,18 @@ Item item_of(const gefenx_adamw_desc& d) {
                 d.step_size, d.wd_factor, d.beta1, d.alpha1, d.beta2, d.alpha2, d.inv_sqrt_bc2, d.eps};
 }
 
-// Elements of one pass of a workgroup.
-constexpr int64_t kPass32 = (int64_t)kT * 8, kPass8 = (int64_t)kT * 16;
+// Elements of a workgroup.  One pass each: workgroups start in order, so what is being written at any
+// time lies in a few runs of memory (four passes: 960 us against 896 on the layer above).
+constexpr int64_t kWg32 = (int64_t)kT * kW32, kWg8 = (int64_t)kT * kBlock8 / kGroup, kWgValues = (int64_t)kT * 4;
+constexpr int64_t kNormPass = (int64_t)kT * 8;
 
-// Calls launch(batch, workgroups) for the tensors of one dtype and moment width, kItems at a time.
-template <class F>
-int for_batches(const gefenx_adamw_desc* d, int n, int dtype, int bits, int64_t pass, int iters, F&& launch) {
+// Calls launch(batch, workgroups) for the tensors that take(descriptor) picks, kItems at a time, `per`
+// elements to a workgroup.
+template <class P, class F>
+int for_batches(const gefenx_adamw_desc* d, int n, int64_t per, P&& take, F&& launch) {
     Batch b;
     b.n = 0;
-    b.iters = iters;
+    b.iters = 1;
     int64_t wgs = 0;
     const auto flush = [&]() -> int {
         if (!b.n) return GEFENX_OK;
@@ -393,9 +418,9 @@ int for_batches(const gefenx_adamw_desc* d, int n, int dtype, int bits, int64_t 
         return rc;
     };
     for (int i = 0; i < n; ++i) {
-        if (d[i].dtype != dtype || (bits && d[i].bits != bits) || d[i].numel == 0) continue;
-        const int64_t w = (d[i].numel + pass * iters - 1) / (pass * iters);
-        if (b.n == kItems || wgs + w > 0x3fffffff) {
+        if (d[i].numel == 0 || !take(d[i])) continue;
+        const int64_t w = (d[i].numel + per - 1) / per;
+        if (b.n == kItems || wgs + w > 0x7fffffff) {
             const int rc = flush();
             if (rc != GEFENX_OK) return rc;
         }
@@ -412,38 +437,46 @@ int64_t total_elems(const gefenx_adamw_desc* d, int n) {
     return s;
 }
 
-int step_iters(int64_t elems, int64_t pass) {
-    return elems >= (int64_t)8192 * pass ? 4 : 1;
-}
-
 int norm_iters(int64_t elems) {
-    const int64_t k = (elems + kNormPartials * kPass32 - 1) / (kNormPartials * kPass32);
+    const int64_t k = (elems + kNormPartials * kNormPass - 1) / (kNormPartials * kNormPass);
     return (int)(k < 1 ? 1 : k);
 }
 
 int64_t norm_partials(const gefenx_adamw_desc* d, int n) {
-    const int64_t per = kPass32 * norm_iters(total_elems(d, n));
+    const int64_t per = kNormPass * norm_iters(total_elems(d, n));
     int64_t s = 0;
     for (int i = 0; i < n; ++i) s += (d[i].numel + per - 1) / per;
     return s;
 }
 
 template <int DT>
-int step_dtype(const gefenx_adamw_desc* d, int n, int64_t elems, const float* coef, hipStream_t s) {
-    int rc = for_batches(d, n, DT, 32, kPass32, step_iters(elems, kPass32), [&](const Batch& b, int wgs) {
+int step_dtype(const gefenx_adamw_desc* d, int n, const float* coef, hipStream_t s) {
+    const auto picks = [](int bits, bool fast) {
+        return [=](const gefenx_adamw_desc& t) {
+            return t.dtype == DT && t.bits == bits && (bits == 32 || (t.eps >= kFastEps) == fast);
+        };
+    };
+    int rc = for_batches(d, n, kWg32, picks(32, false), [&](const Batch& b, int wgs) {
         k_adamw<DT><<<wgs, kT, 0, s>>>(b, coef);
         return launched("gefenx_adamw_step");
     });
-    if (rc != GEFENX_OK) return rc;
-    return for_batches(d, n, DT, 8, kPass8, step_iters(elems, kPass8), [&](const Batch& b, int wgs) {
-        k_adamw8<DT><<<wgs, kT, 0, s>>>(b, coef);
-        return launched("gefenx_adamw_step");
-    });
+    if (rc == GEFENX_OK)
+        rc = for_batches(d, n, kWg8, picks(8, true), [&](const Batch& b, int wgs) {
+            k_adamw8<DT, true><<<wgs, kT, 0, s>>>(b, coef);
+            return launched("gefenx_adamw_step");
+        });
+    if (rc == GEFENX_OK)
+        rc = for_batches(d, n, kWg8, picks(8, false), [&](const Batch& b, int wgs) {
+            k_adamw8<DT, false><<<wgs, kT, 0, s>>>(b, coef);
+            return launched("gefenx_adamw_step");
+        });
+    return rc;
 }
 
 template <int DT>
 int norm_dtype(const gefenx_adamw_desc* d, int n, int iters, double*& at, hipStream_t s) {
-    return for_batches(d, n, DT, 0, kPass32, iters, [&](const Batch& b, int wgs) {
+    return for_batches(d, n, kNormPass * iters, [](const gefenx_adamw_desc& t) { return t.dtype == DT; }, [&](Batch& b, int wgs) {
+        b.iters = iters;
         k_grad_sumsq<DT><<<wgs, kT, 0, s>>>(b, at);
         at += wgs;
         return launched("gefenx_adamw_norm");
@@ -461,10 +494,9 @@ int gefenx_adamw_step(const gefenx_adamw_desc* descs, int n, const float* grad_c
     int rc = validate("gefenx_adamw_step", descs, n, true, true);
     if (rc != GEFENX_OK) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t elems = total_elems(descs, n);
-    rc = step_dtype<F32>(descs, n, elems, grad_coef, s);
-    if (rc == GEFENX_OK) rc = step_dtype<F16>(descs, n, elems, grad_coef, s);
-    if (rc == GEFENX_OK) rc = step_dtype<BF16>(descs, n, elems, grad_coef, s);
+    rc = step_dtype<F32>(descs, n, grad_coef, s);
+    if (rc == GEFENX_OK) rc = step_dtype<F16>(descs, n, grad_coef, s);
+    if (rc == GEFENX_OK) rc = step_dtype<BF16>(descs, n, grad_coef, s);
     return rc;
 }
 
@@ -501,7 +533,7 @@ int gefenx_adamw_moments(const gefenx_adamw_desc* descs, int n, void* stream) {
         if (descs[i].bits != 8 || descs[i].dtype != GEFENX_F32)
             return set_error(GEFENX_EINVAL, "gefenx_adamw_moments: tensor %d: 8-bit moments into fp32 only", i);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    return for_batches(descs, n, F32, 8, kPass32, step_iters(total_elems(descs, n), kPass32), [&](const Batch& b, int wgs) {
+    return for_batches(descs, n, kWgValues, [](const gefenx_adamw_desc&) { return true; }, [&](const Batch& b, int wgs) {
         k_adamw8_values<<<wgs, kT, 0, s>>>(b);
         return launched("gefenx_adamw_moments");
     });

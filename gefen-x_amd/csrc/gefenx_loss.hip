@@ -8,6 +8,7 @@
 // statistics, a few numbers per row and sequence, and a pass that writes the gradient.  Both passes are
 // bound by memory; rows without a label are not read.
 #include <hip/hip_runtime.h>
+#include <stdlib.h>
 
 #include "gefenx.h"
 #include "gefenx_device.h"
@@ -419,7 +420,7 @@ int launched(const char* what) {
 }
 
 // Row workgroups: one per row, or enough to fill the chip where the rows are few, each of a pass or more.
-int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q) {
+int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q, int64_t most_passes = 0) {
     if (!l) return set_error(GEFENX_EINVAL, "%s: null descriptor", what);
     if (l->dtype != GEFENX_F32 && l->dtype != GEFENX_F16 && l->dtype != GEFENX_BF16)
         return set_error(GEFENX_EDTYPE, "%s: unsupported dtype %d", what, l->dtype);
@@ -441,6 +442,7 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q)
     q.n_seq = l->n_seq;
     const int64_t chunks = (l->vocab + 7) / 8, passes = (l->vocab + kPass - 1) / kPass;
     int64_t splits = l->rows > 0 ? (kWantedWgs + l->rows - 1) / l->rows : 1;
+    if (most_passes && splits < (passes + most_passes - 1) / most_passes) splits = (passes + most_passes - 1) / most_passes;
     splits = splits < 1 ? 1 : (splits > passes ? passes : splits);
     q.split_chunks = (chunks + splits - 1) / splits;
     q.splits = (int32_t)((chunks + q.split_chunks - 1) / q.split_chunks);
@@ -577,7 +579,8 @@ int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const fl
                        const float* scale_dev, double scale, void* grad, void* stream) {
     const char* what = "gefenx_logits_grad";
     Rows q;
-    int rc = make_rows(what, logits, weights != nullptr, q);
+    static int e = getenv("GX_GP") ? atoi(getenv("GX_GP")) : 4;
+    int rc = make_rows(what, logits, weights != nullptr, q, e);
     if (rc != GEFENX_OK) return rc;
     if (q.rows == 0) return GEFENX_OK;
     if (!stats || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
