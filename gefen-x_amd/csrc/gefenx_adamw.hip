@@ -60,37 +60,6 @@ __device__ __forceinline__ int find_item(const Batch& b, int w, int& local) {
 // fp32 step of 218M bf16 elements from 793 to 883 us).  Whole runs by vector accesses of any
 // alignment, a tensor's last one by elements.
 
-template <class T, int W> struct Run { T e[W]; };
-
-template <class T, int W>
-__device__ __forceinline__ Run<T, W> load_run(const T* base, int64_t left) {
-    typedef uint32_t V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
-    static_assert(W * sizeof(T) >= 8, "vectors of two words and more");
-    Run<T, W> r;
-    if (left >= W) {
-        const auto v = __builtin_nontemporal_load(GX_GLOBAL_AS(const V, base));
-        __builtin_memcpy(&r, &v, sizeof(r));
-    } else {
-#pragma unroll
-        for (int k = 0; k < W; ++k) r.e[k] = k < left ? *gbl(base + k) : T(0);
-    }
-    return r;
-}
-
-template <class T, int W>
-__device__ __forceinline__ void store_run(T* base, int64_t left, const Run<T, W>& r) {
-    typedef uint32_t V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
-    if (left >= W) {
-        V v;
-        __builtin_memcpy(&v, &r, sizeof(r));
-        __builtin_nontemporal_store(v, GX_GLOBAL_AS(V, base));
-    } else {
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-            if (k < left) *gbl(base + k) = r.e[k];
-    }
-}
-
 // Four codes to a word.
 __device__ __forceinline__ uint32_t load_codes4(const uint8_t* base, int64_t left) {
     typedef uint32_t V __attribute__((aligned(1)));

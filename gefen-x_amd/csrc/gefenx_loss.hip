@@ -8,7 +8,6 @@
 // statistics, a few numbers per row and sequence, and a pass that writes the gradient.  Both passes are
 // bound by memory; rows without a label are not read.
 #include <hip/hip_runtime.h>
-#include <stdlib.h>
 
 #include "gefenx.h"
 #include "gefenx_device.h"
@@ -18,8 +17,8 @@ namespace gx {
 namespace {
 
 constexpr int kT = 256;               // threads of a row workgroup
-constexpr int kPass = kT * 8;         // logits of one pass of it
 constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
+constexpr int64_t kGradPasses = 2;    // passes of a workgroup of the gradient
 constexpr int kSeqT = 1024;           // threads of a sequence workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eRest = (float)(1.44269504088896340736 - (double)kLog2e);
@@ -31,7 +30,7 @@ struct Rows {
     int64_t rows, per_batch, batch_stride, row_stride;
     int64_t vocab, ignore;
     int32_t n_seq, splits;
-    int64_t split_chunks;  // chunks of 8 logits of a split
+    int64_t split_chunks;  // runs of 16 bytes of a split
 };
 
 __device__ __forceinline__ int64_t row_offset(const Rows& q, int64_t r) {
@@ -50,25 +49,13 @@ __device__ __forceinline__ int seq_of(const Rows& q, int64_t r) {
     return lo < q.n_seq && sload(q.cu + lo) <= r ? lo : -1;
 }
 
-// Eight logits; beyond `left` of them -inf, which adds nothing to any sum.
+// Logits go 16 bytes a lane; past the end of a row -inf, which adds nothing to any sum.
+template <int DT> constexpr int kW = 16 / sizeof(typename Elem<DT>::T);
 template <int DT>
-__device__ __forceinline__ void load_logits(const typename Elem<DT>::T* base, int64_t left, Raw8<DT>& r) {
-    if (left >= 8) {
-        load_raw8_any<DT>(base, r);
-        return;
-    }
-    if constexpr (DT == F32) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r.f[k] = k < left ? *gbl(base + k) : -__builtin_inff();
-    } else {
-        constexpr uint32_t kNegInf = DT == BF16 ? 0xff80u : 0xfc00u;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = 2 * k < left ? (uint32_t)*gbl(base + 2 * k) : kNegInf;
-            const uint32_t hi = 2 * k + 1 < left ? (uint32_t)*gbl(base + 2 * k + 1) : kNegInf;
-            r.w[k] = lo | (hi << 16);
-        }
-    }
+__device__ __forceinline__ Run<typename Elem<DT>::T, kW<DT>> load_logits(const typename Elem<DT>::T* base, int64_t left = kW<DT>) {
+    using T = typename Elem<DT>::T;
+    if constexpr (DT == F32) return load_run<T, kW<DT>>(base, left, -__builtin_inff());
+    else return load_run<T, kW<DT>>(base, left, (T)(DT == BF16 ? 0xff80 : 0xfc00));
 }
 
 // The constant's rounding would lean every sum one way, and a sequence adds up thousands of them: its
@@ -97,18 +84,18 @@ struct Soft {
 };
 
 template <int DT, int N>
-__device__ __forceinline__ void add_chunks(Soft& a, const Raw8<DT> (&r)[N]) {
+__device__ __forceinline__ void add_runs(Soft& a, const Run<typename Elem<DT>::T, kW<DT>> (&r)[N]) {
     float top = -__builtin_inff();
 #pragma unroll
     for (int c = 0; c < N; ++c)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, raw_elem<DT>(r[c], k));
+        for (int k = 0; k < kW<DT>; ++k) top = __builtin_fmaxf(top, to_f32<DT>(r[c].e[k]));
     a.rebase(top);
     const float b = a.base();
 #pragma unroll
     for (int c = 0; c < N; ++c)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) a.s += exp_(raw_elem<DT>(r[c], k) - b);
+        for (int k = 0; k < kW<DT>; ++k) a.s += exp_(to_f32<DT>(r[c].e[k]) - b);
 }
 
 __device__ __forceinline__ void wave_join(Soft& a) {
@@ -129,21 +116,21 @@ __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restri
     const int64_t label = sload(q.labels + r);
     if (label == q.ignore) return;
     const T* x = (const T*)q.x + row_offset(q, r);
-    const int64_t chunks = (q.vocab + 7) / 8;
+    constexpr int W = kW<DT>;
+    const int64_t chunks = (q.vocab + W - 1) / W;
     int64_t c = split * q.split_chunks, end = c + q.split_chunks;
     if (end > chunks) end = chunks;
-    const int64_t whole = end * 8 <= q.vocab ? end : end - 1;
+    const int64_t whole = end * W <= q.vocab ? end : end - 1;
     Soft a;
     for (c += threadIdx.x; c + 3 * kT < whole; c += 4 * kT) {
-        Raw8<DT> v[4];
+        Run<T, W> v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_raw8_any<DT>(x + (c + i * kT) * 8, v[i]);
-        add_chunks<DT, 4>(a, v);
+        for (int i = 0; i < 4; ++i) v[i] = load_logits<DT>(x + (c + i * kT) * W);
+        add_runs<DT, 4>(a, v);
     }
     for (; c < end; c += kT) {
-        Raw8<DT> v[1];
-        load_logits<DT>(x + c * 8, q.vocab - c * 8, v[0]);
-        add_chunks<DT, 1>(a, v);
+        const Run<T, W> v[1] = {load_logits<DT>(x + c * W, q.vocab - c * W)};
+        add_runs<DT, 1>(a, v);
     }
     wave_join(a);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(a.m, a.s);
@@ -362,54 +349,48 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
         if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
     }
     T* out = (T*)grad + r * q.vocab;
-    const int64_t chunks = (q.vocab + 7) / 8;
+    constexpr int W = kW<DT>;
+    const int64_t chunks = (q.vocab + W - 1) / W;
     int64_t c = split * q.split_chunks, end = c + q.split_chunks;
     if (end > chunks) end = chunks;
-    const int64_t whole = end * 8 <= q.vocab ? end : end - 1;
+    const int64_t whole = end * W <= q.vocab ? end : end - 1;
     c += threadIdx.x;
     if (coef == 0.0f) {
-        const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (; c < whole; c += kT) store8_any<DT>(out + c * 8, zeros);
-        if (c < end)
-            for (int64_t v = c * 8; v < q.vocab; ++v) out[v] = from_f32<DT>(0.0f);
+        Run<T, W> zeros;
+#pragma unroll
+        for (int i = 0; i < W; ++i) zeros.e[i] = T(0);
+        for (; c < end; c += kT) store_run<T, W>(out + c * W, q.vocab - c * W, zeros);
         return;
     }
     const T* x = (const T*)q.x + row_offset(q, r);
     const float2 st = make_float2(sload(&stats[r].x), sload(&stats[r].y));
     const float each = -coef / st.y;
-    const auto chunk = [&](const Raw8<DT>& v, int64_t at, float g[8]) {
+    const auto finish = [&](Run<T, W>& v, int64_t at) {
+        float g[W];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = each * exp_(raw_elem<DT>(v, i) - st.x);
+        for (int i = 0; i < W; ++i) g[i] = each * exp_(to_f32<DT>(v.e[i]) - st.x);
         const uint64_t here = (uint64_t)(label - at);
-        if (here < 8) {
+        if (here < W) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] += here == (uint64_t)i ? coef : 0.0f;
+            for (int i = 0; i < W; ++i) g[i] += here == (uint64_t)i ? coef : 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g[i]);
     };
-    for (; c + 3 * kT < whole; c += 4 * kT) {
-        Raw8<DT> v[4];
+    for (; c + kT < whole; c += 2 * kT) {
+        Run<T, W> v[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_raw8_any<DT>(x + (c + i * kT) * 8, v[i]);
+        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + (c + i * kT) * W);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float g[8];
-            chunk(v[i], (c + i * kT) * 8, g);
-            store8_any<DT>(out + (c + i * kT) * 8, g);
+        for (int i = 0; i < 2; ++i) {
+            finish(v[i], (c + i * kT) * W);
+            store_run<T, W>(out + (c + i * kT) * W, W, v[i]);
         }
     }
     for (; c < end; c += kT) {
-        Raw8<DT> v;
-        float g[8];
-        const int64_t left = q.vocab - c * 8;
-        load_logits<DT>(x + c * 8, left, v);
-        chunk(v, c * 8, g);
-        if (left >= 8) {
-            store8_any<DT>(out + c * 8, g);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < left) out[c * 8 + i] = from_f32<DT>(g[i]);
-        }
+        Run<T, W> v = load_logits<DT>(x + c * W, q.vocab - c * W);
+        finish(v, c * W);
+        store_run<T, W>(out + c * W, q.vocab - c * W, v);
     }
 }
 
@@ -419,8 +400,9 @@ int launched(const char* what) {
     return e == hipSuccess ? GEFENX_OK : set_error(GEFENX_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
 }
 
-// Row workgroups: one per row, or enough to fill the chip where the rows are few, each of a pass or more.
-int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q, int64_t most_passes = 0) {
+// Row workgroups: one per row, or enough to fill the chip where the rows are few, each of a pass or
+// more; `most`: the most passes of one, 0: any number.
+int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q, int64_t most = 0) {
     if (!l) return set_error(GEFENX_EINVAL, "%s: null descriptor", what);
     if (l->dtype != GEFENX_F32 && l->dtype != GEFENX_F16 && l->dtype != GEFENX_BF16)
         return set_error(GEFENX_EDTYPE, "%s: unsupported dtype %d", what, l->dtype);
@@ -440,10 +422,11 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     q.vocab = l->vocab;
     q.ignore = l->ignore_index;
     q.n_seq = l->n_seq;
-    const int64_t chunks = (l->vocab + 7) / 8, passes = (l->vocab + kPass - 1) / kPass;
+    const int64_t run = l->dtype == GEFENX_F32 ? 4 : 8;
+    const int64_t chunks = (l->vocab + run - 1) / run, passes = (chunks + kT - 1) / kT;
     int64_t splits = l->rows > 0 ? (kWantedWgs + l->rows - 1) / l->rows : 1;
-    if (most_passes && splits < (passes + most_passes - 1) / most_passes) splits = (passes + most_passes - 1) / most_passes;
-    splits = splits < 1 ? 1 : (splits > passes ? passes : splits);
+    if (most && splits * most < passes) splits = (passes + most - 1) / most;
+    splits = splits > passes ? passes : splits;
     q.split_chunks = (chunks + splits - 1) / splits;
     q.splits = (int32_t)((chunks + q.split_chunks - 1) / q.split_chunks);
     return GEFENX_OK;
@@ -579,8 +562,7 @@ int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const fl
                        const float* scale_dev, double scale, void* grad, void* stream) {
     const char* what = "gefenx_logits_grad";
     Rows q;
-    static int e = getenv("GX_GP") ? atoi(getenv("GX_GP")) : 4;
-    int rc = make_rows(what, logits, weights != nullptr, q, e);
+    int rc = make_rows(what, logits, weights != nullptr, q, kGradPasses);
     if (rc != GEFENX_OK) return rc;
     if (q.rows == 0) return GEFENX_OK;
     if (!stats || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
