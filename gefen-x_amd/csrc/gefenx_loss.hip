@@ -30,7 +30,7 @@ struct Rows {
     int64_t rows, per_batch, batch_stride, row_stride;
     int64_t vocab, ignore;
     int32_t n_seq, splits;
-    int64_t split_chunks;  // runs of 16 bytes of a split
+    int64_t split_runs;    // runs of 16 bytes of a split
 };
 
 __device__ __forceinline__ int64_t row_offset(const Rows& q, int64_t r) {
@@ -57,6 +57,39 @@ __device__ __forceinline__ Run<typename Elem<DT>::T, kW<DT>> load_logits(const t
     if constexpr (DT == F32) return load_run<T, kW<DT>>(base, left, -__builtin_inff());
     else return load_run<T, kW<DT>>(base, left, (T)(DT == BF16 ? 0xff80 : 0xfc00));
 }
+
+// A whole run at an odd multiple of 2 bytes (every other row of an odd vocabulary, in 2-byte types):
+// vectors there read at 2.4 TB/s, so the run is put together from words, each of which holds some of it.
+template <int DT>
+__device__ __forceinline__ Run<typename Elem<DT>::T, kW<DT>> load_odd(const typename Elem<DT>::T* base) {
+    if constexpr (DT == F32) {
+        return load_logits<DT>(base);
+    } else {
+        const auto a = load_run<uint32_t, 4>(reinterpret_cast<const uint32_t*>(base - 1), 4);
+        const uint32_t last = *gbl(reinterpret_cast<const uint32_t*>(base + 7));
+        Run<uint32_t, 4> w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.e[i] = __builtin_amdgcn_alignbit(i < 3 ? a.e[i + 1] : last, a.e[i], 16);
+        Run<typename Elem<DT>::T, kW<DT>> r;
+        __builtin_memcpy(&r, &w, sizeof(r));
+        return r;
+    }
+}
+
+// The runs of a row of the gradient start at multiples of 16 bytes, wherever the row does: run 0 is what
+// lies before the first of them.  pad: elements from the multiple before the row to the row.
+template <int W> struct Runs {
+    int64_t vocab, pad;
+    __device__ __forceinline__ Runs(const void* row, int64_t v, int size) : vocab(v), pad((int64_t)(((uintptr_t)row & 15) / size)) {}
+    __device__ __forceinline__ int64_t count() const { return (vocab + pad + W - 1) / W; }
+    __device__ __forceinline__ int64_t begin(int64_t c) const { return c ? c * W - pad : 0; }
+    __device__ __forceinline__ int64_t left(int64_t c) const {
+        const int64_t all = vocab - begin(c);
+        return c || all < W - pad ? all : W - pad;
+    }
+    // runs before this one, but for run 0 where pad, are whole
+    __device__ __forceinline__ int64_t whole(int64_t end) const { return end * W <= vocab + pad ? end : end - 1; }
+};
 
 // The constant's rounding would lean every sum one way, and a sequence adds up thousands of them: its
 // rest goes into the product too.
@@ -117,17 +150,23 @@ __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restri
     if (label == q.ignore) return;
     const T* x = (const T*)q.x + row_offset(q, r);
     constexpr int W = kW<DT>;
-    const int64_t chunks = (q.vocab + W - 1) / W;
-    int64_t c = split * q.split_chunks, end = c + q.split_chunks;
-    if (end > chunks) end = chunks;
+    const int64_t runs = (q.vocab + W - 1) / W;
+    int64_t c = split * q.split_runs, end = c + q.split_runs;
+    if (end > runs) end = runs;
     const int64_t whole = end * W <= q.vocab ? end : end - 1;
     Soft a;
-    for (c += threadIdx.x; c + 3 * kT < whole; c += 4 * kT) {
-        Run<T, W> v[4];
+    c += threadIdx.x;
+    // which logits a lane adds up, and so the sum, does not depend on where the row starts
+    const auto add = [&](auto load) {
+        for (; c + 3 * kT < whole; c += 4 * kT) {
+            Run<T, W> v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = load_logits<DT>(x + (c + i * kT) * W);
-        add_runs<DT, 4>(a, v);
-    }
+            for (int i = 0; i < 4; ++i) v[i] = load(x + (c + i * kT) * W);
+            add_runs<DT, 4>(a, v);
+        }
+    };
+    if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT>(p); });
+    else add([](const T* p) { return load_logits<DT>(p); });
     for (; c < end; c += kT) {
         const Run<T, W> v[1] = {load_logits<DT>(x + c * W, q.vocab - c * W)};
         add_runs<DT, 1>(a, v);
@@ -350,16 +389,16 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
     }
     T* out = (T*)grad + r * q.vocab;
     constexpr int W = kW<DT>;
-    const int64_t chunks = (q.vocab + W - 1) / W;
-    int64_t c = split * q.split_chunks, end = c + q.split_chunks;
-    if (end > chunks) end = chunks;
-    const int64_t whole = end * W <= q.vocab ? end : end - 1;
+    const Runs<W> runs(out, q.vocab, sizeof(T));
+    int64_t c = split * q.split_runs, end = c + q.split_runs;
+    if (end > runs.count()) end = runs.count();
+    const int64_t whole = runs.whole(end);
     c += threadIdx.x;
     if (coef == 0.0f) {
         Run<T, W> zeros;
 #pragma unroll
         for (int i = 0; i < W; ++i) zeros.e[i] = T(0);
-        for (; c < end; c += kT) store_run<T, W>(out + c * W, q.vocab - c * W, zeros);
+        for (; c < end; c += kT) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
         return;
     }
     const T* x = (const T*)q.x + row_offset(q, r);
@@ -377,21 +416,27 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
 #pragma unroll
         for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g[i]);
     };
+    const auto one = [&](int64_t run) {
+        const int64_t at = runs.begin(run), left = runs.left(run);
+        Run<T, W> v = load_logits<DT>(x + at, left);
+        finish(v, at);
+        store_run<T, W>(out + at, left, v);
+    };
+    if (c == 0) {
+        one(0);
+        c += kT;
+    }
     for (; c + kT < whole; c += 2 * kT) {
         Run<T, W> v[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + (c + i * kT) * W);
+        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * kT));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            finish(v[i], (c + i * kT) * W);
-            store_run<T, W>(out + (c + i * kT) * W, W, v[i]);
+            finish(v[i], runs.begin(c + i * kT));
+            store_run<T, W>(out + runs.begin(c + i * kT), W, v[i]);
         }
     }
-    for (; c < end; c += kT) {
-        Run<T, W> v = load_logits<DT>(x + c * W, q.vocab - c * W);
-        finish(v, c * W);
-        store_run<T, W>(out + c * W, q.vocab - c * W, v);
-    }
+    for (; c < end; c += kT) one(c);
 }
 
 // ------------------------------------------------------------ host side
@@ -423,12 +468,13 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     q.ignore = l->ignore_index;
     q.n_seq = l->n_seq;
     const int64_t run = l->dtype == GEFENX_F32 ? 4 : 8;
-    const int64_t chunks = (l->vocab + run - 1) / run, passes = (chunks + kT - 1) / kT;
+    const int64_t runs = (l->vocab + 2 * run - 2) / run;  // as many as a row can have, wherever it starts
+    const int64_t passes = (runs + kT - 1) / kT;
     int64_t splits = l->rows > 0 ? (kWantedWgs + l->rows - 1) / l->rows : 1;
     if (most && splits * most < passes) splits = (passes + most - 1) / most;
     splits = splits > passes ? passes : splits;
-    q.split_chunks = (chunks + splits - 1) / splits;
-    q.splits = (int32_t)((chunks + q.split_chunks - 1) / q.split_chunks);
+    q.split_runs = (runs + splits - 1) / splits;
+    q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
     return GEFENX_OK;
 }
 
