@@ -236,19 +236,24 @@ __device__ __forceinline__ void store8_any(typename Elem<DT>::T* __restrict__ ba
     }
 }
 
-// W consecutive elements (8 bytes or more) at any alignment of their type, streamed; the end of an
-// array, where fewer than W are left, by elements (reads fill up with `beyond`, nothing is written
-// past it).
+// W consecutive elements (8 bytes or more) at any alignment of their type, streamed (reads: unless
+// told otherwise); the end of an array, where fewer than W are left, by elements (reads fill up with
+// `beyond`, nothing is written past it).
 template <class T, int W> struct Run { T e[W]; };
 
-template <class T, int W>
+template <class T, int W, bool STREAM = true>
 __device__ __forceinline__ Run<T, W> load_run(const T* base, int64_t left, T beyond = T(0)) {
     typedef uint32_t V __attribute__((ext_vector_type(W * sizeof(T) / 4), aligned(sizeof(T))));
     static_assert(W * sizeof(T) >= 8, "vectors of two words and more");
     Run<T, W> r;
     if (left >= W) {
-        const auto v = __builtin_nontemporal_load(GX_GLOBAL_AS(const V, base));
-        __builtin_memcpy(&r, &v, sizeof(r));
+        if constexpr (STREAM) {
+            const auto v = __builtin_nontemporal_load(GX_GLOBAL_AS(const V, base));
+            __builtin_memcpy(&r, &v, sizeof(r));
+        } else {
+            const V v = *GX_GLOBAL_AS(const V, base);
+            __builtin_memcpy(&r, &v, sizeof(r));
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < W; ++k) r.e[k] = k < left ? *gbl(base + k) : beyond;

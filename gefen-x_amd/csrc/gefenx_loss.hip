@@ -19,6 +19,7 @@ namespace {
 constexpr int kT = 256;               // threads of a row workgroup
 constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
 constexpr int64_t kGradPasses = 2;    // passes of a workgroup of the gradient
+constexpr int kRowT = 1024;           // threads of a workgroup that keeps a row to itself
 constexpr int kSeqT = 1024;           // threads of a sequence workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eRest = (float)(1.44269504088896340736 - (double)kLog2e);
@@ -51,21 +52,21 @@ __device__ __forceinline__ int seq_of(const Rows& q, int64_t r) {
 
 // Logits go 16 bytes a lane; past the end of a row -inf, which adds nothing to any sum.
 template <int DT> constexpr int kW = 16 / sizeof(typename Elem<DT>::T);
-template <int DT>
+template <int DT, bool STREAM = true>
 __device__ __forceinline__ Run<typename Elem<DT>::T, kW<DT>> load_logits(const typename Elem<DT>::T* base, int64_t left = kW<DT>) {
     using T = typename Elem<DT>::T;
-    if constexpr (DT == F32) return load_run<T, kW<DT>>(base, left, -__builtin_inff());
-    else return load_run<T, kW<DT>>(base, left, (T)(DT == BF16 ? 0xff80 : 0xfc00));
+    if constexpr (DT == F32) return load_run<T, kW<DT>, STREAM>(base, left, -__builtin_inff());
+    else return load_run<T, kW<DT>, STREAM>(base, left, (T)(DT == BF16 ? 0xff80 : 0xfc00));
 }
 
 // A whole run at an odd multiple of 2 bytes (every other row of an odd vocabulary, in 2-byte types):
 // vectors there read at 2.4 TB/s, so the run is put together from words, each of which holds some of it.
-template <int DT>
+template <int DT, bool STREAM = true>
 __device__ __forceinline__ Run<typename Elem<DT>::T, kW<DT>> load_odd(const typename Elem<DT>::T* base) {
     if constexpr (DT == F32) {
-        return load_logits<DT>(base);
+        return load_logits<DT, STREAM>(base);
     } else {
-        const auto a = load_run<uint32_t, 4>(reinterpret_cast<const uint32_t*>(base - 1), 4);
+        const auto a = load_run<uint32_t, 4, STREAM>(reinterpret_cast<const uint32_t*>(base - 1), 4);
         const uint32_t last = *gbl(reinterpret_cast<const uint32_t*>(base + 7));
         Run<uint32_t, 4> w;
 #pragma unroll
@@ -140,45 +141,56 @@ __device__ __forceinline__ void wave_join(Soft& a) {
 }
 
 // ------------------------------------------------------------ row statistics
+// Runs c .. end - 1 of a row, TH lanes at a time; each lane's part.  Which logits a lane adds up, and so
+// the sum, does not depend on where the row starts in memory.
+template <int DT, int TH, bool STREAM>
+__device__ __forceinline__ Soft row_part(const typename Elem<DT>::T* x, int64_t vocab, int64_t c, int64_t end) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = kW<DT>;
+    const int64_t whole = end * W <= vocab ? end : end - 1;
+    Soft a;
+    c += threadIdx.x;
+    const auto add = [&](auto load) {
+        for (; c + 3 * TH < whole; c += 4 * TH) {
+            Run<T, W> v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = load(x + (c + i * TH) * W);
+            add_runs<DT, 4>(a, v);
+        }
+    };
+    if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT, STREAM>(p); });
+    else add([](const T* p) { return load_logits<DT, STREAM>(p); });
+    for (; c < end; c += TH) {
+        const Run<T, W> v[1] = {load_logits<DT, STREAM>(x + c * W, vocab - c * W)};
+        add_runs<DT, 1>(a, v);
+    }
+    return a;
+}
+
+// The workgroup's Soft, in every lane.
+template <int TH>
+__device__ __forceinline__ Soft group_join(Soft a, float2* waves) {
+    wave_join(a);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(a.m, a.s);
+    __syncthreads();
+    a.m = waves[0].x;
+    a.s = waves[0].y;
+#pragma unroll
+    for (int w = 1; w < TH / 64; ++w) a.join(waves[w].x, waves[w].y);
+    return a;
+}
+
 // part[row][split] = {maximum, sum of exp(x - maximum)} of a split of a row.
 template <int DT>
 __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restrict__ part) {
     using T = typename Elem<DT>::T;
     __shared__ float2 waves[kT / 64];
     const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
-    const int64_t label = sload(q.labels + r);
-    if (label == q.ignore) return;
-    const T* x = (const T*)q.x + row_offset(q, r);
-    constexpr int W = kW<DT>;
-    const int64_t runs = (q.vocab + W - 1) / W;
-    int64_t c = split * q.split_runs, end = c + q.split_runs;
-    if (end > runs) end = runs;
-    const int64_t whole = end * W <= q.vocab ? end : end - 1;
-    Soft a;
-    c += threadIdx.x;
-    // which logits a lane adds up, and so the sum, does not depend on where the row starts
-    const auto add = [&](auto load) {
-        for (; c + 3 * kT < whole; c += 4 * kT) {
-            Run<T, W> v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = load(x + (c + i * kT) * W);
-            add_runs<DT, 4>(a, v);
-        }
-    };
-    if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT>(p); });
-    else add([](const T* p) { return load_logits<DT>(p); });
-    for (; c < end; c += kT) {
-        const Run<T, W> v[1] = {load_logits<DT>(x + c * W, q.vocab - c * W)};
-        add_runs<DT, 1>(a, v);
-    }
-    wave_join(a);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(a.m, a.s);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-        for (int w = 1; w < kT / 64; ++w) a.join(waves[w].x, waves[w].y);
-        part[blockIdx.x] = make_float2(a.m, a.s);
-    }
+    if (sload(q.labels + r) == q.ignore) return;
+    const int64_t runs = (q.vocab + kW<DT> - 1) / kW<DT>, begin = split * q.split_runs;
+    const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
+    const Soft a = group_join<kT>(row_part<DT, kT, true>((const T*)q.x + row_offset(q, r), q.vocab, begin, end), waves);
+    if (threadIdx.x == 0) part[blockIdx.x] = make_float2(a.m, a.s);
 }
 
 // ------------------------------------------------------------ tokens and sequences
@@ -221,6 +233,31 @@ __device__ __forceinline__ double token_logp(const Rows& q, int64_t r, int64_t l
     return ((double)x - (double)a.m) - log((double)a.s);
 }
 
+// A token of the policy loss: its loss, KL estimate, whether the clamped term is the minimum, and
+// d loss / d logp, all but for its sequence's weight.
+struct PolicyToken {
+    float each, kl, k;
+    bool clipped;
+};
+__device__ __forceinline__ PolicyToken policy_token(const Token& t, int64_t r, int64_t seq, float logp) {
+    const float adv = *gbl(t.adv + (t.adv_per_row ? r : seq));
+    const float ratio = expf(logp - *gbl(t.old + r));
+    const float bound = __builtin_fminf(__builtin_fmaxf(ratio, t.lo), t.hi);
+    const float plain = ratio * adv, clip = bound * adv;
+    PolicyToken p;
+    p.clipped = clip < plain;
+    p.each = p.clipped ? -clip : -plain;
+    p.k = p.clipped ? 0.0f : -plain;
+    p.kl = 0.0f;
+    if (t.ref) {
+        const float d = *gbl(t.ref + r) - logp, e = expm1f(d);
+        p.kl = e - d;
+        p.each += t.kl_coef * p.kl;
+        p.k -= t.kl_coef * e;
+    }
+    return p;
+}
+
 // One workgroup per sequence (kLogps: per kSeqT / lanes rows), a group of lanes per row.
 template <int DT, int MODE>
 __global__ __launch_bounds__(kSeqT) void k_tokens(const Rows q, const Token t, const float2* __restrict__ part, int lanes,
@@ -260,22 +297,11 @@ __global__ __launch_bounds__(kSeqT) void k_tokens(const Rows q, const Token t, c
                 own.n += 1.0;
             }
             if (MODE == kPolicy && lane == 0) {
-                const float adv = *gbl(t.adv + (t.adv_per_row ? r : (int64_t)blockIdx.x));
-                const float ratio = expf(logp - *gbl(t.old + r));
-                const float bound = __builtin_fminf(__builtin_fmaxf(ratio, t.lo), t.hi);
-                const float plain = ratio * adv, clip = bound * adv;
-                const bool clipped = clip < plain;
-                float each = clipped ? -clip : -plain;
-                k = clipped ? 0.0f : -plain;
-                if (t.ref) {
-                    const float d = *gbl(t.ref + r) - logp;
-                    const float e = expm1f(d);
-                    each += t.kl_coef * (e - d);
-                    k -= t.kl_coef * e;
-                    own.kl += (double)(e - d);
-                }
-                own.a += (double)each;
-                own.clipped += clipped ? 1.0 : 0.0;
+                const PolicyToken p = policy_token(t, r, blockIdx.x, logp);
+                k = p.k;
+                own.a += (double)p.each;
+                own.kl += (double)p.kl;
+                own.clipped += p.clipped ? 1.0 : 0.0;
                 own.n += 1.0;
             }
         }
@@ -311,6 +337,19 @@ __device__ __forceinline__ double block_sum(double v, double* waves) {
     double total = 0.0;
     for (int w = 0; w < kT / 64; ++w) total += waves[w];
     return total;
+}
+
+// The labelled rows of each sequence, and nothing else, in sums.
+__global__ __launch_bounds__(kT) void k_counts(const Rows q, SeqSums* __restrict__ sums) {
+    __shared__ double waves[kT / 64];
+    int64_t begin = q.cu ? (int64_t)sload(q.cu + blockIdx.x) : (int64_t)blockIdx.x * q.per_batch;
+    int64_t end = q.cu ? (int64_t)sload(q.cu + blockIdx.x + 1) : begin + q.per_batch;
+    begin = begin < 0 ? 0 : begin;
+    end = end > q.rows ? q.rows : end;
+    double n = 0.0;
+    for (int64_t r = begin + threadIdx.x; r < end; r += kT) n += *gbl(q.labels + r) != q.ignore ? 1.0 : 0.0;
+    n = block_sum(n, waves);
+    if (threadIdx.x == 0) sums[blockIdx.x] = SeqSums{0.0, 0.0, 0.0, n};
 }
 
 // Rewards of either side, and weights per sequence, the chosen ones first.
@@ -369,16 +408,35 @@ __global__ __launch_bounds__(kT) void k_policy(const SeqSums* __restrict__ sums,
 }
 
 // ------------------------------------------------------------ gradient
-// grad[r][v] = k_r ([v = y_r] - exp(x - max) / sum); k_r = k[r] * weights[sequence] * scale.
+// coef ([v = label] - exp(x - max) / sum) of a run whose first logit is number `at`, in place.
+template <int DT>
+__device__ __forceinline__ void grad_run(Run<typename Elem<DT>::T, kW<DT>>& v, int64_t at, int64_t label, float coef, float each,
+                                         float max) {
+    constexpr int W = kW<DT>;
+    float g[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) g[i] = each * exp_(to_f32<DT>(v.e[i]) - max);
+    const uint64_t here = (uint64_t)(label - at);
+    if (here < W) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) g[i] += here == (uint64_t)i ? coef : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g[i]);
+}
+
+// grad[r][v] = c_r ([v = y_r] - exp(x - max) / sum), c_r = k[r] * weights[sequence] * scale.
+// unlabelled: only the rows without a label, which get zeros.
 template <int DT>
 __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* __restrict__ stats, const float* __restrict__ k,
                                                     const float* __restrict__ weights, const float* __restrict__ scale_dev,
-                                                    float scale, void* __restrict__ grad) {
+                                                    float scale, int unlabelled, void* __restrict__ grad) {
     using T = typename Elem<DT>::T;
     const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
     const int64_t label = sload(q.labels + r);
     float coef = 0.0f;
     if (label != q.ignore) {
+        if (unlabelled) return;
         coef = scale_dev ? sload(scale_dev) * scale : scale;
         if (k) coef *= sload(k + r);
         if (weights) {
@@ -402,24 +460,11 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
         return;
     }
     const T* x = (const T*)q.x + row_offset(q, r);
-    const float2 st = make_float2(sload(&stats[r].x), sload(&stats[r].y));
-    const float each = -coef / st.y;
-    const auto finish = [&](Run<T, W>& v, int64_t at) {
-        float g[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) g[i] = each * exp_(to_f32<DT>(v.e[i]) - st.x);
-        const uint64_t here = (uint64_t)(label - at);
-        if (here < W) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) g[i] += here == (uint64_t)i ? coef : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g[i]);
-    };
+    const float max = sload(&stats[r].x), each = -coef / sload(&stats[r].y);
     const auto one = [&](int64_t run) {
         const int64_t at = runs.begin(run), left = runs.left(run);
         Run<T, W> v = load_logits<DT>(x + at, left);
-        finish(v, at);
+        grad_run<DT>(v, at, label, coef, each, max);
         store_run<T, W>(out + at, left, v);
     };
     if (c == 0) {
@@ -432,11 +477,54 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
         for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * kT));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            finish(v[i], runs.begin(c + i * kT));
+            grad_run<DT>(v[i], runs.begin(c + i * kT), label, coef, each, max);
             store_run<T, W>(out + runs.begin(c + i * kT), W, v[i]);
         }
     }
     for (; c < end; c += kT) one(c);
+}
+
+// Statistics and gradient of a labelled row in one go, where the coefficient needs no other row: two
+// workgroups a CU hold 512 rows (155 MB of 151936 bf16 logits), which the 256 MB cache still has when
+// they are read again, last part first.  part[row] gets the statistics.
+template <int DT>
+__global__ __launch_bounds__(kRowT) void k_policy_rows(const Rows q, const Token t, const float* __restrict__ weights,
+                                                       const float* __restrict__ scale_dev, float scale,
+                                                       float2* __restrict__ part, void* __restrict__ grad) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = kW<DT>;
+    __shared__ float2 waves[kRowT / 64];
+    __shared__ float coef_of;
+    const int64_t r = blockIdx.x, label = sload(q.labels + r);
+    if (label == q.ignore) return;
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const Soft a = group_join<kRowT>(row_part<DT, kRowT, false>(x, q.vocab, 0, (q.vocab + W - 1) / W), waves);
+    if (threadIdx.x == 0) {
+        part[r] = make_float2(a.m, a.s);
+        const int s = seq_of(q, r);
+        float coef = 0.0f;
+        if (s >= 0) coef = (scale_dev ? sload(scale_dev) * scale : scale) * policy_token(t, r, s, (float)token_logp<DT>(q, r, label, a)).k * sload(weights + s);
+        if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+        coef_of = coef;
+    }
+    __syncthreads();
+    const float coef = coef_of, each = -coef / a.s;
+    T* out = (T*)grad + r * q.vocab;
+    const Runs<W> runs(out, q.vocab, sizeof(T));
+    const int64_t n = runs.count();
+    for (int64_t c = (n - 1) / kRowT * kRowT + threadIdx.x; c >= 0; c -= kRowT) {
+        if (c >= n) continue;
+        const int64_t at = runs.begin(c), left = runs.left(c);
+        Run<T, W> v;
+        if (coef == 0.0f) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v.e[i] = T(0);
+        } else {
+            v = load_logits<DT>(x + at, left);
+            grad_run<DT>(v, at, label, coef, each, a.m);
+        }
+        store_run<T, W>(out + at, left, v);
+    }
 }
 
 // ------------------------------------------------------------ host side
@@ -512,10 +600,86 @@ int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const
     });
 }
 
+// Whether the policy gradient goes row by row.  It reads long rows once instead of twice (1 GiB of bf16
+// logits, a quarter of the rows masked: rows of 128256 416 against 486 us, of 65536 401 against 462, of
+// 32768 434 against 445); short ones leave most of its 1024 lanes idle (16384 587 against 469, 8192 851
+// against 530).  Logits that the 256 MB cache holds are read from there the second time anyway, and few
+// rows are split instead.
+bool rows_alone(const gefenx_logits& l) {
+    const int64_t bytes = l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2);
+    return bytes >= (64 << 10) && l.rows >= 1024 && l.rows * bytes > (int64_t)256 << 20;
+}
+
 int need(const char* what, const Rows& q, const void* ws, size_t bytes) {
     if (!ws || bytes < ws_bytes(q))
         return set_error(GEFENX_EINVAL, "%s: workspace of %zu bytes, %zu needed", what, bytes, ws_bytes(q));
     return GEFENX_OK;
+}
+
+int run_grad(const char* what, const gefenx_logits& l, const float* stats, const float* k, const float* weights,
+             const float* scale_dev, double scale, int unlabelled, void* grad, hipStream_t s) {
+    Rows q;
+    const int rc = make_rows(what, &l, false, q, kGradPasses);
+    if (rc != GEFENX_OK) return rc;
+    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
+    return by_dtype(l.dtype, [&](auto dt) {
+        k_logits_grad<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(
+            q, reinterpret_cast<const float2*>(stats), k, weights, scale_dev, (float)scale, unlabelled, grad);
+        return launched(what);
+    });
+}
+
+// A checked call of the policy loss.
+struct Policy {
+    const char* what;
+    Rows q;
+    Token t;
+    int dtype, by_sequence;
+    float *loss, *kl, *clip_fraction, *weights;
+    float2* part;
+    SeqSums* sums;
+    hipStream_t s;
+};
+
+int make_policy(const char* what, const gefenx_logits* logits, const float* old_logps, const float* advantages,
+                int advantages_per_row, const float* ref_logps, double clip_low, double clip_high, double kl_coef,
+                int by_sequence, float* loss, float* kl, float* clip_fraction, float* logps, float* stats, float* k,
+                float* weights, void* workspace, size_t workspace_bytes, void* stream, Policy& p) {
+    p.what = what;
+    int rc = make_rows(what, logits, true, p.q);
+    if (rc == GEFENX_OK) rc = need(what, p.q, workspace, workspace_bytes);
+    if (rc != GEFENX_OK) return rc;
+    if (!loss || !kl || !clip_fraction || !weights || !advantages || (p.q.rows > 0 && (!logps || !stats || !k || !old_logps)))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    p.dtype = logits->dtype;
+    p.by_sequence = by_sequence;
+    p.loss = loss;
+    p.kl = kl;
+    p.clip_fraction = clip_fraction;
+    p.weights = weights;
+    p.part = static_cast<float2*>(workspace);
+    p.sums = reinterpret_cast<SeqSums*>(static_cast<char*>(workspace) + part_bytes(p.q));
+    p.s = static_cast<hipStream_t>(stream);
+    p.t = Token{};
+    p.t.ref = ref_logps;
+    p.t.old = old_logps;
+    p.t.adv = advantages;
+    p.t.adv_per_row = advantages_per_row;
+    p.t.logps = logps;
+    p.t.stats = reinterpret_cast<float2*>(stats);
+    p.t.k = k;
+    p.t.lo = (float)(1.0 - clip_low);
+    p.t.hi = (float)(1.0 + clip_high);
+    p.t.kl_coef = (float)kl_coef;
+    return GEFENX_OK;
+}
+
+// From the rows' statistics to the loss.
+int policy_totals(const Policy& p) {
+    const int rc = run_tokens<kPolicy>(p.what, p.q, p.dtype, p.t, p.part, p.sums, p.s);
+    if (rc != GEFENX_OK) return rc;
+    k_policy<<<1, kT, 0, p.s>>>(p.sums, p.q.n_seq, p.by_sequence, p.loss, p.kl, p.clip_fraction, p.weights);
+    return launched(p.what);
 }
 
 }  // namespace
@@ -576,49 +740,53 @@ int gefenx_policy_loss(const gefenx_logits* logits, const float* old_logps, cons
                        const float* ref_logps, double clip_low, double clip_high, double kl_coef, int by_sequence,
                        float* loss, float* kl, float* clip_fraction, float* logps, float* stats, float* k, float* weights,
                        void* workspace, size_t workspace_bytes, void* stream) {
-    const char* what = "gefenx_policy_loss";
-    Rows q;
-    int rc = make_rows(what, logits, true, q);
-    if (rc == GEFENX_OK) rc = need(what, q, workspace, workspace_bytes);
+    Policy p;
+    int rc = make_policy("gefenx_policy_loss", logits, old_logps, advantages, advantages_per_row, ref_logps, clip_low, clip_high,
+                         kl_coef, by_sequence, loss, kl, clip_fraction, logps, stats, k, weights, workspace, workspace_bytes,
+                         stream, p);
+    if (rc == GEFENX_OK) rc = run_stats(p.what, p.q, p.dtype, p.part, p.s);
+    return rc == GEFENX_OK ? policy_totals(p) : rc;
+}
+
+int gefenx_policy_loss_grad(const gefenx_logits* logits, const float* old_logps, const float* advantages, int advantages_per_row,
+                            const float* ref_logps, double clip_low, double clip_high, double kl_coef, int by_sequence,
+                            float* loss, float* kl, float* clip_fraction, float* logps, float* stats, float* k, float* weights,
+                            const float* scale_dev, double scale, void* grad, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    Policy p;
+    int rc = make_policy("gefenx_policy_loss_grad", logits, old_logps, advantages, advantages_per_row, ref_logps, clip_low,
+                         clip_high, kl_coef, by_sequence, loss, kl, clip_fraction, logps, stats, k, weights, workspace,
+                         workspace_bytes, stream, p);
     if (rc != GEFENX_OK) return rc;
-    if (!loss || !kl || !clip_fraction || !weights || !advantages || (q.rows > 0 && (!logps || !stats || !k || !old_logps)))
-        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    float2* part = static_cast<float2*>(workspace);
-    SeqSums* sums = reinterpret_cast<SeqSums*>(static_cast<char*>(workspace) + part_bytes(q));
-    Token t = {};
-    t.ref = ref_logps;
-    t.old = old_logps;
-    t.adv = advantages;
-    t.adv_per_row = advantages_per_row;
-    t.logps = logps;
-    t.stats = reinterpret_cast<float2*>(stats);
-    t.k = k;
-    t.lo = (float)(1.0 - clip_low);
-    t.hi = (float)(1.0 + clip_high);
-    t.kl_coef = (float)kl_coef;
-    rc = run_stats(what, q, logits->dtype, part, s);
-    if (rc == GEFENX_OK) rc = run_tokens<kPolicy>(what, q, logits->dtype, t, part, sums, s);
+    if (p.q.rows > 0 && !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", p.what);
+    if (!rows_alone(*logits)) {
+        rc = run_stats(p.what, p.q, p.dtype, p.part, p.s);
+        if (rc == GEFENX_OK) rc = policy_totals(p);
+        return rc == GEFENX_OK ? gefenx_logits_grad(logits, stats, k, weights, scale_dev, scale, grad, stream) : rc;
+    }
+    // the sequences' weights come from the labels alone
+    k_counts<<<(uint32_t)p.q.n_seq, kT, 0, p.s>>>(p.q, p.sums);
+    k_policy<<<1, kT, 0, p.s>>>(p.sums, p.q.n_seq, by_sequence, loss, kl, clip_fraction, weights);
+    rc = launched(p.what);
+    if (rc == GEFENX_OK) rc = run_grad(p.what, *logits, nullptr, nullptr, nullptr, nullptr, 0.0, 1, grad, p.s);
     if (rc != GEFENX_OK) return rc;
-    k_policy<<<1, kT, 0, s>>>(sums, q.n_seq, by_sequence, loss, kl, clip_fraction, weights);
-    return launched(what);
+    p.q.splits = 1;
+    rc = by_dtype(p.dtype, [&](auto dt) {
+        k_policy_rows<decltype(dt)::value><<<(uint32_t)p.q.rows, kRowT, 0, p.s>>>(p.q, p.t, weights, scale_dev, (float)scale, p.part,
+                                                                                  grad);
+        return launched(p.what);
+    });
+    return rc == GEFENX_OK ? policy_totals(p) : rc;
 }
 
 int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const float* k, const float* weights,
                        const float* scale_dev, double scale, void* grad, void* stream) {
     const char* what = "gefenx_logits_grad";
     Rows q;
-    int rc = make_rows(what, logits, weights != nullptr, q, kGradPasses);
-    if (rc != GEFENX_OK) return rc;
-    if (q.rows == 0) return GEFENX_OK;
+    const int rc = make_rows(what, logits, weights != nullptr, q);
+    if (rc != GEFENX_OK || q.rows == 0) return rc;
     if (!stats || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
-    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    return by_dtype(logits->dtype, [&](auto dt) {
-        k_logits_grad<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(
-            q, reinterpret_cast<const float2*>(stats), k, weights, scale_dev, (float)scale, grad);
-        return launched(what);
-    });
+    return run_grad(what, *logits, stats, k, weights, scale_dev, scale, 0, grad, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

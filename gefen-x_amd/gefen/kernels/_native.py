@@ -173,6 +173,8 @@ SIGNATURES = {
     "gefenx_token_logps": (_I, [_P, _P, _P, _P, _SZ, _P]),
     "gefenx_preference_loss": (_I, [_P, _P, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "gefenx_policy_loss": (_I, [_P, _P, _P, _I, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gefenx_policy_loss_grad": (_I, [_P, _P, _P, _I, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _P, _D, _P, _P, _SZ,
+                                     _P]),
     "gefenx_logits_grad": (_I, [_P, _P, _P, _P, _P, _D, _P, _P]),
     "gefenx_profile_enable": (_I, [_I]),
     "gefenx_profile_read": (_I, [_I, _P, _P, _P, _P]),

@@ -117,16 +117,20 @@ class _Call:
         n = int(_native.load().gefenx_loss_workspace_bytes(self.ref))
         return torch.empty(max(n, 16), dtype=torch.uint8, device=self.device), n
 
+    def scale(self, scale):
+        """A gradient's scale as (device tensor or None, number)."""
+        if not isinstance(scale, torch.Tensor):
+            return None, float(scale)
+        if scale.numel() != 1 or scale.device != self.device:
+            raise ValueError("grad_scale must be a number or one value on {}".format(self.device))
+        return scale.detach().to(torch.float32), 1.0
+
+    def empty_grad(self):
+        return torch.empty(self.shape, dtype=self.logits.dtype, device=self.device)
+
     def grad(self, stats, k, weights, scale):
         """The gradient of the logits, contiguous in their shape."""
-        out = torch.empty(self.shape, dtype=self.logits.dtype, device=self.device)
-        factor, scale_dev = 1.0, None
-        if isinstance(scale, torch.Tensor):
-            if scale.numel() != 1 or scale.device != self.device:
-                raise ValueError("grad_scale must be a number or one value on {}".format(self.device))
-            scale_dev = scale.detach().to(torch.float32)
-        else:
-            factor = float(scale)
+        (scale_dev, factor), out = self.scale(scale), self.empty_grad()
         with _on_device(self.device):
             _native.check(_native.load().gefenx_logits_grad(
                 self.ref, _ptr(stats), _ptr(k), _ptr(weights), _ptr(scale_dev), factor, _ptr(out), self.stream),
@@ -180,7 +184,8 @@ def _preference_forward(call, ref_logps, beta, smoothing, average):
     return PreferenceLoss(loss, chosen, rejected, logps), stats, weights
 
 
-def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction):
+def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction, grad_scale=None):
+    """The loss and what its gradient needs; with a grad_scale the gradient too."""
     old, ref = call.per_token(old_logps, "old_logps"), call.per_token(ref_logps, "ref_logps")
     if old is None:
         raise ValueError("policy_loss needs old_logps")
@@ -201,13 +206,17 @@ def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high,
             raise ValueError("policy_loss needs advantages")
     loss, kl, clipped, weights = call.empty(), call.empty(), call.empty(), call.empty(call.n_seq)
     logps, stats, k = call.empty(*call.labels.shape), call.empty(call.rows, 2), call.empty(call.rows)
+    args = [call.ref, _ptr(old), _ptr(adv), per_row, _ptr(ref), clip_low, clip_high, kl_coef, 1 if reduction == "sequence" else 0,
+            _ptr(loss), _ptr(kl), _ptr(clipped), _ptr(logps), _ptr(stats), _ptr(k), _ptr(weights)]
+    entry, grad = _native.load().gefenx_policy_loss, None
+    if grad_scale is not None:
+        (scale_dev, factor), grad = call.scale(grad_scale), call.empty_grad()
+        entry = _native.load().gefenx_policy_loss_grad
+        args += [_ptr(scale_dev), factor, _ptr(grad)]
     ws, n = call.workspace()
     with _on_device(call.device):
-        _native.check(_native.load().gefenx_policy_loss(
-            call.ref, _ptr(old), _ptr(adv), per_row, _ptr(ref), clip_low, clip_high, kl_coef,
-            1 if reduction == "sequence" else 0, _ptr(loss), _ptr(kl), _ptr(clipped), _ptr(logps), _ptr(stats), _ptr(k),
-            _ptr(weights), _ptr(ws), n, call.stream), "policy_loss")
-    return PolicyLoss(loss, kl, clipped, logps), stats, k, weights
+        _native.check(entry(*args, _ptr(ws), n, call.stream), "policy_loss")
+    return PolicyLoss(loss, kl, clipped, logps), stats, k, weights, grad
 
 
 # ------------------------------------------------------------ autograd
@@ -290,13 +299,16 @@ def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seq
     reduction: "token", the mean over all labelled tokens, or "sequence", the mean over the sequences that have
     any of their mean; 0 without any.  advantages: one per token, or one per sequence [N]."""
     def forward_of(call):
-        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)
+        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)[:4]
     return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of))
 
 
 def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2,
                          clip_high=0.2, kl_coef=0.0, reduction="token", ignore_index=-100, grad_scale=1.0):
     """(policy_loss(...), gradient of the loss times grad_scale in the logits)."""
+    if grad_scale is None:
+        raise ValueError("grad_scale must be a number or one value on the logits' device")
     call = _Call(logits, labels, ignore_index, cu_seqlens)
-    out, stats, k, weights = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)
-    return out, call.grad(stats, k, weights, grad_scale)
+    out, _, _, _, grad = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction,
+                                         grad_scale)
+    return out, grad

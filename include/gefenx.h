@@ -605,6 +605,15 @@ int gefenx_policy_loss(const gefenx_logits* logits, const float* old_logps, cons
                        float* logps, float* stats, float* k, float* weights, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* gefenx_policy_loss and gefenx_logits_grad in one call: long and many rows are
+ * read once for both.  logps, stats, k, weights are written as there. */
+int gefenx_policy_loss_grad(const gefenx_logits* logits, const float* old_logps, const float* advantages,
+                            int advantages_per_row, const float* ref_logps, double clip_low,
+                            double clip_high, double kl_coef, int by_sequence, float* loss, float* kl,
+                            float* clip_fraction, float* logps, float* stats, float* k, float* weights,
+                            const float* scale_dev, double scale, void* grad, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* grad[r][v] = c_r ([v == label] - softmax(x_r)[v]) in the logits' dtype, [rows,
  * vocab] contiguous, with c_r = k[r] (NULL: 1) * weights[sequence of r] (NULL: 1)
  * * *scale_dev (NULL: 1) * scale, rounded once. */

@@ -481,6 +481,70 @@ def test_positions_past_2_31_elements(dev):
     assert not g[1:-3].any()
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 65541), (torch.float16, 70000), (torch.float32, 33333)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_long_rows_beyond_the_cache(dev, dtype, V, packed):
+    """More than 256 MB of logits in rows of 64 KB and more take statistics and gradient of a row together: against
+    the two passes of the autograd form, and a few rows against 64 bits; masked rows, rows outside, odd starts."""
+    n, S = 8, 310
+    T = n * S
+    gen = torch.Generator(dev).manual_seed(3)
+    wide = (torch.randn(T, V + 3, generator=gen, device=dev) * 2).to(dtype)
+    x = wide[:, 2:V + 2]  # rows start anywhere
+    y = torch.randint(0, V, (T,), generator=gen, device=dev)
+    y[torch.rand(T, generator=gen, device=dev) < 0.3] = IGNORE
+    y[5] = V - 1
+    y[6] = 0
+    old = torch.randn(T, generator=gen, device=dev) * 0.3 - 13
+    ref = torch.randn(T, generator=gen, device=dev) * 0.3 - 13
+    cu, lead = None, (n, S)
+    if packed:
+        cu, lead = torch.tensor([3, 500, 500, 1200, 1201, T - 7], dtype=torch.int32, device=dev), (T,)
+    adv = torch.randn(n if not packed else 5, generator=gen, device=dev)
+    kw = dict(cu_seqlens=cu, kl_coef=0.05, reduction="sequence")
+    args = (y.view(lead), old.view(lead), adv, ref.view(lead))
+    out, g = gefen.policy_loss_and_grad(x.view(*lead, V) if packed else x.unflatten(0, lead), *args, grad_scale=4096.0, **kw)
+    leaf = x.contiguous().view(*lead, V).requires_grad_(True)
+    two = gefen.policy_loss(leaf, *args, **kw)
+    (two.loss * 4096.0).backward()
+    x64 = x[:64].double().cpu()
+    tol = logp_tolerance(x64, y[:64].cpu()).max().item()  # per row; about the same in all
+    assert (out.logps - two.logps).abs().max().item() <= 2 * tol
+    for a, b in ((out.loss, two.loss), (out.kl, two.kl)):
+        assert abs(a.item() - b.item()) <= 1e-5 * (1 + abs(b.item()))
+    assert abs(out.clip_fraction.item() - two.clip_fraction.item()) <= 2.0 / T
+    off = (y.view(lead) == IGNORE).view(T)
+    if packed:
+        off[:3] = off[-7:] = True
+    g, h = g.view(T, V), leaf.grad.view(T, V)
+    assert not g[off].any() and not h[off].any()
+    # ratios grow with the errors of logp: relative 4 tol, and one rounding of either; a token at the clip's edge may part
+    near = (g.float() - h.float()).abs() <= (4 * tol + 2.02 * UNIT[dtype]) * h.float().abs() + 2 * LEAST[dtype]
+    assert (~near.all(1)).sum().item() <= 1
+    again, g2 = gefen.policy_loss_and_grad(x.view(*lead, V) if packed else x.unflatten(0, lead), *args, grad_scale=4096.0, **kw)
+    assert torch.equal(out.loss, again.loss) and torch.equal(g, g2.view(T, V))
+    keep = (~off[:64]).nonzero().view(-1)[:8].cpu()
+    lp = logps64(x64, y[:64].cpu())[keep]
+    assert torch.all((out.logps.view(T)[keep].cpu().double() - lp).abs() <= tol)
+
+
+def test_long_rows_of_bad_values(dev):
+    V = 66000
+    x = torch.randn(2100, V, device=dev).bfloat16()
+    y = torch.randint(0, V, (2100,), device=dev)
+    y[7], y[8], y[9] = V, -1, IGNORE
+    x[9] = float("nan")
+    x[10, 5] = float("nan")
+    x[11, :60000] = -float("inf")
+    y[11] = 65000
+    old = torch.full((2100,), -11.0, device=dev)
+    cu = torch.tensor([0, 2100], dtype=torch.int32, device=dev)
+    out, g = gefen.policy_loss_and_grad(x, y, old, torch.ones(2100, device=dev), cu_seqlens=cu, clip_high=1e9)
+    bad = torch.isnan(g).all(1)
+    assert bad.nonzero().view(-1).tolist() == [7, 8, 10] and torch.isnan(out.loss)
+    assert not torch.isnan(g[~bad]).any() and not g[9].any() and not g[11, :60000].any() and g[11, 65000] != 0
+
+
 def test_refusals(dev):
     x, y = torch.zeros(4, 6, 50, device=dev), torch.zeros(4, 6, dtype=torch.long, device=dev)
     z = torch.zeros(4, 6, device=dev)
