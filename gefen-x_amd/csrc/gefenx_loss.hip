@@ -649,7 +649,7 @@ int make_policy(const char* what, const gefenx_logits* logits, const float* old_
     int rc = make_rows(what, logits, true, p.q);
     if (rc == GEFENX_OK) rc = need(what, p.q, workspace, workspace_bytes);
     if (rc != GEFENX_OK) return rc;
-    if (!loss || !kl || !clip_fraction || !weights || !advantages || (p.q.rows > 0 && (!logps || !stats || !k || !old_logps)))
+    if (!loss || !kl || !clip_fraction || !weights || (p.q.rows > 0 && (!logps || !stats || !k || !old_logps || !advantages)))
         return set_error(GEFENX_EINVAL, "%s: null pointer", what);
     p.dtype = logits->dtype;
     p.by_sequence = by_sequence;

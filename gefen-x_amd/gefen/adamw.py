@@ -21,13 +21,13 @@ import torch
 
 from gefen.gefen import _amp_gate, _amp_native_scaling_required, _on_device
 from gefen.kernels import _native
-from gefen.kernels.automatic_gefen_fused import _dtype_code
 
 BLOCK = 256  # elements per scale of the 8-bit moments
 
 _DESC_STRUCT = struct.Struct("<6QqQ8f2i")
 assert _DESC_STRUCT.size == ctypes.sizeof(_native.AdamWDesc)
-_DTYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))
+_DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.bfloat16: _native.DT_BF16}
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
 _U64 = (1 << 64) - 1
 _GOLDEN = 0x9E3779B97F4A7C15
 # state keys and dtypes by width
@@ -44,6 +44,11 @@ def _mix(z: int) -> int:
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9 & _U64
     z = (z ^ (z >> 27)) * 0x94D049BB133111EB & _U64
     return z ^ (z >> 31)
+
+
+def _pack(rows) -> bytes:
+    """The descriptors of gefenx_adamw_* calls."""
+    return b"".join([_DESC_STRUCT.pack(*row) for row in rows])
 
 
 def _order(t: torch.Tensor):
@@ -124,72 +129,86 @@ class AdamW(torch.optim.Optimizer):
 
     # --------------------------------------------------------------- step
 
-    def _validate_grads(self):
-        """Refuse what cannot be stepped before anything moves."""
-        devices = set()
+    @staticmethod
+    def _refuse_grad(p, g):
+        """What is wrong with a gradient that is not plainly the parameter's."""
+        if g.layout is not torch.strided:
+            raise RuntimeError("AdamW does not support sparse gradients")
+        if hasattr(p, "placements") or hasattr(g, "placements"):
+            raise RuntimeError("AdamW does not step DTensor parameters")
+        if not p.is_cuda or g.device != p.device:
+            raise RuntimeError("AdamW steps HIP device parameters with gradients on the same device: parameter "
+                               "on {}, gradient on {}".format(p.device, g.device))
+        if g.shape != p.shape:
+            raise RuntimeError("gradient shape {} does not match parameter shape {}".format(tuple(g.shape), tuple(p.shape)))
+        if p.dtype not in _DTYPES:
+            raise NotImplementedError("AdamW is not implemented for {}".format(p.dtype))
+        if g.dtype is not p.dtype:
+            raise RuntimeError("gradient dtype {} does not match parameter dtype {}".format(g.dtype, p.dtype))
+
+    def _checked(self):
+        """[(group, [(index, parameter, gradient, state), ...]), ...] of what there is to step; refuses what cannot
+        be stepped before anything moves."""
+        found, devices, index, known = [], set(), 0, self.state
         for group in self.param_groups:
+            bits, members = group["state_bits"], []
             for p in group["params"]:
+                index += 1
                 g = p.grad
                 if g is None:
                     continue
-                if g.layout is not torch.strided:
-                    raise RuntimeError("AdamW does not support sparse gradients")
-                if hasattr(p, "placements") or hasattr(g, "placements"):
-                    raise RuntimeError("AdamW does not step DTensor parameters")
-                if p.device.type != "cuda" or g.device != p.device:
-                    raise RuntimeError("AdamW steps HIP device parameters with gradients on the same device: parameter "
-                                       "on {}, gradient on {}".format(p.device, g.device))
-                if g.shape != p.shape:
-                    raise RuntimeError("gradient shape {} does not match parameter shape {}".format(
-                        tuple(g.shape), tuple(p.shape)))
-                if p.dtype not in _DTYPES:
-                    raise NotImplementedError("AdamW is not implemented for {}".format(p.dtype))
-                if g.dtype is not p.dtype:
-                    raise RuntimeError("gradient dtype {} does not match parameter dtype {}".format(g.dtype, p.dtype))
+                dtype = p.dtype
+                if not (type(g) is torch.Tensor and type(p) in _PLAIN and g.dtype is dtype and dtype in _DTYPES
+                        and p.is_cuda and g.is_cuda and g.layout is torch.strided and g.shape == p.shape
+                        and g.get_device() == p.get_device()):
+                    self._refuse_grad(p, g)
                 if not p.is_contiguous():
                     _order(p)
-                if self.state.get(p):
-                    self._check_state(p, self.state[p], group["state_bits"])
-                devices.add(p.device)
+                state = known.get(p)
+                if state:
+                    self._check_state(p, state, bits)
+                devices.add(p.get_device())
+                members.append((index, p, g, state))
+            if members:
+                found.append((group, members))
         if self.max_grad_norm is not None and len(devices) > 1:
-            raise RuntimeError("AdamW with max_grad_norm steps parameters of one device, got {}".format(
-                sorted(str(d) for d in devices)))
+            raise RuntimeError("AdamW with max_grad_norm steps parameters of one device, got devices {}".format(sorted(devices)))
+        return found
 
     @staticmethod
     def _check_state(p, state, bits):
-        blocks = -(-p.numel() // BLOCK)
+        n, device, contiguous = p.numel(), p.get_device(), p.is_contiguous()
         for key, dtype in _STATE[bits].items():
             t = state.get(key)
-            if not torch.is_tensor(t) or t.dtype is not dtype:
+            if type(t) is not torch.Tensor or t.dtype is not dtype:
                 raise ValueError("AdamW with state_bits={} needs {} as {}, got {}".format(
-                    bits, key, dtype, t.dtype if torch.is_tensor(t) else type(t).__name__))
+                    bits, key, dtype, t.dtype if isinstance(t, torch.Tensor) else type(t).__name__))
             if bits == 32:
                 fits = t.shape == p.shape
             else:
-                fits = t.numel() == (blocks if key.endswith("scale") else p.numel()) and t.is_contiguous()
-            if not fits or t.device != p.device:
+                fits = t.numel() == (-(-n // BLOCK) if dtype is torch.float32 else n) and t.is_contiguous()
+            if not fits or t.get_device() != device:
                 raise ValueError("AdamW state {} (shape {}, {}) does not belong to a parameter of shape {} on {}".format(
                     key, tuple(t.shape), t.device, tuple(p.shape), p.device))
-        if bits == 8 and state.get("order") != _order(p):
-            raise ValueError("AdamW's 8-bit state follows the storage order of the parameter it was made for "
-                             "({}); this one is stored as {}".format(state.get("order"), _order(p)))
+        if bits == 8:
+            order = state.get("order")
+            if not (contiguous and order is None) and order != _order(p):
+                raise ValueError("AdamW's 8-bit state follows the storage order of the parameter it was made for "
+                                 "({}); this one is stored as {}".format(order, _order(p)))
 
-    def _state_of(self, p, bits):
-        state = self.state[p]
-        if not state:
-            state["step"] = 0
-            if bits == 32:
-                like = p if _dense(p) else p.contiguous()
-                state["exp_avg"] = torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format)
-                state["exp_avg_sq"] = torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format)
-            else:
-                blocks = -(-p.numel() // BLOCK)
-                state["exp_avg"] = torch.zeros(p.numel(), dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
-                state["exp_avg_sq"] = torch.zeros(p.numel(), dtype=torch.uint8, device=p.device)
-                state["exp_avg_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-                state["exp_avg_sq_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-                state["order"] = _order(p)
-        return state
+    @staticmethod
+    def _new_state(p, bits):
+        if bits == 32:
+            like = p if _dense(p) else p.contiguous()
+            return {"step": 0,
+                    "exp_avg": torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format),
+                    "exp_avg_sq": torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format)}
+        blocks, dev = -(-p.numel() // BLOCK), p.device
+        return {"step": 0,
+                "exp_avg": torch.zeros(p.numel(), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                "exp_avg_sq": torch.zeros(p.numel(), dtype=torch.uint8, device=dev),
+                "exp_avg_scale": torch.zeros(blocks, dtype=torch.float32, device=dev),
+                "exp_avg_sq_scale": torch.zeros(blocks, dtype=torch.float32, device=dev), "order": _order(p)}
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -197,69 +216,77 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self._validate_grads()
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        found = self._checked()
+        if found and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step cannot be captured into a graph: its bias corrections are host values")
         if not _amp_gate(self):
             return loss
         self.grad_norm = None
         batches = {}  # device -> descriptors, parameters to write back, tensors that the launch reads
-        index = 0
-        for group in self.param_groups:
+        for group, members in found:
             lr, (beta1, beta2), bits = float(group["lr"]), group["betas"], group["state_bits"]
             eps, wdf = float(group["eps"]), 1.0 - lr * float(group["weight_decay"])
-            for p in group["params"]:
-                index += 1
-                grad = p.grad
-                if grad is None:
-                    continue
-                state = self._state_of(p, bits)
+            last = None
+            for index, p, grad, state in members:
+                if not state:
+                    state = self.state[p] = self._new_state(p, bits)
                 state["step"] = t = int(state["step"]) + 1
-                if p.numel() == 0:
+                if t != last:
+                    step_size, rbc2, last = lr / (1.0 - beta1 ** t), 1.0 / math.sqrt(1.0 - beta2 ** t), t
+                n = p.numel()
+                if n == 0:
                     continue
-                rows, back, held = batches.setdefault(p.device, ([], [], []))
-                work = p
-                if not _dense(p):
-                    work = p.contiguous()
-                    back.append((p, work))
-                if not _same_layout(grad, work) or not _dense(grad):
-                    grad = torch.empty_like(work).copy_(grad)
-                m, v = state["exp_avg"], state["exp_avg_sq"]
+                device = p.get_device()
+                if device not in batches:
+                    batches[device] = ([], [], [])
+                rows, back, held = batches[device]
+                work, m, v = p, state["exp_avg"], state["exp_avg_sq"]
+                if not (p.is_contiguous() and grad.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+                    work, grad, m, v = self._laid_out(p, grad, state, bits, back)
+                    held.append((work, grad))
                 key = ms = vs = 0
                 if bits == 8:
                     ms, vs = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
                     key = _mix(_mix(self.seed + _GOLDEN * index) + _GOLDEN * t)
-                else:
-                    for name in ("exp_avg", "exp_avg_sq"):
-                        if not _dense(state[name]) or not _same_layout(state[name], work):
-                            state[name] = torch.empty_like(work, dtype=torch.float32).copy_(state[name])
-                    m, v = state["exp_avg"], state["exp_avg_sq"]
-                held.append((work, grad))
-                rows.append((work.data_ptr(), grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, p.numel(), key,
-                             lr / (1.0 - beta1 ** t), wdf, beta1, 1.0 - beta1, beta2, 1.0 - beta2,
-                             1.0 / math.sqrt(1.0 - beta2 ** t), eps, _dtype_code(p.dtype), bits))
+                rows.append((work.data_ptr(), grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n, key, step_size, wdf,
+                             beta1, 1.0 - beta1, beta2, 1.0 - beta2, rbc2, eps, _DTYPES[p.dtype], bits))
         for device, (rows, back, _) in batches.items():
+            device = torch.device("cuda", device)
             with _on_device(device):
                 self._launch(device, rows)
             for p, work in back:
                 p.copy_(work)
         return loss
 
+    @staticmethod
+    def _laid_out(p, grad, state, bits, back):
+        """Parameter, gradient and moments as runs of memory in one order; a parameter with gaps is stepped in a
+        copy that `back` says to write back."""
+        work = p
+        if not _dense(p):
+            work = p.contiguous()
+            back.append((p, work))
+        if not _same_layout(grad, work) or not _dense(grad):
+            grad = torch.empty_like(work).copy_(grad)
+        if bits == 32:
+            for name in ("exp_avg", "exp_avg_sq"):
+                if not _dense(state[name]) or not _same_layout(state[name], work):
+                    state[name] = torch.empty_like(work, dtype=torch.float32).copy_(state[name])
+        return work, grad, state["exp_avg"], state["exp_avg_sq"]
+
     def _launch(self, device, rows):
         lib = _native.load()
-        descs = ctypes.create_string_buffer(len(rows) * _DESC_STRUCT.size)
-        for i, row in enumerate(rows):
-            _DESC_STRUCT.pack_into(descs, i * _DESC_STRUCT.size, *row)
+        descs = _pack(rows)
         stream = torch.cuda.current_stream(device).cuda_stream
         coef = None
         if self.max_grad_norm is not None:
             bytes_ = int(lib.gefenx_adamw_norm_workspace_bytes(descs, len(rows)))
             ws = torch.empty(bytes_, dtype=torch.uint8, device=device)
             out = torch.empty(2, dtype=torch.float32, device=device)
-            _native.check(lib.gefenx_adamw_norm(descs, len(rows), self.max_grad_norm, out.data_ptr(), ws.data_ptr(),
-                                                bytes_, stream), "AdamW gradient norm")
-            self.grad_norm = out[0]
             coef = out.data_ptr() + 4
+            _native.check(lib.gefenx_adamw_norm(descs, len(rows), self.max_grad_norm, coef - 4, ws.data_ptr(), bytes_, stream),
+                          "AdamW gradient norm")
+            self.grad_norm = out[0]
         _native.check(lib.gefenx_adamw_step(descs, len(rows), coef, stream), "AdamW step")
 
     # ------------------------------------------------------------ moments
@@ -272,30 +299,32 @@ class AdamW(torch.optim.Optimizer):
         the codes stand for, flat, in the order the parameter is stored in.
         None for a parameter that has not been stepped."""
         bits_of = {p: group["state_bits"] for group in self.param_groups for p in group["params"]}
-        got, batches = [], {}
+        got, batches, known = [], {}, self.state
         for p in bits_of if params is None else params:
-            if p not in bits_of:
+            bits = bits_of.get(p)
+            if bits is None:
                 raise ValueError("moments() of a tensor that this optimizer does not step")
-            state = self.state.get(p)
+            state = known.get(p)
             if not state:
                 got.append(None)
                 continue
-            self._check_state(p, state, bits_of[p])
-            if bits_of[p] == 32:
-                got.append((state["exp_avg"], state["exp_avg_sq"]))
+            self._check_state(p, state, bits)
+            m, v = state["exp_avg"], state["exp_avg_sq"]
+            if bits == 32:
+                got.append((m, v))
                 continue
-            m, v = (torch.empty(p.numel(), dtype=torch.float32, device=p.device) for _ in range(2))
-            got.append((m, v))
-            if p.numel():
-                batches.setdefault(p.device, []).append(
-                    (m.data_ptr(), v.data_ptr(), state["exp_avg"].data_ptr(), state["exp_avg_sq"].data_ptr(),
-                     state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr(), p.numel(), 0,
-                     0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, _native.DT_F32, 8))
+            n = p.numel()
+            to_m, to_v = torch.empty_like(m, dtype=torch.float32), torch.empty_like(v, dtype=torch.float32)
+            got.append((to_m, to_v))
+            if n:
+                batches.setdefault(p.get_device(), []).append(
+                    (to_m.data_ptr(), to_v.data_ptr(), m.data_ptr(), v.data_ptr(), state["exp_avg_scale"].data_ptr(),
+                     state["exp_avg_sq_scale"].data_ptr(), n, 0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, _native.DT_F32, 8))
         for device, rows in batches.items():
-            descs = b"".join(_DESC_STRUCT.pack(*row) for row in rows)
+            device = torch.device("cuda", device)
             with _on_device(device):
                 _native.check(_native.load().gefenx_adamw_moments(
-                    descs, len(rows), torch.cuda.current_stream(device).cuda_stream), "AdamW moments")
+                    _pack(rows), len(rows), torch.cuda.current_stream(device).cuda_stream), "AdamW moments")
         return got
 
     # --------------------------------------------------------- checkpoint

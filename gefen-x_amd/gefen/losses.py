@@ -31,9 +31,8 @@ from torch.autograd.function import once_differentiable
 
 from gefen.gefen import _on_device
 from gefen.kernels import _native
-from gefen.kernels.automatic_gefen_fused import _dtype_code
 
-_DTYPES = frozenset((torch.float32, torch.float16, torch.bfloat16))
+_DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.bfloat16: _native.DT_BF16}
 
 
 class PreferenceLoss(NamedTuple):
@@ -84,19 +83,36 @@ class _Call:
                 raise ValueError("logits are [sequences, tokens, vocab], or [tokens, vocab] with cu_seqlens, got shape "
                                  "{}".format(tuple(logits.shape)))
             self.n_seq = logits.shape[0]
-        x = logits.detach()
-        if x.dim() > 3 or (x.stride(-1) != 1 and x.shape[-1] > 1):
-            x = x.contiguous()
-        x = x.reshape(-1, self.vocab) if x.dim() > 3 else x
-        x = x[(None,) * (3 - x.dim())]  # [batches, rows of a batch, vocab]
-        self.logits, self.labels = x, labels.detach().contiguous()
-        self.rows = self.labels.numel()
+        x = logits
+        if x.dim() > 3 or (x.stride(-1) != 1 and self.vocab > 1):
+            x = x.detach().contiguous()
+        # rows r of the leading dims: batches of `per` rows
+        if x.dim() == 3:
+            per, strides = x.shape[1], x.stride()[:2]
+        elif x.dim() == 2:
+            per, strides = x.shape[0], (0, x.stride(0))
+        else:  # one row, or contiguous
+            per, strides = labels.numel(), (0, self.vocab)
+        self.logits, self.labels = x, labels if labels.is_contiguous() else labels.contiguous()
+        self.rows = labels.numel()
         self.desc = _native.Logits(
-            logits=x.data_ptr(), labels=self.labels.data_ptr(), cu_seqlens=None if self.cu is None else self.cu.data_ptr(),
-            rows=self.rows, rows_per_batch=max(1, x.shape[1]), batch_stride=x.stride(0), row_stride=x.stride(1),
-            vocab=self.vocab, ignore_index=int(ignore_index), dtype=_dtype_code(x.dtype), n_seq=self.n_seq)
+            x.data_ptr(), self.labels.data_ptr(), None if self.cu is None else self.cu.data_ptr(), self.rows, max(1, per),
+            strides[0], strides[1], self.vocab, int(ignore_index), _DTYPES[x.dtype], self.n_seq)
         self.ref = ctypes.byref(self.desc)
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
+
+    @classmethod
+    def again(cls, desc, logits, labels, ignore_index, cu_seqlens=None, sequences=True):
+        """The call of a forward pass for its backward: by its descriptor, where that reads the saved tensors
+        themselves (not copies that are gone, nor tensors that hooks have moved)."""
+        if (desc.logits != logits.data_ptr() or desc.labels != labels.data_ptr()
+                or desc.cu_seqlens != (None if cu_seqlens is None else cu_seqlens.data_ptr())):
+            return cls(logits, labels, ignore_index, cu_seqlens, sequences)
+        call = cls.__new__(cls)
+        call.desc, call.ref = desc, ctypes.byref(desc)
+        call.device, call.shape, call.logits, call.labels = logits.device, logits.shape, logits, labels
+        call.stream = torch.cuda.current_stream(call.device).cuda_stream
+        return call
 
     def per_token(self, t, name):
         """A per-token input as the kernels read it, or None."""
@@ -108,10 +124,20 @@ class _Call:
                 name, tuple(self.labels.shape), self.device,
                 "{} of shape {} on {}".format(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor)
                 else type(t).__name__))
-        return t.detach().to(torch.float32).contiguous()
+        return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().to(torch.float32).contiguous()
 
     def empty(self, *shape):
         return torch.empty(shape, dtype=torch.float32, device=self.device)
+
+    def saved(self):
+        """One buffer for what the gradient needs (row statistics [rows, 2], row coefficients [rows], sequence weights
+        [n_seq]), and the pointers of the three."""
+        t = torch.empty(3 * self.desc.rows + self.desc.n_seq + 1, dtype=torch.float32, device=self.device)
+        return t, self.saved_ptrs(t)
+
+    def saved_ptrs(self, t):
+        at, rows = t.data_ptr(), self.desc.rows
+        return at, at + 8 * rows, at + 12 * rows
 
     def workspace(self):
         n = int(_native.load().gefenx_loss_workspace_bytes(self.ref))
@@ -123,17 +149,18 @@ class _Call:
             return None, float(scale)
         if scale.numel() != 1 or scale.device != self.device:
             raise ValueError("grad_scale must be a number or one value on {}".format(self.device))
-        return scale.detach().to(torch.float32), 1.0
+        return scale if scale.dtype is torch.float32 else scale.detach().to(torch.float32), 1.0
 
     def empty_grad(self):
         return torch.empty(self.shape, dtype=self.logits.dtype, device=self.device)
 
-    def grad(self, stats, k, weights, scale):
-        """The gradient of the logits, contiguous in their shape."""
+    def grad(self, saved, k, weighted, scale):
+        """The gradient of the logits, contiguous in their shape; k: pointer of the row coefficients, or None."""
         (scale_dev, factor), out = self.scale(scale), self.empty_grad()
+        stats, _, weights = self.saved_ptrs(saved)
         with _on_device(self.device):
             _native.check(_native.load().gefenx_logits_grad(
-                self.ref, _ptr(stats), _ptr(k), _ptr(weights), _ptr(scale_dev), factor, _ptr(out), self.stream),
+                self.ref, stats, k, weights if weighted else None, _ptr(scale_dev), factor, out.data_ptr(), self.stream),
                 "logits gradient")
         return out
 
@@ -159,12 +186,12 @@ def _finite(value, name):
 # ------------------------------------------------------------ forward passes
 
 def _logps_forward(call):
-    logps, stats = call.empty(*call.labels.shape), call.empty(call.rows, 2)
+    logps, (saved, ptrs) = call.empty(*call.labels.shape), call.saved()
     ws, n = call.workspace()
     with _on_device(call.device):
-        _native.check(_native.load().gefenx_token_logps(call.ref, _ptr(logps), _ptr(stats), _ptr(ws), n, call.stream),
+        _native.check(_native.load().gefenx_token_logps(call.ref, logps.data_ptr(), ptrs[0], ws.data_ptr(), n, call.stream),
                       "token_logps")
-    return logps, stats
+    return logps, saved
 
 
 def _preference_forward(call, ref_logps, beta, smoothing, average):
@@ -174,14 +201,14 @@ def _preference_forward(call, ref_logps, beta, smoothing, average):
     ref = call.per_token(ref_logps, "ref_logps")
     beta, smoothing = _finite(beta, "beta"), _probability(smoothing, "label_smoothing", 0.5)
     pairs = call.n_seq // 2
-    loss, chosen, rejected, weights = call.empty(), call.empty(pairs), call.empty(pairs), call.empty(call.n_seq)
-    logps, stats = call.empty(*call.labels.shape), call.empty(call.rows, 2)
+    loss, chosen, rejected = call.empty(), call.empty(pairs), call.empty(pairs)
+    logps, (saved, (stats, _, weights)) = call.empty(*call.labels.shape), call.saved()
     ws, n = call.workspace()
     with _on_device(call.device):
         _native.check(_native.load().gefenx_preference_loss(
-            call.ref, _ptr(ref), beta, smoothing, 1 if average else 0, _ptr(loss), _ptr(chosen), _ptr(rejected),
-            _ptr(logps), _ptr(stats), _ptr(weights), _ptr(ws), n, call.stream), "preference_loss")
-    return PreferenceLoss(loss, chosen, rejected, logps), stats, weights
+            call.ref, _ptr(ref), beta, smoothing, 1 if average else 0, loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(),
+            logps.data_ptr(), stats, weights, ws.data_ptr(), n, call.stream), "preference_loss")
+    return PreferenceLoss(loss, chosen, rejected, logps), saved
 
 
 def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction, grad_scale=None):
@@ -204,19 +231,20 @@ def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high,
         adv, per_row = call.per_token(advantages, "advantages (one per token or one per sequence)"), 1
         if adv is None:
             raise ValueError("policy_loss needs advantages")
-    loss, kl, clipped, weights = call.empty(), call.empty(), call.empty(), call.empty(call.n_seq)
-    logps, stats, k = call.empty(*call.labels.shape), call.empty(call.rows, 2), call.empty(call.rows)
-    args = [call.ref, _ptr(old), _ptr(adv), per_row, _ptr(ref), clip_low, clip_high, kl_coef, 1 if reduction == "sequence" else 0,
-            _ptr(loss), _ptr(kl), _ptr(clipped), _ptr(logps), _ptr(stats), _ptr(k), _ptr(weights)]
+    loss, kl, clipped, logps = call.empty(), call.empty(), call.empty(), call.empty(*call.labels.shape)
+    saved, (stats, k, weights) = call.saved()
+    args = [call.ref, old.data_ptr(), adv.data_ptr(), per_row, _ptr(ref), clip_low, clip_high, kl_coef,
+            1 if reduction == "sequence" else 0, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), logps.data_ptr(), stats, k,
+            weights]
     entry, grad = _native.load().gefenx_policy_loss, None
     if grad_scale is not None:
         (scale_dev, factor), grad = call.scale(grad_scale), call.empty_grad()
         entry = _native.load().gefenx_policy_loss_grad
-        args += [_ptr(scale_dev), factor, _ptr(grad)]
+        args += [_ptr(scale_dev), factor, grad.data_ptr()]
     ws, n = call.workspace()
     with _on_device(call.device):
-        _native.check(entry(*args, _ptr(ws), n, call.stream), "policy_loss")
-    return PolicyLoss(loss, kl, clipped, logps), stats, k, weights, grad
+        _native.check(entry(*args, ws.data_ptr(), n, call.stream), "policy_loss")
+    return PolicyLoss(loss, kl, clipped, logps), saved, grad
 
 
 # ------------------------------------------------------------ autograd
@@ -224,28 +252,31 @@ def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high,
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ignore_index):
-        logps, stats = _logps_forward(_Call(logits, labels, ignore_index, sequences=False))
-        ctx.ignore_index = ignore_index
-        ctx.save_for_backward(logits, labels, stats)
+        call = _Call(logits, labels, ignore_index, sequences=False)
+        logps, saved = _logps_forward(call)
+        ctx.ignore_index, ctx.desc = ignore_index, call.desc
+        ctx.save_for_backward(logits, labels, saved)
         return logps
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        logits, labels, stats = ctx.saved_tensors
-        call = _Call(logits, labels, ctx.ignore_index, sequences=False)
-        return call.grad(stats, call.per_token(grad, "gradient"), None, 1.0), None, None
+        logits, labels, saved = ctx.saved_tensors
+        call = _Call.again(ctx.desc, logits, labels, ctx.ignore_index, sequences=False)
+        k = call.per_token(grad, "gradient")
+        return call.grad(saved, k.data_ptr(), False, 1.0), None, None
 
 
 class _SequenceLoss(torch.autograd.Function):
-    """Both sequence losses: `forward_of` returns the outputs and what the gradient needs."""
+    """Both sequence losses: `forward_of` returns the outputs and what the gradient needs; by_row: whether rows
+    have coefficients of their own."""
 
     @staticmethod
-    def forward(ctx, logits, labels, cu_seqlens, ignore_index, forward_of):
+    def forward(ctx, logits, labels, cu_seqlens, ignore_index, forward_of, by_row):
         call = _Call(logits, labels, ignore_index, cu_seqlens)
-        out, stats, k, weights = forward_of(call)
-        ctx.ignore_index = ignore_index
-        ctx.save_for_backward(logits, labels, cu_seqlens, stats, k, weights)
+        out, saved = forward_of(call)
+        ctx.ignore_index, ctx.desc, ctx.by_row = ignore_index, call.desc, by_row
+        ctx.save_for_backward(logits, labels, cu_seqlens, saved)
         ctx.mark_non_differentiable(*out[1:])
         ctx.set_materialize_grads(False)
         return tuple(out)
@@ -254,9 +285,11 @@ class _SequenceLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, *unused):
         if grad is None:
-            return None, None, None, None, None
-        logits, labels, cu_seqlens, stats, k, weights = ctx.saved_tensors
-        return _Call(logits, labels, ctx.ignore_index, cu_seqlens).grad(stats, k, weights, grad), None, None, None, None
+            return None, None, None, None, None, None
+        logits, labels, cu_seqlens, saved = ctx.saved_tensors
+        call = _Call.again(ctx.desc, logits, labels, ctx.ignore_index, cu_seqlens)
+        k = call.saved_ptrs(saved)[1] if ctx.by_row else None
+        return call.grad(saved, k, True, grad), None, None, None, None, None
 
 
 def token_logps(logits, labels, *, ignore_index=-100):
@@ -277,17 +310,16 @@ def preference_loss(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1
     without any has reward 0).  ref_logps: the reference model's token_logps;
     None: zeros."""
     def forward_of(call):
-        out, stats, weights = _preference_forward(call, ref_logps, beta, label_smoothing, average)
-        return out, stats, None, weights
-    return PreferenceLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of))
+        return _preference_forward(call, ref_logps, beta, label_smoothing, average)
+    return PreferenceLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of, False))
 
 
 def preference_loss_and_grad(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0,
                              average=False, ignore_index=-100, grad_scale=1.0):
     """(preference_loss(...), gradient of the loss times grad_scale in the logits)."""
     call = _Call(logits, labels, ignore_index, cu_seqlens)
-    out, stats, weights = _preference_forward(call, ref_logps, beta, label_smoothing, average)
-    return out, call.grad(stats, None, weights, grad_scale)
+    out, saved = _preference_forward(call, ref_logps, beta, label_smoothing, average)
+    return out, call.grad(saved, None, True, grad_scale)
 
 
 def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2, clip_high=0.2,
@@ -299,8 +331,8 @@ def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seq
     reduction: "token", the mean over all labelled tokens, or "sequence", the mean over the sequences that have
     any of their mean; 0 without any.  advantages: one per token, or one per sequence [N]."""
     def forward_of(call):
-        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)[:4]
-    return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of))
+        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)[:2]
+    return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of, True))
 
 
 def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2,
@@ -309,6 +341,6 @@ def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, 
     if grad_scale is None:
         raise ValueError("grad_scale must be a number or one value on the logits' device")
     call = _Call(logits, labels, ignore_index, cu_seqlens)
-    out, _, _, _, grad = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction,
-                                         grad_scale)
+    out, _, grad = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction,
+                                   grad_scale)
     return out, grad

@@ -387,6 +387,8 @@ def test_nothing_to_learn_from(dev):
         assert out.loss.item() == 0 and out.kl.item() == 0 and out.clip_fraction.item() == 0 and not g.any()
     out, g = gefen.preference_loss_and_grad(x[:, :0], y[:, :0])
     assert abs(out.loss.item() - math.log(2)) < 1e-6 and g.shape == (4, 0, 100)
+    out, g = gefen.policy_loss_and_grad(x[:, :0], y[:, :0], z[:, :0], z[:, :0])
+    assert out.loss.item() == 0 and g.shape == (4, 0, 100)
     cu = torch.tensor([0, 0, 0], dtype=torch.int32, device=dev)
     out, g = gefen.preference_loss_and_grad(x[0, :0], y[0, :0], cu_seqlens=cu)
     assert abs(out.loss.item() - math.log(2)) < 1e-6
@@ -438,6 +440,30 @@ def test_scales(dev):
     again.loss.backward()
     _, half = gefen.policy_loss_and_grad(d.logits(), *args, grad_scale=0.5)
     assert torch.equal(leaf.grad, half)
+
+
+def test_backward_of_copies_and_of_moved_tensors(dev):
+    """Logits, labels and cu_seqlens that the forward pass had to copy, and saved tensors that hooks moved away."""
+    d = Data([30, 20], 500, torch.float32, dev, packed=True)
+    y, ref = d.row(d.labels), d.row(d.ref)
+    plain = d.logits(True)
+    gefen.preference_loss(plain, y, ref, cu_seqlens=d.cu).loss.backward()
+    odd = d.x.t().contiguous().to(dev).requires_grad_(True)  # [V, T]
+    every = torch.stack([y, y], 1)[:, 0]                     # stride 2
+    gefen.preference_loss(odd.t(), every, ref, cu_seqlens=d.cu.long()).loss.backward()
+    assert torch.equal(odd.grad.t(), plain.grad)
+    leaf = d.logits(True)
+    with torch.autograd.graph.save_on_cpu():
+        out = gefen.preference_loss(leaf * 1.0, y, ref, cu_seqlens=d.cu)
+    torch.empty(1 << 20, device=dev).fill_(float("nan"))
+    out.loss.backward()
+    assert torch.equal(leaf.grad, plain.grad)
+    twice = d.logits(True)
+    out = gefen.preference_loss(twice, y, ref, cu_seqlens=d.cu)
+    with torch.no_grad():
+        twice.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        out.loss.backward()
 
 
 def test_runs_repeat_bit_for_bit_and_on_other_streams(dev):
