@@ -18,6 +18,11 @@ namespace {
 
 constexpr int kT = 256;               // threads of a row workgroup
 constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
+// Rows of up to so many runs of 16 bytes go to a wave each where there are enough of them: a workgroup is
+// a barrier and more than its share of lanes for them (statistics and gradient of 16384 rows, us: 1000
+// bf16 logits 26.6 and 26.2 -> 12.9 and 18.6, 4096 37.6 and 58.0 -> 23.4 and 53.4; 8192, 1024 runs, 44.0
+// and 102 against 43.3 and 117).
+constexpr int64_t kShortRuns = 768;
 constexpr int64_t kGradPasses = 2;    // passes of a workgroup of the gradient
 constexpr int kRowT = 1024;           // threads of a workgroup that keeps a row to itself
 constexpr int kSeqT = 1024;           // threads of a sequence workgroup
@@ -30,7 +35,7 @@ struct Rows {
     const int32_t* cu;
     int64_t rows, per_batch, batch_stride, row_stride;
     int64_t vocab, ignore;
-    int32_t n_seq, splits;
+    int32_t n_seq, splits, per;  // per: rows of a workgroup
     int64_t split_runs;    // runs of 16 bytes of a split
 };
 
@@ -144,12 +149,12 @@ __device__ __forceinline__ void wave_join(Soft& a) {
 // Runs c .. end - 1 of a row, TH lanes at a time; each lane's part.  Which logits a lane adds up, and so
 // the sum, does not depend on where the row starts in memory.
 template <int DT, int TH, bool STREAM>
-__device__ __forceinline__ Soft row_part(const typename Elem<DT>::T* x, int64_t vocab, int64_t c, int64_t end) {
+__device__ __forceinline__ Soft row_part(const typename Elem<DT>::T* x, int64_t vocab, int64_t c, int64_t end, int lane) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>;
     const int64_t whole = end * W <= vocab ? end : end - 1;
     Soft a;
-    c += threadIdx.x;
+    c += lane;
     const auto add = [&](auto load) {
         for (; c + 3 * TH < whole; c += 4 * TH) {
             Run<T, W> v[4];
@@ -180,17 +185,23 @@ __device__ __forceinline__ Soft group_join(Soft a, float2* waves) {
     return a;
 }
 
-// part[row][split] = {maximum, sum of exp(x - maximum)} of a split of a row.
-template <int DT>
+// part[row][split] = {maximum, sum of exp(x - maximum)} of a split of a row.  PER rows to a workgroup:
+// one, or one for each of its waves (rows without splits).
+template <int DT, int PER>
 __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restrict__ part) {
     using T = typename Elem<DT>::T;
+    constexpr int TH = kT / PER;
     __shared__ float2 waves[kT / 64];
-    const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
-    if (sload(q.labels + r) == q.ignore) return;
+    const int lane = threadIdx.x % TH;
+    const int64_t at = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
+    const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
+    if (r >= q.rows || sload(q.labels + r) == q.ignore) return;
     const int64_t runs = (q.vocab + kW<DT> - 1) / kW<DT>, begin = split * q.split_runs;
     const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
-    const Soft a = group_join<kT>(row_part<DT, kT, true>((const T*)q.x + row_offset(q, r), q.vocab, begin, end), waves);
-    if (threadIdx.x == 0) part[blockIdx.x] = make_float2(a.m, a.s);
+    Soft a = row_part<DT, TH, true>((const T*)q.x + row_offset(q, r), q.vocab, begin, end, lane);
+    if constexpr (PER > 1) wave_join(a);
+    else a = group_join<kT>(a, waves);
+    if (lane == 0) part[at] = make_float2(a.m, a.s);
 }
 
 // ------------------------------------------------------------ tokens and sequences
@@ -426,13 +437,16 @@ __device__ __forceinline__ void grad_run(Run<typename Elem<DT>::T, kW<DT>>& v, i
 }
 
 // grad[r][v] = c_r ([v = y_r] - exp(x - max) / sum), c_r = k[r] * weights[sequence] * scale.
-// unlabelled: only the rows without a label, which get zeros.
-template <int DT>
+// unlabelled: only the rows without a label, which get zeros.  PER: as above.
+template <int DT, int PER>
 __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* __restrict__ stats, const float* __restrict__ k,
                                                     const float* __restrict__ weights, const float* __restrict__ scale_dev,
                                                     float scale, int unlabelled, void* __restrict__ grad) {
     using T = typename Elem<DT>::T;
-    const int64_t r = blockIdx.x / (uint32_t)q.splits, split = blockIdx.x % (uint32_t)q.splits;
+    constexpr int TH = kT / PER;
+    const int64_t wg = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
+    const int64_t r = PER > 1 ? wg : wg / (uint32_t)q.splits, split = PER > 1 ? 0 : wg % (uint32_t)q.splits;
+    if (r >= q.rows) return;
     const int64_t label = sload(q.labels + r);
     float coef = 0.0f;
     if (label != q.ignore) {
@@ -451,12 +465,12 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
     int64_t c = split * q.split_runs, end = c + q.split_runs;
     if (end > runs.count()) end = runs.count();
     const int64_t whole = runs.whole(end);
-    c += threadIdx.x;
+    c += threadIdx.x % TH;
     if (coef == 0.0f) {
         Run<T, W> zeros;
 #pragma unroll
         for (int i = 0; i < W; ++i) zeros.e[i] = T(0);
-        for (; c < end; c += kT) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
+        for (; c < end; c += TH) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
         return;
     }
     const T* x = (const T*)q.x + row_offset(q, r);
@@ -469,19 +483,19 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
     };
     if (c == 0) {
         one(0);
-        c += kT;
+        c += TH;
     }
-    for (; c + kT < whole; c += 2 * kT) {
+    for (; c + TH < whole; c += 2 * TH) {
         Run<T, W> v[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * kT));
+        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * TH));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            grad_run<DT>(v[i], runs.begin(c + i * kT), label, coef, each, max);
-            store_run<T, W>(out + runs.begin(c + i * kT), W, v[i]);
+            grad_run<DT>(v[i], runs.begin(c + i * TH), label, coef, each, max);
+            store_run<T, W>(out + runs.begin(c + i * TH), W, v[i]);
         }
     }
-    for (; c < end; c += kT) one(c);
+    for (; c < end; c += TH) one(c);
 }
 
 // Statistics and gradient of a labelled row in one go, where the coefficient needs no other row: two
@@ -498,7 +512,7 @@ __global__ __launch_bounds__(kRowT) void k_policy_rows(const Rows q, const Token
     const int64_t r = blockIdx.x, label = sload(q.labels + r);
     if (label == q.ignore) return;
     const T* x = (const T*)q.x + row_offset(q, r);
-    const Soft a = group_join<kRowT>(row_part<DT, kRowT, false>(x, q.vocab, 0, (q.vocab + W - 1) / W), waves);
+    const Soft a = group_join<kRowT>(row_part<DT, kRowT, false>(x, q.vocab, 0, (q.vocab + W - 1) / W, threadIdx.x), waves);
     if (threadIdx.x == 0) {
         part[r] = make_float2(a.m, a.s);
         const int s = seq_of(q, r);
@@ -563,6 +577,11 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     splits = splits > passes ? passes : splits;
     q.split_runs = (runs + splits - 1) / splits;
     q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
+    q.per = runs <= kShortRuns && l->rows >= kWantedWgs ? kT / 64 : 1;
+    if (q.per > 1) {
+        q.splits = 1;
+        q.split_runs = runs;
+    }
     return GEFENX_OK;
 }
 
@@ -583,7 +602,9 @@ int run_stats(const char* what, const Rows& q, int dtype, float2* part, hipStrea
     if (q.rows == 0) return GEFENX_OK;
     if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
     return by_dtype(dtype, [&](auto dt) {
-        k_row_stats<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, part);
+        constexpr int DT = decltype(dt)::value;
+        if (q.per > 1) k_row_stats<DT, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, part);
+        else k_row_stats<DT, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, part);
         return launched(what);
     });
 }
@@ -623,8 +644,14 @@ int run_grad(const char* what, const gefenx_logits& l, const float* stats, const
     if (rc != GEFENX_OK) return rc;
     if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
     return by_dtype(l.dtype, [&](auto dt) {
-        k_logits_grad<decltype(dt)::value><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(
-            q, reinterpret_cast<const float2*>(stats), k, weights, scale_dev, (float)scale, unlabelled, grad);
+        constexpr int DT = decltype(dt)::value;
+        const float2* st = reinterpret_cast<const float2*>(stats);
+        if (q.per > 1)
+            k_logits_grad<DT, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, st, k, weights, scale_dev,
+                                                                                             (float)scale, unlabelled, grad);
+        else
+            k_logits_grad<DT, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, st, k, weights, scale_dev, (float)scale,
+                                                                              unlabelled, grad);
         return launched(what);
     });
 }
