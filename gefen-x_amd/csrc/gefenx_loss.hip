@@ -23,7 +23,11 @@ constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on
 // bf16 logits 26.6 and 26.2 -> 12.9 and 18.6, 4096 37.6 and 58.0 -> 23.4 and 53.4; 8192, 1024 runs, 44.0
 // and 102 against 43.3 and 117).
 constexpr int64_t kShortRuns = 768;
-constexpr int64_t kGradPasses = 2;    // passes of a workgroup of the gradient
+// Passes of a workgroup of the gradient, and where it only writes zeros beside rows it leaves alone.  What
+// is being written at any time should lie close together, and a workgroup costs its start (gradient of
+// 16384 x 151936 bf16, 9216 rows labelled, 1 / 2 / 4 / 8 passes: 1490 / 1400 / 1425 / 1512 us; the whole
+// policy loss on it with zeros in 1 / 2 / 4 / 8: 1650 / 1554 / 1532 / 1573).
+constexpr int64_t kGradPasses = 2, kZeroPasses = 4;
 constexpr int kRowT = 1024;           // threads of a workgroup that keeps a row to itself
 constexpr int kSeqT = 1024;           // threads of a sequence workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -640,7 +644,7 @@ int need(const char* what, const Rows& q, const void* ws, size_t bytes) {
 int run_grad(const char* what, const gefenx_logits& l, const float* stats, const float* k, const float* weights,
              const float* scale_dev, double scale, int unlabelled, void* grad, hipStream_t s) {
     Rows q;
-    const int rc = make_rows(what, &l, false, q, kGradPasses);
+    const int rc = make_rows(what, &l, false, q, unlabelled ? kZeroPasses : kGradPasses);
     if (rc != GEFENX_OK) return rc;
     if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
     return by_dtype(l.dtype, [&](auto dt) {

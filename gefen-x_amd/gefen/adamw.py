@@ -60,7 +60,7 @@ def _order(t: torch.Tensor):
     reach = 1  # elements spanned by the inner dims
     for d in reversed(dims):
         if t.stride(d) < reach:
-            raise ValueError("AdamW cannot step a parameter whose elements share memory (shape {}, strides {})".format(
+            raise ValueError("AdamW cannot step a parameter whose elements may share memory (shape {}, strides {})".format(
                 tuple(t.shape), t.stride()))
         reach += (t.shape[d] - 1) * t.stride(d)
     return tuple(dims)
@@ -313,6 +313,8 @@ class AdamW(torch.optim.Optimizer):
             if bits == 32:
                 got.append((m, v))
                 continue
+            if not p.is_cuda:
+                raise RuntimeError("AdamW reads 8-bit moments on a HIP device only; the parameter is on {}".format(p.device))
             n = p.numel()
             to_m, to_v = torch.empty_like(m, dtype=torch.float32), torch.empty_like(v, dtype=torch.float32)
             got.append((to_m, to_v))

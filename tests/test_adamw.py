@@ -144,6 +144,13 @@ def test_moments_of_foreign_tensors_are_refused():
     assert opt.moments() == [None]
 
 
+def test_host_state_of_8_bits_is_not_read_on_a_device():
+    p, opt = one(300, state_bits=8)
+    opt.load_state_dict({"state": {0: state8(300)}, "param_groups": opt.state_dict()["param_groups"]})
+    with pytest.raises(RuntimeError, match="HIP device"):
+        opt.moments()
+
+
 # ------------------------------------------------ the formats, by their restatement
 
 def test_v_code_round_trip_and_order():
