@@ -22,6 +22,8 @@ constexpr int kGroup = 16;               // lanes that share such a block, two c
 constexpr float kTiny = 0x1p-126f;       // smallest scale: its reciprocal, and 448 of them, are finite
 constexpr int kCode0 = 761;              // bits(x) >> 20 of v's code c is c + 761: code 255 is x = 1
 constexpr int64_t kNormPartials = 4096;  // about so many partial sums of the gradient norm
+// A launch has fewer than 2^32 threads; a tensor has its workgroups in one.
+constexpr int64_t kMaxWgs = ((int64_t)1 << 32) / kT - 1, kMaxNumel = (int64_t)1 << 33;
 
 struct Item {
     void* p;
@@ -351,7 +353,7 @@ int validate(const char* what, const gefenx_adamw_desc* d, int n, bool state, bo
             return set_error(GEFENX_EDTYPE, "%s: tensor %d: unsupported dtype %d", what, i, d[i].dtype);
         if (d[i].bits != 8 && d[i].bits != 32)
             return set_error(GEFENX_EINVAL, "%s: tensor %d: moments of %d bits (8 or 32)", what, i, d[i].bits);
-        if (d[i].numel < 0 || d[i].numel >= (int64_t)1 << 40)
+        if (d[i].numel < 0 || d[i].numel > kMaxNumel)
             return set_error(GEFENX_EINVAL, "%s: tensor %d: bad numel %lld", what, i, (long long)d[i].numel);
         if (d[i].numel == 0) continue;
         const bool scales = d[i].bits == 32 || (d[i].exp_avg_scale && d[i].exp_avg_sq_scale);
@@ -389,7 +391,7 @@ int for_batches(const gefenx_adamw_desc* d, int n, int64_t per, P&& take, F&& la
     for (int i = 0; i < n; ++i) {
         if (d[i].numel == 0 || !take(d[i])) continue;
         const int64_t w = (d[i].numel + per - 1) / per;
-        if (b.n == kItems || wgs + w > 0x7fffffff) {
+        if (b.n == kItems || wgs + w > kMaxWgs) {
             const int rc = flush();
             if (rc != GEFENX_OK) return rc;
         }

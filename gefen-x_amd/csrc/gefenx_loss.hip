@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kT = 256;               // threads of a row workgroup
 constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
+constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;  // of a launch
 // Rows of up to so many runs of 16 bytes go to a wave each where there are enough of them: a workgroup is
 // a barrier and more than its share of lanes for them (statistics and gradient of 16384 rows, us: 1000
 // bf16 logits 26.6 and 26.2 -> 12.9 and 18.6, 4096 37.6 and 58.0 -> 23.4 and 53.4; 8192, 1024 runs, 44.0
@@ -460,8 +461,10 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
         if (weights) {
             const int s = seq_of(q, r);
             coef = s >= 0 ? coef * sload(weights + s) : 0.0f;
+            if (s >= 0 && (uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+        } else if ((uint64_t)label >= (uint64_t)q.vocab) {
+            coef = __uint_as_float(0x7fc00000u);
         }
-        if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
     }
     T* out = (T*)grad + r * q.vocab;
     constexpr int W = kW<DT>;
@@ -522,7 +525,7 @@ __global__ __launch_bounds__(kRowT) void k_policy_rows(const Rows q, const Token
         const int s = seq_of(q, r);
         float coef = 0.0f;
         if (s >= 0) coef = (scale_dev ? sload(scale_dev) * scale : scale) * policy_token(t, r, s, (float)token_logp<DT>(q, r, label, a)).k * sload(weights + s);
-        if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+        if (s >= 0 && (uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
         coef_of = coef;
     }
     __syncthreads();
@@ -560,6 +563,7 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     if (l->rows < 0 || l->vocab < 1 || l->rows > 0x7fffffff || l->vocab > 0x7fffffff || l->rows_per_batch < 1)
         return set_error(GEFENX_EINVAL, "%s: bad sizes (rows=%lld of %lld, vocab=%lld)", what, (long long)l->rows,
                          (long long)l->rows_per_batch, (long long)l->vocab);
+    if (l->n_seq < 0 || l->n_seq > kMaxThreads / kSeqT) return set_error(GEFENX_EINVAL, "%s: bad sequences (%d)", what, l->n_seq);
     if (l->rows > 0 && (!l->logits || !l->labels)) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
     if (sequences && (l->n_seq < 1 || (!l->cu_seqlens && l->rows != 0 && l->rows != l->n_seq * l->rows_per_batch)))
         return set_error(GEFENX_EINVAL, "%s: bad sequences (%d over %lld rows)", what, l->n_seq, (long long)l->rows);
@@ -579,6 +583,7 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     int64_t splits = l->rows > 0 ? (kWantedWgs + l->rows - 1) / l->rows : 1;
     if (most && splits * most < passes) splits = (passes + most - 1) / most;
     splits = splits > passes ? passes : splits;
+    if (l->rows * splits > kMaxThreads / kT) splits = kMaxThreads / kT / l->rows < 1 ? 1 : kMaxThreads / kT / l->rows;
     q.split_runs = (runs + splits - 1) / splits;
     q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
     q.per = runs <= kShortRuns && l->rows >= kWantedWgs ? kT / 64 : 1;
@@ -586,6 +591,8 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
         q.splits = 1;
         q.split_runs = runs;
     }
+    if ((l->rows * q.splits + q.per - 1) / q.per > kMaxThreads / kT)
+        return set_error(GEFENX_EINVAL, "%s: too many rows (%lld)", what, (long long)l->rows);
     return GEFENX_OK;
 }
 
@@ -604,7 +611,6 @@ int by_dtype(int dtype, F&& f) {
 
 int run_stats(const char* what, const Rows& q, int dtype, float2* part, hipStream_t s) {
     if (q.rows == 0) return GEFENX_OK;
-    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
     return by_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (q.per > 1) k_row_stats<DT, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, part);
@@ -632,7 +638,7 @@ int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const
 // rows are split instead.
 bool rows_alone(const gefenx_logits& l) {
     const int64_t bytes = l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2);
-    return bytes >= (64 << 10) && l.rows >= 1024 && l.rows * bytes > (int64_t)256 << 20;
+    return bytes >= (64 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)256 << 20;
 }
 
 int need(const char* what, const Rows& q, const void* ws, size_t bytes) {
@@ -646,7 +652,6 @@ int run_grad(const char* what, const gefenx_logits& l, const float* stats, const
     Rows q;
     const int rc = make_rows(what, &l, false, q, unlabelled ? kZeroPasses : kGradPasses);
     if (rc != GEFENX_OK) return rc;
-    if (q.rows * q.splits > 0x7fffffff) return set_error(GEFENX_EINVAL, "%s: too many rows", what);
     return by_dtype(l.dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         const float2* st = reinterpret_cast<const float2*>(stats);

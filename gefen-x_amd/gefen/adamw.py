@@ -339,9 +339,10 @@ class AdamW(torch.optim.Optimizer):
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("loaded state dict has other parameter groups than this optimizer")
-        new = {}
+        new, widths = {}, []
         for group, old in zip(groups, saved):
             bits = old.get("state_bits", group["state_bits"])
+            widths.append(bits)
             if bits not in _STATE:
                 raise ValueError("state_bits must be 8 or 32 but is: {!r}".format(bits))
             for p, i in zip(group["params"], old["params"]):
@@ -366,7 +367,7 @@ class AdamW(torch.optim.Optimizer):
                 self._check_state(p, state, bits)
                 new[p] = state
         super().load_state_dict({"state": {}, "param_groups": saved})
-        for group in self.param_groups:
-            group.setdefault("state_bits", self.defaults["state_bits"])
+        for group, bits in zip(self.param_groups, widths):
+            group["state_bits"] = bits
         self.state.clear()
         self.state.update(new)

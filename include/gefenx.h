@@ -511,7 +511,7 @@ int gefenx_gemm_nt_bf16(const void* A, const void* B, const void* C, void* D, in
  *               finalizer of key + 0x9E3779B97F4A7C15 * (i / 4 + 1).
  *   A block with an inf or NaN gets the scale NaN.
  * Elements are taken in storage order: p, grad and the averages are each numel
- * contiguous elements, at any alignment of their type.
+ * contiguous elements (at most 2^33), at any alignment of their type.
  * ---------------------------------------------------------------------- */
 typedef struct gefenx_adamw_desc {
     void* p;

@@ -125,6 +125,14 @@ def test_torch_checkpoint_loads_and_goes_back():
     back.load_state_dict({"state": opt.state_dict()["state"], "param_groups": theirs.state_dict()["param_groups"]})
 
 
+def test_groups_keep_their_width_where_a_checkpoint_names_none():
+    a, b = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(300))
+    opt = gefen.AdamW([{"params": [a]}, {"params": [b], "state_bits": 8}])
+    groups = [{k: v for k, v in g.items() if k != "state_bits"} for g in opt.state_dict()["param_groups"]]
+    opt.load_state_dict({"state": {1: state8(300)}, "param_groups": groups})
+    assert [g["state_bits"] for g in opt.param_groups] == [32, 8] and opt.state[b]["step"] == 7
+
+
 def test_other_groups_are_refused():
     _, opt = one()
     with pytest.raises(ValueError, match="parameter groups"):

@@ -405,6 +405,9 @@ def test_packed_sequences_with_empty_ones_and_rows_outside(dev):
     assert torch.equal(out.loss, want.loss) and torch.equal(out.chosen_rewards, want.chosen_rewards)
     assert torch.equal(g[2:15], gw) and not g[:2].any() and not g[15:].any()
     assert not out.logps[:2].any() and not out.logps[15:].any() and torch.equal(out.logps[2:15], want.logps)
+    y[0], y[17] = 64, -5  # no logits of these numbers, but nobody asks for them
+    again, g2 = gefen.preference_loss_and_grad(x, y, ref, cu_seqlens=cu)
+    assert torch.equal(again.loss, out.loss) and torch.equal(g2, g)
 
 
 def test_padded_and_packed_agree(dev):

@@ -26,7 +26,7 @@ def test_bad_descriptors_are_refused_on_the_host():
     lib = _native.load()
     good = dict(logits=64, labels=64, rows=4, rows_per_batch=2, batch_stride=10, row_stride=5, vocab=5, dtype=0, n_seq=2)
     assert lib.gefenx_loss_workspace_bytes(ctypes.byref(_native.Logits(**good))) > 0
-    for change in ({"dtype": 3}, {"vocab": 0}, {"rows": -1}, {"rows_per_batch": 0}, {"labels": None}, {"rows": 1 << 31}):
+    for change in ({"dtype": 3}, {"vocab": 0}, {"rows": -1}, {"rows_per_batch": 0}, {"labels": None}, {"rows": 1 << 31}, {"rows": 1 << 30}, {"n_seq": -1}, {"n_seq": 1 << 30}):
         d = _native.Logits(**{**good, **change})
         assert lib.gefenx_loss_workspace_bytes(ctypes.byref(d)) == 0, change
         assert lib.gefenx_token_logps(ctypes.byref(d), 64, 64, 64, 1 << 20, None) == (-2 if "dtype" in change else -1), change
