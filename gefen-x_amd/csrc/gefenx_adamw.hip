@@ -11,6 +11,7 @@
 #include "gefenx.h"
 #include "gefenx_device.h"
 #include "gefenx_internal.h"
+#include "gefenx_run.h"
 
 namespace gx {
 namespace {
