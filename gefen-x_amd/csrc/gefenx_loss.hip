@@ -31,6 +31,7 @@ constexpr int64_t kShortRuns = 768;
 // policy loss on it with zeros in 1 / 2 / 4 / 8: 1650 / 1554 / 1532 / 1573).
 constexpr int64_t kGradPasses = 2, kZeroPasses = 4;
 constexpr int kRowT = 1024;           // threads of a workgroup that keeps a row to itself
+constexpr int kKeptLds = 4, kKeptRegs = 2;  // steps of a row (16 KB) that it keeps on chip
 constexpr int kSeqT = 1024;           // threads of a sequence workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eRest = (float)(1.44269504088896340736 - (double)kLog2e);
@@ -506,46 +507,89 @@ __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* 
     for (; c < end; c += TH) one(c);
 }
 
-// Statistics and gradient of a labelled row in one go, where the coefficient needs no other row: two
-// workgroups a CU hold 512 rows (155 MB of 151936 bf16 logits), which the 256 MB cache still has when
-// they are read again, last part first.  part[row] gets the statistics.
-template <int DT>
-__global__ __launch_bounds__(kRowT) void k_policy_rows(const Rows q, const Token t, const float* __restrict__ weights,
+// Statistics and gradient of a labelled row in one go, where the coefficient needs no other row.  Two
+// workgroups a CU hold 512 rows (155 MB of 151936 bf16 logits), which the 256 MB cache still has when they
+// are read again, last part first.  KEEP: every row of the gradient starts at a multiple of 16 bytes, so
+// both passes cut it into the same runs, and its last steps stay in LDS and registers between them (8192
+// rows of 128256 bf16 logits 898 -> 847 us, of 65536 469 -> 442; two more steps in registers spill: 944).
+// part[row] gets the statistics.
+template <int DT, bool KEEP>
+__global__ __launch_bounds__(kRowT, 2 * kRowT / 256) void k_policy_rows(const Rows q, const Token t, const float* __restrict__ weights,
                                                        const float* __restrict__ scale_dev, float scale,
                                                        float2* __restrict__ part, void* __restrict__ grad) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>;
     __shared__ float2 waves[kRowT / 64];
     __shared__ float coef_of;
+    __shared__ Run<T, W> kept[KEEP ? kKeptLds * kRowT : 1];
     const int64_t r = blockIdx.x, label = sload(q.labels + r);
     if (label == q.ignore) return;
     const T* x = (const T*)q.x + row_offset(q, r);
-    const Soft a = group_join<kRowT>(row_part<DT, kRowT, false>(x, q.vocab, 0, (q.vocab + W - 1) / W, threadIdx.x), waves);
+    const int64_t n = (q.vocab + W - 1) / W, steps = (n + kRowT - 1) / kRowT;
+    // steps of kRowT runs: those before `first` are read twice
+    constexpr int kKept = kKeptLds + kKeptRegs;
+    const int64_t first = KEEP ? (steps > kKept ? steps - kKept : 0) : steps;
+    const auto number = [&](int i) { return (first + i) * kRowT + threadIdx.x; };  // of kept run i
+    Soft a = row_part<DT, kRowT, false>(x, q.vocab, 0, first * kRowT < n ? first * kRowT : n, threadIdx.x);
+    Run<T, W> held[kKeptRegs];
+    if constexpr (KEEP) {
+        // what lies past the row's end reads as -inf
+#pragma unroll
+        for (int i = 0; i < kKeptLds; i += 2) {
+            Run<T, W> v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[j] = load_logits<DT>(x + number(i + j) * W, q.vocab - number(i + j) * W);
+            add_runs<DT, 2>(a, v);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) kept[(i + j) * kRowT + threadIdx.x] = v[j];
+        }
+#pragma unroll
+        for (int i = 0; i < kKeptRegs; ++i)
+            held[i] = load_logits<DT>(x + number(kKeptLds + i) * W, q.vocab - number(kKeptLds + i) * W);
+        add_runs<DT, kKeptRegs>(a, held);
+    }
+    a = group_join<kRowT>(a, waves);
     if (threadIdx.x == 0) {
         part[r] = make_float2(a.m, a.s);
         const int s = seq_of(q, r);
         float coef = 0.0f;
-        if (s >= 0) coef = (scale_dev ? sload(scale_dev) * scale : scale) * policy_token(t, r, s, (float)token_logp<DT>(q, r, label, a)).k * sload(weights + s);
-        if (s >= 0 && (uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+        if (s >= 0) {
+            const float logp = (float)token_logp<DT>(q, r, label, a);
+            coef = (scale_dev ? sload(scale_dev) * scale : scale) * policy_token(t, r, s, logp).k * sload(weights + s);
+            if ((uint64_t)label >= (uint64_t)q.vocab) coef = __uint_as_float(0x7fc00000u);
+        }
         coef_of = coef;
     }
     __syncthreads();
     const float coef = coef_of, each = -coef / a.s;
     T* out = (T*)grad + r * q.vocab;
     const Runs<W> runs(out, q.vocab, sizeof(T));
-    const int64_t n = runs.count();
-    for (int64_t c = (n - 1) / kRowT * kRowT + threadIdx.x; c >= 0; c -= kRowT) {
-        if (c >= n) continue;
-        const int64_t at = runs.begin(c), left = runs.left(c);
-        Run<T, W> v;
+    const auto put = [&](Run<T, W>& v, int64_t c) {
+        const int64_t at = runs.begin(c);
         if (coef == 0.0f) {
 #pragma unroll
             for (int i = 0; i < W; ++i) v.e[i] = T(0);
         } else {
-            v = load_logits<DT>(x + at, left);
             grad_run<DT>(v, at, label, coef, each, a.m);
         }
-        store_run<T, W>(out + at, left, v);
+        store_run<T, W>(out + at, runs.left(c), v);
+    };
+    int64_t c = (runs.count() - 1) / kRowT * kRowT + threadIdx.x;
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = kKeptRegs - 1; i >= 0; --i) put(held[i], number(kKeptLds + i));
+#pragma unroll
+        for (int i = kKeptLds - 1; i >= 0; --i) {
+            Run<T, W> v = kept[i * kRowT + threadIdx.x];
+            put(v, number(i));
+        }
+        c = (first - 1) * kRowT + threadIdx.x;
+    }
+    for (; c >= 0; c -= kRowT) {
+        if (c >= runs.count()) continue;
+        Run<T, W> v;
+        if (coef != 0.0f) v = load_logits<DT>(x + runs.begin(c), runs.left(c));
+        put(v, c);
     }
 }
 
@@ -632,14 +676,14 @@ int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const
     });
 }
 
-// Whether the policy gradient goes row by row.  It reads long rows once instead of twice (1 GiB of bf16
-// logits, a quarter of the rows masked: rows of 128256 416 against 486 us, of 65536 401 against 462, of
-// 32768 434 against 445); short ones leave most of its 1024 lanes idle (16384 587 against 469, 8192 851
-// against 530).  Logits that the 256 MB cache holds are read from there the second time anyway, and few
-// rows are split instead.
+// Whether the policy gradient goes row by row.  It reads long rows from memory once instead of twice (1 GiB
+// of bf16 logits, a quarter of the rows masked: rows of 128256 416 against 486 us, of 65536 401 against
+// 462, of 32768 434 against 445); short ones leave most of its 1024 lanes idle (16384 587 against 469).
+// Logits that the 256 MB cache holds are read from there the second time anyway, and few rows are split
+// instead.
 bool rows_alone(const gefenx_logits& l) {
     const int64_t bytes = l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2);
-    return bytes >= (64 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)256 << 20;
+    return bytes >= (128 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)256 << 20;
 }
 
 int need(const char* what, const Rows& q, const void* ws, size_t bytes) {
@@ -809,8 +853,10 @@ int gefenx_policy_loss_grad(const gefenx_logits* logits, const float* old_logps,
     if (rc != GEFENX_OK) return rc;
     p.q.splits = 1;
     rc = by_dtype(p.dtype, [&](auto dt) {
-        k_policy_rows<decltype(dt)::value><<<(uint32_t)p.q.rows, kRowT, 0, p.s>>>(p.q, p.t, weights, scale_dev, (float)scale, p.part,
-                                                                                  grad);
+        constexpr int DT = decltype(dt)::value;
+        const bool keep = ((uintptr_t)grad & 15) == 0 && p.q.vocab % kW<DT> == 0;
+        const auto kernel = keep ? k_policy_rows<DT, true> : k_policy_rows<DT, false>;
+        kernel<<<(uint32_t)p.q.rows, kRowT, 0, p.s>>>(p.q, p.t, weights, scale_dev, (float)scale, p.part, grad);
         return launched(p.what);
     });
     return rc == GEFENX_OK ? policy_totals(p) : rc;

@@ -510,7 +510,8 @@ def test_positions_past_2_31_elements(dev):
     assert not g[1:-3].any()
 
 
-@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 65541), (torch.float16, 70000), (torch.float32, 33333)])
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 65541), (torch.bfloat16, 65600), (torch.bfloat16, 114696),
+                                     (torch.float16, 70000), (torch.float32, 33333), (torch.float32, 33336)])
 @pytest.mark.parametrize("packed", [False, True])
 def test_long_rows_beyond_the_cache(dev, dtype, V, packed):
     """More than 256 MB of logits in rows of 64 KB and more take statistics and gradient of a row together: against
