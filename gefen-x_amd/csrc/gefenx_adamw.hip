@@ -125,6 +125,7 @@ __device__ __forceinline__ float stepped(const Item& t, float p, float m, float 
 }
 
 // ------------------------------------------------------------ fp32 moments
+// 22 bytes an element (bf16): 218M elements 790-817 us, 5.9-6.1 TB/s, where a copy of 2 GiB reaches 5.8.
 constexpr int kW32 = 4;  // elements of a lane
 template <int DT>
 __global__ __launch_bounds__(kT) void k_adamw(const Batch b, const float* __restrict__ coef) {
@@ -213,7 +214,9 @@ __device__ __forceinline__ float block_scale(float amax) {
 }
 
 // A block of 256 elements by 16 lanes, each with N runs of W of them: the moments stay in registers
-// between the block's maxima and its codes.
+// between the block's maxima and its codes, and the maxima cross lanes within a DPP row.  10.06 bytes an
+// element (bf16): 1.05e9 elements 1.80 ms, 5.9 TB/s; with the exact square root and division the
+// arithmetic takes longer than the memory (218M elements 368 -> 523 us).
 template <int DT, bool FAST>
 __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __restrict__ coef) {
     using T = typename Elem<DT>::T;
@@ -277,7 +280,8 @@ __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __res
     }
 }
 
-// The values that 8-bit moments stand for: Item::p and Item::g are where m's and v's go.
+// The values that 8-bit moments stand for: Item::p and Item::g are where m's and v's go.  Mostly writes:
+// 1.05e9 elements 1.68 ms, 6.3 TB/s.
 __global__ __launch_bounds__(kT) void k_adamw8_values(const Batch b) {
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
@@ -294,7 +298,8 @@ __global__ __launch_bounds__(kT) void k_adamw8_values(const Batch b) {
 }
 
 // ------------------------------------------------------------ gradient norm
-// Sums of squares in float64, one partial per workgroup, added up by one workgroup in a fixed order.
+// Sums of squares in float64, one partial per workgroup, added up by one workgroup in a fixed order.  One
+// read of the gradients: 436 MB 67 us, 6.5 TB/s (a read alone reaches 7.1).
 template <int DT>
 __global__ __launch_bounds__(kT) void k_grad_sumsq(const Batch b, double* __restrict__ partials) {
     using T = typename Elem<DT>::T;

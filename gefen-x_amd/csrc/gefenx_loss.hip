@@ -202,7 +202,8 @@ __device__ __forceinline__ Soft group_join(Soft a, float2* waves) {
 }
 
 // part[row][split] = {maximum, sum of exp(x - maximum)} of a split of a row.  PER rows to a workgroup:
-// one, or one for each of its waves (rows without splits).
+// one, or one for each of its waves (rows without splits).  One pass with the running maximum, corrected
+// once in 32 logits; a read: 9169 rows of 151936 bf16 logits 415 us, 6.7 TB/s (a read alone reaches 7.1).
 template <int DT, int PER>
 __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restrict__ part) {
     using T = typename Elem<DT>::T;
@@ -285,6 +286,7 @@ __device__ __forceinline__ PolicyToken policy_token(const Token& t, int64_t r, i
     return p;
 }
 
+// From the rows' statistics to log-probabilities and sums: waits for a few dependent reads, 4-7 us.
 // One workgroup per sequence (kLogps: per kSeqT / lanes rows), a group of lanes per row.
 template <int DT, int MODE>
 __global__ __launch_bounds__(kSeqT) void k_tokens(const Rows q, const Token t, const float2* __restrict__ part, int lanes,
@@ -453,7 +455,8 @@ __device__ __forceinline__ void grad_run(Run<typename Elem<DT>::T, kW<DT>>& v, i
 }
 
 // grad[r][v] = c_r ([v = y_r] - exp(x - max) / sum), c_r = k[r] * weights[sequence] * scale.
-// unlabelled: only the rows without a label, which get zeros.  PER: as above.
+// unlabelled: only the rows without a label, which get zeros.  PER: as above.  A read and a write: 8192 rows
+// of 128256 bf16 logits, 4998 of them labelled, 580 us, 5.8 TB/s, a copy's rate.
 template <int DT, int PER>
 __global__ __launch_bounds__(kT) void k_logits_grad(const Rows q, const float2* __restrict__ stats, const float* __restrict__ k,
                                                     const float* __restrict__ weights, const float* __restrict__ scale_dev,
