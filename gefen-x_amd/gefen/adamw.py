@@ -210,8 +210,16 @@ class AdamW(torch.optim.Optimizer):
                 "exp_avg_scale": torch.zeros(blocks, dtype=torch.float32, device=dev),
                 "exp_avg_sq_scale": torch.zeros(blocks, dtype=torch.float32, device=dev), "order": _order(p)}
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # a torch.compile'd caller runs it eagerly between its graphs: launches go through ctypes
+        return (self._step_outside_graphs if torch.compiler.is_compiling() else self._step)(closure)
+
+    @torch.compiler.disable
+    def _step_outside_graphs(self, closure):
+        return self._step(closure)
+
+    @torch.no_grad()
+    def _step(self, closure):
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -24,6 +24,7 @@ GradScaler's) multiplies it before it is rounded to the logits' type.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -45,8 +46,8 @@ class PreferenceLoss(NamedTuple):
 
 
 class PolicyLoss(NamedTuple):
-    """loss, mean KL estimate and share of clipped tokens (0-dim), the labels'
-    log-probabilities (0 where ignored)."""
+    """loss, mean KL estimate (0 without ref_logps) and share of clipped tokens
+    (0-dim), the labels' log-probabilities (0 where ignored)."""
     loss: torch.Tensor
     kl: torch.Tensor
     clip_fraction: torch.Tensor
@@ -292,12 +293,24 @@ class _SequenceLoss(torch.autograd.Function):
         return call.grad(saved, k, True, grad), None, None, None, None, None
 
 
+def _outside_graphs(fn):
+    """fn, run eagerly between the graphs of a torch.compile'd caller (its launches go through ctypes)."""
+    eager = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        return (eager if torch.compiler.is_compiling() else fn)(*args, **kwargs)
+    return call
+
+
+@_outside_graphs
 def token_logps(logits, labels, *, ignore_index=-100):
     """log softmax(logits)[label] of every row, fp32 in the labels' shape (0
     where ignored); differentiable in the logits."""
     return _TokenLogps.apply(logits, labels, ignore_index)
 
 
+@_outside_graphs
 def preference_loss(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0, average=False,
                     ignore_index=-100):
     """Preference loss of pairs of sequences, the chosen ones first:
@@ -314,6 +327,7 @@ def preference_loss(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1
     return PreferenceLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of, False))
 
 
+@_outside_graphs
 def preference_loss_and_grad(logits, labels, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0,
                              average=False, ignore_index=-100, grad_scale=1.0):
     """(preference_loss(...), gradient of the loss times grad_scale in the logits)."""
@@ -322,6 +336,7 @@ def preference_loss_and_grad(logits, labels, ref_logps=None, *, cu_seqlens=None,
     return out, call.grad(saved, None, True, grad_scale)
 
 
+@_outside_graphs
 def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2, clip_high=0.2,
                 kl_coef=0.0, reduction="token", ignore_index=-100):
     """Clipped policy loss with a KL term; per labelled token, with q = exp(logp - old_logp), d = ref_logp - logp:
@@ -335,6 +350,7 @@ def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seq
     return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of, True))
 
 
+@_outside_graphs
 def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2,
                          clip_high=0.2, kl_coef=0.0, reduction="token", ignore_index=-100, grad_scale=1.0):
     """(policy_loss(...), gradient of the loss times grad_scale in the logits)."""
