@@ -17,9 +17,9 @@ namespace gx {
 namespace {
 
 constexpr int kT = 256;                  // threads of a workgroup
-constexpr int kItems = 36;               // tensors of a launch: 36 * 100 bytes of kernel arguments
+constexpr int kItems = 36;               // tensors of a launch: 36 * 108 bytes of kernel arguments
 constexpr int kBlock8 = 256;             // elements per scale of the 8-bit moments
-constexpr int kGroup = 16;               // lanes that share such a block, two chunks of 8 elements each
+constexpr int kGroup = 16;               // lanes that share such a block, 16 elements each
 constexpr float kTiny = 0x1p-126f;       // smallest scale: its reciprocal, and 448 of them, are finite
 constexpr int kCode0 = 761;              // bits(x) >> 20 of v's code c is c + 761: code 255 is x = 1
 constexpr int64_t kNormPartials = 4096;  // about so many partial sums of the gradient norm
@@ -36,7 +36,18 @@ struct Item {
     int64_t n;
     uint64_t key;
     float step, wdf, b1, a1, b2, a2, rbc2, eps;
+    const gefenx_adamw_row* row;  // captured steps: where step, wdf, rbc2 and key are
 };
+
+// What of an Item changes from step to step.
+struct Scalars {
+    float step, wdf, rbc2;
+    uint64_t key;
+};
+__device__ __forceinline__ Scalars scalars_of(const Item& t) {
+    if (!t.row) return Scalars{t.step, t.wdf, t.rbc2, t.key};
+    return Scalars{sload(&t.row->step_size), sload(&t.row->wd_factor), sload(&t.row->inv_sqrt_bc2), sload(&t.row->key)};
+}
 
 struct Batch {
     Item it[kItems];
@@ -114,13 +125,13 @@ __device__ __forceinline__ void advance(const Item& t, float g, float& m, float&
 // is under 2^-24 eps for eps >= kFastEps and 1 / sqrt(bc2) up to 2^6.
 constexpr float kFastEps = 1e-10f;
 template <bool FAST>
-__device__ __forceinline__ float stepped(const Item& t, float p, float m, float v) {
+__device__ __forceinline__ float stepped(const Scalars& s, float eps, float p, float m, float v) {
     if constexpr (FAST) {
-        const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v), t.rbc2, t.eps);
-        return __builtin_fmaf(-t.step, m * __builtin_amdgcn_rcpf(d), p * t.wdf);
+        const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v), s.rbc2, eps);
+        return __builtin_fmaf(-s.step, m * __builtin_amdgcn_rcpf(d), p * s.wdf);
     } else {
-        const float d = __builtin_fmaf(__builtin_sqrtf(v), t.rbc2, t.eps);
-        return __builtin_fmaf(-t.step, m / d, p * t.wdf);
+        const float d = __builtin_fmaf(__builtin_sqrtf(v), s.rbc2, eps);
+        return __builtin_fmaf(-s.step, m / d, p * s.wdf);
     }
 }
 
@@ -132,6 +143,7 @@ __global__ __launch_bounds__(kT) void k_adamw(const Batch b, const float* __rest
     using T = typename Elem<DT>::T;
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
+    const Scalars sc = scalars_of(t);
     const float c = coef ? sload(coef) : 1.0f;
     const int64_t at = ((int64_t)local * kT + threadIdx.x) * kW32;
     const int64_t left = t.n - at;
@@ -142,7 +154,7 @@ __global__ __launch_bounds__(kT) void k_adamw(const Batch b, const float* __rest
 #pragma unroll
     for (int k = 0; k < kW32; ++k) {
         advance(t, to_f32<DT>(g.e[k]) * c, m.e[k], v.e[k]);
-        p.e[k] = from_f32<DT>(stepped<false>(t, to_f32<DT>(p.e[k]), m.e[k], v.e[k]));
+        p.e[k] = from_f32<DT>(stepped<false>(sc, t.eps, to_f32<DT>(p.e[k]), m.e[k], v.e[k]));
     }
     store_run<float, kW32>((float*)t.m + at, left, m);
     store_run<float, kW32>((float*)t.v + at, left, v);
@@ -223,6 +235,7 @@ __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __res
     constexpr int W = 16 / sizeof(T), N = kBlock8 / (kGroup * W);
     int local;
     const Item& t = b.it[find_item(b, (int)blockIdx.x, local)];
+    const Scalars sc = scalars_of(t);
     const float c = coef ? sload(coef) : 1.0f;
     const int lane = threadIdx.x & (kGroup - 1);
     const int64_t blk = (int64_t)local * (kT / kGroup) + threadIdx.x / kGroup;
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __res
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             advance(t, to_f32<DT>(g[h].e[k]) * c, m[h][k], v[h][k]);
-            p[h].e[k] = from_f32<DT>(stepped<FAST>(t, to_f32<DT>(p[h].e[k]), m[h][k], v[h][k]));
+            p[h].e[k] = from_f32<DT>(stepped<FAST>(sc, t.eps, to_f32<DT>(p[h].e[k]), m[h][k], v[h][k]));
             const uint32_t mb = __float_as_uint(m[h][k]) & 0x7fffffffu, vb = __float_as_uint(v[h][k]) & 0x7fffffffu;
             mx = mb > mx ? mb : mx;
             vx = vb > vx ? vb : vx;
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(kT) void k_adamw8(const Batch b, const float* __res
 #pragma unroll
         for (int i = 0; i < W / 4; ++i) {
             mc[h][i] = encode_m(m[h] + 4 * i, minv);
-            vc[h][i] = encode_v(v[h] + 4 * i, vinv, t.key, at + 4 * i);
+            vc[h][i] = encode_v(v[h] + 4 * i, vinv, sc.key, at + 4 * i);
         }
         store_codes<W>((uint8_t*)t.m + at, left, mc[h]);
         store_codes<W>((uint8_t*)t.v + at, left, vc[h]);
@@ -346,6 +359,33 @@ __global__ __launch_bounds__(1024) void k_grad_norm(const double* __restrict__ p
     }
 }
 
+// ------------------------------------------------------------ captured steps
+constexpr int kCounters = 56;
+struct Counters {
+    gefenx_adamw_counter c[kCounters];
+    int32_t n;
+};
+static_assert(sizeof(Counters) <= 4080, "kernel arguments");
+
+// One thread a tensor: the step counter goes up by one, and its row gets what the host would have computed
+// from it, in float64 as there.
+__global__ __launch_bounds__(64) void k_adamw_counters(const Counters q) {
+    const int i = threadIdx.x;
+    if (i >= q.n) return;
+    const gefenx_adamw_counter& c = q.c[i];
+    const float t = *gbl(c.step) + 1.0f;
+    *gbl(c.step) = t;
+    const double lr = !c.lr_dev ? c.lr
+                      : c.lr_dtype == GEFENX_F64 ? *gbl((const double*)c.lr_dev) : (double)*gbl((const float*)c.lr_dev);
+    gefenx_adamw_row r;
+    r.step_size = (float)(lr / (1.0 - pow(c.beta1, (double)t)));
+    r.wd_factor = (float)(1.0 - lr * c.weight_decay);
+    r.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(c.beta2, (double)t)));
+    r.reserved = 0;
+    r.key = mix64(c.key0 + 0x9E3779B97F4A7C15ULL * (uint64_t)t);
+    *c.row = r;
+}
+
 // ------------------------------------------------------------ host side
 int launched(const char* what) {
     const hipError_t e = hipGetLastError();
@@ -371,7 +411,7 @@ int validate(const char* what, const gefenx_adamw_desc* d, int n, bool state, bo
 
 Item item_of(const gefenx_adamw_desc& d) {
     return Item{d.p, d.grad, d.exp_avg, d.exp_avg_sq, d.exp_avg_scale, d.exp_avg_sq_scale, d.numel, d.key,
-                d.step_size, d.wd_factor, d.beta1, d.alpha1, d.beta2, d.alpha2, d.inv_sqrt_bc2, d.eps};
+                d.step_size, d.wd_factor, d.beta1, d.alpha1, d.beta2, d.alpha2, d.inv_sqrt_bc2, d.eps, d.row};
 }
 
 // Elements of a workgroup.  One pass each: workgroups start in order, so what is being written at any
@@ -501,6 +541,25 @@ int gefenx_adamw_norm(const gefenx_adamw_desc* descs, int n, double max_norm, fl
     if (rc != GEFENX_OK) return rc;
     k_grad_norm<<<1, 1024, 0, s>>>(static_cast<const double*>(workspace), partials, max_norm, norm_out);
     return launched("gefenx_adamw_norm");
+}
+
+int gefenx_adamw_advance(const gefenx_adamw_counter* counters, int n, void* stream) {
+    const char* what = "gefenx_adamw_advance";
+    if (n < 0 || (n > 0 && !counters)) return set_error(GEFENX_EINVAL, "%s: bad array (n=%d)", what, n);
+    for (int i = 0; i < n; ++i) {
+        if (!counters[i].step || !counters[i].row) return set_error(GEFENX_EINVAL, "%s: tensor %d: null pointer", what, i);
+        if (counters[i].lr_dev && counters[i].lr_dtype != GEFENX_F32 && counters[i].lr_dtype != GEFENX_F64)
+            return set_error(GEFENX_EDTYPE, "%s: tensor %d: unsupported lr dtype %d", what, i, counters[i].lr_dtype);
+    }
+    for (int at = 0; at < n; at += kCounters) {
+        Counters q;
+        q.n = n - at < kCounters ? n - at : kCounters;
+        for (int i = 0; i < q.n; ++i) q.c[i] = counters[at + i];
+        k_adamw_counters<<<1, 64, 0, static_cast<hipStream_t>(stream)>>>(q);
+        const int rc = launched(what);
+        if (rc != GEFENX_OK) return rc;
+    }
+    return GEFENX_OK;
 }
 
 int gefenx_adamw_moments(const gefenx_adamw_desc* descs, int n, void* stream) {

@@ -24,8 +24,10 @@ from gefen.kernels import _native
 
 BLOCK = 256  # elements per scale of the 8-bit moments
 
-_DESC_STRUCT = struct.Struct("<6QqQ8f2i")
+_DESC_STRUCT = struct.Struct("<6QqQ8f2iQ")
+_COUNTER_STRUCT = struct.Struct("<3Q4dQ2i")
 assert _DESC_STRUCT.size == ctypes.sizeof(_native.AdamWDesc)
+assert _COUNTER_STRUCT.size == ctypes.sizeof(_native.AdamWCounter)
 _DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.bfloat16: _native.DT_BF16}
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
 _U64 = (1 << 64) - 1
@@ -46,9 +48,9 @@ def _mix(z: int) -> int:
     return z ^ (z >> 31)
 
 
-def _pack(rows) -> bytes:
+def _pack(rows, form=_DESC_STRUCT) -> bytes:
     """The descriptors of gefenx_adamw_* calls."""
-    return b"".join([_DESC_STRUCT.pack(*row) for row in rows])
+    return b"".join([form.pack(*row) for row in rows])
 
 
 def _order(t: torch.Tensor):
@@ -108,17 +110,21 @@ class AdamW(torch.optim.Optimizer):
     A parameter's elements are stepped in place in the order it is stored in.
     Slices with gaps, and gradients laid out otherwise than their parameter,
     go through a contiguous copy.  Work is enqueued on the current stream; the
-    step does not wait for the GPU and cannot be captured into a graph (the
-    bias corrections are host values).
+    step does not wait for the GPU.  capturable=True: step counters are 0-dim
+    device tensors and a step can be captured into a graph and replayed (each
+    parameter's first step runs eagerly; an lr on the device is read at every
+    replay, one on the host is what it was at capture).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
-                 max_grad_norm=None, seed=0):
+                 max_grad_norm=None, seed=0, capturable=False):
         if max_grad_norm is not None and not (float(max_grad_norm) > 0.0 and math.isfinite(float(max_grad_norm))):
             raise ValueError("max_grad_norm must be positive and finite but is: {!r}".format(max_grad_norm))
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         self.seed = int(seed)
+        self.capturable = bool(capturable)
         self.grad_norm = None
+        self._rows = {}  # capturable: parameter -> device row of what changes from step to step
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
     def add_param_group(self, param_group):
@@ -137,7 +143,8 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
 
     def __getstate__(self):
-        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, seed=self.seed, grad_norm=self.grad_norm)
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, seed=self.seed, grad_norm=self.grad_norm,
+                    capturable=self.capturable, _rows={})
 
     @property
     def _step_supports_amp_scaling(self) -> bool:
@@ -182,6 +189,11 @@ class AdamW(torch.optim.Optimizer):
                 if not p.is_contiguous():
                     _order(p)
                 state = known.get(p)
+                if state and self.capturable:
+                    step = state.get("step")
+                    if not (isinstance(step, torch.Tensor) and step.dtype is torch.float32 and step.numel() == 1
+                            and step.get_device() == p.get_device()):
+                        raise ValueError("AdamW capturable needs the step counter as an fp32 value on {}".format(p.device))
                 if state and not _plainly_fits(p, state, bits):
                     self._check_state(p, state, bits)
                 devices.add(p.get_device())
@@ -213,15 +225,18 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW's 8-bit state follows the storage order of the parameter it was made for "
                                  "({}); this one is stored as {}".format(order, _order(p)))
 
-    @staticmethod
-    def _new_state(p, bits):
+    def _counter(self, p, value):
+        """A step counter: a number, or under capturable a 0-dim device tensor."""
+        return torch.full((), float(value), dtype=torch.float32, device=p.device) if self.capturable else int(value)
+
+    def _new_state(self, p, bits):
         if bits == 32:
             like = p if _dense(p) else p.contiguous()
-            return {"step": 0,
+            return {"step": self._counter(p, 0),
                     "exp_avg": torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format),
                     "exp_avg_sq": torch.zeros_like(like, dtype=torch.float32, memory_format=torch.preserve_format)}
         blocks, dev = -(-p.numel() // BLOCK), p.device
-        return {"step": 0,
+        return {"step": self._counter(p, 0),
                 "exp_avg": torch.zeros(p.numel(), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
                 "exp_avg_sq": torch.zeros(p.numel(), dtype=torch.uint8, device=dev),
                 "exp_avg_scale": torch.zeros(blocks, dtype=torch.float32, device=dev),
@@ -242,29 +257,41 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         found = self._checked()
-        if found and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW.step cannot be captured into a graph: its bias corrections are host values")
+        capturing = bool(found) and torch.cuda.is_current_stream_capturing()
+        if capturing:
+            self._check_capture(found)
         if not _amp_gate(self):
             return loss
         self.grad_norm = None
-        batches = {}  # device -> descriptors, parameters to write back, tensors that the launch reads
+        batches = {}  # device -> descriptors, counters, parameters to write back, tensors that the launch reads
         for group, members in found:
-            lr, (beta1, beta2), bits = float(group["lr"]), group["betas"], group["state_bits"]
-            eps, wdf = float(group["eps"]), 1.0 - lr * float(group["weight_decay"])
-            last = None
+            (beta1, beta2), bits, lr_tensor = group["betas"], group["state_bits"], None
+            eps, decay, last = float(group["eps"]), float(group["weight_decay"]), None
+            if self.capturable:
+                lr, lr_tensor = self._lr_of(group["lr"])
+            else:
+                lr = float(group["lr"])
+            wdf, step_size, rbc2 = 1.0 - lr * decay, 0.0, 0.0
             for index, p, grad, state in members:
                 if not state:
                     state = self.state[p] = self._new_state(p, bits)
-                state["step"] = t = int(state["step"]) + 1
-                if t != last:
-                    step_size, rbc2, last = lr / (1.0 - beta1 ** t), 1.0 / math.sqrt(1.0 - beta2 ** t), t
-                n = p.numel()
-                if n == 0:
-                    continue
                 device = p.get_device()
                 if device not in batches:
-                    batches[device] = ([], [], [])
-                rows, back, held = batches[device]
+                    batches[device] = ([], [], [], [])
+                rows, counters, back, held = batches[device]
+                row, n = 0, p.numel()
+                if self.capturable:
+                    row = self._row_of(p).data_ptr()
+                    counters.append((state["step"].data_ptr(), row, 0 if lr_tensor is None else lr_tensor.data_ptr(), lr, decay,
+                                     beta1, beta2, _mix(self.seed + _GOLDEN * index),
+                                     _native.DT_F64 if lr_tensor is not None and lr_tensor.dtype is torch.float64
+                                     else _native.DT_F32, 0))
+                else:
+                    state["step"] = t = int(state["step"]) + 1
+                    if t != last:
+                        step_size, rbc2, last = lr / (1.0 - beta1 ** t), 1.0 / math.sqrt(1.0 - beta2 ** t), t
+                if n == 0:
+                    continue
                 work, m, v = p, state["exp_avg"], state["exp_avg_sq"]
                 if not (p.is_contiguous() and grad.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
                     work, grad, m, v = self._laid_out(p, grad, state, bits, back)
@@ -272,16 +299,47 @@ class AdamW(torch.optim.Optimizer):
                 key = ms = vs = 0
                 if bits == 8:
                     ms, vs = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
-                    key = _mix(_mix(self.seed + _GOLDEN * index) + _GOLDEN * t)
+                    if not row:
+                        key = _mix(_mix(self.seed + _GOLDEN * index) + _GOLDEN * t)
                 rows.append((work.data_ptr(), grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n, key, step_size, wdf,
-                             beta1, 1.0 - beta1, beta2, 1.0 - beta2, rbc2, eps, _DTYPES[p.dtype], bits))
-        for device, (rows, back, _) in batches.items():
+                             beta1, 1.0 - beta1, beta2, 1.0 - beta2, rbc2, eps, _DTYPES[p.dtype], bits, row))
+        for device, (rows, counters, back, _) in batches.items():
             device = torch.device("cuda", device)
             with _on_device(device):
-                self._launch(device, rows)
+                self._launch(device, rows, counters)
             for p, work in back:
                 p.copy_(work)
         return loss
+
+    def _check_capture(self, found):
+        """What a captured step asks for: everything that it keeps exists, and stays where it is."""
+        if not self.capturable:
+            raise RuntimeError("AdamW.step is captured into a graph with capturable=True only: its bias corrections are "
+                               "host values otherwise")
+        for group, members in found:
+            for _, p, _, state in members:
+                if not state or p not in self._rows:
+                    raise RuntimeError("AdamW capturable: a parameter's first step runs eagerly, before the capture")
+                if group["state_bits"] == 32:
+                    moments, dense = (state["exp_avg"], state["exp_avg_sq"]), _dense(p)
+                    if not all(_dense(m) and _same_layout(m, p) if dense else m.is_contiguous() for m in moments):
+                        raise RuntimeError("AdamW capturable: moments laid out otherwise than their parameter need an eager "
+                                           "step before the capture")
+
+    @staticmethod
+    def _lr_of(lr):
+        """(host value, None), or (0.0, device tensor) where the kernels read it."""
+        if not isinstance(lr, torch.Tensor) or not lr.is_cuda:
+            return float(lr), None
+        if lr.numel() != 1 or lr.dtype not in (torch.float32, torch.float64):
+            raise ValueError("a device lr is one fp32 or fp64 value, got {} of shape {}".format(lr.dtype, tuple(lr.shape)))
+        return 0.0, lr
+
+    def _row_of(self, p):
+        row = self._rows.get(p)
+        if row is None or row.get_device() != p.get_device():
+            row = self._rows[p] = torch.zeros(3, dtype=torch.int64, device=p.device)
+        return row
 
     @staticmethod
     def _laid_out(p, grad, state, bits, back):
@@ -299,10 +357,12 @@ class AdamW(torch.optim.Optimizer):
                     state[name] = torch.empty_like(work, dtype=torch.float32).copy_(state[name])
         return work, grad, state["exp_avg"], state["exp_avg_sq"]
 
-    def _launch(self, device, rows):
+    def _launch(self, device, rows, counters):
         lib = _native.load()
         descs = _pack(rows)
         stream = torch.cuda.current_stream(device).cuda_stream
+        if counters:
+            _native.check(lib.gefenx_adamw_advance(_pack(counters, _COUNTER_STRUCT), len(counters), stream), "AdamW counters")
         coef = None
         if self.max_grad_norm is not None:
             bytes_ = int(lib.gefenx_adamw_norm_workspace_bytes(descs, len(rows)))
@@ -347,7 +407,7 @@ class AdamW(torch.optim.Optimizer):
             if n:
                 batches.setdefault(p.get_device(), []).append(
                     (to_m.data_ptr(), to_v.data_ptr(), m.data_ptr(), v.data_ptr(), state["exp_avg_scale"].data_ptr(),
-                     state["exp_avg_sq_scale"].data_ptr(), n, 0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, _native.DT_F32, 8))
+                     state["exp_avg_sq_scale"].data_ptr(), n, 0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, _native.DT_F32, 8, 0))
         for device, rows in batches.items():
             device = torch.device("cuda", device)
             with _on_device(device):
@@ -375,7 +435,7 @@ class AdamW(torch.optim.Optimizer):
                 entry = state_dict["state"].get(i)
                 if not entry:
                     continue
-                state = {"step": int(entry["step"])}
+                state = {"step": self._counter(p, int(entry["step"]))}
                 for key, dtype in _STATE[bits].items():
                     t = entry.get(key)
                     if not torch.is_tensor(t):

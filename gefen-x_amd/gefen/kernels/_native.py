@@ -93,7 +93,18 @@ class AdamWDesc(ctypes.Structure):
         ("step_size", ctypes.c_float), ("wd_factor", ctypes.c_float),
         ("beta1", ctypes.c_float), ("alpha1", ctypes.c_float), ("beta2", ctypes.c_float), ("alpha2", ctypes.c_float),
         ("inv_sqrt_bc2", ctypes.c_float), ("eps", ctypes.c_float),
-        ("dtype", ctypes.c_int32), ("bits", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("bits", ctypes.c_int32), ("row", ctypes.c_void_p),
+    ]
+
+
+class AdamWCounter(ctypes.Structure):
+    """Mirror of ``gefenx_adamw_counter`` (include/gefenx.h)."""
+
+    _fields_ = [
+        ("step", ctypes.c_void_p), ("row", ctypes.c_void_p), ("lr_dev", ctypes.c_void_p),
+        ("lr", ctypes.c_double), ("weight_decay", ctypes.c_double),
+        ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("key0", ctypes.c_uint64),
+        ("lr_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -168,6 +179,7 @@ SIGNATURES = {
     "gefenx_adamw_step": (_I, [_P, _I, _P, _P]),
     "gefenx_adamw_norm_workspace_bytes": (_SZ, [_P, _I]),
     "gefenx_adamw_norm": (_I, [_P, _I, _D, _P, _P, _SZ, _P]),
+    "gefenx_adamw_advance": (_I, [_P, _I, _P]),
     "gefenx_adamw_moments": (_I, [_P, _I, _P]),
     "gefenx_loss_workspace_bytes": (_SZ, [_P]),
     "gefenx_token_logps": (_I, [_P, _P, _P, _P, _SZ, _P]),

@@ -513,6 +513,12 @@ int gefenx_gemm_nt_bf16(const void* A, const void* B, const void* C, void* D, in
  * Elements are taken in storage order: p, grad and the averages are each numel
  * contiguous elements (at most 2^33), at any alignment of their type.
  * ---------------------------------------------------------------------- */
+/* What changes from step to step, in device memory (gefenx_adamw_advance). */
+typedef struct gefenx_adamw_row {
+    float step_size, wd_factor, inv_sqrt_bc2, reserved;
+    uint64_t key;
+} gefenx_adamw_row;
+
 typedef struct gefenx_adamw_desc {
     void* p;
     const void* grad;
@@ -530,11 +536,29 @@ typedef struct gefenx_adamw_desc {
     float eps;
     int32_t dtype;       /* gefenx_dtype of p and grad */
     int32_t bits;        /* 8 or 32 */
+    const gefenx_adamw_row* row; /* NULL, or a device row read instead of step_size,
+                                  * wd_factor, inv_sqrt_bc2 and key */
 } gefenx_adamw_desc;
 
 /* Step every tensor of descs[n] (read during the call).  grad_coef: NULL, or a
  * device float that the gradients are multiplied by (gefenx_adamw_norm's). */
 int gefenx_adamw_step(const gefenx_adamw_desc* descs, int n, const float* grad_coef, void* stream);
+
+/* The counters of captured steps: *step += 1 (t from here), then
+ *   row = {lr / (1 - beta1^t), 1 - lr * weight_decay, 1 / sqrt(1 - beta2^t), 0,
+ *          SplitMix64's finalizer of key0 + 0x9E3779B97F4A7C15 * t}
+ * in float64, rounded to float.  Enqueues kernels that hold the array's values
+ * (the device values behind its pointers are read when they run). */
+typedef struct gefenx_adamw_counter {
+    float* step;             /* device fp32 0-dim */
+    gefenx_adamw_row* row;   /* device */
+    const void* lr_dev;      /* NULL: lr; else a device 0-dim lr of lr_dtype */
+    double lr, weight_decay, beta1, beta2;
+    uint64_t key0;
+    int32_t lr_dtype;        /* GEFENX_F32 or GEFENX_F64 */
+    int32_t reserved;
+} gefenx_adamw_counter;
+int gefenx_adamw_advance(const gefenx_adamw_counter* counters, int n, void* stream);
 
 /* The 2-norm of all gradients together and the factor that clips them:
  * norm_out (device float[2]) = {norm, min(1, max_norm / (norm + 1e-6))}; sums

@@ -443,6 +443,83 @@ def test_refusals(dev):
             opt.step()
 
 
+def captured(opt, warm):
+    """A graph of opt.step(), after one eager step."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm()
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return graph
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_equal_eager_steps(dev, bits):
+    """A captured step, replayed with other gradients, a device lr that changes and eager work between: the eager
+    run's moments bit for bit (8-bit codes follow the counters' random bits), its parameters but for roundings of the
+    bias corrections (computed in float64 on either side, a unit of fp32 apart at most)."""
+    sizes = [(300,), (40, 33), (1,), (0,), (5000,)] + [(17,)] * 60
+    base = tensors(sizes, torch.float32, 1, dev)
+    base[1] = base[1].t()
+    ps = [[torch.nn.Parameter(t.detach().clone()) for t in base] for _ in range(2)]
+    lr = torch.tensor(1e-2, device=dev, dtype=torch.float64)
+    kw = dict(betas=(B1, B2), weight_decay=WD, state_bits=bits, max_grad_norm=3.0, seed=4)
+    graphed = gefen.AdamW([{"params": ps[0][:2], "lr": lr}, {"params": ps[0][2:], "lr": 5e-3}], capturable=True, **kw)
+    eager = gefen.AdamW([{"params": ps[1][:2], "lr": 1e-2}, {"params": ps[1][2:], "lr": 5e-3}], **kw)
+    grads = [[torch.zeros_like(p) for p in side] for side in ps]
+    for side, g in zip(ps, grads):
+        for p, x in zip(side, g):
+            p.grad = x
+
+    def fill(step):
+        for i, s in enumerate(sizes):
+            x = tensors([s], torch.float32, 100 * step + i, dev)[0]
+            for g in grads:
+                g[i].copy_(x.t() if i == 1 else x)
+    graph = captured(graphed, lambda: fill(0))
+    fill(0)
+    eager.step()
+    for step in range(1, 5):
+        fill(step)
+        lr.fill_(1e-2 * step)
+        eager.param_groups[0]["lr"] = 1e-2 * step
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        _ = (base[0] * 2).sum().item()
+        assert torch.equal(graphed.grad_norm, eager.grad_norm)
+        for a, b in zip(graphed.moments(), eager.moments()):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        for a, b in zip(*ps):
+            assert (a - b).abs().max().item() <= 2.0 ** -22 * (1 + step) if a.numel() else True
+        assert all(float(graphed.state[p]["step"]) == step + 1 for p in ps[0])
+    again = gefen.AdamW([{"params": ps[1][:2]}, {"params": ps[1][2:]}], **kw)
+    again.load_state_dict(graphed.state_dict())
+    assert again.state[ps[1][0]]["step"] == 5
+
+
+def test_captures_that_are_refused(dev):
+    def grab(opt):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.ones(8, device=dev)
+    with pytest.raises(RuntimeError, match="first step"):
+        grab(gefen.AdamW([p], capturable=True))
+    opt = gefen.AdamW([p], capturable=True)
+    opt.step()
+    opt.state[p]["step"] = 1
+    with pytest.raises(ValueError, match="step counter"):
+        opt.step()
+    with pytest.raises(ValueError, match="device lr"):
+        opt = gefen.AdamW([p], lr=torch.tensor(0.1, device=dev, dtype=torch.float16), capturable=True)
+        opt.step()
+
+
 def test_bad_descriptors_are_refused(dev):
     from gefen.kernels import _native
     lib = _native.load()

@@ -486,6 +486,36 @@ def test_runs_repeat_bit_for_bit_and_on_other_streams(dev):
     assert all(torch.equal(a, b) for a, b in zip(first, other)) and torch.equal(g, h)
 
 
+@pytest.mark.parametrize("V,S", [(3001, 20), (131080, 260)])
+def test_captured_losses_replay(dev, V, S):
+    """The fused calls in a graph, replayed on other logits with eager work between, against eager calls; both the
+    split rows and the rows of their own."""
+    n = 4
+    x = torch.zeros(n, S, V, device=dev, dtype=torch.bfloat16)
+    y = torch.randint(0, V, (n, S), device=dev)
+    y[:, :3] = IGNORE
+    old, adv = torch.full((n, S), -8.0, device=dev), torch.randn(n, device=dev)
+
+    def both():
+        return (gefen.preference_loss_and_grad(x, y, old, average=True),
+                gefen.policy_loss_and_grad(x, y, old, adv, old, kl_coef=0.1))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for k in range(3):
+        x.copy_(torch.randn(n, S, V, generator=torch.Generator(dev).manual_seed(k), device=dev))
+        graph.replay()
+        want = both()
+        torch.cuda.synchronize()
+        for (a, ga), (b, gb) in zip(got, want):
+            assert all(torch.equal(i, j) for i, j in zip(a, b)) and torch.equal(ga, gb)
+
+
 def test_positions_past_2_31_elements(dev):
     rows, V = 16500, 131072 + 8
     x = torch.zeros(rows, V, dtype=torch.bfloat16, device=dev)
