@@ -392,9 +392,9 @@ __global__ __launch_bounds__(kT) void k_preference(const SeqSums* __restrict__ s
         const SeqSums c = sums[j], r = sums[pairs + j];
         const double wc = beta / (average && c.n > 0.0 ? c.n : 1.0), wr = beta / (average && r.n > 0.0 ? r.n : 1.0);
         const double h = c.a * wc - r.a * wr;
-        // log s(h) = min(h, 0) - log(1 + e^-|h|)
+        // log s(h) = min(h, 0) - log(1 + e^-|h|); without smoothing h may be +inf
         const double tail = log1p(exp(-fabs(h)));
-        loss += (1.0 - smoothing) * (tail - fmin(h, 0.0)) + smoothing * (tail + fmax(h, 0.0));
+        loss += (1.0 - smoothing) * (tail - fmin(h, 0.0)) + (smoothing > 0.0 ? smoothing * (tail + fmax(h, 0.0)) : 0.0);
         const double k = (1.0 / (1.0 + exp(-h)) - (1.0 - smoothing)) / pairs;
         chosen[j] = (float)(c.a * wc);
         rejected[j] = (float)(r.a * wr);

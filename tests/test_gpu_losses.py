@@ -365,6 +365,21 @@ def test_labels_of_no_weight_and_rows_of_no_value(dev):
     assert torch.isfinite(leaf.grad[0]).all() and leaf.grad[0, 7].item() == 1.0
 
 
+def test_preference_of_impossible_answers(dev):
+    """An answer with a label at -inf: rejected, its pair is won (loss 0, no gradient); chosen, it is lost (loss inf,
+    the gradient that of a lost pair); both sides: NaN."""
+    x = torch.zeros(6, 2, 40, device=dev)
+    y = torch.full((6, 2), 3, dtype=torch.long, device=dev)
+    x[3, 1, 3] = x[1, 0, 3] = -float("inf")
+    out, g = gefen.preference_loss_and_grad(x[[0, 3]].contiguous(), y[:2])
+    assert out.loss.item() == 0.0 and not g.any() and out.rejected_rewards[0].item() == -float("inf")
+    out, g = gefen.preference_loss_and_grad(x[[1, 0]].contiguous(), y[:2], beta=0.5)
+    assert out.loss.item() == float("inf") and torch.isfinite(g).all()
+    assert g[0, 0, 3].item() == -0.5 and abs(g[1, 0, 3].item() - 0.5 * (1 - 1 / 40)) < 1e-6
+    out, g = gefen.preference_loss_and_grad(x[[1, 3]].contiguous(), y[:2])
+    assert torch.isnan(out.loss)
+
+
 def test_labels_out_of_range_make_their_results_nan(dev):
     x = torch.randn(4, 100, device=dev, requires_grad=True)
     y = torch.tensor([100, -1, 1 << 40, 5], device=dev)
