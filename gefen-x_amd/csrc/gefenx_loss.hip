@@ -22,6 +22,10 @@ namespace {
 constexpr int kT = 256;               // threads of a row workgroup
 constexpr int64_t kWantedWgs = 2048;  // row workgroups that fill the chip: 8 on each CU
 constexpr int kLine = 128;            // bytes of a cache line
+// Logits up to so much are read for the statistics by ordinary loads, and the gradient finds what the 256 MB
+// cache still has of them (a quarter of the rows masked, both passes: 205 MB 94.5 -> 88 us, 482 MB 200 ->
+// 191; streamed loads beyond: 2.1 GB 851 against 870).
+constexpr int64_t kCachedBytes = (int64_t)512 << 20;
 constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;  // of a launch
 // Rows of up to so many runs of 16 bytes go to a wave each where there are enough of them: a workgroup is
 // a barrier and more than its share of lanes for them (statistics and gradient of 16384 rows, us: 1000
@@ -49,7 +53,8 @@ struct Rows {
     const int32_t* cu;
     int64_t rows, per_batch, batch_stride, row_stride;
     int64_t vocab, ignore;
-    int32_t n_seq, splits, per;  // per: rows of a workgroup
+    int32_t n_seq, splits;
+    int32_t per, cached;   // rows of a workgroup; whether the statistics' reads are left in the cache
     int64_t split_runs;    // runs of 16 bytes of a split
 };
 
@@ -215,7 +220,8 @@ __global__ __launch_bounds__(kT) void k_row_stats(const Rows q, float2* __restri
     if (r >= q.rows || sload(q.labels + r) == q.ignore) return;
     const int64_t runs = (q.vocab + kW<DT> - 1) / kW<DT>, begin = split * q.split_runs;
     const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
-    Soft a = row_part<DT, TH, true>((const T*)q.x + row_offset(q, r), q.vocab, begin, end, lane);
+    const T* x = (const T*)q.x + row_offset(q, r);
+    Soft a = q.cached ? row_part<DT, TH, false>(x, q.vocab, begin, end, lane) : row_part<DT, TH, true>(x, q.vocab, begin, end, lane);
     if constexpr (PER > 1) wave_join(a);
     else a = group_join<kT>(a, waves);
     if (lane == 0) part[at] = make_float2(a.m, a.s);
@@ -650,6 +656,7 @@ int make_rows(const char* what, const gefenx_logits* l, bool sequences, Rows& q,
     const int64_t line = kLine / 16;
     q.split_runs = ((runs + splits - 1) / splits + line - 1) / line * line;
     q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
+    q.cached = l->rows * l->vocab * size <= kCachedBytes;
     q.per = runs <= kShortRuns && l->rows >= kWantedWgs ? kT / 64 : 1;
     if (q.per > 1) {
         q.splits = 1;
