@@ -702,14 +702,14 @@ int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const
     });
 }
 
-// Whether the policy gradient goes row by row.  It reads long rows from memory once instead of twice (1 GiB
-// of bf16 logits, a quarter of the rows masked: rows of 128256 416 against 486 us, of 65536 401 against
-// 462, of 32768 434 against 445); short ones leave most of its 1024 lanes idle (16384 587 against 469).
-// Logits that the 256 MB cache holds are read from there the second time anyway, and few rows are split
-// instead.
+// Whether the policy gradient goes row by row.  It reads long rows from memory once instead of twice (1.2 GB,
+// few rows masked: bf16 rows of 128256 422 against 485 us, of 65536 411 against 486, fp32 rows
+// of 32768 382 against 488; 1 GiB of bf16 rows of 32768 434 against 445, of 16384, which leave most of its
+// 1024 lanes idle, 587 against 469).  Of fewer logits the cache still has most the second time (bf16 rows of
+// 128256: 300 MB 141 against 125, 400 MB 170 against 167, 520 MB 204 against 216), and few rows are split.
 bool rows_alone(const gefenx_logits& l) {
     const int64_t bytes = l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2);
-    return bytes >= (128 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)256 << 20;
+    return bytes >= (128 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)400 << 20;
 }
 
 int need(const char* what, const Rows& q, const void* ws, size_t bytes) {

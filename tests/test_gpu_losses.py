@@ -501,7 +501,7 @@ def test_runs_repeat_bit_for_bit_and_on_other_streams(dev):
     assert all(torch.equal(a, b) for a, b in zip(first, other)) and torch.equal(g, h)
 
 
-@pytest.mark.parametrize("V,S", [(3001, 20), (131080, 260)])
+@pytest.mark.parametrize("V,S", [(3001, 20), (131080, 420)])
 def test_captured_losses_replay(dev, V, S):
     """The fused calls in a graph, replayed on other logits with eager work between, against eager calls; both the
     split rows and the rows of their own."""
@@ -559,9 +559,9 @@ def test_positions_past_2_31_elements(dev):
                                      (torch.float16, 70000), (torch.float32, 33333), (torch.float32, 33336)])
 @pytest.mark.parametrize("packed", [False, True])
 def test_long_rows_beyond_the_cache(dev, dtype, V, packed):
-    """More than 256 MB of logits in rows of 64 KB and more take statistics and gradient of a row together: against
+    """More than 400 MB of logits in rows of 128 KB and more take statistics and gradient of a row together: against
     the two passes of the autograd form, and a few rows against 64 bits; masked rows, rows outside, odd starts."""
-    n, S = 8, 310
+    n, S = 8, 410
     T = n * S
     gen = torch.Generator(dev).manual_seed(3)
     wide = (torch.randn(T, V + 3, generator=gen, device=dev) * 2).to(dtype)
@@ -604,17 +604,17 @@ def test_long_rows_beyond_the_cache(dev, dtype, V, packed):
 
 
 def test_long_rows_of_bad_values(dev):
-    V = 66000
-    x = torch.randn(2100, V, device=dev).bfloat16()
-    y = torch.randint(0, V, (2100,), device=dev)
+    V, T = 66000, 3300
+    x = torch.randn(T, V, device=dev).bfloat16()
+    y = torch.randint(0, V, (T,), device=dev)
     y[7], y[8], y[9] = V, -1, IGNORE
     x[9] = float("nan")
     x[10, 5] = float("nan")
     x[11, :60000] = -float("inf")
     y[11] = 65000
-    old = torch.full((2100,), -11.0, device=dev)
-    cu = torch.tensor([0, 2100], dtype=torch.int32, device=dev)
-    out, g = gefen.policy_loss_and_grad(x, y, old, torch.ones(2100, device=dev), cu_seqlens=cu, clip_high=1e9)
+    old = torch.full((T,), -11.0, device=dev)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    out, g = gefen.policy_loss_and_grad(x, y, old, torch.ones(T, device=dev), cu_seqlens=cu, clip_high=1e9)
     bad = torch.isnan(g).all(1)
     assert bad.nonzero().view(-1).tolist() == [7, 8, 10] and torch.isnan(out.loss)
     assert not torch.isnan(g[~bad]).any() and not g[9].any() and not g[11, :60000].any() and g[11, 65000] != 0
