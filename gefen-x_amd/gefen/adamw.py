@@ -97,6 +97,16 @@ def _plainly_fits(p, state, bits) -> bool:
             and vs.is_contiguous() and p.is_contiguous() and state.get("order") is None)
 
 
+def _refuse_variants(group):
+    """Options of torch's class, by argument or checkpoint, that would be another formula."""
+    for name in ("amsgrad", "maximize"):
+        if group.get(name):
+            raise ValueError("AdamW has no {} (a parameter group asks for it)".format(name))
+    if not group.get("decoupled_weight_decay", True) and float(group["weight_decay"]) != 0.0:
+        raise ValueError("AdamW decays weights apart from the gradient; a parameter group asks for "
+                         "decoupled_weight_decay=False")
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) over fp32, fp16 or bf16 parameters.
 
@@ -140,6 +150,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("Invalid weight_decay value: {}".format(wd))
         if group["state_bits"] not in _STATE:
             raise ValueError("state_bits must be 8 or 32 but is: {!r}".format(group["state_bits"]))
+        _refuse_variants(group)
         super().add_param_group(param_group)
 
     def __getstate__(self):
@@ -420,8 +431,9 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Loads this class's checkpoints, and torch.optim.AdamW's where
-        state_bits is 32 (fp32 moments from any floating type).  The state is
-        copied; a mismatch is refused before anything changes."""
+        state_bits is 32 (fp32 moments from any floating type; amsgrad and
+        maximize are refused).  The state is copied; a mismatch is refused
+        before anything changes."""
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("loaded state dict has other parameter groups than this optimizer")
@@ -431,6 +443,7 @@ class AdamW(torch.optim.Optimizer):
             widths.append(bits)
             if bits not in _STATE:
                 raise ValueError("state_bits must be 8 or 32 but is: {!r}".format(bits))
+            _refuse_variants(old)
             for p, i in zip(group["params"], old["params"]):
                 entry = state_dict["state"].get(i)
                 if not entry:

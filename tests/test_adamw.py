@@ -125,6 +125,33 @@ def test_torch_checkpoint_loads_and_goes_back():
     back.load_state_dict({"state": opt.state_dict()["state"], "param_groups": theirs.state_dict()["param_groups"]})
 
 
+@pytest.mark.parametrize("kw", [dict(amsgrad=True), dict(maximize=True)])
+def test_variants_of_the_formula_are_refused(kw):
+    a, b = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    a.grad = torch.ones(4)
+    theirs = torch.optim.AdamW([a], **kw)
+    theirs.step()
+    opt = gefen.AdamW([b])
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        opt.load_state_dict(theirs.state_dict())
+    assert not opt.state and not opt.param_groups[0].get(next(iter(kw)))
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        gefen.AdamW([dict(params=[b], **kw)])
+
+
+def test_checkpoint_with_coupled_decay_is_refused():
+    a, b = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    a.grad = torch.ones(4)
+    theirs = torch.optim.Adam([a], weight_decay=0.1)
+    theirs.step()
+    opt = gefen.AdamW([b])
+    with pytest.raises(ValueError, match="decoupled"):
+        opt.load_state_dict(theirs.state_dict())
+    theirs.param_groups[0]["weight_decay"] = 0.0  # the same formula either way
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.state[b]["step"] == 1
+
+
 def test_groups_keep_their_width_where_a_checkpoint_names_none():
     a, b = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(300))
     opt = gefen.AdamW([{"params": [a]}, {"params": [b], "state_bits": 8}])
