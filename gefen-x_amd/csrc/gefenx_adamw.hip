@@ -136,7 +136,7 @@ __device__ __forceinline__ float stepped(const Scalars& s, float eps, float p, f
 }
 
 // ------------------------------------------------------------ fp32 moments
-// 22 bytes an element (bf16): 218M elements 790-817 us, 5.9-6.1 TB/s, where a copy of 2 GiB reaches 5.8.
+// 22 bytes an element (bf16): 218M elements 785-817 us, 5.9-6.1 TB/s, where a copy of 2 GiB reaches 5.8.
 constexpr int kW32 = 4;  // elements of a lane
 template <int DT>
 __global__ __launch_bounds__(kT) void k_adamw(const Batch b, const float* __restrict__ coef) {
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kT) void k_adamw8_values(const Batch b) {
 
 // ------------------------------------------------------------ gradient norm
 // Sums of squares in float64, one partial per workgroup, added up by one workgroup in a fixed order.  One
-// read of the gradients: 436 MB 67 us, 6.5 TB/s (a read alone reaches 7.1).  Ordinary loads, not streamed
+// read of the gradients: 436 MB 67-77 us, 5.7-6.5 TB/s (a read alone reaches 7.1).  Ordinary loads, not streamed
 // ones: the step that follows finds part of them in the 256 MB cache (both 884 -> 851 us, with 8-bit
 // moments 448 -> 421; 92M elements 355 -> 335).
 template <int DT>
