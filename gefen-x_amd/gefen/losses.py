@@ -84,30 +84,46 @@ class _Call:
                 raise ValueError("logits are [sequences, tokens, vocab], or [tokens, vocab] with cu_seqlens, got shape "
                                  "{}".format(tuple(logits.shape)))
             self.n_seq = logits.shape[0]
-        x = logits
-        if x.dim() > 3 or (x.stride(-1) != 1 and self.vocab > 1):
+        x, placed = logits, self._placed(logits)
+        if placed is None:
             x = x.detach().contiguous()
-        # rows r of the leading dims: batches of `per` rows
-        if x.dim() == 3:
-            per, strides = x.shape[1], x.stride()[:2]
-        elif x.dim() == 2:
-            per, strides = x.shape[0], (0, x.stride(0))
-        else:  # one row, or contiguous
-            per, strides = labels.numel(), (0, self.vocab)
+            placed = self._placed(x)
         self.logits, self.labels = x, labels if labels.is_contiguous() else labels.contiguous()
         self.rows = labels.numel()
         self.desc = _native.Logits(
-            x.data_ptr(), self.labels.data_ptr(), None if self.cu is None else self.cu.data_ptr(), self.rows, max(1, per),
-            strides[0], strides[1], self.vocab, int(ignore_index), _DTYPES[x.dtype], self.n_seq)
+            x.data_ptr(), self.labels.data_ptr(), None if self.cu is None else self.cu.data_ptr(), self.rows, *placed,
+            self.vocab, int(ignore_index), _DTYPES[x.dtype], self.n_seq)
         self.ref = ctypes.byref(self.desc)
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
 
+    @staticmethod
+    def _placed(x):
+        """How the rows of logits lie in memory: rows of a batch, batch stride, row stride; None: not so that the
+        kernels read them in place."""
+        if x.stride(-1) != 1 and x.shape[-1] > 1 and x.numel() > 0:
+            return None
+        if x.dim() == 3:
+            return max(1, x.shape[1]), x.stride(0), x.stride(1)
+        if x.dim() == 2:
+            return max(1, x.shape[0]), 0, x.stride(0)
+        if x.dim() > 3 and not x.is_contiguous():
+            return None
+        return max(1, x.numel() // x.shape[-1]), 0, x.shape[-1]
+
     @classmethod
     def again(cls, desc, logits, labels, ignore_index, cu_seqlens=None, sequences=True):
-        """The call of a forward pass for its backward: by its descriptor, where that reads the saved tensors
-        themselves (not copies that are gone, nor tensors that hooks have moved)."""
-        if (desc.logits != logits.data_ptr() or desc.labels != labels.data_ptr()
-                or desc.cu_seqlens != (None if cu_seqlens is None else cu_seqlens.data_ptr())):
+        """The call of a forward pass for its backward: by its descriptor, where that says how the saved tensors lie.
+        An address alone does not: copies that the forward pass made are gone, hooks may have moved the tensors and
+        laid them out anew, and either may have left its address to the other."""
+        fits = (desc.logits == logits.data_ptr() and desc.labels == labels.data_ptr()
+                and desc.dtype == _DTYPES.get(logits.dtype) and desc.vocab == logits.shape[-1]
+                and cls._placed(logits) == (desc.rows_per_batch, desc.batch_stride, desc.row_stride)
+                and desc.rows == labels.numel() and labels.shape == logits.shape[:-1]
+                and labels.dtype is torch.int64 and labels.is_contiguous())
+        if fits and cu_seqlens is not None:
+            fits = (desc.cu_seqlens == cu_seqlens.data_ptr() and cu_seqlens.dtype is torch.int32
+                    and cu_seqlens.is_contiguous() and desc.n_seq == cu_seqlens.numel() - 1)
+        if not fits:
             return cls(logits, labels, ignore_index, cu_seqlens, sequences)
         call = cls.__new__(cls)
         call.desc, call.ref = desc, ctypes.byref(desc)

@@ -484,6 +484,40 @@ def test_backward_of_copies_and_of_moved_tensors(dev):
         out.loss.backward()
 
 
+@pytest.mark.parametrize("offsets", [None, torch.int32, torch.int64])
+@pytest.mark.parametrize("which", ["logps", "preference", "policy"])
+def test_backward_of_moved_views(dev, which, offsets):
+    """Slices of padded logits and of every sequence's rows but the last, and either type of offsets, moved to the host
+    and back between the passes while the memory they came from is free to be taken: the gradient of the plain call."""
+    n, S, V = 4, 33, 1000
+    g = torch.Generator().manual_seed(2)
+    h = torch.randn(n, S + 1, V + 24, generator=g).to(dev)
+    y = torch.randint(0, V, (n, S), generator=g).to(dev)
+    ref, adv = torch.randn(n, S, generator=g).to(dev) - 7, torch.randn(n, generator=g).to(dev)
+    cu = None if offsets is None else torch.arange(0, n * S + 1, S, dtype=offsets, device=dev)
+
+    def loss(leaf):
+        x, args = (leaf * 1.0)[:, :-1, :V], [y, ref]
+        if cu is not None:  # rows of a padded vocabulary, one sequence after another
+            x, args = (leaf[:, :-1] * 1.0).reshape(n * S, V + 24)[:, :V], [y.view(-1), ref.view(-1)]
+        if which == "logps":
+            return (gefen.token_logps(x, args[0]) * args[1]).sum()
+        if which == "preference":
+            return gefen.preference_loss(x, *args, cu_seqlens=cu).loss
+        return gefen.policy_loss(x, *args, adv, args[1], cu_seqlens=cu, kl_coef=0.1).loss
+    got = []
+    for moved in (False, True):
+        leaf = h.clone().requires_grad_(True)
+        if moved:
+            with torch.autograd.graph.save_on_cpu():
+                out = loss(leaf)
+        else:
+            out = loss(leaf)
+        out.backward()
+        got.append(leaf.grad)
+    assert got[0].any() and torch.equal(*got)
+
+
 def test_runs_repeat_bit_for_bit_and_on_other_streams(dev):
     d = Data([200, 300, 250, 280], 3001, torch.bfloat16, dev, packed=True)
     args = (d.logits(), d.row(d.labels), d.row(d.old), d.row(d.adv), d.row(d.ref))

@@ -37,3 +37,41 @@ def test_bad_descriptors_are_refused_on_the_host():
     small = _native.Logits(**good)
     assert lib.gefenx_token_logps(ctypes.byref(small), 64, 64, 64, 8, None) == -1
     assert "workspace" in _native.last_error()
+
+
+@pytest.mark.parametrize("change", ["strides", "batches", "vocabulary", "type", "label strides", "label type", "offset type", "offset count"])
+def test_backward_takes_no_descriptor_by_its_address_alone(change, monkeypatch):
+    """Saved tensors that came back at the addresses of the forward pass's, but laid out otherwise, are described anew
+    (which host tensors refuse); the same ones are not."""
+    import types
+    from gefen import losses
+    from gefen.kernels import _native
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    memory, labels, cu = torch.zeros(4096), torch.zeros(64, dtype=torch.int64), torch.tensor([0, 3, 6], dtype=torch.int32)
+    packed = change.startswith("offset")
+    x, y = (memory.as_strided((6, 8), (12, 1)), labels[:6]) if packed else (memory.as_strided((2, 3, 8), (48, 12, 1)),
+                                                                          labels[:6].view(2, 3))
+    desc = _native.Logits(x.data_ptr(), y.data_ptr(), cu.data_ptr() if packed else None, 6, 6 if packed else 3,
+                          0 if packed else 48, 12, 8, -100, _native.DT_F32, 2)
+    offsets = cu if packed else None
+    assert losses._Call.again(desc, x, y, -100, offsets).desc is desc
+    if change == "strides":
+        x = memory.as_strided((2, 3, 8), (24, 8, 1))
+    elif change == "batches":  # [:, :-1] of four rows, come back without the fourth
+        x = memory.as_strided((2, 3, 8), (36, 12, 1))
+    elif change == "vocabulary":
+        x = memory.as_strided((2, 3, 7), (48, 12, 1))
+    elif change == "type":
+        x = memory.view(torch.bfloat16).as_strided((2, 3, 8), (48, 12, 1))
+    elif change == "label strides":
+        y = labels.as_strided((2, 3), (6, 2))
+    elif change == "label type":
+        y = labels.view(torch.int32)[:6].view(2, 3)
+    elif change == "offset type":
+        offsets = torch.tensor([0, 3, 6])
+        desc.cu_seqlens = offsets.data_ptr()
+    else:
+        offsets = torch.zeros(4, dtype=torch.int32)
+        desc.cu_seqlens = offsets.data_ptr()
+    with pytest.raises(ValueError, match="HIP device"):
+        losses._Call.again(desc, x, y, -100, offsets)
