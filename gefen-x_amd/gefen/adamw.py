@@ -73,6 +73,12 @@ def _dense(t: torch.Tensor) -> bool:
     return t.is_contiguous() or t.numel() == 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
 
 
+def _code_order(p: torch.Tensor):
+    """The order of a parameter's 8-bit moments: that of the memory it is stepped in, which for one with gaps is a
+    contiguous copy (None, as for a contiguous parameter)."""
+    return _order(p) if _dense(p) else None
+
+
 def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two dense tensors of one shape hold their elements in the same order."""
     if a.is_contiguous() and b.is_contiguous():
@@ -232,9 +238,9 @@ class AdamW(torch.optim.Optimizer):
                     key, tuple(t.shape), t.device, tuple(p.shape), p.device))
         if bits == 8:
             order = state.get("order")
-            if not (contiguous and order is None) and order != _order(p):
+            if not (contiguous and order is None) and order != _code_order(p):
                 raise ValueError("AdamW's 8-bit state follows the storage order of the parameter it was made for "
-                                 "({}); this one is stored as {}".format(order, _order(p)))
+                                 "({}); this one is stepped in {}".format(order, _code_order(p)))
 
     def _counter(self, p, value):
         """A step counter: a number, or under capturable a 0-dim device tensor."""
@@ -251,7 +257,7 @@ class AdamW(torch.optim.Optimizer):
                 "exp_avg": torch.zeros(p.numel(), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
                 "exp_avg_sq": torch.zeros(p.numel(), dtype=torch.uint8, device=dev),
                 "exp_avg_scale": torch.zeros(blocks, dtype=torch.float32, device=dev),
-                "exp_avg_sq_scale": torch.zeros(blocks, dtype=torch.float32, device=dev), "order": _order(p)}
+                "exp_avg_sq_scale": torch.zeros(blocks, dtype=torch.float32, device=dev), "order": _code_order(p)}
 
     def step(self, closure=None):
         # a torch.compile'd caller runs it eagerly between its graphs: launches go through ctypes
@@ -392,8 +398,9 @@ class AdamW(torch.optim.Optimizer):
         """[(exp_avg, exp_avg_sq), ...] in fp32 for each parameter (default:
         all, in group order), laid out as the state is: with 32 bits the
         state's own tensors, in the parameter's shape; with 8 the values that
-        the codes stand for, flat, in the order the parameter is stored in.
-        None for a parameter that has not been stepped."""
+        the codes stand for, flat, in the order the parameter is stored in
+        (row by row where it has gaps).  None for a parameter that has not
+        been stepped."""
         bits_of = {p: group["state_bits"] for group in self.param_groups for p in group["params"]}
         got, batches, known = [], {}, self.state
         for p in bits_of if params is None else params:
@@ -460,9 +467,10 @@ class AdamW(torch.optim.Optimizer):
                     moved = raw.to(p.device, copy=True)
                     state[key] = moved.view(torch.float8_e4m3fn) if t.dtype is torch.float8_e4m3fn else moved
                 if bits == 8:
-                    # without an order: in the storage order of the parameter that it is loaded for
-                    order = entry["order"] if "order" in entry else _order(p)
-                    state["order"] = None if order is None else tuple(order)
+                    # without an order: in that of the parameter that it is loaded for
+                    order = entry["order"] if "order" in entry else _code_order(p)
+                    # dims in ascending order: row-major by another name
+                    state["order"] = None if order is None or list(order) == sorted(order) else tuple(order)
                 self._check_state(p, state, bits)
                 new[p] = state
         super().load_state_dict({"state": {}, "param_groups": saved})

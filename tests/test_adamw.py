@@ -111,6 +111,32 @@ def test_checkpoint_of_another_storage_order_is_refused():
     assert opt.state[turned]["order"] == (1, 0)
 
 
+def test_state_of_8_bits_follows_the_memory_that_is_stepped():
+    """A parameter with gaps is stepped in a row-major copy: its state is that of a contiguous parameter, whichever way
+    it is turned, and is not taken for that of a dense turned one."""
+    rows, turned, dense, flat = (torch.nn.Parameter(t) for t in (
+        torch.ones(4, 9)[:, :6], torch.ones(9, 6)[:, :4].t()[:, :6], torch.ones(6, 4).t(), torch.ones(4, 6)))
+    states = {}
+    for p in (rows, turned, dense, flat):
+        opt = gefen.AdamW([p], state_bits=8)
+        states[p] = opt._new_state(p, 8)
+        opt._check_state(p, states[p], 8)
+    assert [states[p]["order"] for p in (rows, turned, dense, flat)] == [None, None, (1, 0), None]
+    for p, fits in ((rows, True), (turned, True), (flat, True), (dense, False)):
+        opt = gefen.AdamW([p], state_bits=8)
+        saved = {"state": {0: states[turned]}, "param_groups": opt.state_dict()["param_groups"]}
+        if fits:
+            opt.load_state_dict(saved)
+            # row-major by its dims, as saved for a parameter with gaps
+            opt.load_state_dict(dict(saved, state={0: dict(states[turned], order=(0, 1))}))
+        else:
+            with pytest.raises(ValueError, match="storage order"):
+                opt.load_state_dict(saved)
+    opt = gefen.AdamW([turned], state_bits=8)
+    with pytest.raises(ValueError, match="storage order"):
+        opt.load_state_dict({"state": {0: states[dense]}, "param_groups": opt.state_dict()["param_groups"]})
+
+
 def test_torch_checkpoint_loads_and_goes_back():
     a = torch.nn.Parameter(torch.ones(5, 3))
     theirs = torch.optim.AdamW([a], lr=0.1)

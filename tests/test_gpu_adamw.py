@@ -174,6 +174,24 @@ def test_gaps_and_gradients_of_another_layout(dev, bits):
     assert torch.equal(c, like[2])
 
 
+def test_moments_of_a_turned_parameter_with_gaps(dev):
+    """Row by row, as a contiguous parameter's, whose checkpoint goes on from there bit for bit."""
+    wide, g = tensors([(40, 100)], torch.float32, 1, dev)[0], tensors([(33, 40)] * 2, torch.float32, 2, dev)
+    turned = torch.nn.Parameter(wide[:, 10:43].t())
+    flat = torch.nn.Parameter(turned.detach().contiguous())
+    opts = [gefen.AdamW([p], state_bits=8) for p in (turned, flat)]
+    for p, o in zip((turned, flat), opts):
+        p.grad = g[0]
+        o.step()
+    assert all(torch.equal(a, b) for a, b in zip(opts[0].moments()[0], opts[1].moments()[0]))
+    opts[1].load_state_dict(opts[0].state_dict())
+    for p, o in zip((turned, flat), opts):
+        p.grad = g[1]
+        o.step()
+    assert torch.equal(turned, flat)
+    assert all(torch.equal(a, b) for a, b in zip(opts[0].moments()[0], opts[1].moments()[0]))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_clipping_by_the_global_norm(dev, dtype, bits):
