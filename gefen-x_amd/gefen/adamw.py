@@ -18,6 +18,7 @@ import math
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from gefen.gefen import _amp_gate, _amp_native_scaling_required, _on_device
 from gefen.kernels import _native
@@ -126,7 +127,9 @@ class AdamW(torch.optim.Optimizer):
     A parameter's elements are stepped in place in the order it is stored in.
     Slices with gaps, and gradients laid out otherwise than their parameter,
     go through a contiguous copy.  Work is enqueued on the current stream; the
-    step does not wait for the GPU.  capturable=True: step counters are 0-dim
+    step does not wait for the GPU.  A backward pass through a graph that has
+    saved a parameter from before the step raises, as after any write in
+    place (a captured step's replays are not seen).  capturable=True: step counters are 0-dim
     device tensors and a step can be captured into a graph and replayed (each
     parameter's first step runs eagerly; an lr on the device is read at every
     replay, one on the host is what it was at capture).
@@ -281,6 +284,7 @@ class AdamW(torch.optim.Optimizer):
             return loss
         self.grad_norm = None
         batches = {}  # device -> descriptors, counters, parameters to write back, tensors that the launch reads
+        stepped = []
         for group, members in found:
             (beta1, beta2), bits, lr_tensor = group["betas"], group["state_bits"], None
             eps, decay, last = float(group["eps"]), float(group["weight_decay"]), None
@@ -309,6 +313,7 @@ class AdamW(torch.optim.Optimizer):
                         step_size, rbc2, last = lr / (1.0 - beta1 ** t), 1.0 / math.sqrt(1.0 - beta2 ** t), t
                 if n == 0:
                     continue
+                stepped.append(p)
                 work, m, v = p, state["exp_avg"], state["exp_avg_sq"]
                 if not (p.is_contiguous() and grad.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
                     work, grad, m, v = self._laid_out(p, grad, state, bits, back)
@@ -320,6 +325,8 @@ class AdamW(torch.optim.Optimizer):
                         key = _mix(_mix(self.seed + _GOLDEN * index) + _GOLDEN * t)
                 rows.append((work.data_ptr(), grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n, key, step_size, wdf,
                              beta1, 1.0 - beta1, beta2, 1.0 - beta2, rbc2, eps, _DTYPES[p.dtype], bits, row))
+        # the kernels write behind autograd's back: a graph that has saved a parameter must not go on with its new values
+        increment_version(stepped)
         for device, (rows, counters, back, _) in batches.items():
             device = torch.device("cuda", device)
             with _on_device(device):

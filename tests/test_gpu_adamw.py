@@ -327,6 +327,28 @@ def test_second_moment_in_8_bits_is_unbiased(dev):
     assert ((v8 / v32 - 1) ** 2).mean().sqrt().item() < 0.5
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_graphs_that_saved_a_parameter_end_with_the_step(dev, bits, capturable):
+    """A second backward pass through weights that were stepped in between raises; through others it does not."""
+    x = torch.ones(5, 8, device=dev, requires_grad=True)
+    w, idle = (torch.nn.Parameter(torch.ones(8, 8, device=dev)) for _ in range(2))
+    turned = torch.nn.Parameter(torch.ones(8, 8, device=dev).t())
+    opt = gefen.AdamW([w, idle, turned], state_bits=bits, capturable=capturable)
+    for p in (w, turned, idle):
+        out = (x @ p).sum()
+        out.backward(retain_graph=True)
+        if p is idle:
+            idle.grad = None
+        opt.step()
+        opt.zero_grad()
+        if p is idle:
+            out.backward()
+        else:
+            with pytest.raises(RuntimeError, match="modified"):
+                out.backward()
+
+
 def test_same_seed_same_run(dev):
     def go(seed):
         p = torch.nn.Parameter(torch.ones(5000, device=dev))
