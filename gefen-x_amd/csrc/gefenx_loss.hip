@@ -401,7 +401,8 @@ __global__ __launch_bounds__(kT) void k_preference(const SeqSums* __restrict__ s
         // log s(h) = min(h, 0) - log(1 + e^-|h|); without smoothing h may be +inf
         const double tail = log1p(exp(-fabs(h)));
         loss += (1.0 - smoothing) * (tail - fmin(h, 0.0)) + (smoothing > 0.0 ? smoothing * (tail + fmax(h, 0.0)) : 0.0);
-        const double k = (1.0 / (1.0 + exp(-h)) - (1.0 - smoothing)) / pairs;
+        // s(h) - (1 - e) as e - s(-h): a won pair's is all in s(-h), which 1 - s(h) would lose
+        const double k = (smoothing - 1.0 / (1.0 + exp(h))) / pairs;
         chosen[j] = (float)(c.a * wc);
         rejected[j] = (float)(r.a * wr);
         weights[j] = (float)(k * wc);

@@ -240,6 +240,34 @@ def test_policy(dev, lengths, V, dtype, packed):
             assert torch.all((g.cpu().double().view(d.T, V) - x.grad).abs() <= tol_g)
 
 
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_preference_of_decided_pairs(dev, smoothing):
+    """Pairs won and lost by far: the gradient of a won one falls off as exp(-h), to the last digit."""
+    hs = [25.0, 33.0, 36.5, 40.0, 60.0, 80.0, -30.0, -60.0]
+    n, S, V = len(hs), 3, 50
+    d = Data([S] * (2 * n), V, torch.float32, dev, packed=False)  # no row is masked: 3 // 5 = 0
+    ref = logps64(d.x64, d.labels).view(2 * n, S)
+    ref[:n] -= torch.tensor(hs, dtype=torch.float64)[:, None] / S
+    ref = ref.float()
+    x = d.x64.clone().requires_grad_(True)
+    loss, reward = preference64(x, d.labels, d.spans, ref.double().view(-1), 1.0, smoothing, False)
+    loss.backward()
+    out, grad = gefen.preference_loss_and_grad(d.logits(), d.row(d.labels), ref.to(dev), beta=1.0, label_smoothing=smoothing)
+    h = (reward[:n] - reward[n:]).detach()
+    assert (h - torch.tensor(hs).double()).abs().max() < 1e-3
+    # s(-h) changes by a share of at most the error of h, the tokens' of both answers
+    tol = logp_tolerance(d.x64, d.labels)
+    dh = (per_sequence(tol, d.spans)[:n] + per_sequence(tol, d.spans)[n:]).repeat(2)[d.seq_of_rows()]
+    k = (torch.sigmoid(-h) - smoothing).abs() / n
+    slip = torch.sigmoid(-h) / n
+    k, slip = (t.repeat(2)[d.seq_of_rows()] for t in (k, slip))
+    p = torch.softmax(d.x64, -1)
+    hot = torch.zeros_like(p).scatter_(1, d.labels[:, None], 1.0)
+    tol_g = grad_tolerance(x.grad, d.x64, d.labels, 8 * U, k, torch.float32) + (slip * dh)[:, None] * (p + hot)
+    assert torch.all((grad.cpu().double().view(d.T, V) - x.grad).abs() <= tol_g)
+    assert abs(out.loss.item() - loss.item()) <= dh.max() + 2 * U * abs(loss.item())
+
+
 def test_gradients_against_differences(dev):
     """Central differences of the 64-bit losses, step 1e-5: third derivatives (below 10 here) leave 1e-9."""
     d = Data([4, 5], 6, torch.float32, dev, packed=False)
