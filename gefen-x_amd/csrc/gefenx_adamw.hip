@@ -121,9 +121,7 @@ __device__ __forceinline__ void advance(const Item& t, float g, float& m, float&
     v = v * t.b2 + g * g * t.a2;
 }
 // FAST: the hardware's square root and reciprocal, 1 unit each, as good as the exact ones before p
-// rounds.  That square root takes v below 2^-126 for 0, which eps has to drown: sqrt(2^-126) / sqrt(bc2)
-// is under 2^-24 eps for eps >= kFastEps and 1 / sqrt(bc2) up to 2^6.
-constexpr float kFastEps = 1e-10f;
+// rounds.  That square root takes v below 2^-126 for 0, which eps has to drown: drowns().
 template <bool FAST>
 __device__ __forceinline__ float stepped(const Scalars& s, float eps, float p, float m, float v) {
     if constexpr (FAST) {
@@ -468,11 +466,15 @@ int64_t norm_partials(const gefenx_adamw_desc* d, int n) {
     return s;
 }
 
+// Whether eps is 2^24 times all that sqrt(v) / sqrt(bc2) can be for v < 2^-126.  bc2 = 1 - b2^t is
+// 1 - b2 at least, so 2^-63 / sqrt(1 - b2) <= 2^-24 eps at every step (eps = 1e-8: b2 up to 1 - 3.3e-8).
+bool drowns(float eps, float alpha2) { return (double)eps * eps * alpha2 >= 0x1p-78; }
+
 template <int DT>
 int step_dtype(const gefenx_adamw_desc* d, int n, const float* coef, hipStream_t s) {
     const auto picks = [](int bits, bool fast) {
         return [=](const gefenx_adamw_desc& t) {
-            return t.dtype == DT && t.bits == bits && (bits == 32 || (t.eps >= kFastEps) == fast);
+            return t.dtype == DT && t.bits == bits && (bits == 32 || drowns(t.eps, t.alpha2) == fast);
         };
     };
     int rc = for_batches(d, n, kWg32, picks(32, false), [&](const Batch& b, int wgs) {

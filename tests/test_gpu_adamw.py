@@ -11,6 +11,7 @@ pytestmark = pytest.mark.gpu
 
 LR, B1, B2, EPS, WD = 1e-2, 0.9, 0.99, 1e-8, 0.1
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+U = 2.0 ** -24
 
 
 @pytest.fixture(scope="module")
@@ -278,6 +279,23 @@ def test_extreme_scales_of_8_bit_blocks(dev):
     # the first step's size is lr wherever the square neither vanishes nor loses bits
     sound = want_v > 1e-30
     assert (p.detach().cpu()[sound] + LR).abs().max() <= LR * 1e-6
+
+
+@pytest.mark.parametrize("eps", [1e-12, 1e-10, 1e-9, 1e-8])
+@pytest.mark.parametrize("beta2", [0.9, 0.9999, 1 - 2.0 ** -23])
+def test_second_moments_below_the_normal_numbers(dev, beta2, eps):
+    """v below 2^-126 where 1 / sqrt(1 - beta2) lifts its root to a share of eps: 8 bits step as the formula says, to 16
+    roundings (fewer than that many operations are in it)."""
+    g = torch.cat([torch.linspace(0.05, 1.0, 256) * 2.0 ** -63 / math.sqrt(1 - beta2), torch.linspace(0.1, 1, 256) * 1e-3])
+    p = torch.nn.Parameter(torch.zeros(512, device=dev))
+    p.grad = g.to(dev)
+    opt = gefen.AdamW([p], lr=LR, betas=(B1, beta2), eps=eps, weight_decay=0.0, state_bits=8)
+    opt.step()
+    m, v = ref.moments32(torch.zeros(512), torch.zeros(512), g, B1, beta2)
+    assert v[:256].max() < 2.0 ** -125 and (v[:256] > 0).all()
+    # from the rounded moments: those of denormal v are no matter of the step
+    want = -LR / (1 - B1) * m.double() / (v.double().sqrt() / math.sqrt(1 - beta2) + eps)
+    assert torch.all((p.detach().cpu().double() - want).abs() <= 16 * U * want.abs())
 
 
 def test_every_float8_code_decodes_and_encodes_as_torch_does(dev):
