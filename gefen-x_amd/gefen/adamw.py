@@ -447,7 +447,31 @@ class AdamW(torch.optim.Optimizer):
         """Loads this class's checkpoints, and torch.optim.AdamW's where
         state_bits is 32 (fp32 moments from any floating type; amsgrad and
         maximize are refused).  The state is copied; a mismatch is refused
-        before anything changes."""
+        before anything changes.  Hooks run as torch's class runs them: what
+        pre-hooks return is loaded, post-hooks find it in place."""
+        new, widths = {}, []
+
+        def take(_, state_dict):  # after every pre-hook
+            got, bits = self._loaded(state_dict)
+            new.update(got)
+            widths.extend(bits)
+            return dict(state_dict, state={})  # torch's class would cast codes
+
+        def install(_):  # before every post-hook
+            for group, bits in zip(self.param_groups, widths):
+                group["state_bits"] = bits
+            self.state.clear()
+            self.state.update(new)
+        handles = [self.register_load_state_dict_pre_hook(take),
+                   self.register_load_state_dict_post_hook(install, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
+
+    def _loaded(self, state_dict):
+        """What a checkpoint holds for this optimizer: ({parameter: state}, width of each group)."""
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("loaded state dict has other parameter groups than this optimizer")
@@ -480,8 +504,4 @@ class AdamW(torch.optim.Optimizer):
                     state["order"] = None if order is None or list(order) == sorted(order) else tuple(order)
                 self._check_state(p, state, bits)
                 new[p] = state
-        super().load_state_dict({"state": {}, "param_groups": saved})
-        for group, bits in zip(self.param_groups, widths):
-            group["state_bits"] = bits
-        self.state.clear()
-        self.state.update(new)
+        return new, widths

@@ -192,6 +192,35 @@ def test_other_groups_are_refused():
         opt.load_state_dict({"state": {}, "param_groups": []})
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hooks_of_loading_see_what_is_loaded(bits):
+    """Pre-hooks get the checkpoint and may replace it, post-hooks find its state in place, none stays behind."""
+    p, opt = one(300, state_bits=bits)
+    entry = state8(300) if bits == 8 else {"step": 7, "exp_avg": torch.rand(300), "exp_avg_sq": torch.rand(300)}
+    saved = {"state": {0: entry}, "param_groups": opt.state_dict()["param_groups"]}
+    seen = []
+
+    def later(optimizer, state_dict):
+        seen.append(state_dict["state"][0]["step"])
+        return dict(state_dict, state={0: dict(state_dict["state"][0], step=9)})
+    opt.register_load_state_dict_pre_hook(later)
+    opt.register_load_state_dict_pre_hook(lambda optimizer, state_dict: seen.append(state_dict["state"][0]["step"]))
+    opt.register_load_state_dict_post_hook(lambda optimizer: seen.append(optimizer.state[p]["step"]), prepend=True)
+    opt.register_load_state_dict_post_hook(lambda optimizer: optimizer.state[p].update(step=10))
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert seen == [7, 9, 9] and opt.state[p]["step"] == 10 and saved["state"][0]["step"] == 7
+        assert opt.param_groups[0]["state_bits"] == bits
+        seen.clear()
+    bad = dict(saved, state={0: dict(entry, exp_avg=torch.zeros(5))})
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+    assert seen == [7, 9] and opt.state[p]["step"] == 10
+    seen.clear()
+    opt.load_state_dict(saved)
+    assert seen == [7, 9, 9]
+
+
 def test_copies_keep_the_options():
     _, opt = one(max_grad_norm=2.0, seed=5)
     for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
