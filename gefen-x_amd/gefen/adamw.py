@@ -20,7 +20,7 @@ import struct
 import torch
 from torch.autograd.graph import increment_version
 
-from gefen.gefen import _amp_gate, _amp_native_scaling_required, _on_device
+from gefen.gefen import _amp_gate, _amp_native_scaling_required, _on_device, _outside_graphs
 from gefen.kernels import _native
 
 BLOCK = 256  # elements per scale of the 8-bit moments
@@ -262,16 +262,9 @@ class AdamW(torch.optim.Optimizer):
                 "exp_avg_scale": torch.zeros(blocks, dtype=torch.float32, device=dev),
                 "exp_avg_sq_scale": torch.zeros(blocks, dtype=torch.float32, device=dev), "order": _code_order(p)}
 
-    def step(self, closure=None):
-        # a torch.compile'd caller runs it eagerly between its graphs: launches go through ctypes
-        return (self._step_outside_graphs if torch.compiler.is_compiling() else self._step)(closure)
-
-    @torch.compiler.disable
-    def _step_outside_graphs(self, closure):
-        return self._step(closure)
-
+    @_outside_graphs
     @torch.no_grad()
-    def _step(self, closure):
+    def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import logging
 import math
 import os
@@ -102,6 +103,17 @@ def _on_device(device):
     if device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def _outside_graphs(fn):
+    """fn, run eagerly between the graphs of a torch.compile'd caller (its launches go through ctypes)."""
+    # as torch.compiler.disable, which imports torch._dynamo at once (0.6 s of an import of this package)
+    eager = getattr(torch, "_disable_dynamo", torch.compiler.disable)(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        return (eager if torch.compiler.is_compiling() else fn)(*args, **kwargs)
+    return call
 
 
 def automatic_partition_view(flat_tensor: torch.Tensor, period: int) -> torch.Tensor:

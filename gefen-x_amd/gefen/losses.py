@@ -24,13 +24,12 @@ GradScaler's) multiplies it before it is rounded to the logits' type.
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from gefen.gefen import _on_device
+from gefen.gefen import _on_device, _outside_graphs
 from gefen.kernels import _native
 
 _DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.bfloat16: _native.DT_BF16}
@@ -307,16 +306,6 @@ class _SequenceLoss(torch.autograd.Function):
         call = _Call.again(ctx.desc, logits, labels, ctx.ignore_index, cu_seqlens)
         k = call.saved_ptrs(saved)[1] if ctx.by_row else None
         return call.grad(saved, k, True, grad), None, None, None, None, None
-
-
-def _outside_graphs(fn):
-    """fn, run eagerly between the graphs of a torch.compile'd caller (its launches go through ctypes)."""
-    eager = torch.compiler.disable(fn)
-
-    @functools.wraps(fn)
-    def call(*args, **kwargs):
-        return (eager if torch.compiler.is_compiling() else fn)(*args, **kwargs)
-    return call
 
 
 @_outside_graphs

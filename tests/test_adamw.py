@@ -1,6 +1,9 @@
 """AdamW's host side: arguments, layouts, checkpoints, and the 8-bit formats' restatement (no GPU)."""
 import copy
+import os
 import pickle
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -225,6 +228,15 @@ def test_copies_keep_the_options():
     _, opt = one(max_grad_norm=2.0, seed=5)
     for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
         assert other.max_grad_norm == 2.0 and other.seed == 5 and other.grad_norm is None
+
+
+def test_import_leaves_the_compiler_alone():
+    """torch._dynamo, an import of half a second, is for callers who compile."""
+    package = os.path.dirname(os.path.dirname(os.path.abspath(gefen.__file__)))
+    code = "import sys, gefen; print('torch._dynamo' in sys.modules)"
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=True,
+                         env=dict(os.environ, PYTHONPATH=package))
+    assert out.stdout.strip() == "False"
 
 
 def test_moments_of_foreign_tensors_are_refused():
