@@ -227,7 +227,31 @@ def _preference_forward(call, ref_logps, beta, smoothing, average):
     return PreferenceLoss(loss, chosen, rejected, logps), saved
 
 
-def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction, grad_scale=None):
+def _advantages(call, advantages, per):
+    """The advantages as the kernels read them, and whether they are one per token."""
+    if per not in (None, "token", "sequence"):
+        raise ValueError("advantages_per must be 'token' or 'sequence' but is: {!r}".format(per))
+    each = isinstance(advantages, torch.Tensor) and advantages.shape == (call.n_seq,)
+    if each and per is None and advantages.shape == call.labels.shape:
+        # packed, with as many rows as sequences: the same either way where each has one row, which only the offsets know
+        if torch.cuda.is_current_stream_capturing() or not torch.equal(
+                call.cu, torch.arange(call.n_seq + 1, dtype=torch.int32, device=call.device)):
+            raise ValueError("advantages of shape {} may be one per token or one per sequence: say which by "
+                             "advantages_per".format(tuple(advantages.shape)))
+        per = "token"
+    if per == "token" or (per is None and not each):
+        adv = call.per_token(advantages, "advantages (one per token or one per sequence)")
+        if adv is None:
+            raise ValueError("policy_loss needs advantages")
+        return adv, 1
+    if not each or advantages.device != call.device or not advantages.is_floating_point():
+        raise ValueError("advantages per sequence must be a floating tensor of shape {} on {}".format(
+            (call.n_seq,), call.device))
+    return advantages.detach().to(torch.float32).contiguous(), 0
+
+
+def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction, advantages_per,
+                    grad_scale=None):
     """The loss and what its gradient needs; with a grad_scale the gradient too."""
     old, ref = call.per_token(old_logps, "old_logps"), call.per_token(ref_logps, "ref_logps")
     if old is None:
@@ -240,13 +264,7 @@ def _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high,
     kl_coef = _finite(kl_coef, "kl_coef")
     if kl_coef and ref is None:
         raise ValueError("kl_coef={} needs ref_logps".format(kl_coef))
-    if (isinstance(advantages, torch.Tensor) and advantages.shape == (call.n_seq,) != call.labels.shape
-            and advantages.device == call.device and advantages.is_floating_point()):
-        adv, per_row = advantages.detach().to(torch.float32).contiguous(), 0
-    else:
-        adv, per_row = call.per_token(advantages, "advantages (one per token or one per sequence)"), 1
-        if adv is None:
-            raise ValueError("policy_loss needs advantages")
+    adv, per_row = _advantages(call, advantages, advantages_per)
     loss, kl, clipped, logps = call.empty(), call.empty(), call.empty(), call.empty(*call.labels.shape)
     saved, (stats, k, weights) = call.saved()
     args = [call.ref, old.data_ptr(), adv.data_ptr(), per_row, _ptr(ref), clip_low, clip_high, kl_coef,
@@ -343,25 +361,28 @@ def preference_loss_and_grad(logits, labels, ref_logps=None, *, cu_seqlens=None,
 
 @_outside_graphs
 def policy_loss(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2, clip_high=0.2,
-                kl_coef=0.0, reduction="token", ignore_index=-100):
+                kl_coef=0.0, reduction="token", advantages_per=None, ignore_index=-100):
     """Clipped policy loss with a KL term; per labelled token, with q = exp(logp - old_logp), d = ref_logp - logp:
 
         -min(q A, clamp(q, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(d) - d - 1)
 
     reduction: "token", the mean over all labelled tokens, or "sequence", the mean over the sequences that have
-    any of their mean; 0 without any.  advantages: one per token, or one per sequence [N]."""
+    any of their mean; 0 without any.  advantages: one per token, or one per sequence [N]; advantages_per ("token" or
+    "sequence") says which where packed logits have as many rows as sequences (left out there, the call waits for
+    cu_seqlens and is refused unless every sequence has one row)."""
     def forward_of(call):
-        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction)[:2]
+        return _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction,
+                               advantages_per)[:2]
     return PolicyLoss(*_SequenceLoss.apply(logits, labels, cu_seqlens, ignore_index, forward_of, True))
 
 
 @_outside_graphs
 def policy_loss_and_grad(logits, labels, old_logps, advantages, ref_logps=None, *, cu_seqlens=None, clip_low=0.2,
-                         clip_high=0.2, kl_coef=0.0, reduction="token", ignore_index=-100, grad_scale=1.0):
+                         clip_high=0.2, kl_coef=0.0, reduction="token", advantages_per=None, ignore_index=-100, grad_scale=1.0):
     """(policy_loss(...), gradient of the loss times grad_scale in the logits)."""
     if grad_scale is None:
         raise ValueError("grad_scale must be a number or one value on the logits' device")
     call = _Call(logits, labels, ignore_index, cu_seqlens)
     out, _, grad = _policy_forward(call, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, reduction,
-                                   grad_scale)
+                                   advantages_per, grad_scale)
     return out, grad

@@ -453,6 +453,34 @@ def test_packed_sequences_with_empty_ones_and_rows_outside(dev):
     assert torch.equal(again.loss, out.loss) and torch.equal(g2, g)
 
 
+def test_advantages_of_as_many_tokens_as_sequences(dev):
+    """Packed logits with a row per sequence on average: what [N] advantages belong to has to be said, unless every
+    sequence has one row."""
+    x, y = torch.randn(3, 50, device=dev), torch.tensor([4, 5, 6], device=dev)
+    old, adv = gefen.token_logps(x, y).detach(), torch.tensor([1.0, -2.0, 4.0], device=dev)
+    for f in (gefen.policy_loss, gefen.policy_loss_and_grad):
+        run = lambda cu, **kw: f(x, y, old, adv, cu_seqlens=torch.tensor(cu, device=dev), **kw)  # noqa: E731, B023
+        loss = lambda out: (out if f is gefen.policy_loss else out[0]).loss.item()  # noqa: E731, B023
+        for cu in ([0, 0, 2, 3], [0, 1, 2, 2]):
+            with pytest.raises(ValueError, match="advantages_per"):
+                run(cu)
+        # ratios are 1: the loss is minus the mean advantage of the tokens
+        assert abs(loss(run([0, 0, 2, 3], advantages_per="token")) + 1.0) < 1e-6
+        assert abs(loss(run([0, 0, 2, 3], advantages_per="sequence")) - 0.0) < 1e-6   # -2, -2, 4
+        for per in (None, "token", "sequence"):
+            assert abs(loss(run([0, 1, 2, 3], advantages_per=per)) + 1.0) < 1e-6
+        with pytest.raises(ValueError, match="advantages_per"):
+            run([0, 1, 2, 3], advantages_per="row")
+        with pytest.raises(ValueError, match="advantages"):  # two sequences, three tokens
+            run([0, 1, 3], advantages_per="sequence")
+        with pytest.raises(ValueError, match="advantages"):
+            f(x, y, old, adv[:2], cu_seqlens=torch.tensor([0, 1, 3], device=dev), advantages_per="token")
+    out, grad = gefen.policy_loss_and_grad(x, y, old, adv, cu_seqlens=torch.tensor([0, 0, 2, 3], device=dev),
+                                           advantages_per="sequence")
+    want, g = gefen.policy_loss_and_grad(x, y, old, adv[[1, 1, 2]], cu_seqlens=torch.tensor([0, 1, 2, 3], device=dev))
+    assert torch.equal(out.loss, want.loss) and torch.equal(grad, g)
+
+
 def test_padded_and_packed_agree(dev):
     d = Data([40, 31, 25, 33], 500, torch.bfloat16, dev, packed=False)
     keep = torch.cat([torch.arange(i * 40, i * 40 + n) for i, n in enumerate([40, 31, 25, 33])])
