@@ -195,7 +195,10 @@ class AdamW(torch.optim.Optimizer):
         be stepped before anything moves."""
         found, devices, index, known = [], set(), 0, self.state
         for group in self.param_groups:
-            bits, members = group["state_bits"], []
+            bits, members, lr_device = group["state_bits"], [], None
+            if self.capturable:
+                _, lr_tensor = self._lr_of(group["lr"])
+                lr_device = None if lr_tensor is None else lr_tensor.get_device()
             for p in group["params"]:
                 index += 1
                 g = p.grad
@@ -208,6 +211,9 @@ class AdamW(torch.optim.Optimizer):
                     self._refuse_grad(p, g)
                 if not p.is_contiguous():
                     _order(p)
+                if lr_device is not None and lr_device != p.get_device():
+                    raise ValueError("a device lr is read by the parameters' kernels: it is on device {}, a parameter on "
+                                     "{}".format(lr_device, p.device))
                 state = known.get(p)
                 if state and self.capturable:
                     step = state.get("step")

@@ -578,6 +578,19 @@ def test_captures_that_are_refused(dev):
         opt.step()
 
 
+def test_a_device_lr_of_another_device_is_refused(dev, monkeypatch):
+    """Before anything moves: its pointer would go to the parameters' kernels."""
+    import types
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.ones(8, device=dev)
+    opt = gefen.AdamW([p], capturable=True)
+    elsewhere = types.SimpleNamespace(get_device=lambda: dev.index + 1, dtype=torch.float32)  # no pointer to follow
+    monkeypatch.setattr(gefen.AdamW, "_lr_of", staticmethod(lambda lr: (0.0, elsewhere)))
+    with pytest.raises(ValueError, match="device lr"):
+        opt.step()
+    assert not opt.state and torch.equal(p.detach(), torch.ones(8, device=dev))
+
+
 def test_bad_descriptors_are_refused(dev):
     from gefen.kernels import _native
     lib = _native.load()
