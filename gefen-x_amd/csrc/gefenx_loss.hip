@@ -708,6 +708,7 @@ int run_tokens(const char* what, const Rows& q, int dtype, const Token& t, const
 // of 32768 382 against 488; 1 GiB of bf16 rows of 32768 434 against 445, of 16384, which leave most of its
 // 1024 lanes idle, 587 against 469).  Of fewer logits the cache still has most the second time (bf16 rows of
 // 128256: 300 MB 141 against 125, 400 MB 170 against 167, 520 MB 204 against 216), and few rows are split.
+// All rows count: how many are masked only the device knows.
 bool rows_alone(const gefenx_logits& l) {
     const int64_t bytes = l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2);
     return bytes >= (128 << 10) && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)400 << 20;

@@ -129,10 +129,13 @@ class AdamW(torch.optim.Optimizer):
     go through a contiguous copy.  Work is enqueued on the current stream; the
     step does not wait for the GPU.  A backward pass through a graph that has
     saved a parameter from before the step raises, as after any write in
-    place (a captured step's replays are not seen).  capturable=True: step counters are 0-dim
-    device tensors and a step can be captured into a graph and replayed (each
-    parameter's first step runs eagerly; an lr on the device is read at every
-    replay, one on the host is what it was at capture).
+    place (a captured step's replays are not seen).
+
+    capturable=True: step counters are 0-dim device tensors and a step can be
+    captured into a graph and replayed (each parameter's first step runs
+    eagerly; an lr on the device, the parameters', is read at every replay, one
+    on the host is what it was at capture).  load_state_dict makes new state:
+    graphs captured before it step the old one and are not to be replayed.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,

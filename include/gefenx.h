@@ -496,7 +496,9 @@ int gefenx_gemm_nt_bf16(const void* A, const void* B, const void* C, void* D, in
 /* ------------------------------------------------------------------------
  * AdamW over many tensors, the exponential averages in fp32 or in 8 bits.  No
  * counterpart in the reference, which leaves AdamW to torch
- * (hybrid.py:546-560).  Per element, in fp32, each operation rounded:
+ * (hybrid.py:546-560).  Per element, in fp32, m and v rounded after each operation, p once from
+ * a term that is within a few units of fp32 (bits == 8: the hardware's square root and quotient where
+ * eps^2 * alpha2 >= 2^-78 makes up for v < 2^-126, which that root takes for 0):
  *   g' = coef * g,  m <- m * beta1 + g' * alpha1,  v <- v * beta2 + g'^2 * alpha2
  *   p  <- D(p * wd_factor - step_size * m / (sqrt(v) * inv_sqrt_bc2 + eps))
  * bits == 32: exp_avg, exp_avg_sq are fp32 [numel], the scales NULL.
