@@ -1,0 +1,1023 @@
+// gefenx_tokens.hip -- statistics of tokens over the logits of a language model, and distillation from a teacher's
+// likeliest tokens, with the gradients of the logits.
+//
+// With z = x / tau, m = max z, S = sum exp(z - m), T = sum (z - m) exp(z - m), q = exp(z - m) / S:
+//   statistics:   log q[y];  entropy H = log S - T / S;  the largest x, ties by the lowest index
+//     d / d z_v = [v = y] g + sum_j [v = i_j] g_j - q_v (g + sum_j g_j + g_H (log q_v + H))
+//   distillation: D = sum_j p_j (log p_j - log q[i_j]), and for the others r (log r - log rho) with
+//     r = 1 - sum p, rho = 1 - sum q[i_j] = R / S, R the sum over the logits outside of the teacher's tokens
+//     d D / d z_v = (P + r) q_v - p_v for the teacher's tokens, q_v (P + r - r / rho) elsewhere
+//     loss = mean over rows of (1 - w) tau^2 D - w log softmax(x)[y]
+// A pass over the logits for the sums, a few numbers per row, and a pass that writes the gradient.
+#include "gefenx_logits.h"
+
+namespace gx {
+namespace {
+
+constexpr int kMaxTop = 128;      // likeliest tokens of a row
+constexpr int kMaxTeacher = 512;  // a teacher's tokens of a row
+constexpr int kMergeKeys = 2048;  // candidates of a row's splits that are merged
+constexpr int kBits = 16384;      // runs of a workgroup's part of a row where some are marked
+constexpr int64_t kTokenGradPasses = 2;
+// Differences from the maximum stop here: exp is 0 from there at any temperature, and 0 times it is 0.
+constexpr float kFar = -1e25f;
+
+// exp(d / tau) = 2^(d (hi + lo)), hi + lo = log2(e) / tau.  lo > 0: -inf times either is -inf.
+struct Heat {
+    float hi, lo, inv;
+    double inv64;
+};
+__device__ __forceinline__ float heat_exp(float d, const Heat& h) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, h.lo, d * h.hi));
+}
+
+// A running maximum m of x and s = sum exp((x - m) / tau); u: sum of (x - m) exp((x - m) / tau), or of exp(x - m).
+// The maximum of nothing is -inf, and -inf logits add 0; NaN and +inf logits make the sums NaN.
+enum { kNone = 0, kEntropy = 1, kPlain = 2 };
+template <int U> struct Sums {
+    float m = -__builtin_inff(), s = 0.0f, u = 0.0f;
+    __device__ __forceinline__ void rebase(float m2, const Heat& h) {
+        if (m2 > m) {
+            const float d = m - m2, f = heat_exp(d, h);
+            if (U == kEntropy) u = f * __builtin_fmaf(s, __builtin_fmaxf(d, kFar), u);
+            if (U == kPlain) u = u * exp_(d);
+            s = s * f;
+            m = m2;
+        }
+    }
+    __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.0f : m; }
+    __device__ __forceinline__ void add(float x, float b, const Heat& h) {
+        const float d = x - b, e = heat_exp(d, h);
+        s += e;
+        if (U == kEntropy) u = __builtin_fmaf(__builtin_fmaxf(d, kFar), e, u);
+        if (U == kPlain) u += exp_(d);
+    }
+    __device__ __forceinline__ void join(float m2, float s2, float u2, const Heat& h) {
+        const float top = m2 > m ? m2 : m;
+        const float b = top == -__builtin_inff() ? 0.0f : top;
+        const float da = m - b, db = m2 - b, fa = heat_exp(da, h), fb = heat_exp(db, h);
+        if (U == kEntropy)
+            u = fa * __builtin_fmaf(s, __builtin_fmaxf(da, kFar), u) + fb * __builtin_fmaf(s2, __builtin_fmaxf(db, kFar), u2);
+        if (U == kPlain) u = u * exp_(da) + u2 * exp_(db);
+        s = s * fa + s2 * fb;
+        m = top;
+    }
+};
+
+template <int U>
+__device__ __forceinline__ void wave_join(Sums<U>& a, const Heat& h, int lanes = 64) {
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor(a.m, off, 64), s2 = __shfl_xor(a.s, off, 64), u2 = __shfl_xor(a.u, off, 64);
+        a.join(m2, s2, u2, h);
+    }
+}
+
+template <int U>
+__device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* waves) {
+    wave_join(a, h);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float4(a.m, a.s, a.u, 0.0f);
+    __syncthreads();
+    a.m = waves[0].x;
+    a.s = waves[0].y;
+    a.u = waves[0].z;
+#pragma unroll
+    for (int w = 1; w < kT / 64; ++w) a.join(waves[w].x, waves[w].y, waves[w].z, h);
+    return a;
+}
+
+template <int DT, int U, int N>
+__device__ __forceinline__ void add_runs(Sums<U>& a, const Run<typename Elem<DT>::T, kW<DT>> (&r)[N], const Heat& h) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int k = 0; k < kW<DT>; ++k) top = __builtin_fmaxf(top, to_f32<DT>(r[c].e[k]));
+    a.rebase(top, h);
+    const float b = a.base();
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int k = 0; k < kW<DT>; ++k) a.add(to_f32<DT>(r[c].e[k]), b, h);
+}
+
+// Runs c .. end - 1 of a row, TH lanes at a time; each lane's sums.  skip(run): a run that is left out.  Which
+// logits a lane adds up does not depend on where the row starts in memory.
+template <int DT, int U, int TH, bool STREAM, class Skip>
+__device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t c, int64_t end, int lane,
+                                            const Heat& h, Skip&& skip) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = kW<DT>;
+    const int64_t whole = end * W <= vocab ? end : end - 1;
+    Sums<U> a;
+    c += lane;
+    const auto put = [&](Run<T, W>& v, int64_t run) {
+        if (skip(run)) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) v.e[k] = DT == F32 ? (T)-__builtin_inff() : (T)(DT == BF16 ? 0xff80 : 0xfc00);
+        }
+    };
+    const auto add = [&](auto load) {
+        for (; c + 3 * TH < whole; c += 4 * TH) {
+            Run<T, W> v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = load(x + (c + i * TH) * W);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(v[i], c + i * TH);
+            add_runs<DT, U, 4>(a, v, h);
+        }
+    };
+    if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT, STREAM>(p); });
+    else add([](const T* p) { return load_logits<DT, STREAM>(p); });
+    for (; c < end; c += TH) {
+        Run<T, W> v[1] = {load_logits<DT, STREAM>(x + c * W, vocab - c * W)};
+        put(v[0], c);
+        add_runs<DT, U, 1>(a, v, h);
+    }
+    return a;
+}
+
+// ------------------------------------------------------------ the likeliest tokens
+// Logits in the order of their values as whole numbers above 0, NaN above all; -0 is 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    x += 0.0f;
+    const uint32_t b = __float_as_uint(x);
+    if (x != x) return 0xffffffffu;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+    if (o == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+// Order and column as one number: of equal logits the lower column is the larger.  0 is no logit.
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t column) { return (uint64_t)order << 32 | (uint32_t)~column; }
+
+struct Select {
+    uint32_t bins[256];
+    uint32_t count, digit, above;
+    uint32_t waves[kT / 64];
+};
+
+// The `top` largest keys of columns first .. last - 1 of a row, in no order, 0 behind them, by digits of 8 bits of
+// the order from the highest: after the last one the order of the top-th largest is known, larger ones are taken as
+// they come, equal ones by column.
+template <int DT>
+__device__ __forceinline__ void select_keys(const typename Elem<DT>::T* x, int64_t first, int64_t last, int top, Select& at,
+                                            uint64_t* __restrict__ out) {
+    const auto order = [&](int64_t v) { return order_of(to_f32<DT>(*gbl(x + v))); };
+    if (last - first <= top) {
+        for (int64_t i = threadIdx.x; i < top; i += kT) out[i] = first + i < last ? key_of(order(first + i), (uint32_t)(first + i)) : 0;
+        return;
+    }
+    uint32_t prefix = 0, mask = 0, want = (uint32_t)top;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        at.bins[threadIdx.x] = 0;
+        at.count = 0;
+        __syncthreads();
+        for (int64_t v = first + threadIdx.x; v < last; v += kT) {
+            const uint32_t o = order(v);
+            if ((o & mask) == prefix) atomicAdd(&at.bins[o >> shift & 255], 1u);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t above = 0, d = 255;
+            while (d > 0 && above + at.bins[d] < want) above += at.bins[d--];
+            at.digit = d;
+            at.above = above;
+        }
+        __syncthreads();
+        want -= at.above;
+        prefix |= at.digit << shift;
+        mask |= 255u << shift;
+    }
+    for (int64_t v = first + threadIdx.x; v < last; v += kT) {
+        const uint32_t o = order(v);
+        if (o > prefix) out[atomicAdd(&at.count, 1u)] = key_of(o, (uint32_t)v);
+    }
+    uint32_t taken = 0;
+    for (int64_t begin = first; taken < want && begin < last; begin += kT) {
+        const int64_t v = begin + threadIdx.x;
+        const bool equal = v < last && order(v) == prefix;
+        const uint64_t who = __ballot(equal);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) at.waves[threadIdx.x >> 6] = (uint32_t)__popcll(who);
+        __syncthreads();
+        uint32_t before = taken + (uint32_t)__popcll(who & (((uint64_t)1 << (threadIdx.x & 63)) - 1));
+        for (int w = 0; w < kT / 64; ++w) {
+            if (w < (int)(threadIdx.x >> 6)) before += at.waves[w];
+            taken += at.waves[w];
+        }
+        if (equal && before < want) out[top - want + before] = key_of(prefix, (uint32_t)v);
+    }
+}
+
+// part[row][split] = the sums of a split of a row, keys[row][split][top] its largest.  PER rows to a workgroup: one,
+// or one for each of its waves (rows without splits, no keys).
+template <int DT, int PER>
+__global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, float4* __restrict__ part,
+                                                   uint64_t* __restrict__ keys) {
+    using T = typename Elem<DT>::T;
+    constexpr int TH = kT / PER, W = kW<DT>;
+    __shared__ float4 waves[kT / 64];
+    __shared__ Select select;
+    const int lane = threadIdx.x % TH;
+    const int64_t at = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
+    const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
+    if (r >= q.rows || (q.labels && sload(q.labels + r) == q.ignore)) return;
+    const int64_t runs = (q.vocab + W - 1) / W, begin = split * q.split_runs;
+    const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const auto none = [](int64_t) { return false; };
+    Sums<kEntropy> a = q.cached || top ? row_sums<DT, kEntropy, TH, false>(x, q.vocab, begin, end, lane, h, none)
+                                       : row_sums<DT, kEntropy, TH, true>(x, q.vocab, begin, end, lane, h, none);
+    if constexpr (PER > 1) wave_join(a, h);
+    else a = group_join(a, h, waves);
+    if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
+    if constexpr (PER == 1) {
+        if (top) {
+            const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
+            select_keys<DT>(x, first, last, top, select, keys + at * top);
+        }
+    }
+}
+
+struct Statistics {
+    float *logps, *entropy, *top_logps;
+    int64_t* top_ids;
+    float4* stats;  // {maximum, sum, log of the sum, entropy}
+};
+
+// What the rows' sums and keys come to: a workgroup per row with keys, else a group of lanes per row.
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat h, int top, const Statistics out,
+                                                        const float4* __restrict__ part, const uint64_t* __restrict__ keys,
+                                                        int lanes) {
+    using T = typename Elem<DT>::T;
+    __shared__ uint64_t all[TOP ? kMergeKeys : 1];
+    __shared__ double base;
+    const int lane = TOP ? threadIdx.x : threadIdx.x % lanes;
+    const int64_t r = TOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kT / lanes) + threadIdx.x / lanes;
+    if (r >= q.rows) return;
+    const int64_t label = q.labels ? *gbl(q.labels + r) : 0;
+    const bool counts = !q.labels || label != q.ignore;
+    if (!counts) {
+        if (lane == 0) {
+            if (out.logps) out.logps[r] = 0.0f;
+            out.entropy[r] = 0.0f;
+            out.stats[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+        }
+        if (TOP && lane < top) {
+            out.top_ids[r * top + lane] = 0;
+            out.top_logps[r * top + lane] = -__builtin_inff();
+        }
+        return;
+    }
+    if (!TOP || threadIdx.x < 64) {
+        Sums<kEntropy> a;
+        for (int i = lane; i < q.splits; i += TOP ? 64 : lanes) {
+            const float4 p = part[r * q.splits + i];
+            a.join(p.x, p.y, p.z, h);
+        }
+        wave_join(a, h, TOP ? 64 : lanes);
+        const double log_sum = log((double)a.s), lse = (double)a.m * h.inv64 + log_sum;
+        const float entropy = (float)(log_sum - (double)a.u / (double)a.s * h.inv64);
+        if (lane == 0) {
+            if (out.logps) {
+                const bool in = label >= 0 && label < q.vocab;
+                const float xl = in ? to_f32<DT>(*gbl((const T*)q.x + row_offset(q, r) + label)) : 0.0f;
+                out.logps[r] = in ? (float)(((double)xl - (double)a.m) * h.inv64 - log_sum) : __uint_as_float(0x7fc00000u);
+            }
+            out.entropy[r] = entropy;
+            out.stats[r] = make_float4(a.m, a.s, (float)log_sum, entropy);
+            if (TOP) base = lse;
+        }
+    }
+    if constexpr (TOP) {
+        const int n = q.splits * top;
+        for (int i = threadIdx.x; i < n; i += kT) all[i] = keys[r * n + i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kT) {
+            const uint64_t key = all[i];
+            if (key == 0) continue;
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += all[j] > key ? 1 : 0;
+            if (rank < top) {
+                out.top_ids[r * top + rank] = (int64_t)(uint32_t)~(uint32_t)key;
+                out.top_logps[r * top + rank] = (float)((double)value_of((uint32_t)(key >> 32)) * h.inv64 - base);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ distillation: a row's loss
+struct Teacher {
+    const void* ids;
+    const float* logps;
+    int32_t top, ids64, rest;
+    float soft;      // (1 - w) tau: of d loss / d x against d D / d z
+    double loss;     // (1 - w) tau^2
+    double hard;     // w
+};
+enum { kBucket = 0, kDrop = 1, kNormalize = 2 };
+
+__device__ __forceinline__ int64_t teacher_id(const Teacher& t, int64_t i) {
+    return t.ids64 ? *gbl((const int64_t*)t.ids + i) : (int64_t)*gbl((const int32_t*)t.ids + i);
+}
+
+// What the gradient of a row needs but for its weight: e^((x - other_m) / tau) other, of the teacher's tokens
+// e^((x - m) / tau) mine - soft p, and e^(x - m) plain; p = exp(log p - log_mass).
+struct Slope {
+    float m, other_m, mine, other, plain, log_mass, unused[2];
+};
+
+// part[row][split]: the sums of a split of a row; BUCKET: without the runs that hold a token of the teacher.
+template <int DT, int U, bool BUCKET, int PER>
+__global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, const Teacher t, float4* __restrict__ part) {
+    using T = typename Elem<DT>::T;
+    constexpr int TH = kT / PER, W = kW<DT>;
+    __shared__ float4 waves[kT / 64];
+    __shared__ uint32_t marks[BUCKET ? (PER > 1 ? PER * ((int)kShortRuns / 32 + 1) : kBits / 32) : 1];
+    const int lane = threadIdx.x % TH, wave = PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
+    const int64_t at = (int64_t)blockIdx.x * PER + wave;
+    const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
+    const bool counts = r < q.rows && sload(q.labels + r) != q.ignore;
+    if (PER == 1 && !counts) return;
+    const int64_t runs = (q.vocab + W - 1) / W, begin = split * q.split_runs;
+    const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
+    uint32_t* mine = marks + (PER > 1 ? wave * ((int)kShortRuns / 32 + 1) : 0);
+    if constexpr (BUCKET) {
+        for (int i = lane; i < (int)((end - begin + 31) / 32); i += TH) mine[i] = 0;
+        __syncthreads();
+        if (counts)
+            for (int j = lane; j < t.top; j += TH) {
+                const int64_t id = teacher_id(t, r * t.top + j);
+                const int64_t run = id >= 0 && id < q.vocab ? id / W : -1;
+                if (run >= begin && run < end && *gbl(t.logps + r * t.top + j) != -__builtin_inff())
+                    atomicOr(&mine[(run - begin) >> 5], 1u << ((run - begin) & 31));
+            }
+        __syncthreads();
+    }
+    if (!counts) return;
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const auto skip = [&](int64_t run) { return BUCKET && (mine[(run - begin) >> 5] >> ((run - begin) & 31) & 1); };
+    Sums<U> a = q.cached ? row_sums<DT, U, TH, false>(x, q.vocab, begin, end, lane, h, skip)
+                         : row_sums<DT, U, TH, true>(x, q.vocab, begin, end, lane, h, skip);
+    if constexpr (PER > 1) wave_join(a, h);
+    else a = group_join(a, h, waves);
+    if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
+}
+
+// From a row's sums to its loss and slope, a wave per row, in float64: the divergence is what is left of terms that
+// cancel.  BUCKET: the runs with tokens of the teacher are added up here, the others apart from the teacher's.
+template <int DT, int U, bool BUCKET>
+__global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h, const Teacher t, const float4* __restrict__ part,
+                                                     double2* __restrict__ each, float* __restrict__ divergence,
+                                                     Slope* __restrict__ slopes) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = kW<DT>;
+    __shared__ int32_t ids[kMaxTeacher];
+    const int64_t r = blockIdx.x, label = sload(q.labels + r);
+    const int lane = threadIdx.x;
+    if (label == q.ignore || (q.n_seq > 0 && seq_of(q, r) < 0)) {
+        if (lane == 0) {
+            each[r] = make_double2(0.0, 0.0);
+            divergence[r] = 0.0f;
+        }
+        return;
+    }
+    const T* x = (const T*)q.x + row_offset(q, r);
+    // mass and sum of p (log p - z) over the teacher's tokens; one outside of the vocabulary makes the row NaN
+    double mass = 0.0, cross = 0.0;
+    for (int j = lane; j < t.top; j += 64) {
+        const int64_t id = teacher_id(t, r * t.top + j);
+        const float lp = *gbl(t.logps + r * t.top + j);
+        const bool held = lp != -__builtin_inff(), in = id >= 0 && id < q.vocab;
+        ids[j] = held && in ? (int32_t)id : -1;
+        if (!held) continue;
+        const double p = in ? exp((double)lp) : __longlong_as_double(0x7ff8000000000000ll);
+        mass += p;
+        if (p > 0.0) cross += p * ((double)lp - (in ? (double)to_f32<DT>(*gbl(x + id)) * h.inv64 : 0.0));
+    }
+    __syncthreads();
+    mass = wave_allsum_d(mass);
+    cross = wave_allsum_d(cross);
+    double log_mass = 0.0;
+    if (t.rest == kNormalize) {
+        // the same sum with p / mass: log p - log mass
+        const bool some = !(mass <= 0.0);
+        log_mass = some ? log(mass) : 0.0;
+        cross = some ? cross / mass - log_mass : 0.0;
+        mass = some ? mass / mass : 0.0;
+    }
+    Sums<U> a;
+    for (int i = lane; i < q.splits; i += 64) {
+        const float4 p = part[r * q.splits + i];
+        a.join(p.x, p.y, p.z, h);
+    }
+    Sums<U> known;
+    if constexpr (BUCKET) {
+        for (int j = lane; j < t.top; j += 64) {
+            const int32_t id = ids[j];
+            if (id < 0) continue;
+            bool first = true, first_run = true;
+            for (int i = 0; i < j; ++i) {
+                first &= ids[i] != id;
+                first_run &= ids[i] < 0 || ids[i] / W != id / W;
+            }
+            if (first) {
+                const float v = to_f32<DT>(*gbl(x + id));
+                known.rebase(v, h);
+                known.add(v, known.base(), h);
+            }
+            if (!first_run) continue;
+            const int32_t start = id / W * W;
+            uint32_t taken = 0;
+            for (int i = 0; i < t.top; ++i) {
+                const uint32_t off = (uint32_t)(ids[i] - start);
+                if (ids[i] >= 0 && off < (uint32_t)W) taken |= 1u << off;
+            }
+            for (int k = 0; k < W; ++k) {
+                if (taken >> k & 1 || start + k >= q.vocab) continue;
+                const float v = to_f32<DT>(*gbl(x + start + k));
+                a.rebase(v, h);
+                a.add(v, a.base(), h);
+            }
+        }
+        wave_join(known, h);
+    }
+    wave_join(a, h);
+    Sums<U> total = a;
+    if constexpr (BUCKET) total.join(known.m, known.s, known.u, h);
+    if (lane != 0) return;
+    const double sum = (double)total.s, log_sum = log(sum), m = (double)total.m;
+    double d = cross + mass * (m * h.inv64 + log_sum), rest = 0.0, other = 0.0;
+    Slope s = {};
+    if constexpr (BUCKET) {
+        if (mass < 1.0 && a.s != 0.0f) {
+            rest = 1.0 - mass;
+            // the teacher's tokens against the others, the log of 1 / rho - 1
+            const double odds = log((double)known.s / (double)a.s) + ((double)known.m - (double)a.m) * h.inv64;
+            d += rest * (log1p(-mass) + (odds > 50.0 ? odds : log1p(exp(odds))));
+            other = rest / (double)a.s;
+        }
+    }
+    const double whole = mass + rest;
+    const bool apart = BUCKET && a.s != 0.0f;
+    const double shift = apart ? exp(((double)a.m - m) * h.inv64) : 1.0;
+    double mine = t.soft * whole / sum, others = t.soft * (whole / sum * shift - other), plain = 0.0, nll = 0.0;
+    if (t.hard > 0.0) {
+        const double sum1 = U == kPlain ? (double)total.u : sum;
+        const bool in = label >= 0 && label < q.vocab;
+        nll = in ? log(sum1) - ((double)to_f32<DT>(*gbl(x + label)) - m) : __longlong_as_double(0x7ff8000000000000ll);
+        if (U == kPlain) {
+            plain = t.hard / sum1;
+        } else {
+            mine += t.hard / sum;
+            others += t.hard / sum * shift;
+        }
+        if (!in) mine = others = nll;
+    }
+    each[r] = make_double2(d, nll);
+    divergence[r] = (float)d;
+    s.m = total.m;
+    s.other_m = apart ? a.m : total.m;
+    s.mine = (float)mine;
+    s.other = (float)others;
+    s.plain = (float)plain;
+    s.log_mass = (float)log_mass;
+    slopes[r] = s;
+}
+
+struct DistillSums {
+    double divergence, nll, n;
+};
+
+// One workgroup per sequence, or one for all rows where there are none.
+__global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const double2* __restrict__ each, DistillSums* __restrict__ sums) {
+    __shared__ DistillSums waves[kSeqT / 64];
+    int64_t begin = 0, end = q.rows;
+    if (q.n_seq > 0) {
+        begin = q.cu ? (int64_t)sload(q.cu + blockIdx.x) : (int64_t)blockIdx.x * q.per_batch;
+        end = q.cu ? (int64_t)sload(q.cu + blockIdx.x + 1) : begin + q.per_batch;
+    }
+    begin = begin < 0 ? 0 : begin;
+    end = end > q.rows ? q.rows : end;
+    DistillSums own = {0.0, 0.0, 0.0};
+    for (int64_t r = begin + threadIdx.x; r < end; r += kSeqT) {
+        if (*gbl(q.labels + r) == q.ignore) continue;
+        const double2 e = each[r];
+        own.divergence += e.x;
+        own.nll += e.y;
+        own.n += 1.0;
+    }
+    own.divergence = wave_sum_d(own.divergence);
+    own.nll = wave_sum_d(own.nll);
+    own.n = wave_sum_d(own.n);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = own;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kSeqT / 64; ++w) {
+            own.divergence += waves[w].divergence;
+            own.nll += waves[w].nll;
+            own.n += waves[w].n;
+        }
+        sums[blockIdx.x] = own;
+    }
+}
+
+// Loss, means of both parts, weights per sequence.
+__global__ __launch_bounds__(kT) void k_distill_total(const DistillSums* __restrict__ sums, int n_seq, int by_sequence, const Teacher t,
+                                                      float* __restrict__ loss_out, float* __restrict__ divergence_out,
+                                                      float* __restrict__ nll_out, float* __restrict__ weights) {
+    __shared__ double waves[kT / 64];
+    double n = 0.0, seqs = 0.0;
+    for (int i = threadIdx.x; i < n_seq; i += kT) {
+        n += sums[i].n;
+        seqs += sums[i].n > 0.0 ? 1.0 : 0.0;
+    }
+    n = block_sum(n, waves);
+    seqs = block_sum(seqs, waves);
+    double divergence = 0.0, nll = 0.0;
+    for (int i = threadIdx.x; i < n_seq; i += kT) {
+        const double w = sums[i].n > 0.0 ? (by_sequence ? 1.0 / (sums[i].n * seqs) : 1.0 / n) : 0.0;
+        if (w > 0.0) {
+            divergence += sums[i].divergence * w;
+            nll += sums[i].nll * w;
+        }
+        weights[i] = (float)w;
+    }
+    divergence = block_sum(divergence, waves);
+    nll = block_sum(nll, waves);
+    if (threadIdx.x == 0) {
+        // a part of weight 0 is not there, whatever it would be
+        *loss_out = (float)((t.loss != 0.0 ? t.loss * divergence : 0.0) + (t.hard != 0.0 ? t.hard * nll : 0.0));
+        *divergence_out = (float)divergence;
+        *nll_out = (float)nll;
+    }
+}
+
+// ------------------------------------------------------------ gradients
+struct Upstream {                // what the statistics' gradient takes
+    const float4* stats;
+    const float *logps, *entropy, *top;  // gradients; each may be null
+    const int64_t* ids;
+    int32_t top_n;
+};
+struct Downhill {                // what the distillation's takes
+    const Slope* slopes;
+    const float *weights, *scale_dev;
+    float scale;
+    Teacher t;
+};
+
+// A row's gradient: an element by its logit, and what is added at some columns.
+struct StatisticsGrad {
+    Upstream g;
+    __device__ __forceinline__ int entries() const { return g.top ? g.top_n : 0; }
+    struct Row {
+        float m, log_sum, entropy, all, slope, label_extra, inv_sum;
+        const float* top;
+        const int64_t* ids;
+        bool zero;
+    };
+    __device__ __forceinline__ Row row(const Rows& q, const Heat& h, int64_t r, int64_t label, int lane) const {
+        Row o;
+        const float4* s = g.stats + r;
+        o.m = sload(&s->x);
+        o.inv_sum = 1.0f / sload(&s->y);
+        o.log_sum = sload(&s->z);
+        o.entropy = sload(&s->w);
+        o.top = g.top ? g.top + r * g.top_n : nullptr;
+        o.ids = g.ids + r * g.top_n;
+        const float up = g.logps ? sload(g.logps + r) * h.inv : 0.0f;
+        float sum = 0.0f;
+        if (g.top) {
+            for (int j = lane; j < g.top_n; j += 64) sum += *gbl(o.top + j);
+            sum = wave_sum(sum);
+        }
+        o.label_extra = up;
+        o.all = -(up + sum * h.inv);
+        o.slope = g.entropy ? -sload(g.entropy + r) * h.inv : 0.0f;
+        if (g.logps && (uint64_t)label >= (uint64_t)q.vocab) o.all = __uint_as_float(0x7fc00000u);
+        o.zero = false;
+        return o;
+    }
+    __device__ __forceinline__ float at(const Row& o, const Heat& h, float x, bool) const {
+        const float d = x - o.m, p = heat_exp(d, h) * o.inv_sum;
+        const float logq = __builtin_fmaxf(d, kFar) * h.inv - o.log_sum;
+        return p * __builtin_fmaf(o.slope, logq + o.entropy, o.all);
+    }
+    __device__ __forceinline__ bool entry(const Row& o, const Rows& q, const Heat& h, int j, int64_t& id, float& extra) const {
+        id = *gbl(o.ids + j);
+        extra = *gbl(o.top + j) * h.inv;
+        return (uint64_t)id < (uint64_t)q.vocab;
+    }
+};
+
+template <bool PLAIN>
+struct DistillGrad {
+    Downhill g;
+    __device__ __forceinline__ int entries() const { return g.t.top; }
+    struct Row {
+        float m, other_m, mine, other, plain, log_mass, label_extra, soft;
+        int64_t first;
+        bool zero;
+    };
+    __device__ __forceinline__ Row row(const Rows& q, const Heat&, int64_t r, int64_t, int) const {
+        Row o;
+        float w = g.scale_dev ? sload(g.scale_dev) * g.scale : g.scale;
+        const int s = q.n_seq > 0 ? seq_of(q, r) : 0;
+        w = s >= 0 ? w * sload(g.weights + s) : 0.0f;
+        const Slope* p = g.slopes + r;
+        o.m = sload(&p->m);
+        o.other_m = sload(&p->other_m);
+        o.mine = sload(&p->mine) * w;
+        o.other = sload(&p->other) * w;
+        o.plain = sload(&p->plain) * w;
+        o.log_mass = sload(&p->log_mass);
+        o.label_extra = g.t.hard > 0.0 ? -(float)g.t.hard * w : 0.0f;
+        o.soft = g.t.soft * w;
+        o.first = r * g.t.top;
+        o.zero = w == 0.0f;
+        return o;
+    }
+    __device__ __forceinline__ float at(const Row& o, const Heat& h, float x, bool teacher) const {
+        float y = teacher ? heat_exp(x - o.m, h) * o.mine : heat_exp(x - o.other_m, h) * o.other;
+        if (PLAIN) y = __builtin_fmaf(exp_(x - o.m), o.plain, y);
+        return y;
+    }
+    __device__ __forceinline__ bool entry(const Row& o, const Rows& q, const Heat&, int j, int64_t& id, float& extra) const {
+        id = teacher_id(g.t, o.first + j);
+        const float lp = *gbl(g.t.logps + o.first + j);
+        extra = -o.soft * exp_(lp - o.log_mass);
+        return lp != -__builtin_inff() && (uint64_t)id < (uint64_t)q.vocab;
+    }
+};
+
+// The gradient of a split of a row, in runs of 16 bytes from the ends of cache lines.  Runs that hold a label or one
+// of the entries are marked, left out of the pass, and written element by element afterwards.
+template <int DT, class G, int PER>
+__global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, const G g, void* __restrict__ grad) {
+    using T = typename Elem<DT>::T;
+    constexpr int TH = kT / PER, W = kW<DT>;
+    constexpr int kMarks = PER > 1 ? (int)kShortRuns / 32 + 2 : kBits / 32;
+    constexpr int kEntries = (PER > 1 ? kMaxTop : kMaxTeacher) + 1;
+    __shared__ uint32_t marks[PER][kMarks];
+    __shared__ uint32_t ids[PER][kEntries];  // highest bit: the label
+    __shared__ float extras[PER][kEntries];
+    __shared__ int counts[PER];
+    const int lane = threadIdx.x % TH, wave = PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
+    const int64_t wg = (int64_t)blockIdx.x * PER + wave;
+    const int64_t r = PER > 1 ? wg : wg / (uint32_t)q.splits, split = PER > 1 ? 0 : wg % (uint32_t)q.splits;
+    const bool row = r < q.rows;
+    const int64_t label = row && q.labels ? sload(q.labels + r) : 0;
+    const bool learns = row && (!q.labels || label != q.ignore);
+    T* out = (T*)grad + r * q.vocab;
+    const Runs<W> runs(out, q.vocab, sizeof(T));
+    int64_t c = split * q.split_runs, end = c + q.split_runs;
+    if (end > runs.count()) end = runs.count();
+    const int64_t first = c, whole = runs.whole(end);
+    typename G::Row o;
+    o.zero = true;
+    if (learns) o = g.row(q, h, r, label, threadIdx.x & 63);
+    const bool works = learns && !o.zero;
+    if (PER > 1 || works) {
+        for (int i = lane; i < (int)((end - first + 31) / 32); i += TH) marks[wave][i] = 0;
+        __syncthreads();
+        if (works && lane < 64) {  // in the entries' order, so that what meets at a column adds up in it
+            int n = 0;
+            const int all = g.entries();
+            for (int j0 = 0; j0 < all + 1; j0 += 64) {
+                const int j = j0 + lane;
+                int64_t id = -1;
+                float extra = 0.0f;
+                bool in = false;
+                if (j < all) in = g.entry(o, q, h, j, id, extra);
+                else if (j == all && q.labels && o.label_extra != 0.0f) {
+                    id = label;
+                    extra = o.label_extra;
+                    in = (uint64_t)id < (uint64_t)q.vocab;
+                }
+                const int64_t run = in ? (id + runs.pad) / W : -1;
+                in = in && run >= first && run < end;
+                const uint64_t who = __ballot(in);
+                if (in) {
+                    const int at = n + (int)__popcll(who & (((uint64_t)1 << lane) - 1));
+                    ids[wave][at] = (uint32_t)id | (j == all ? 0x80000000u : 0u);
+                    extras[wave][at] = extra;
+                    atomicOr(&marks[wave][(run - first) >> 5], 1u << ((run - first) & 31));
+                }
+                n += (int)__popcll(who);
+            }
+            if (lane == 0) counts[wave] = n;
+        }
+        __syncthreads();
+    }
+    if (!row) return;
+    c += lane;
+    if (!works) {
+        Run<T, W> zeros;
+#pragma unroll
+        for (int i = 0; i < W; ++i) zeros.e[i] = T(0);
+        for (; c < end; c += TH) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
+        return;
+    }
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const auto marked = [&](int64_t run) { return marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1; };
+    const auto finish = [&](Run<T, W>& v) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g.at(o, h, to_f32<DT>(v.e[i]), false));
+    };
+    const auto one = [&](int64_t run) {
+        const int64_t at = runs.begin(run), left = runs.left(run);
+        Run<T, W> v = load_logits<DT>(x + at, left);
+        finish(v);
+        if (!marked(run)) store_run<T, W>(out + at, left, v);
+    };
+    if (runs.at_start(c)) {
+        one(c);
+        c += TH;
+    }
+    for (; c + TH < whole; c += 2 * TH) {
+        Run<T, W> v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * TH));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            finish(v[i]);
+            if (!marked(c + i * TH)) store_run<T, W>(out + runs.begin(c + i * TH), W, v[i]);
+        }
+    }
+    for (; c < end; c += TH) one(c);
+    const int n = counts[wave];
+    for (int i = lane; i < n; i += TH) {
+        const int64_t run = ((int64_t)(ids[wave][i] & 0x7fffffffu) + runs.pad) / W;
+        bool first_of = true;
+        for (int j = 0; j < i; ++j) first_of &= ((int64_t)(ids[wave][j] & 0x7fffffffu) + runs.pad) / W != run;
+        if (!first_of) continue;
+        const int64_t at = runs.begin(run), left = runs.left(run);
+        for (int k = 0; k < W && k < left; ++k) {
+            float extra = 0.0f;
+            bool teacher = false;
+            for (int j = 0; j < n; ++j) {
+                const uint32_t id = ids[wave][j];
+                if ((int64_t)(id & 0x7fffffffu) != at + k) continue;
+                extra += extras[wave][j];
+                teacher |= !(id >> 31);
+            }
+            *gbl(out + at + k) = from_f32<DT>(g.at(o, h, to_f32<DT>(*gbl(x + at + k)), teacher) + extra);
+        }
+    }
+}
+
+// ------------------------------------------------------------ host side
+int make_heat(const char* what, double temperature, Heat& h) {
+    if (!(temperature >= 1e-4 && temperature <= 1e4))
+        return set_error(GEFENX_EINVAL, "%s: temperature %g is not in [1e-4, 1e4]", what, temperature);
+    const double c = 1.44269504088896340736 / temperature;
+    h.hi = (float)c;
+    if ((double)h.hi >= c) h.hi = nextafterf(h.hi, 0.0f);
+    h.lo = (float)(c - (double)h.hi);
+    h.inv64 = 1.0 / temperature;
+    h.inv = (float)h.inv64;
+    return GEFENX_OK;
+}
+
+void set_splits(const gefenx_logits& l, Rows& q, int64_t splits) {
+    const int64_t run = l.dtype == GEFENX_F32 ? 4 : 8, size = 16 / run;
+    const int64_t runs = (l.vocab + kLine / size - 1 + run - 1) / run, line = kLine / 16;
+    splits = std::max<int64_t>(splits, 1);
+    q.split_runs = ((runs + splits - 1) / splits + line - 1) / line * line;
+    q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
+}
+
+// How rows are split for the statistics with `top` keys a split.
+int statistics_rows(const char* what, const gefenx_logits* l, int top, Rows& q) {
+    if (top < 0 || top > kMaxTop) return set_error(GEFENX_EINVAL, "%s: top %d is not in [0, %d]", what, top, kMaxTop);
+    const int rc = make_rows(what, l, false, q, 0, false);
+    if (rc != GEFENX_OK) return rc;
+    if (top > l->vocab) return set_error(GEFENX_EINVAL, "%s: top %d of %lld logits", what, top, (long long)l->vocab);
+    if (top && q.per > 1) {
+        q.per = 1;
+        set_splits(*l, q, 1);
+    }
+    if (top && q.splits * top > kMergeKeys) set_splits(*l, q, kMergeKeys / top);
+    if (q.rows * q.splits > kMaxThreads / kT)
+        return set_error(GEFENX_EINVAL, "%s: too many rows (%lld)", what, (long long)l->rows);
+    return GEFENX_OK;
+}
+
+// ... and where runs of a split are marked.
+int marked_rows(const char* what, const gefenx_logits* l, bool sequences, bool labelled, int64_t most, Rows& q) {
+    const int rc = make_rows(what, l, sequences, q, most, labelled);
+    if (rc != GEFENX_OK) return rc;
+    if (q.split_runs > kBits) set_splits(*l, q, q.splits * ((q.split_runs + kBits - 1) / kBits) + 1);
+    if (q.split_runs > kBits || q.rows * q.splits > kMaxThreads / kT)
+        return set_error(GEFENX_EINVAL, "%s: too many logits (%lld x %lld)", what, (long long)l->rows, (long long)l->vocab);
+    return GEFENX_OK;
+}
+
+size_t sums_bytes(const Rows& q) { return align16(sizeof(float4) * (size_t)q.rows * (size_t)q.splits); }
+size_t keys_bytes(const Rows& q, int top) { return 8 * (size_t)q.rows * (size_t)q.splits * (size_t)top; }
+
+int enough(const char* what, const void* ws, size_t bytes, size_t needed) {
+    if (!ws || bytes < needed) return set_error(GEFENX_EINVAL, "%s: workspace of %zu bytes, %zu needed", what, bytes, needed);
+    return GEFENX_OK;
+}
+
+template <class G>
+int run_tokens_grad(const char* what, const Rows& q, int dtype, const Heat& h, const G& g, void* grad, hipStream_t s) {
+    return by_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (q.per > 1) k_tokens_grad<DT, G, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, g, grad);
+        else k_tokens_grad<DT, G, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, g, grad);
+        return launched(what);
+    });
+}
+
+// A checked call of the distillation.
+struct Distill {
+    const char* what;
+    Rows q;
+    Heat h;
+    Teacher t;
+    int dtype, by_sequence;
+    float4* part;
+    double2* each;
+    DistillSums* sums;
+    size_t bytes;
+    hipStream_t s;
+};
+
+int make_distill(const char* what, const gefenx_logits* l, const gefenx_teacher* t, int64_t most, Distill& d) {
+    d.what = what;
+    if (!t) return set_error(GEFENX_EINVAL, "%s: null descriptor", what);
+    const int rc = marked_rows(what, l, t->by_sequence != 0 || (l && l->cu_seqlens), true, most, d.q);
+    if (rc != GEFENX_OK) return rc;
+    if (t->top < 1 || t->top > kMaxTeacher)
+        return set_error(GEFENX_EINVAL, "%s: %d tokens of the teacher are not in [1, %d]", what, t->top, kMaxTeacher);
+    if (t->rest < kBucket || t->rest > kNormalize) return set_error(GEFENX_EINVAL, "%s: rest %d", what, t->rest);
+    if (!(t->hard_weight >= 0.0 && t->hard_weight <= 1.0))
+        return set_error(GEFENX_EINVAL, "%s: hard_weight %g is not in [0, 1]", what, t->hard_weight);
+    if (l->rows > 0 && (!t->ids || !t->logps)) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const int rh = make_heat(what, t->temperature, d.h);
+    if (rh != GEFENX_OK) return rh;
+    if (!l->cu_seqlens && !t->by_sequence) d.q.n_seq = 0;
+    if (d.q.per > 1 && t->top > kMaxTop) {
+        d.q.per = 1;
+        set_splits(*l, d.q, 1);
+    }
+    d.dtype = l->dtype;
+    d.by_sequence = t->by_sequence;
+    d.t = Teacher{t->ids, t->logps, t->top, t->ids64, t->rest, (float)((1.0 - t->hard_weight) * t->temperature),
+                  (1.0 - t->hard_weight) * t->temperature * t->temperature, t->hard_weight};
+    d.bytes = sums_bytes(d.q) + sizeof(double2) * (size_t)d.q.rows + sizeof(DistillSums) * (size_t)std::max(d.q.n_seq, 1);
+    return GEFENX_OK;
+}
+
+int distill_forward(Distill& d, float* loss, float* divergence, float* nll, float* token_divergence, void* slopes, float* weights,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = d.what;
+    int rc = enough(what, workspace, workspace_bytes, d.bytes);
+    if (rc != GEFENX_OK) return rc;
+    if (!loss || !divergence || !nll || !weights || (d.q.rows > 0 && (!token_divergence || !slopes)))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    char* ws = static_cast<char*>(workspace);
+    d.part = reinterpret_cast<float4*>(ws);
+    d.each = reinterpret_cast<double2*>(ws + sums_bytes(d.q));
+    d.sums = reinterpret_cast<DistillSums*>(d.each + d.q.rows);
+    d.s = static_cast<hipStream_t>(stream);
+    const Rows& q = d.q;
+    const bool plain = d.t.hard > 0.0 && d.h.inv64 != 1.0;
+    if (q.rows > 0) {
+        rc = by_dtype(d.dtype, [&](auto dt) {
+            constexpr int DT = decltype(dt)::value;
+            const auto go = [&](auto u, auto bucket) {
+                constexpr int U = decltype(u)::value;
+                constexpr bool B = decltype(bucket)::value;
+                if (q.per > 1) k_distill<DT, U, B, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, d.s>>>(q, d.h, d.t, d.part);
+                else k_distill<DT, U, B, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, d.s>>>(q, d.h, d.t, d.part);
+                k_distill_rows<DT, U, B><<<(uint32_t)q.rows, 64, 0, d.s>>>(q, d.h, d.t, d.part, d.each, token_divergence,
+                                                                         static_cast<Slope*>(slopes));
+            };
+            using N = std::integral_constant<int, kNone>;
+            using P = std::integral_constant<int, kPlain>;
+            if (d.t.rest == kBucket) {
+                if (plain) go(P(), std::true_type());
+                else go(N(), std::true_type());
+            } else {
+                if (plain) go(P(), std::false_type());
+                else go(N(), std::false_type());
+            }
+            return launched(what);
+        });
+        if (rc != GEFENX_OK) return rc;
+    }
+    const int n = std::max(q.n_seq, 1);
+    k_distill_sums<<<(uint32_t)n, kSeqT, 0, d.s>>>(q, d.each, d.sums);
+    k_distill_total<<<1, kT, 0, d.s>>>(d.sums, n, d.by_sequence, d.t, loss, divergence, nll, weights);
+    return launched(what);
+}
+
+int distill_grad(const char* what, const gefenx_logits* l, const gefenx_teacher* t, const void* slopes, const float* weights,
+                 const float* scale_dev, double scale, void* grad, void* stream) {
+    Distill d;
+    const int rc = make_distill(what, l, t, kTokenGradPasses, d);
+    if (rc != GEFENX_OK || d.q.rows == 0) return rc;
+    if (!slopes || !weights || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const Downhill g = {static_cast<const Slope*>(slopes), weights, scale_dev, (float)scale, d.t};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (d.t.hard > 0.0 && d.h.inv64 != 1.0) return run_tokens_grad(what, d.q, d.dtype, d.h, DistillGrad<true>{g}, grad, s);
+    return run_tokens_grad(what, d.q, d.dtype, d.h, DistillGrad<false>{g}, grad, s);
+}
+
+}  // namespace
+}  // namespace gx
+
+using namespace gx;
+
+extern "C" {
+
+size_t gefenx_token_statistics_workspace_bytes(const gefenx_logits* logits, int top) {
+    Rows q;
+    if (statistics_rows("gefenx_token_statistics_workspace_bytes", logits, top, q) != GEFENX_OK) return 0;
+    return sums_bytes(q) + keys_bytes(q, top) + 16;
+}
+
+int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int top, float* logps, float* entropy,
+                            int64_t* top_ids, float* top_logps, float* stats, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    const char* what = "gefenx_token_statistics";
+    Rows q;
+    Heat h;
+    int rc = statistics_rows(what, logits, top, q);
+    if (rc == GEFENX_OK) rc = make_heat(what, temperature, h);
+    if (rc == GEFENX_OK) rc = enough(what, workspace, workspace_bytes, sums_bytes(q) + keys_bytes(q, top));
+    if (rc != GEFENX_OK || q.rows == 0) return rc;
+    if (!entropy || !stats || (q.labels && !logps) || (!q.labels && logps) || (top && (!top_ids || !top_logps)))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    float4* part = static_cast<float4*>(workspace);
+    uint64_t* keys = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + sums_bytes(q));
+    const Statistics out = {logps, entropy, top_logps, top_ids, reinterpret_cast<float4*>(stats)};
+    return by_dtype(logits->dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (q.per > 1) k_statistics<DT, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, top, part, keys);
+        else k_statistics<DT, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, top, part, keys);
+        int lanes = 1;
+        while (lanes < q.splits && lanes < 64) lanes *= 2;
+        if (top) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
+        else k_statistics_rows<DT, false><<<(uint32_t)((q.rows * lanes + kT - 1) / kT), kT, 0, s>>>(q, h, top, out, part, keys, lanes);
+        return launched(what);
+    });
+}
+
+int gefenx_token_statistics_grad(const gefenx_logits* logits, double temperature, int top, const float* stats,
+                                 const int64_t* top_ids, const float* logps_grad, const float* entropy_grad,
+                                 const float* top_logps_grad, void* grad, void* stream) {
+    const char* what = "gefenx_token_statistics_grad";
+    Rows q;
+    Heat h;
+    int rc = marked_rows(what, logits, false, false, kTokenGradPasses, q);
+    if (rc == GEFENX_OK) rc = make_heat(what, temperature, h);
+    if (rc != GEFENX_OK) return rc;
+    if (top < 0 || top > kMaxTop) return set_error(GEFENX_EINVAL, "%s: top %d is not in [0, %d]", what, top, kMaxTop);
+    if (q.rows == 0) return GEFENX_OK;
+    if (!stats || !grad || (top_logps_grad && !top_ids) || (logps_grad && !q.labels))
+        return set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    const StatisticsGrad g = {{reinterpret_cast<const float4*>(stats), logps_grad, entropy_grad, top ? top_logps_grad : nullptr,
+                               top_ids, top}};
+    return run_tokens_grad(what, q, logits->dtype, h, g, grad, static_cast<hipStream_t>(stream));
+}
+
+size_t gefenx_distillation_workspace_bytes(const gefenx_logits* logits, const gefenx_teacher* teacher) {
+    Distill d;
+    return make_distill("gefenx_distillation_workspace_bytes", logits, teacher, 0, d) == GEFENX_OK ? d.bytes + 16 : 0;
+}
+
+int gefenx_distillation_loss(const gefenx_logits* logits, const gefenx_teacher* teacher, float* loss, float* divergence,
+                             float* nll, float* token_divergence, float* slopes, float* weights, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    Distill d;
+    const int rc = make_distill("gefenx_distillation_loss", logits, teacher, 0, d);
+    if (rc != GEFENX_OK) return rc;
+    return distill_forward(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+}
+
+int gefenx_distillation_grad(const gefenx_logits* logits, const gefenx_teacher* teacher, const float* slopes,
+                             const float* weights, const float* scale_dev, double scale, void* grad, void* stream) {
+    return distill_grad("gefenx_distillation_grad", logits, teacher, slopes, weights, scale_dev, scale, grad, stream);
+}
+
+int gefenx_distillation_loss_grad(const gefenx_logits* logits, const gefenx_teacher* teacher, float* loss, float* divergence,
+                                  float* nll, float* token_divergence, float* slopes, float* weights, const float* scale_dev,
+                                  double scale, void* grad, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "gefenx_distillation_loss_grad";
+    Distill d;
+    int rc = make_distill(what, logits, teacher, 0, d);
+    if (rc == GEFENX_OK && d.q.rows > 0 && !grad) rc = set_error(GEFENX_EINVAL, "%s: null pointer", what);
+    if (rc == GEFENX_OK) rc = distill_forward(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    return rc == GEFENX_OK ? distill_grad(what, logits, teacher, slopes, weights, scale_dev, scale, grad, stream) : rc;
+}
+
+}  // extern "C"

@@ -21,7 +21,10 @@ from gefen.hybrid import GefenMuonHybrid
 from gefen.losses import (PolicyLoss, PreferenceLoss, policy_loss, policy_loss_and_grad, preference_loss,
                           preference_loss_and_grad, token_logps)
 from gefen.params import DEFAULT_BACKUP_SUBSTRINGS, is_muon_param, split_params_for_muon, validate_split
+from gefen.tokens import (DistillationLoss, TokenStatistics, distillation_loss, distillation_loss_and_grad,
+                          token_statistics)
 
 __all__ = ["AdamW", "Gefen", "GefenMuon", "GefenMuonHybrid", "split_params_for_muon", "validate_split", "is_muon_param",
            "PolicyLoss", "PreferenceLoss", "policy_loss", "policy_loss_and_grad", "preference_loss",
-           "preference_loss_and_grad", "token_logps", "DEFAULT_BACKUP_SUBSTRINGS", "kernels", "__version__"]
+           "preference_loss_and_grad", "token_logps", "DistillationLoss", "TokenStatistics", "distillation_loss",
+           "distillation_loss_and_grad", "token_statistics", "DEFAULT_BACKUP_SUBSTRINGS", "kernels", "__version__"]

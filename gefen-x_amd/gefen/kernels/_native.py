@@ -120,6 +120,16 @@ class Logits(ctypes.Structure):
     ]
 
 
+class Teacher(ctypes.Structure):
+    """Mirror of ``gefenx_teacher`` (include/gefenx.h)."""
+
+    _fields_ = [
+        ("ids", ctypes.c_void_p), ("logps", ctypes.c_void_p),
+        ("temperature", ctypes.c_double), ("hard_weight", ctypes.c_double),
+        ("top", ctypes.c_int32), ("ids64", ctypes.c_int32), ("rest", ctypes.c_int32), ("by_sequence", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -188,6 +198,13 @@ SIGNATURES = {
     "gefenx_policy_loss_grad": (_I, [_P, _P, _P, _I, _P, _D, _D, _D, _I, _P, _P, _P, _P, _P, _P, _P, _P, _D, _P, _P, _SZ,
                                      _P]),
     "gefenx_logits_grad": (_I, [_P, _P, _P, _P, _P, _D, _P, _P]),
+    "gefenx_token_statistics_workspace_bytes": (_SZ, [_P, _I]),
+    "gefenx_token_statistics": (_I, [_P, _D, _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gefenx_token_statistics_grad": (_I, [_P, _D, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "gefenx_distillation_workspace_bytes": (_SZ, [_P, _P]),
+    "gefenx_distillation_loss": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "gefenx_distillation_grad": (_I, [_P, _P, _P, _P, _P, _D, _P, _P]),
+    "gefenx_distillation_loss_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _D, _P, _P, _SZ, _P]),
     "gefenx_profile_enable": (_I, [_I]),
     "gefenx_profile_read": (_I, [_I, _P, _P, _P, _P]),
     "gefenx_profile_reset": (_I, []),

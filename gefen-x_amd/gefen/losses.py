@@ -54,10 +54,11 @@ class PolicyLoss(NamedTuple):
 
 
 class _Call:
-    """The logits of one call, checked, and the descriptor that the kernels read them by."""
+    """The logits of one call, checked, and the descriptor that the kernels read them by.  labelled: whether there have to
+    be labels; without them every row counts."""
 
-    def __init__(self, logits, labels, ignore_index, cu_seqlens=None, sequences=True):
-        if not isinstance(logits, torch.Tensor) or not isinstance(labels, torch.Tensor):
+    def __init__(self, logits, labels, ignore_index, cu_seqlens=None, sequences=True, labelled=True):
+        if not isinstance(logits, torch.Tensor) or not (isinstance(labels, torch.Tensor) or (labels is None and not labelled)):
             raise TypeError("logits and labels must be tensors")
         if logits.device.type != "cuda":
             raise ValueError("Expected logits on a HIP device, got {}".format(logits.device))
@@ -65,10 +66,11 @@ class _Call:
             raise NotImplementedError("logits of {} are not implemented (fp32, fp16, bf16)".format(logits.dtype))
         if logits.dim() < 1 or logits.shape[-1] < 1:
             raise ValueError("logits need a vocabulary dimension, got shape {}".format(tuple(logits.shape)))
-        if labels.dtype != torch.int64 or labels.shape != logits.shape[:-1] or labels.device != logits.device:
+        if labels is not None and (labels.dtype != torch.int64 or labels.shape != logits.shape[:-1]
+                                   or labels.device != logits.device):
             raise ValueError("labels must be int64 of shape {} on {}, got {} of shape {} on {}".format(
                 tuple(logits.shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
-        self.device, self.shape, self.vocab = logits.device, logits.shape, logits.shape[-1]
+        self.device, self.shape, self.lead, self.vocab = logits.device, logits.shape, logits.shape[:-1], logits.shape[-1]
         self.n_seq, self.cu = 0, None
         if cu_seqlens is not None:
             if logits.dim() != 2:
@@ -87,10 +89,10 @@ class _Call:
         if placed is None:
             x = x.detach().contiguous()
             placed = self._placed(x)
-        self.logits, self.labels = x, labels if labels.is_contiguous() else labels.contiguous()
-        self.rows = labels.numel()
+        self.logits, self.labels = x, labels if labels is None or labels.is_contiguous() else labels.contiguous()
+        self.rows = self.lead.numel()
         self.desc = _native.Logits(
-            x.data_ptr(), self.labels.data_ptr(), None if self.cu is None else self.cu.data_ptr(), self.rows, *placed,
+            x.data_ptr(), _ptr(self.labels), None if self.cu is None else self.cu.data_ptr(), self.rows, *placed,
             self.vocab, int(ignore_index), _DTYPES[x.dtype], self.n_seq)
         self.ref = ctypes.byref(self.desc)
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
@@ -110,23 +112,24 @@ class _Call:
         return max(1, x.numel() // x.shape[-1]), 0, x.shape[-1]
 
     @classmethod
-    def again(cls, desc, logits, labels, ignore_index, cu_seqlens=None, sequences=True):
+    def again(cls, desc, logits, labels, ignore_index, cu_seqlens=None, sequences=True, labelled=True):
         """The call of a forward pass for its backward: by its descriptor, where that says how the saved tensors lie.
         An address alone does not: copies that the forward pass made are gone, hooks may have moved the tensors and
         laid them out anew, and either may have left its address to the other."""
-        fits = (desc.logits == logits.data_ptr() and desc.labels == labels.data_ptr()
-                and desc.dtype == _DTYPES.get(logits.dtype) and desc.vocab == logits.shape[-1]
+        fits = (desc.logits == logits.data_ptr() and desc.dtype == _DTYPES.get(logits.dtype) and desc.vocab == logits.shape[-1]
                 and cls._placed(logits) == (desc.rows_per_batch, desc.batch_stride, desc.row_stride)
-                and desc.rows == labels.numel() and labels.shape == logits.shape[:-1]
-                and labels.dtype is torch.int64 and labels.is_contiguous())
+                and desc.rows == logits.shape[:-1].numel() and desc.labels == _ptr(labels))
+        if fits and labels is not None:
+            fits = labels.shape == logits.shape[:-1] and labels.dtype is torch.int64 and labels.is_contiguous()
         if fits and cu_seqlens is not None:
             fits = (desc.cu_seqlens == cu_seqlens.data_ptr() and cu_seqlens.dtype is torch.int32
                     and cu_seqlens.is_contiguous() and desc.n_seq == cu_seqlens.numel() - 1)
         if not fits:
-            return cls(logits, labels, ignore_index, cu_seqlens, sequences)
+            return cls(logits, labels, ignore_index, cu_seqlens, sequences, labelled)
         call = cls.__new__(cls)
         call.desc, call.ref = desc, ctypes.byref(desc)
-        call.device, call.shape, call.logits, call.labels = logits.device, logits.shape, logits, labels
+        call.device, call.shape, call.lead, call.logits, call.labels = (logits.device, logits.shape, logits.shape[:-1],
+                                                                        logits, labels)
         call.stream = torch.cuda.current_stream(call.device).cuda_stream
         return call
 
@@ -134,10 +137,10 @@ class _Call:
         """A per-token input as the kernels read it, or None."""
         if t is None:
             return None
-        if not isinstance(t, torch.Tensor) or t.shape != self.labels.shape or t.device != self.device \
+        if not isinstance(t, torch.Tensor) or t.shape != self.lead or t.device != self.device \
                 or not t.is_floating_point():
             raise ValueError("{} must be a floating tensor of the labels' shape {} on {}, got {}".format(
-                name, tuple(self.labels.shape), self.device,
+                name, tuple(self.lead), self.device,
                 "{} of shape {} on {}".format(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor)
                 else type(t).__name__))
         return t if t.dtype is torch.float32 and t.is_contiguous() else t.detach().to(torch.float32).contiguous()

@@ -647,6 +647,73 @@ int gefenx_logits_grad(const gefenx_logits* logits, const float* stats, const fl
                        const float* scale_dev, double scale, void* grad, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Statistics of tokens, and distillation from a teacher's likeliest tokens.  No
+ * counterpart in the reference.  Logits are divided by `temperature`, in [1e-4,
+ * 1e4]; rows and labels as above.  All calls enqueue kernels on `stream` and
+ * allocate nothing.
+ * ---------------------------------------------------------------------- */
+
+/* Of softmax(x / temperature) of each row: the label's log-probability (fp32
+ * [rows]), the entropy (fp32 [rows]) and the `top` (0 .. 128, <= vocab) largest
+ * logits, falling, ties by the lowest index, NaN above all: ids int64 [rows,
+ * top], log-probabilities fp32 [rows, top].  Rows that are ignored: 0, 0, and
+ * ids 0 of log-probability -inf.  logits->labels NULL: every row counts, logps
+ * is NULL.  A label outside of the vocabulary makes its log-probability NaN.
+ * stats: fp32 [rows, 4] for the gradient.  workspace: any contents. */
+size_t gefenx_token_statistics_workspace_bytes(const gefenx_logits* logits, int top);
+int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int top, float* logps, float* entropy,
+                            int64_t* top_ids, float* top_logps, float* stats, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* The gradient of the logits [rows, vocab], contiguous, in their dtype, from those
+ * of log-probabilities, entropies and top log-probabilities (fp32, as above; each
+ * may be NULL: zeros). */
+int gefenx_token_statistics_grad(const gefenx_logits* logits, double temperature, int top, const float* stats,
+                                 const int64_t* top_ids, const float* logps_grad, const float* entropy_grad,
+                                 const float* top_logps_grad, void* grad, void* stream);
+
+/* A teacher's tokens: `top` (1 .. 512) ids and log-probabilities per row; an entry
+ * of log-probability -inf holds none (its id is not used), any other id outside of
+ * [0, vocab) makes its row's results NaN. */
+enum gefenx_rest { GEFENX_REST_BUCKET = 0, GEFENX_REST_DROP = 1, GEFENX_REST_NORMALIZE = 2 };
+typedef struct gefenx_teacher {
+    const void* ids;          /* device int64 (ids64) or int32 [rows, top] */
+    const float* logps;       /* device fp32 [rows, top] */
+    double temperature;
+    double hard_weight;       /* w, in [0, 1] */
+    int32_t top, ids64, rest, by_sequence;
+} gefenx_teacher;
+
+/* With p the teacher's probabilities, P their sum and q = softmax(x / temperature),
+ * per row that counts
+ *   D = sum p (log p - log q)                                            DROP
+ *   the same of p / P (0 where P = 0)                                    NORMALIZE
+ *   DROP's + r log(r / rho), r = max(0, 1 - P), rho = 1 - sum of q over
+ *   the teacher's ids; without that term where rho is 0 by itself        BUCKET
+ *   nll = -log softmax(x)[label]  (0 with hard_weight 0, which asks nothing of the label)
+ * and loss = (1 - w) temperature^2 mean D + w mean nll; means over the rows that
+ * count or (by_sequence) over the sequences that have any of theirs; 0 without any.
+ * logits->n_seq and cu_seqlens as above; neither by_sequence nor cu_seqlens: all
+ * rows are taken together, n_seq is not used.  Written: loss[1], divergence[1],
+ * nll[1] (both means), token_divergence[rows] (0 where ignored), and slopes [rows,
+ * 8] / weights [max(n_seq, 1)] for the gradient. */
+size_t gefenx_distillation_workspace_bytes(const gefenx_logits* logits, const gefenx_teacher* teacher);
+int gefenx_distillation_loss(const gefenx_logits* logits, const gefenx_teacher* teacher, float* loss, float* divergence,
+                             float* nll, float* token_divergence, float* slopes, float* weights, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* The gradient of the loss in the logits [rows, vocab], contiguous, in their dtype,
+ * times *scale_dev (NULL: 1) * scale, rounded once. */
+int gefenx_distillation_grad(const gefenx_logits* logits, const gefenx_teacher* teacher, const float* slopes,
+                             const float* weights, const float* scale_dev, double scale, void* grad, void* stream);
+
+/* Both in one call. */
+int gefenx_distillation_loss_grad(const gefenx_logits* logits, const gefenx_teacher* teacher, float* loss,
+                                  float* divergence, float* nll, float* token_divergence, float* slopes, float* weights,
+                                  const float* scale_dev, double scale, void* grad, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Kernel timing.  When enabled, every update-kernel launch is bracketed by
  * HIP events on its own stream and tagged with its kind and algorithmic
  * bytes (compulsory traffic of the step it belongs to); gefenx_profile_read
