@@ -85,8 +85,9 @@ __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* 
     return a;
 }
 
+// Adds N runs; their maximum.
 template <int DT, int U, int N>
-__device__ __forceinline__ void add_runs(Sums<U>& a, const Run<typename Elem<DT>::T, kW<DT>> (&r)[N], const Heat& h) {
+__device__ __forceinline__ float add_runs(Sums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, const Heat& h) {
     float top = -__builtin_inff();
 #pragma unroll
     for (int c = 0; c < N; ++c)
@@ -98,18 +99,24 @@ __device__ __forceinline__ void add_runs(Sums<U>& a, const Run<typename Elem<DT>
     for (int c = 0; c < N; ++c)
 #pragma unroll
         for (int k = 0; k < kW<DT>; ++k) a.add(to_f32<DT>(r[c].e[k]), b, h);
+    return top;
 }
 
-// Runs c .. end - 1 of a row, TH lanes at a time; each lane's sums.  skip(run): a run that is left out.  Which
-// logits a lane adds up does not depend on where the row starts in memory.
-template <int DT, int U, int TH, bool STREAM, class Skip>
-__device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t c, int64_t end, int lane,
-                                            const Heat& h, Skip&& skip) {
+constexpr int kStep = 4;  // runs of a lane in flight
+
+// Runs begin .. end - 1 of a row, TH lanes at a time in steps of kStep runs each; each lane's sums.  skip(run): a
+// run that is left out; note(step, maximum): what a lane found in each step.  Which logits a lane adds up does not
+// depend on where the row starts in memory.
+template <int DT, int U, int TH, bool STREAM, class Skip, class Note>
+__device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t begin, int64_t end, int lane,
+                                            const Heat& h, Skip&& skip, Note&& note) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>;
     const int64_t whole = end * W <= vocab ? end : end - 1;
+    const int64_t last = end * W < vocab ? end * W : vocab;  // column behind the part
     Sums<U> a;
-    c += lane;
+    int64_t c = begin;
+    int step = 0;
     const auto put = [&](Run<T, W>& v, int64_t run) {
         if (skip(run)) {
 #pragma unroll
@@ -117,21 +124,32 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
         }
     };
     const auto add = [&](auto load) {
-        for (; c + 3 * TH < whole; c += 4 * TH) {
-            Run<T, W> v[4];
+        for (; c + kStep * TH <= whole; c += kStep * TH, ++step) {
+            Run<T, W> v[kStep];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = load(x + (c + i * TH) * W);
+            for (int i = 0; i < kStep; ++i) v[i] = load(x + (c + lane + i * TH) * W);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put(v[i], c + i * TH);
-            add_runs<DT, U, 4>(a, v, h);
+            for (int i = 0; i < kStep; ++i) put(v[i], c + lane + i * TH);
+            note(step, add_runs<DT, U, kStep>(a, v, h));
         }
     };
     if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT, STREAM>(p); });
     else add([](const T* p) { return load_logits<DT, STREAM>(p); });
-    for (; c < end; c += TH) {
-        Run<T, W> v[1] = {load_logits<DT, STREAM>(x + c * W, vocab - c * W)};
-        put(v[0], c);
-        add_runs<DT, U, 1>(a, v, h);
+    if (c < end) {  // the last step, of which some runs are missing or not whole
+        Run<T, W> v[kStep];
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+            const int64_t at = (c + lane + i * TH) * W;
+            v[i] = load_logits<DT, STREAM>(x + at, last - at);
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+            if (c + i * TH >= end) break;
+            if (c + lane + i * TH < end) put(v[i], c + lane + i * TH);
+            top = __builtin_fmaxf(top, add_runs<DT, U, 1>(a, v + i, h));
+        }
+        note(step, top);
     }
     return a;
 }
@@ -156,6 +174,27 @@ struct Select {
     uint32_t count, digit, above;
     uint32_t waves[kT / 64];
 };
+
+// The first `want` columns of first .. last - 1 whose order is `order`, as keys; waves: of kT / 64.
+template <int DT>
+__device__ __forceinline__ void first_equal(const typename Elem<DT>::T* x, int64_t first, int64_t last, uint32_t order,
+                                            uint32_t want, uint32_t* waves, uint64_t* __restrict__ out) {
+    uint32_t taken = 0;
+    for (int64_t begin = first; taken < want && begin < last; begin += kT) {
+        const int64_t v = begin + threadIdx.x;
+        const bool equal = v < last && order_of(to_f32<DT>(*gbl(x + v))) == order;
+        const uint64_t who = __ballot(equal);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = (uint32_t)__popcll(who);
+        __syncthreads();
+        uint32_t before = taken + (uint32_t)__popcll(who & (((uint64_t)1 << (threadIdx.x & 63)) - 1));
+        for (int w = 0; w < kT / 64; ++w) {
+            if (w < (int)(threadIdx.x >> 6)) before += waves[w];
+            taken += waves[w];
+        }
+        if (equal && before < want) out[before] = key_of(order, (uint32_t)v);
+    }
+}
 
 // The `top` largest keys of columns first .. last - 1 of a row, in no order, 0 behind them, by digits of 8 bits of
 // the order from the highest: after the last one the order of the top-th largest is known, larger ones are taken as
@@ -194,83 +233,240 @@ __device__ __forceinline__ void select_keys(const typename Elem<DT>::T* x, int64
         const uint32_t o = order(v);
         if (o > prefix) out[atomicAdd(&at.count, 1u)] = key_of(o, (uint32_t)v);
     }
-    uint32_t taken = 0;
-    for (int64_t begin = first; taken < want && begin < last; begin += kT) {
-        const int64_t v = begin + threadIdx.x;
-        const bool equal = v < last && order(v) == prefix;
-        const uint64_t who = __ballot(equal);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) at.waves[threadIdx.x >> 6] = (uint32_t)__popcll(who);
-        __syncthreads();
-        uint32_t before = taken + (uint32_t)__popcll(who & (((uint64_t)1 << (threadIdx.x & 63)) - 1));
-        for (int w = 0; w < kT / 64; ++w) {
-            if (w < (int)(threadIdx.x >> 6)) before += at.waves[w];
-            taken += at.waves[w];
-        }
-        if (equal && before < want) out[top - want + before] = key_of(prefix, (uint32_t)v);
-    }
+    first_equal<DT>(x, first, last, prefix, want, at.waves, out + (top - want));
 }
 
-// part[row][split] = the sums of a split of a row, keys[row][split][top] its largest.  PER rows to a workgroup: one,
-// or one for each of its waves (rows without splits, no keys).
-template <int DT, int PER>
-__global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, float4* __restrict__ part,
-                                                   uint64_t* __restrict__ keys) {
-    using T = typename Elem<DT>::T;
-    constexpr int TH = kT / PER, W = kW<DT>;
-    __shared__ float4 waves[kT / 64];
-    __shared__ Select select;
-    const int lane = threadIdx.x % TH;
-    const int64_t at = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
-    const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
-    if (r >= q.rows || (q.labels && sload(q.labels + r) == q.ignore)) return;
-    const int64_t runs = (q.vocab + W - 1) / W, begin = split * q.split_runs;
-    const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
-    const T* x = (const T*)q.x + row_offset(q, r);
-    const auto none = [](int64_t) { return false; };
-    Sums<kEntropy> a = q.cached || top ? row_sums<DT, kEntropy, TH, false>(x, q.vocab, begin, end, lane, h, none)
-                                       : row_sums<DT, kEntropy, TH, true>(x, q.vocab, begin, end, lane, h, none);
-    if constexpr (PER > 1) wave_join(a, h);
-    else a = group_join(a, h, waves);
-    if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
-    if constexpr (PER == 1) {
-        if (top) {
-            const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
-            select_keys<DT>(x, first, last, top, select, keys + at * top);
-        }
+// The want-th largest (want <= kT) of the orders that a workgroup's lanes bring, by bits from the highest; every wave
+// looks through all of them, four to a lane.
+__device__ __forceinline__ uint32_t largest_of_lanes(uint32_t own, int want, uint32_t* all) {
+    all[threadIdx.x] = own;
+    __syncthreads();
+    uint32_t v[kT / 64];
+#pragma unroll
+    for (int i = 0; i < kT / 64; ++i) v[i] = all[i * 64 + (threadIdx.x & 63)];
+    uint32_t found = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t next = found | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kT / 64; ++i) n += (int)__popcll(__ballot(v[i] >= next));
+        if (n >= want) found = next;
     }
+    return found;
 }
 
+// What the rows come to.
 struct Statistics {
     float *logps, *entropy, *top_logps;
     int64_t* top_ids;
     float4* stats;  // {maximum, sum, log of the sum, entropy}
 };
 
-// What the rows' sums and keys come to: a workgroup per row with keys, else a group of lanes per row.
+__device__ __forceinline__ void ignored_row(const Statistics& out, int64_t r, int top, int lane, int lanes) {
+    if (lane == 0) {
+        if (out.logps) out.logps[r] = 0.0f;
+        out.entropy[r] = 0.0f;
+        out.stats[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+    }
+    for (int i = lane; i < top; i += lanes) {
+        out.top_ids[r * top + i] = 0;
+        out.top_logps[r * top + i] = -__builtin_inff();
+    }
+}
+
+// A row's sums to its results, by one lane; log sum exp(x / tau).
+template <int DT>
+__device__ __forceinline__ double row_results(const Rows& q, const Heat& h, const Statistics& out, int64_t r, int64_t label,
+                                              const Sums<kEntropy>& a) {
+    using T = typename Elem<DT>::T;
+    const double log_sum = log((double)a.s);
+    const float entropy = (float)(log_sum - (double)a.u / (double)a.s * h.inv64);
+    if (out.logps) {
+        const bool in = label >= 0 && label < q.vocab;
+        const float x = in ? to_f32<DT>(*gbl((const T*)q.x + row_offset(q, r) + label)) : 0.0f;
+        out.logps[r] = in ? (float)(((double)x - (double)a.m) * h.inv64 - log_sum) : __uint_as_float(0x7fc00000u);
+    }
+    out.entropy[r] = entropy;
+    out.stats[r] = make_float4(a.m, a.s, (float)log_sum, entropy);
+    return (double)a.m * h.inv64 + log_sum;
+}
+
+__device__ __forceinline__ void top_result(const Heat& h, const Statistics& out, int64_t at, uint64_t key, double log_sum_exp) {
+    out.top_ids[at] = (int64_t)(uint32_t)~(uint32_t)key;
+    out.top_logps[at] = (float)((double)value_of((uint32_t)(key >> 32)) * h.inv64 - log_sum_exp);
+}
+
+// The place of each of n keys (no two alike) among them: put(place, key) for the `top` largest.
+template <class Put>
+__device__ __forceinline__ void by_rank(const uint64_t* keys, int n, int top, Put&& put) {
+    for (int i = threadIdx.x; i < n; i += kT) {
+        const uint64_t key = keys[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += keys[j] > key ? 1 : 0;
+        if (rank < top) put(rank, key);
+    }
+}
+
+constexpr int kSlots = 20;        // of a lane: the maxima of its steps
+// Candidates that there is room for; short rows may have all of their logits among them.
+__host__ __device__ constexpr int room(int slots) { return slots > 4 ? 512 : 1024; }
+constexpr int kSuspects = 384;    // slots that are looked through again
+struct Hunt {
+    uint32_t orders[kT];
+    uint16_t suspects[kSuspects];
+    uint32_t n_suspects, n_candidates;
+    double log_sum_exp;
+};
+
+// part[row][split] = the sums of a split of a row, keys[row][split][top] its largest, 0 where there are fewer; a whole
+// row's results at once.  PER rows to a workgroup: one, or one for each of its waves (rows without splits, no keys).
+//
+// The likeliest tokens cost the pass a maximum of each step of a lane, kept in LDS.  The top-th largest of the lanes'
+// maxima is a bound that at least `top` logits reach; the few steps that reach it are read again, what reaches it in
+// them are the candidates, and counting the larger ones gives each its place.  More candidates than there is room for
+// (equal logits), NaN and +inf go through select_keys.
+template <int DT, int PER, bool TOP>
+__global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, const Statistics out,
+                                                   float4* __restrict__ part, uint64_t* __restrict__ keys) {
+    using T = typename Elem<DT>::T;
+    constexpr int TH = kT / PER, W = kW<DT>;
+    __shared__ float4 waves[kT / 64];
+    __shared__ std::conditional_t<TOP, Hunt, char> hunt_;
+    extern __shared__ uint64_t dynamic[];
+    const int lane = threadIdx.x % TH;
+    const int64_t at = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
+    const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
+    if (r >= q.rows) return;
+    const int64_t label = q.labels ? sload(q.labels + r) : 0;
+    const bool alone = PER > 1 || q.splits == 1;
+    if (q.labels && label == q.ignore) {
+        if (alone) ignored_row(out, r, top, lane, TH);
+        return;
+    }
+    const int64_t runs = (q.vocab + W - 1) / W, begin = split * q.split_runs;
+    const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const auto none = [](int64_t) { return false; };
+    float* tops = reinterpret_cast<float*>(dynamic);
+    const auto note = [&](int step, float m) {
+        if constexpr (TOP) {
+            float* slot = tops + step / steps_of_slot * kT + threadIdx.x;
+            *slot = step % steps_of_slot ? __builtin_fmaxf(*slot, m) : m;
+        }
+    };
+    Sums<kEntropy> a = q.cached ? row_sums<DT, kEntropy, TH, false>(x, q.vocab, begin, end, lane, h, none, note)
+                                : row_sums<DT, kEntropy, TH, true>(x, q.vocab, begin, end, lane, h, none, note);
+    const float own = a.m;
+    if constexpr (PER > 1) wave_join(a, h);
+    else a = group_join(a, h, waves);
+    if constexpr (!TOP) {
+        if (lane == 0) {
+            if (alone) row_results<DT>(q, h, out, r, label, a);
+            else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
+        }
+    } else {
+        Hunt& hunt = hunt_;
+        if (threadIdx.x == 0) {
+            hunt.n_suspects = hunt.n_candidates = 0;
+            if (alone) hunt.log_sum_exp = row_results<DT>(q, h, out, r, label, a);
+            else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
+        }
+        const float bound = value_of(largest_of_lanes(order_of(own), top, hunt.orders));  // a barrier inside
+        const int64_t steps = begin < end ? (end - begin + kStep * TH - 1) / (kStep * TH) : 0;
+        const int slots = (int)((steps + steps_of_slot - 1) / steps_of_slot), each = kStep * steps_of_slot;  // runs of a slot
+        const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
+        uint64_t* mine = keys + at * top;
+        uint64_t* candidates = dynamic + kT / 2 * slots;  // behind the maxima
+        const uint32_t most = room(slots);
+        // those that reach the bound, or (above) that are over it; whether there was room for all
+        const auto gather = [&](bool above) {
+            for (int i = 0; i < slots; ++i) {
+                const float m = tops[i * kT + threadIdx.x];
+                if (above ? m > bound : m >= bound) {
+                    const uint32_t n = atomicAdd(&hunt.n_suspects, 1u);
+                    if (n < kSuspects) hunt.suspects[n] = (uint16_t)(i * kT + threadIdx.x);
+                }
+            }
+            __syncthreads();
+            const uint32_t suspects = hunt.n_suspects;
+            if (suspects > kSuspects) return false;
+            for (int i = threadIdx.x; i < (int)suspects * each; i += kT) {
+                const int s = hunt.suspects[i / each], slot = s / kT, who = s % kT;
+                const int64_t run = begin + who + ((int64_t)slot * each + i % each) * TH, col = run * W;
+                if (run >= end) continue;
+                const Run<T, W> v = load_logits<DT, false>(x + col, last - col);
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const float f = to_f32<DT>(v.e[k]);
+                    if ((above ? f > bound : f >= bound) && col + k < last) {
+                        const uint32_t n = atomicAdd(&hunt.n_candidates, 1u);
+                        if (n < most) candidates[n] = key_of(order_of(f), (uint32_t)(col + k));
+                    }
+                }
+            }
+            __syncthreads();
+            return hunt.n_candidates <= most;
+        };
+        bool found = a.s == a.s && gather(false);
+        if (!found && a.s == a.s) {  // many are equal to the bound: those over it, then the first of the others
+            __syncthreads();
+            if (threadIdx.x == 0) hunt.n_suspects = hunt.n_candidates = 0;
+            __syncthreads();
+            found = gather(true);
+            const uint32_t over = hunt.n_candidates;
+            if (found && over < (uint32_t)top) {
+                first_equal<DT>(x, first, last, order_of(bound), (uint32_t)top - over, hunt.orders, candidates + over);
+                __syncthreads();
+                if (threadIdx.x == 0) hunt.n_candidates = (uint32_t)(last - first < top ? last - first : top);
+                __syncthreads();
+            }
+        }
+        if (!found) {
+            __syncthreads();
+            select_keys<DT>(x, first, last, top, *reinterpret_cast<Select*>(dynamic), mine);
+            if (!alone) return;
+            __threadfence_block();
+            __syncthreads();
+            for (int i = threadIdx.x; i < top; i += kT) dynamic[i] = mine[i];
+            __syncthreads();
+            by_rank(dynamic, top, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+            return;
+        }
+        const int n = (int)hunt.n_candidates;
+        if (alone) {
+            by_rank(candidates, n, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+        } else {
+            for (int i = n + threadIdx.x; i < top; i += kT) mine[i] = 0;
+            by_rank(candidates, n, top, [&](int rank, uint64_t key) { mine[rank] = key; });
+        }
+    }
+}
+
+// What the splits of rows come to: a workgroup per row with keys, else a group of lanes per row.
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat h, int top, const Statistics out,
                                                         const float4* __restrict__ part, const uint64_t* __restrict__ keys,
                                                         int lanes) {
-    using T = typename Elem<DT>::T;
-    __shared__ uint64_t all[TOP ? kMergeKeys : 1];
-    __shared__ double base;
+    __shared__ uint64_t candidates[TOP ? kMergeKeys : 1];
+    __shared__ uint32_t orders[TOP ? kT : 1];
+    __shared__ uint32_t count;
+    __shared__ double log_sum_exp;
     const int lane = TOP ? threadIdx.x : threadIdx.x % lanes;
     const int64_t r = TOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kT / lanes) + threadIdx.x / lanes;
     if (r >= q.rows) return;
     const int64_t label = q.labels ? *gbl(q.labels + r) : 0;
-    const bool counts = !q.labels || label != q.ignore;
-    if (!counts) {
-        if (lane == 0) {
-            if (out.logps) out.logps[r] = 0.0f;
-            out.entropy[r] = 0.0f;
-            out.stats[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+    if (q.labels && label == q.ignore) return ignored_row(out, r, top, lane, TOP ? kT : lanes);
+    uint64_t own[kMergeKeys / kT];
+    uint64_t most = 0;
+    const int n = q.splits * top;
+    if constexpr (TOP) {
+#pragma unroll
+        for (int i = 0; i < kMergeKeys / kT; ++i) {
+            const int j = i * kT + threadIdx.x;
+            own[i] = j < n ? *gbl(keys + r * n + j) : 0;
+            most = own[i] > most ? own[i] : most;
         }
-        if (TOP && lane < top) {
-            out.top_ids[r * top + lane] = 0;
-            out.top_logps[r * top + lane] = -__builtin_inff();
-        }
-        return;
+        if (threadIdx.x == 0) count = 0;
     }
     if (!TOP || threadIdx.x < 64) {
         Sums<kEntropy> a;
@@ -279,33 +475,18 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
             a.join(p.x, p.y, p.z, h);
         }
         wave_join(a, h, TOP ? 64 : lanes);
-        const double log_sum = log((double)a.s), lse = (double)a.m * h.inv64 + log_sum;
-        const float entropy = (float)(log_sum - (double)a.u / (double)a.s * h.inv64);
         if (lane == 0) {
-            if (out.logps) {
-                const bool in = label >= 0 && label < q.vocab;
-                const float xl = in ? to_f32<DT>(*gbl((const T*)q.x + row_offset(q, r) + label)) : 0.0f;
-                out.logps[r] = in ? (float)(((double)xl - (double)a.m) * h.inv64 - log_sum) : __uint_as_float(0x7fc00000u);
-            }
-            out.entropy[r] = entropy;
-            out.stats[r] = make_float4(a.m, a.s, (float)log_sum, entropy);
-            if (TOP) base = lse;
+            const double lse = row_results<DT>(q, h, out, r, label, a);
+            if (TOP) log_sum_exp = lse;
         }
     }
     if constexpr (TOP) {
-        const int n = q.splits * top;
-        for (int i = threadIdx.x; i < n; i += kT) all[i] = keys[r * n + i];
+        const uint32_t bound = largest_of_lanes((uint32_t)(most >> 32), top, orders);
+#pragma unroll
+        for (int i = 0; i < kMergeKeys / kT; ++i)
+            if (own[i] != 0 && (uint32_t)(own[i] >> 32) >= bound) candidates[atomicAdd(&count, 1u)] = own[i];
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kT) {
-            const uint64_t key = all[i];
-            if (key == 0) continue;
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += all[j] > key ? 1 : 0;
-            if (rank < top) {
-                out.top_ids[r * top + rank] = (int64_t)(uint32_t)~(uint32_t)key;
-                out.top_logps[r * top + rank] = (float)((double)value_of((uint32_t)(key >> 32)) * h.inv64 - base);
-            }
-        }
+        by_rank(candidates, (int)count, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, log_sum_exp); });
     }
 }
 
@@ -360,8 +541,9 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
     if (!counts) return;
     const T* x = (const T*)q.x + row_offset(q, r);
     const auto skip = [&](int64_t run) { return BUCKET && (mine[(run - begin) >> 5] >> ((run - begin) & 31) & 1); };
-    Sums<U> a = q.cached ? row_sums<DT, U, TH, false>(x, q.vocab, begin, end, lane, h, skip)
-                         : row_sums<DT, U, TH, true>(x, q.vocab, begin, end, lane, h, skip);
+    const auto note = [](int, float) {};
+    Sums<U> a = q.cached ? row_sums<DT, U, TH, false>(x, q.vocab, begin, end, lane, h, skip, note)
+                         : row_sums<DT, U, TH, true>(x, q.vocab, begin, end, lane, h, skip, note);
     if constexpr (PER > 1) wave_join(a, h);
     else a = group_join(a, h, waves);
     if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
@@ -962,12 +1144,22 @@ int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int
     const Statistics out = {logps, entropy, top_logps, top_ids, reinterpret_cast<float4*>(stats)};
     return by_dtype(logits->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (q.per > 1) k_statistics<DT, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, top, part, keys);
-        else k_statistics<DT, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, top, part, keys);
-        int lanes = 1;
-        while (lanes < q.splits && lanes < 64) lanes *= 2;
-        if (top) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
-        else k_statistics_rows<DT, false><<<(uint32_t)((q.rows * lanes + kT - 1) / kT), kT, 0, s>>>(q, h, top, out, part, keys, lanes);
+        if (top) {
+            constexpr int W = kW<DT>;
+            const int64_t runs = std::min(q.split_runs, (q.vocab + W - 1) / W), steps = (runs + kStep * kT - 1) / (kStep * kT);
+            const int per = (int)((steps + kSlots - 1) / kSlots), slots = (int)((steps + per - 1) / per);
+            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * room(slots);
+            k_statistics<DT, 1, true><<<(uint32_t)(q.rows * q.splits), kT, lds, s>>>(q, h, top, per, out, part, keys);
+            if (q.splits > 1) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
+        } else if (q.per > 1) {
+            k_statistics<DT, kT / 64, false><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, 0, 1, out, part, keys);
+        } else {
+            k_statistics<DT, 1, false><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, 0, 1, out, part, keys);
+            int lanes = 1;
+            while (lanes < q.splits && lanes < 64) lanes *= 2;
+            if (q.splits > 1)
+                k_statistics_rows<DT, false><<<(uint32_t)((q.rows * lanes + kT - 1) / kT), kT, 0, s>>>(q, h, 0, out, part, keys, lanes);
+        }
         return launched(what);
     });
 }
