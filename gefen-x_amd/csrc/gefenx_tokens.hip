@@ -18,7 +18,7 @@ constexpr int kMaxTop = 128;      // likeliest tokens of a row
 constexpr int kMaxTeacher = 512;  // a teacher's tokens of a row
 constexpr int kMergeKeys = 2048;  // candidates of a row's splits that are merged
 constexpr int kBits = 16384;      // runs of a workgroup's part of a row where some are marked
-constexpr int64_t kTokenGradPasses = 2;
+constexpr int kGradRuns = 2;       // of a lane of the gradient in flight
 // Differences from the maximum stop here: exp is 0 from there at any temperature, and 0 times it is 0.
 constexpr float kFar = -1e25f;
 
@@ -856,47 +856,55 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
     const bool learns = row && (!q.labels || label != q.ignore);
     T* out = (T*)grad + r * q.vocab;
     const Runs<W> runs(out, q.vocab, sizeof(T));
-    int64_t c = split * q.split_runs, end = c + q.split_runs;
+    const int64_t first = split * q.split_runs;
+    int64_t end = first + q.split_runs;
     if (end > runs.count()) end = runs.count();
-    const int64_t first = c, whole = runs.whole(end);
+    int64_t c = first + lane;
+    // the logits are on their way while the row's numbers and entries are found
+    const T* x = (const T*)q.x + row_offset(q, r);
+    Run<T, W> v[kGradRuns];
+    const auto load = [&]() {
+#pragma unroll
+        for (int i = 0; i < kGradRuns; ++i)
+            if (c + i * TH < end) v[i] = load_logits<DT>(x + runs.begin(c + i * TH), runs.left(c + i * TH));
+    };
     typename G::Row o;
     o.zero = true;
-    if (learns) o = g.row(q, h, r, label, threadIdx.x & 63);
-    const bool works = learns && !o.zero;
-    if (PER > 1 || works) {
-        for (int i = lane; i < (int)((end - first + 31) / 32); i += TH) marks[wave][i] = 0;
-        __syncthreads();
-        if (works && lane < 64) {  // in the entries' order, so that what meets at a column adds up in it
-            int n = 0;
-            const int all = g.entries();
-            for (int j0 = 0; j0 < all + 1; j0 += 64) {
-                const int j = j0 + lane;
-                int64_t id = -1;
-                float extra = 0.0f;
-                bool in = false;
-                if (j < all) in = g.entry(o, q, h, j, id, extra);
-                else if (j == all && q.labels && o.label_extra != 0.0f) {
-                    id = label;
-                    extra = o.label_extra;
-                    in = (uint64_t)id < (uint64_t)q.vocab;
-                }
-                const int64_t run = in ? (id + runs.pad) / W : -1;
-                in = in && run >= first && run < end;
-                const uint64_t who = __ballot(in);
-                if (in) {
-                    const int at = n + (int)__popcll(who & (((uint64_t)1 << lane) - 1));
-                    ids[wave][at] = (uint32_t)id | (j == all ? 0x80000000u : 0u);
-                    extras[wave][at] = extra;
-                    atomicOr(&marks[wave][(run - first) >> 5], 1u << ((run - first) & 31));
-                }
-                n += (int)__popcll(who);
-            }
-            if (lane == 0) counts[wave] = n;
-        }
-        __syncthreads();
+    if (learns) {
+        load();
+        o = g.row(q, h, r, label, threadIdx.x & 63);
     }
+    const bool works = learns && !o.zero;
+    if (works && lane < 64) {  // in the entries' order, so that what meets at a column adds up in it
+        for (int i = lane; i < (int)((end - first + 31) / 32); i += 64) marks[wave][i] = 0;
+        int n = 0;
+        const int all = g.entries();
+        for (int j0 = 0; j0 < all + 1; j0 += 64) {
+            const int j = j0 + lane;
+            int64_t id = -1;
+            float extra = 0.0f;
+            bool in = false;
+            if (j < all) in = g.entry(o, q, h, j, id, extra);
+            else if (j == all && q.labels && o.label_extra != 0.0f) {
+                id = label;
+                extra = o.label_extra;
+                in = (uint64_t)id < (uint64_t)q.vocab;
+            }
+            const int64_t run = in ? (id + runs.pad) / W : -1;
+            in = in && run >= first && run < end;
+            const uint64_t who = __ballot(in);
+            if (in) {
+                const int at = n + (int)__popcll(who & (((uint64_t)1 << lane) - 1));
+                ids[wave][at] = (uint32_t)id | (j == all ? 0x80000000u : 0u);
+                extras[wave][at] = extra;
+                atomicOr(&marks[wave][(run - first) >> 5], 1u << ((run - first) & 31));
+            }
+            n += (int)__popcll(who);
+        }
+        if (lane == 0) counts[wave] = n;
+    }
+    if (PER > 1 || works) __syncthreads();
     if (!row) return;
-    c += lane;
     if (!works) {
         Run<T, W> zeros;
 #pragma unroll
@@ -904,33 +912,19 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
         for (; c < end; c += TH) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
         return;
     }
-    const T* x = (const T*)q.x + row_offset(q, r);
-    const auto marked = [&](int64_t run) { return marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1; };
-    const auto finish = [&](Run<T, W>& v) {
+    for (;;) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v.e[i] = from_f32<DT>(g.at(o, h, to_f32<DT>(v.e[i]), false));
-    };
-    const auto one = [&](int64_t run) {
-        const int64_t at = runs.begin(run), left = runs.left(run);
-        Run<T, W> v = load_logits<DT>(x + at, left);
-        finish(v);
-        if (!marked(run)) store_run<T, W>(out + at, left, v);
-    };
-    if (runs.at_start(c)) {
-        one(c);
-        c += TH;
-    }
-    for (; c + TH < whole; c += 2 * TH) {
-        Run<T, W> v[2];
+        for (int i = 0; i < kGradRuns; ++i) {
+            const int64_t run = c + i * TH;
+            if (run >= end) break;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + runs.begin(c + i * TH));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            finish(v[i]);
-            if (!marked(c + i * TH)) store_run<T, W>(out + runs.begin(c + i * TH), W, v[i]);
+            for (int k = 0; k < W; ++k) v[i].e[k] = from_f32<DT>(g.at(o, h, to_f32<DT>(v[i].e[k]), false));
+            if (!(marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1)) store_run<T, W>(out + runs.begin(run), runs.left(run), v[i]);
         }
+        c += kGradRuns * TH;
+        if (c >= end) break;
+        load();
     }
-    for (; c < end; c += TH) one(c);
     const int n = counts[wave];
     for (int i = lane; i < n; i += TH) {
         const int64_t run = ((int64_t)(ids[wave][i] & 0x7fffffffu) + runs.pad) / W;
@@ -1104,7 +1098,7 @@ int distill_forward(Distill& d, float* loss, float* divergence, float* nll, floa
 int distill_grad(const char* what, const gefenx_logits* l, const gefenx_teacher* t, const void* slopes, const float* weights,
                  const float* scale_dev, double scale, void* grad, void* stream) {
     Distill d;
-    const int rc = make_distill(what, l, t, kTokenGradPasses, d);
+    const int rc = make_distill(what, l, t, kGradRuns, d);
     if (rc != GEFENX_OK || d.q.rows == 0) return rc;
     if (!slopes || !weights || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
     const Downhill g = {static_cast<const Slope*>(slopes), weights, scale_dev, (float)scale, d.t};
@@ -1170,7 +1164,7 @@ int gefenx_token_statistics_grad(const gefenx_logits* logits, double temperature
     const char* what = "gefenx_token_statistics_grad";
     Rows q;
     Heat h;
-    int rc = marked_rows(what, logits, false, false, kTokenGradPasses, q);
+    int rc = marked_rows(what, logits, false, false, kGradRuns, q);
     if (rc == GEFENX_OK) rc = make_heat(what, temperature, h);
     if (rc != GEFENX_OK) return rc;
     if (top < 0 || top > kMaxTop) return set_error(GEFENX_EINVAL, "%s: top %d is not in [0, %d]", what, top, kMaxTop);
