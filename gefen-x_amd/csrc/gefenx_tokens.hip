@@ -18,7 +18,6 @@ constexpr int kMaxTop = 128;      // likeliest tokens of a row
 constexpr int kMaxTeacher = 512;  // a teacher's tokens of a row
 constexpr int kMergeKeys = 2048;  // candidates of a row's splits that are merged
 constexpr int kBits = 16384;      // runs of a workgroup's part of a row where some are marked
-constexpr int kGradRuns = 2;       // of a lane of the gradient in flight
 // Differences from the maximum stop here: exp is 0 from there at any temperature, and 0 times it is 0.
 constexpr float kFar = -1e25f;
 
@@ -752,8 +751,11 @@ struct Downhill {                // what the distillation's takes
     Teacher t;
 };
 
-// A row's gradient: an element by its logit, and what is added at some columns.
+// A row's gradient: an element by its logit, and what is added at some columns.  kRuns: runs of a lane in flight, and
+// all of a workgroup's; the statistics' row costs it more (4096 x 151936 bf16, 2 / 4 runs: 385 / 369 us; the
+// distillation of 8192 x 128256 581 / 612).
 struct StatisticsGrad {
+    static constexpr int kRuns = 4;
     Upstream g;
     __device__ __forceinline__ int entries() const { return g.top ? g.top_n : 0; }
     struct Row {
@@ -798,6 +800,7 @@ struct StatisticsGrad {
 
 template <bool PLAIN>
 struct DistillGrad {
+    static constexpr int kRuns = 2;
     Downhill g;
     __device__ __forceinline__ int entries() const { return g.t.top; }
     struct Row {
@@ -837,7 +840,7 @@ struct DistillGrad {
 };
 
 // The gradient of a split of a row, in runs of 16 bytes from the ends of cache lines.  Runs that hold a label or one
-// of the entries are marked, left out of the pass, and written element by element afterwards.
+// of the entries are marked; the lanes that have them look through the split's list.
 template <int DT, class G, int PER>
 __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, const G g, void* __restrict__ grad) {
     using T = typename Elem<DT>::T;
@@ -862,10 +865,10 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
     int64_t c = first + lane;
     // the logits are on their way while the row's numbers and entries are found
     const T* x = (const T*)q.x + row_offset(q, r);
-    Run<T, W> v[kGradRuns];
+    Run<T, W> v[G::kRuns];
     const auto load = [&]() {
 #pragma unroll
-        for (int i = 0; i < kGradRuns; ++i)
+        for (int i = 0; i < G::kRuns; ++i)
             if (c + i * TH < end) v[i] = load_logits<DT>(x + runs.begin(c + i * TH), runs.left(c + i * TH));
     };
     typename G::Row o;
@@ -912,37 +915,40 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
         for (; c < end; c += TH) store_run<T, W>(out + runs.begin(c), runs.left(c), zeros);
         return;
     }
+    const int n = counts[wave];
     for (;;) {
 #pragma unroll
-        for (int i = 0; i < kGradRuns; ++i) {
+        for (int i = 0; i < G::kRuns; ++i) {
             const int64_t run = c + i * TH;
             if (run >= end) break;
+            const int64_t at = runs.begin(run);
+            float y[W];
 #pragma unroll
-            for (int k = 0; k < W; ++k) v[i].e[k] = from_f32<DT>(g.at(o, h, to_f32<DT>(v[i].e[k]), false));
-            if (!(marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1)) store_run<T, W>(out + runs.begin(run), runs.left(run), v[i]);
+            for (int k = 0; k < W; ++k) y[k] = g.at(o, h, to_f32<DT>(v[i].e[k]), false);
+            if (marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1) {
+                float extra[W] = {};
+                uint32_t named = 0;
+                for (int j = 0; j < n; ++j) {
+                    const uint32_t id = ids[wave][j], off = (id & 0x7fffffffu) - (uint32_t)at;
+                    if (off >= (uint32_t)W) continue;
+                    const float e = extras[wave][j];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) extra[k] += (uint32_t)k == off ? e : 0.0f;
+                    named |= (id >> 31 ^ 1u) << off;
+                }
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    if (named >> k & 1) y[k] = g.at(o, h, to_f32<DT>(v[i].e[k]), true);
+                    y[k] += extra[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[i].e[k] = from_f32<DT>(y[k]);
+            store_run<T, W>(out + at, runs.left(run), v[i]);
         }
-        c += kGradRuns * TH;
+        c += G::kRuns * TH;
         if (c >= end) break;
         load();
-    }
-    const int n = counts[wave];
-    for (int i = lane; i < n; i += TH) {
-        const int64_t run = ((int64_t)(ids[wave][i] & 0x7fffffffu) + runs.pad) / W;
-        bool first_of = true;
-        for (int j = 0; j < i; ++j) first_of &= ((int64_t)(ids[wave][j] & 0x7fffffffu) + runs.pad) / W != run;
-        if (!first_of) continue;
-        const int64_t at = runs.begin(run), left = runs.left(run);
-        for (int k = 0; k < W && k < left; ++k) {
-            float extra = 0.0f;
-            bool teacher = false;
-            for (int j = 0; j < n; ++j) {
-                const uint32_t id = ids[wave][j];
-                if ((int64_t)(id & 0x7fffffffu) != at + k) continue;
-                extra += extras[wave][j];
-                teacher |= !(id >> 31);
-            }
-            *gbl(out + at + k) = from_f32<DT>(g.at(o, h, to_f32<DT>(*gbl(x + at + k)), teacher) + extra);
-        }
     }
 }
 
@@ -1098,7 +1104,7 @@ int distill_forward(Distill& d, float* loss, float* divergence, float* nll, floa
 int distill_grad(const char* what, const gefenx_logits* l, const gefenx_teacher* t, const void* slopes, const float* weights,
                  const float* scale_dev, double scale, void* grad, void* stream) {
     Distill d;
-    const int rc = make_distill(what, l, t, kGradRuns, d);
+    const int rc = make_distill(what, l, t, DistillGrad<false>::kRuns, d);
     if (rc != GEFENX_OK || d.q.rows == 0) return rc;
     if (!slopes || !weights || !grad) return set_error(GEFENX_EINVAL, "%s: null pointer", what);
     const Downhill g = {static_cast<const Slope*>(slopes), weights, scale_dev, (float)scale, d.t};
@@ -1164,7 +1170,7 @@ int gefenx_token_statistics_grad(const gefenx_logits* logits, double temperature
     const char* what = "gefenx_token_statistics_grad";
     Rows q;
     Heat h;
-    int rc = marked_rows(what, logits, false, false, kGradRuns, q);
+    int rc = marked_rows(what, logits, false, false, StatisticsGrad::kRuns, q);
     if (rc == GEFENX_OK) rc = make_heat(what, temperature, h);
     if (rc != GEFENX_OK) return rc;
     if (top < 0 || top > kMaxTop) return set_error(GEFENX_EINVAL, "%s: top %d is not in [0, %d]", what, top, kMaxTop);
