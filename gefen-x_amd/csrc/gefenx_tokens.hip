@@ -21,9 +21,10 @@ constexpr int kBits = 16384;      // runs of a workgroup's part of a row where s
 // Differences from the maximum stop here: exp is 0 from there at any temperature, and 0 times it is 0.
 constexpr float kFar = -1e25f;
 
-// exp(d / tau) = 2^(d (hi + lo)), hi + lo = log2(e) / tau.  lo > 0: -inf times either is -inf.
+// exp(d / tau) = 2^(d (hi + lo)), hi + lo = log2(e) / tau.  lo > 0: -inf times either is -inf.  inv_hi: 1 / hi; tilt:
+// (hi / (hi + lo) - 1) / tau.
 struct Heat {
-    float hi, lo, inv;
+    float hi, lo, inv, inv_hi, tilt;
     double inv64;
 };
 __device__ __forceinline__ float heat_exp(float d, const Heat& h) {
@@ -84,27 +85,89 @@ __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* 
     return a;
 }
 
+// Sums as a lane takes them over its logits: 2^(x hi - M) with M = m hi rounded is one fused operation where
+// 2^((x - m) (hi + lo)) is three (the statistics of 4096 x 128256 bf16 are bound by such operations as much as by
+// memory).  What M's rounding and hi's make of the sums is known and put right in sums(): 2^(m hi - M) for all of
+// them, and by hi alone s grows by (hi / (hi + lo) - 1) sum z exp(z), which u gives; without u the product with lo is
+// taken too.  Beyond kHuge, where x hi may overflow (rows of the type's lowest value), the difference is taken first.
+constexpr float kHuge = 1e30f;
+template <int U> struct LaneSums {
+    float m = -__builtin_inff(), s = 0.0f, u = 0.0f, minus = 0.0f, minus1 = 0.0f;  // -M, and that of exp(x)
+    __device__ __forceinline__ bool huge() const { return __builtin_fabsf(m) > kHuge && m != -__builtin_inff(); }
+    __device__ __forceinline__ void rebase(float m2, const Heat& h) {
+        if (!(m2 > m)) return;
+        const float next = -(m2 * h.hi), next1 = -(m2 * kLog2e);
+        if (m != -__builtin_inff()) {
+            const bool apart = huge() || __builtin_fabsf(m2) > kHuge;
+            const float d = apart ? (m - m2) * h.hi : next - minus, f = __builtin_amdgcn_exp2f(d);
+            if (U == kEntropy) u = f * __builtin_fmaf(s, __builtin_fmaxf(d, kFar), u);
+            if (U == kPlain) u *= __builtin_amdgcn_exp2f(apart ? (m - m2) * kLog2e : next1 - minus1);
+            s *= f;
+        }
+        m = m2;
+        minus = next;
+        minus1 = next1;
+    }
+    __device__ __forceinline__ void exponent(float y) {
+        const float e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        if (U == kEntropy) u = __builtin_fmaf(__builtin_fmaxf(y, kFar), e, u);
+    }
+    __device__ __forceinline__ void add(float x, const Heat& h) {
+        const float y = __builtin_fmaf(x, h.hi, minus);
+        exponent(U == kEntropy ? y : __builtin_fmaf(x, h.lo, y));
+        if (U == kPlain) u += __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, minus1)));
+    }
+    __device__ __forceinline__ void add_far(float x, const Heat& h) {
+        const float d = x - m;
+        exponent(d * h.hi);
+        if (U == kPlain) u += exp_(d);
+    }
+    __device__ __forceinline__ Sums<U> sums(const Heat& h) const {
+        Sums<U> a;
+        a.m = m;
+        float off = 0.0f, off1 = 0.0f;
+        if (m != -__builtin_inff() && !huge()) {
+            off = __builtin_fmaf(m, h.hi, minus);
+            if (U != kEntropy) off = __builtin_fmaf(m, h.lo, off);
+            off1 = __builtin_fmaf(m, kLog2eRest, __builtin_fmaf(m, kLog2e, minus1));
+        }
+        const float f = __builtin_amdgcn_exp2f(-off);
+        a.s = s * f;
+        if (U == kEntropy) {
+            a.u = __builtin_fmaf(-off, s, u) * f * h.inv_hi;
+            a.s = __builtin_fmaf(-h.tilt, a.u, a.s);
+        }
+        if (U == kPlain) a.u = u * __builtin_amdgcn_exp2f(-off1);
+        return a;
+    }
+};
+
 // Adds N runs; their maximum.
 template <int DT, int U, int N>
-__device__ __forceinline__ float add_runs(Sums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, const Heat& h) {
+__device__ __forceinline__ float add_runs(LaneSums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, const Heat& h) {
     float top = -__builtin_inff();
 #pragma unroll
     for (int c = 0; c < N; ++c)
 #pragma unroll
         for (int k = 0; k < kW<DT>; ++k) top = __builtin_fmaxf(top, to_f32<DT>(r[c].e[k]));
     a.rebase(top, h);
-    const float b = a.base();
+    if (a.huge()) {
+        for (int c = 0; c < N; ++c)
+            for (int k = 0; k < kW<DT>; ++k) a.add_far(to_f32<DT>(r[c].e[k]), h);
+    } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c)
+        for (int c = 0; c < N; ++c)
 #pragma unroll
-        for (int k = 0; k < kW<DT>; ++k) a.add(to_f32<DT>(r[c].e[k]), b, h);
+            for (int k = 0; k < kW<DT>; ++k) a.add(to_f32<DT>(r[c].e[k]), h);
+    }
     return top;
 }
 
 constexpr int kStep = 4;  // runs of a lane in flight
 
 // Runs begin .. end - 1 of a row, TH lanes at a time in steps of kStep runs each; each lane's sums.  skip(run): a
-// run that is left out; note(step, maximum): what a lane found in each step.  Which logits a lane adds up does not
+// run that is left out; note(maximum): what a lane found in a step.  Which logits a lane adds up does not
 // depend on where the row starts in memory.
 template <int DT, int U, int TH, bool STREAM, class Skip, class Note>
 __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t begin, int64_t end, int lane,
@@ -113,9 +176,8 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
     constexpr int W = kW<DT>;
     const int64_t whole = end * W <= vocab ? end : end - 1;
     const int64_t last = end * W < vocab ? end * W : vocab;  // column behind the part
-    Sums<U> a;
+    LaneSums<U> a;
     int64_t c = begin;
-    int step = 0;
     const auto put = [&](Run<T, W>& v, int64_t run) {
         if (skip(run)) {
 #pragma unroll
@@ -123,13 +185,13 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
         }
     };
     const auto add = [&](auto load) {
-        for (; c + kStep * TH <= whole; c += kStep * TH, ++step) {
+        for (; c + kStep * TH <= whole; c += kStep * TH) {
             Run<T, W> v[kStep];
 #pragma unroll
             for (int i = 0; i < kStep; ++i) v[i] = load(x + (c + lane + i * TH) * W);
 #pragma unroll
             for (int i = 0; i < kStep; ++i) put(v[i], c + lane + i * TH);
-            note(step, add_runs<DT, U, kStep>(a, v, h));
+            note(add_runs<DT, U, kStep>(a, v, h));
         }
     };
     if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT, STREAM>(p); });
@@ -148,9 +210,9 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
             if (c + lane + i * TH < end) put(v[i], c + lane + i * TH);
             top = __builtin_fmaxf(top, add_runs<DT, U, 1>(a, v + i, h));
         }
-        note(step, top);
+        note(top);
     }
-    return a;
+    return a.sums(h);
 }
 
 // ------------------------------------------------------------ the likeliest tokens
@@ -168,28 +230,43 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 // Order and column as one number: of equal logits the lower column is the larger.  0 is no logit.
 __device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t column) { return (uint64_t)order << 32 | (uint32_t)~column; }
 
-struct Select {
+// A barrier of a group of lanes: a workgroup, or a wave of it.
+template <int TH> __device__ __forceinline__ void meet() {
+    if constexpr (TH == kT) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int TH> struct Select {
     uint32_t bins[256];
     uint32_t count, digit, above;
-    uint32_t waves[kT / 64];
+    uint32_t waves[TH / 64];
 };
 
-// The first `want` columns of first .. last - 1 whose order is `order`, as keys; waves: of kT / 64.
-template <int DT>
+// The first `want` columns of first .. last - 1 whose order is `order`, as keys; waves: of TH / 64.
+template <int DT, int TH>
 __device__ __forceinline__ void first_equal(const typename Elem<DT>::T* x, int64_t first, int64_t last, uint32_t order,
                                             uint32_t want, uint32_t* waves, uint64_t* __restrict__ out) {
+    const int lane = threadIdx.x % TH;
     uint32_t taken = 0;
-    for (int64_t begin = first; taken < want && begin < last; begin += kT) {
-        const int64_t v = begin + threadIdx.x;
+    for (int64_t begin = first; taken < want && begin < last; begin += TH) {
+        const int64_t v = begin + lane;
         const bool equal = v < last && order_of(to_f32<DT>(*gbl(x + v))) == order;
         const uint64_t who = __ballot(equal);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = (uint32_t)__popcll(who);
-        __syncthreads();
-        uint32_t before = taken + (uint32_t)__popcll(who & (((uint64_t)1 << (threadIdx.x & 63)) - 1));
-        for (int w = 0; w < kT / 64; ++w) {
-            if (w < (int)(threadIdx.x >> 6)) before += waves[w];
-            taken += waves[w];
+        uint32_t before = taken + (uint32_t)__popcll(who & (((uint64_t)1 << (lane & 63)) - 1));
+        if constexpr (TH == 64) {
+            taken += (uint32_t)__popcll(who);
+        } else {
+            __syncthreads();
+            if ((lane & 63) == 0) waves[lane >> 6] = (uint32_t)__popcll(who);
+            __syncthreads();
+            for (int w = 0; w < TH / 64; ++w) {
+                if (w < lane >> 6) before += waves[w];
+                taken += waves[w];
+            }
         }
         if (equal && before < want) out[before] = key_of(order, (uint32_t)v);
     }
@@ -198,60 +275,67 @@ __device__ __forceinline__ void first_equal(const typename Elem<DT>::T* x, int64
 // The `top` largest keys of columns first .. last - 1 of a row, in no order, 0 behind them, by digits of 8 bits of
 // the order from the highest: after the last one the order of the top-th largest is known, larger ones are taken as
 // they come, equal ones by column.
-template <int DT>
-__device__ __forceinline__ void select_keys(const typename Elem<DT>::T* x, int64_t first, int64_t last, int top, Select& at,
+template <int DT, int TH>
+__device__ __forceinline__ void select_keys(const typename Elem<DT>::T* x, int64_t first, int64_t last, int top, Select<TH>& at,
                                             uint64_t* __restrict__ out) {
+    const int lane = threadIdx.x % TH;
     const auto order = [&](int64_t v) { return order_of(to_f32<DT>(*gbl(x + v))); };
     if (last - first <= top) {
-        for (int64_t i = threadIdx.x; i < top; i += kT) out[i] = first + i < last ? key_of(order(first + i), (uint32_t)(first + i)) : 0;
+        for (int64_t i = lane; i < top; i += TH) out[i] = first + i < last ? key_of(order(first + i), (uint32_t)(first + i)) : 0;
         return;
     }
     uint32_t prefix = 0, mask = 0, want = (uint32_t)top;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        at.bins[threadIdx.x] = 0;
+        meet<TH>();
+        for (int i = lane; i < 256; i += TH) at.bins[i] = 0;
         at.count = 0;
-        __syncthreads();
-        for (int64_t v = first + threadIdx.x; v < last; v += kT) {
+        meet<TH>();
+        for (int64_t v = first + lane; v < last; v += TH) {
             const uint32_t o = order(v);
             if ((o & mask) == prefix) atomicAdd(&at.bins[o >> shift & 255], 1u);
         }
-        __syncthreads();
-        if (threadIdx.x == 0) {
+        meet<TH>();
+        if (lane == 0) {
             uint32_t above = 0, d = 255;
             while (d > 0 && above + at.bins[d] < want) above += at.bins[d--];
             at.digit = d;
             at.above = above;
         }
-        __syncthreads();
+        meet<TH>();
         want -= at.above;
         prefix |= at.digit << shift;
         mask |= 255u << shift;
     }
-    for (int64_t v = first + threadIdx.x; v < last; v += kT) {
+    for (int64_t v = first + lane; v < last; v += TH) {
         const uint32_t o = order(v);
         if (o > prefix) out[atomicAdd(&at.count, 1u)] = key_of(o, (uint32_t)v);
     }
-    first_equal<DT>(x, first, last, prefix, want, at.waves, out + (top - want));
+    first_equal<DT, TH>(x, first, last, prefix, want, at.waves, out + (top - want));
 }
 
-// The want-th largest (want <= kT) of the orders that a workgroup's lanes bring, by bits from the highest; every wave
-// looks through all of them, four to a lane.
+// The want-th largest (want <= TH) of the orders that a group's lanes bring, or 0, by bits from the highest that the
+// type's values tell apart; every wave looks through all of them, TH / 64 to a lane.
+template <int DT, int TH>
 __device__ __forceinline__ uint32_t largest_of_lanes(uint32_t own, int want, uint32_t* all) {
-    all[threadIdx.x] = own;
-    __syncthreads();
-    uint32_t v[kT / 64];
+    constexpr int kLast = DT == F32 ? 0 : DT == F16 ? 13 : 16, N = TH / 64;
+    uint32_t v[N] = {own};
+    if constexpr (N > 1) {
+        all[threadIdx.x] = own;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kT / 64; ++i) v[i] = all[i * 64 + (threadIdx.x & 63)];
+        for (int i = 0; i < N; ++i) v[i] = all[i * 64 + (threadIdx.x & 63)];
+    }
     uint32_t found = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+#pragma unroll 4
+    for (int bit = 31; bit >= kLast; --bit) {
         const uint32_t next = found | 1u << bit;
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < kT / 64; ++i) n += (int)__popcll(__ballot(v[i] >= next));
+        for (int i = 0; i < N; ++i) n += (int)__popcll(__ballot(v[i] >= next));
         if (n >= want) found = next;
     }
-    return found;
+    // below, a value's order has zeros where it is positive and ones where it is negative
+    return found | (found >> 31 || found == 0 ? 0 : (1u << kLast) - 1);
 }
 
 // What the rows come to.
@@ -296,9 +380,9 @@ __device__ __forceinline__ void top_result(const Heat& h, const Statistics& out,
 }
 
 // The place of each of n keys (no two alike) among them: put(place, key) for the `top` largest.
-template <class Put>
+template <int TH, class Put>
 __device__ __forceinline__ void by_rank(const uint64_t* keys, int n, int top, Put&& put) {
-    for (int i = threadIdx.x; i < n; i += kT) {
+    for (int i = threadIdx.x % TH; i < n; i += TH) {
         const uint64_t key = keys[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += keys[j] > key ? 1 : 0;
@@ -306,34 +390,37 @@ __device__ __forceinline__ void by_rank(const uint64_t* keys, int n, int top, Pu
     }
 }
 
-constexpr int kSlots = 20;        // of a lane: the maxima of its steps
-// Candidates that there is room for; short rows may have all of their logits among them.
-__host__ __device__ constexpr int room(int slots) { return slots > 4 ? 512 : 1024; }
-constexpr int kSuspects = 384;    // slots that are looked through again
-struct Hunt {
-    uint32_t orders[kT];
-    uint16_t suspects[kSuspects];
+// Maxima of a lane's steps that are kept; how many of them are looked through again, and candidates that there is room
+// for (short rows may have all of their logits among them).
+constexpr int kSlots = 20, kWaveSlots = (int)kShortRuns / (64 * kStep);
+constexpr int kWaveTop = 32;  // likeliest tokens that a wave finds for a row of its own
+template <int TH> constexpr int kSuspects = TH == kT ? 384 : 128;
+template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 512 : 1024; }
+template <int TH> struct Hunt {
+    uint32_t orders[TH == kT ? kT : TH / 64];
+    uint16_t suspects[kSuspects<TH>];
     uint32_t n_suspects, n_candidates;
     double log_sum_exp;
 };
 
 // part[row][split] = the sums of a split of a row, keys[row][split][top] its largest, 0 where there are fewer; a whole
-// row's results at once.  PER rows to a workgroup: one, or one for each of its waves (rows without splits, no keys).
+// row's results at once.  PER rows to a workgroup: one, or one for each of its waves (rows without splits).
 //
 // The likeliest tokens cost the pass a maximum of each step of a lane, kept in LDS.  The top-th largest of the lanes'
 // maxima is a bound that at least `top` logits reach; the few steps that reach it are read again, what reaches it in
 // them are the candidates, and counting the larger ones gives each its place.  More candidates than there is room for
-// (equal logits), NaN and +inf go through select_keys.
+// (equal logits) are those over the bound and the first of the equal ones; NaN, +inf and what is left go through
+// select_keys.
 template <int DT, int PER, bool TOP>
 __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, const Statistics out,
                                                    float4* __restrict__ part, uint64_t* __restrict__ keys) {
     using T = typename Elem<DT>::T;
     constexpr int TH = kT / PER, W = kW<DT>;
     __shared__ float4 waves[kT / 64];
-    __shared__ std::conditional_t<TOP, Hunt, char> hunt_;
+    __shared__ std::conditional_t<TOP, Hunt<TH>, char> hunts[PER];
     extern __shared__ uint64_t dynamic[];
-    const int lane = threadIdx.x % TH;
-    const int64_t at = (int64_t)blockIdx.x * PER + (PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0);
+    const int lane = threadIdx.x % TH, wave = PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
+    const int64_t at = (int64_t)blockIdx.x * PER + wave;
     const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
     if (r >= q.rows) return;
     const int64_t label = q.labels ? sload(q.labels + r) : 0;
@@ -346,11 +433,21 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
     const T* x = (const T*)q.x + row_offset(q, r);
     const auto none = [](int64_t) { return false; };
-    float* tops = reinterpret_cast<float*>(dynamic);
-    const auto note = [&](int step, float m) {
+    const int slots = TOP && begin < end ? (int)(((end - begin + kStep * TH - 1) / (kStep * TH) + steps_of_slot - 1) / steps_of_slot) : 0;
+    uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1)) : 0);
+    float* tops = reinterpret_cast<float*>(own_lds);
+    float* slot = tops + lane;
+    float held = -__builtin_inff();
+    int to_go = steps_of_slot;
+    const auto note = [&](float m) {
         if constexpr (TOP) {
-            float* slot = tops + step / steps_of_slot * kT + threadIdx.x;
-            *slot = step % steps_of_slot ? __builtin_fmaxf(*slot, m) : m;
+            held = __builtin_fmaxf(held, m);
+            *slot = held;
+            if (--to_go == 0) {
+                to_go = steps_of_slot;
+                held = -__builtin_inff();
+                slot += TH;
+            }
         }
     };
     Sums<kEntropy> a = q.cached ? row_sums<DT, kEntropy, TH, false>(x, q.vocab, begin, end, lane, h, none, note)
@@ -364,34 +461,34 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
     } else {
-        Hunt& hunt = hunt_;
-        if (threadIdx.x == 0) {
+        Hunt<TH>& hunt = hunts[wave];
+        if (lane == 0) {
             hunt.n_suspects = hunt.n_candidates = 0;
             if (alone) hunt.log_sum_exp = row_results<DT>(q, h, out, r, label, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
-        const float bound = value_of(largest_of_lanes(order_of(own), top, hunt.orders));  // a barrier inside
-        const int64_t steps = begin < end ? (end - begin + kStep * TH - 1) / (kStep * TH) : 0;
-        const int slots = (int)((steps + steps_of_slot - 1) / steps_of_slot), each = kStep * steps_of_slot;  // runs of a slot
+        const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, hunt.orders));  // a barrier inside
+        meet<TH>();
+        const int each = kStep * steps_of_slot;  // runs of a slot
         const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
         uint64_t* mine = keys + at * top;
-        uint64_t* candidates = dynamic + kT / 2 * slots;  // behind the maxima
-        const uint32_t most = room(slots);
+        uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
+        const uint32_t most = room<TH>(slots);
         // those that reach the bound, or (above) that are over it; whether there was room for all
         const auto gather = [&](bool above) {
             for (int i = 0; i < slots; ++i) {
-                const float m = tops[i * kT + threadIdx.x];
+                const float m = tops[i * TH + lane];
                 if (above ? m > bound : m >= bound) {
                     const uint32_t n = atomicAdd(&hunt.n_suspects, 1u);
-                    if (n < kSuspects) hunt.suspects[n] = (uint16_t)(i * kT + threadIdx.x);
+                    if (n < kSuspects<TH>) hunt.suspects[n] = (uint16_t)(i * TH + lane);
                 }
             }
-            __syncthreads();
+            meet<TH>();
             const uint32_t suspects = hunt.n_suspects;
-            if (suspects > kSuspects) return false;
-            for (int i = threadIdx.x; i < (int)suspects * each; i += kT) {
-                const int s = hunt.suspects[i / each], slot = s / kT, who = s % kT;
-                const int64_t run = begin + who + ((int64_t)slot * each + i % each) * TH, col = run * W;
+            if (suspects > kSuspects<TH>) return false;
+            for (int i = lane; i < (int)suspects * each; i += TH) {
+                const int s = hunt.suspects[i / each], place = s / TH, who = s % TH;
+                const int64_t run = begin + who + ((int64_t)place * each + i % each) * TH, col = run * W;
                 if (run >= end) continue;
                 const Run<T, W> v = load_logits<DT, false>(x + col, last - col);
 #pragma unroll
@@ -403,40 +500,40 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
                     }
                 }
             }
-            __syncthreads();
+            meet<TH>();
             return hunt.n_candidates <= most;
         };
         bool found = a.s == a.s && gather(false);
-        if (!found && a.s == a.s) {  // many are equal to the bound: those over it, then the first of the others
-            __syncthreads();
-            if (threadIdx.x == 0) hunt.n_suspects = hunt.n_candidates = 0;
-            __syncthreads();
+        if (!found && a.s == a.s) {
+            meet<TH>();
+            if (lane == 0) hunt.n_suspects = hunt.n_candidates = 0;
+            meet<TH>();
             found = gather(true);
             const uint32_t over = hunt.n_candidates;
             if (found && over < (uint32_t)top) {
-                first_equal<DT>(x, first, last, order_of(bound), (uint32_t)top - over, hunt.orders, candidates + over);
-                __syncthreads();
-                if (threadIdx.x == 0) hunt.n_candidates = (uint32_t)(last - first < top ? last - first : top);
-                __syncthreads();
+                first_equal<DT, TH>(x, first, last, order_of(bound), (uint32_t)top - over, hunt.orders, candidates + over);
+                meet<TH>();
+                if (lane == 0) hunt.n_candidates = (uint32_t)(last - first < top ? last - first : top);
+                meet<TH>();
             }
         }
         if (!found) {
-            __syncthreads();
-            select_keys<DT>(x, first, last, top, *reinterpret_cast<Select*>(dynamic), mine);
+            meet<TH>();
+            select_keys<DT, TH>(x, first, last, top, *reinterpret_cast<Select<TH>*>(own_lds), mine);
             if (!alone) return;
             __threadfence_block();
-            __syncthreads();
-            for (int i = threadIdx.x; i < top; i += kT) dynamic[i] = mine[i];
-            __syncthreads();
-            by_rank(dynamic, top, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+            meet<TH>();
+            for (int i = lane; i < top; i += TH) own_lds[i] = mine[i];
+            meet<TH>();
+            by_rank<TH>(own_lds, top, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
             return;
         }
         const int n = (int)hunt.n_candidates;
         if (alone) {
-            by_rank(candidates, n, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+            by_rank<TH>(candidates, n, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
         } else {
-            for (int i = n + threadIdx.x; i < top; i += kT) mine[i] = 0;
-            by_rank(candidates, n, top, [&](int rank, uint64_t key) { mine[rank] = key; });
+            for (int i = n + lane; i < top; i += TH) mine[i] = 0;
+            by_rank<TH>(candidates, n, top, [&](int rank, uint64_t key) { mine[rank] = key; });
         }
     }
 }
@@ -480,12 +577,12 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
         }
     }
     if constexpr (TOP) {
-        const uint32_t bound = largest_of_lanes((uint32_t)(most >> 32), top, orders);
+        const uint32_t bound = largest_of_lanes<DT, kT>((uint32_t)(most >> 32), top, orders);
 #pragma unroll
         for (int i = 0; i < kMergeKeys / kT; ++i)
             if (own[i] != 0 && (uint32_t)(own[i] >> 32) >= bound) candidates[atomicAdd(&count, 1u)] = own[i];
         __syncthreads();
-        by_rank(candidates, (int)count, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, log_sum_exp); });
+        by_rank<kT>(candidates, (int)count, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, log_sum_exp); });
     }
 }
 
@@ -540,7 +637,7 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
     if (!counts) return;
     const T* x = (const T*)q.x + row_offset(q, r);
     const auto skip = [&](int64_t run) { return BUCKET && (mine[(run - begin) >> 5] >> ((run - begin) & 31) & 1); };
-    const auto note = [](int, float) {};
+    const auto note = [](float) {};
     Sums<U> a = q.cached ? row_sums<DT, U, TH, false>(x, q.vocab, begin, end, lane, h, skip, note)
                          : row_sums<DT, U, TH, true>(x, q.vocab, begin, end, lane, h, skip, note);
     if constexpr (PER > 1) wave_join(a, h);
@@ -962,6 +1059,8 @@ int make_heat(const char* what, double temperature, Heat& h) {
     h.lo = (float)(c - (double)h.hi);
     h.inv64 = 1.0 / temperature;
     h.inv = (float)h.inv64;
+    h.inv_hi = (float)(1.0 / (double)h.hi);
+    h.tilt = (float)(((double)h.hi / c - 1.0) * h.inv64);
     return GEFENX_OK;
 }
 
@@ -979,7 +1078,7 @@ int statistics_rows(const char* what, const gefenx_logits* l, int top, Rows& q) 
     const int rc = make_rows(what, l, false, q, 0, false);
     if (rc != GEFENX_OK) return rc;
     if (top > l->vocab) return set_error(GEFENX_EINVAL, "%s: top %d of %lld logits", what, top, (long long)l->vocab);
-    if (top && q.per > 1) {
+    if (top > kWaveTop && q.per > 1) {
         q.per = 1;
         set_splits(*l, q, 1);
     }
@@ -1144,11 +1243,14 @@ int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int
     const Statistics out = {logps, entropy, top_logps, top_ids, reinterpret_cast<float4*>(stats)};
     return by_dtype(logits->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (top) {
+        if (top && q.per > 1) {
+            const size_t lds = kT / 64 * (sizeof(float) * 64 * kWaveSlots + sizeof(uint64_t) * room<64>(1));
+            k_statistics<DT, kT / 64, true><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, lds, s>>>(q, h, top, 1, out, part, keys);
+        } else if (top) {
             constexpr int W = kW<DT>;
             const int64_t runs = std::min(q.split_runs, (q.vocab + W - 1) / W), steps = (runs + kStep * kT - 1) / (kStep * kT);
             const int per = (int)((steps + kSlots - 1) / kSlots), slots = (int)((steps + per - 1) / per);
-            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * room(slots);
+            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * room<kT>(slots);
             k_statistics<DT, 1, true><<<(uint32_t)(q.rows * q.splits), kT, lds, s>>>(q, h, top, per, out, part, keys);
             if (q.splits > 1) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
         } else if (q.per > 1) {
