@@ -14,6 +14,7 @@
 namespace gx {
 namespace {
 
+constexpr int64_t kCus = 256;
 constexpr int kMaxTop = 128;      // likeliest tokens of a row
 constexpr int kMaxTeacher = 512;  // a teacher's tokens of a row
 constexpr int kMergeKeys = 2048;  // candidates of a row's splits that are merged
@@ -1072,26 +1073,37 @@ void set_splits(const gefenx_logits& l, Rows& q, int64_t splits) {
     q.splits = (int32_t)((runs + q.split_runs - 1) / q.split_runs);
 }
 
+// How a row is split for its sums.  A split is a round of dependent reads and joins of its own, and its results go through
+// a second kernel, so rows are split only where there are fewer than two workgroups a CU, and into no less than 4 passes
+// (statistics with 20 tokens, us, whole / 2 / 4 / 8 / 16 splits: 1 x 128256 bf16 20 / 18 / 15 / 13 / 12, 64 x 151936
+// 23 / 21 / 17 / 16 / 18, 400 x 50257, 25 passes, 19 / 24 / 25 / 29 / 40, 400 x 151936 fp32 58 / 51 / 55 / 57 / 63;
+// 4096 x 128256 with 64 tokens 197 / 232 / 265 in 4).
+void split_sums(const gefenx_logits& l, Rows& q) {
+    if (q.per > 1) return;
+    const int64_t passes = (l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2) + 16 * kT - 1) / (16 * kT);
+    const int64_t wanted = (2 * kCus + q.rows - 1) / std::max<int64_t>(q.rows, 1);
+    set_splits(l, q, passes < 32 ? 1 : std::min(wanted, passes / 4));
+}
+
 // How rows are split for the statistics with `top` keys a split.
 int statistics_rows(const char* what, const gefenx_logits* l, int top, Rows& q) {
     if (top < 0 || top > kMaxTop) return set_error(GEFENX_EINVAL, "%s: top %d is not in [0, %d]", what, top, kMaxTop);
     const int rc = make_rows(what, l, false, q, 0, false);
     if (rc != GEFENX_OK) return rc;
     if (top > l->vocab) return set_error(GEFENX_EINVAL, "%s: top %d of %lld logits", what, top, (long long)l->vocab);
-    if (top > kWaveTop && q.per > 1) {
-        q.per = 1;
-        set_splits(*l, q, 1);
-    }
+    if (top > kWaveTop) q.per = 1;
+    split_sums(*l, q);
     if (top && q.splits * top > kMergeKeys) set_splits(*l, q, kMergeKeys / top);
     if (q.rows * q.splits > kMaxThreads / kT)
         return set_error(GEFENX_EINVAL, "%s: too many rows (%lld)", what, (long long)l->rows);
     return GEFENX_OK;
 }
 
-// ... and where runs of a split are marked.
+// ... and where runs of a split are marked; most: the most passes of the gradient, 0: for the sums.
 int marked_rows(const char* what, const gefenx_logits* l, bool sequences, bool labelled, int64_t most, Rows& q) {
     const int rc = make_rows(what, l, sequences, q, most, labelled);
     if (rc != GEFENX_OK) return rc;
+    if (!most) split_sums(*l, q);
     if (q.split_runs > kBits) set_splits(*l, q, q.splits * ((q.split_runs + kBits - 1) / kBits) + 1);
     if (q.split_runs > kBits || q.rows * q.splits > kMaxThreads / kT)
         return set_error(GEFENX_EINVAL, "%s: too many logits (%lld x %lld)", what, (long long)l->rows, (long long)l->vocab);
