@@ -109,19 +109,20 @@ template <int U> struct LaneSums {
         minus = next;
         minus1 = next1;
     }
-    __device__ __forceinline__ void exponent(float y) {
+    // FAR: y may be -inf, whose exponential of 0 times it would be NaN
+    template <bool FAR> __device__ __forceinline__ void exponent(float y) {
         const float e = __builtin_amdgcn_exp2f(y);
         s += e;
-        if (U == kEntropy) u = __builtin_fmaf(__builtin_fmaxf(y, kFar), e, u);
+        if (U == kEntropy) u = __builtin_fmaf(FAR ? __builtin_fmaxf(y, kFar) : y, e, u);
     }
-    __device__ __forceinline__ void add(float x, const Heat& h) {
+    template <bool FAR> __device__ __forceinline__ void add(float x, const Heat& h) {
         const float y = __builtin_fmaf(x, h.hi, minus);
-        exponent(U == kEntropy ? y : __builtin_fmaf(x, h.lo, y));
+        exponent<FAR>(U == kEntropy ? y : __builtin_fmaf(x, h.lo, y));
         if (U == kPlain) u += __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, minus1)));
     }
     __device__ __forceinline__ void add_far(float x, const Heat& h) {
         const float d = x - m;
-        exponent(d * h.hi);
+        exponent<true>(d * h.hi);
         if (U == kPlain) u += exp_(d);
     }
     __device__ __forceinline__ Sums<U> sums(const Heat& h) const {
@@ -144,23 +145,60 @@ template <int U> struct LaneSums {
     }
 };
 
+// The largest of N runs; fp16 goes two at a time.
+template <int DT, int N>
+__device__ __forceinline__ float largest(const Run<typename Elem<DT>::T, kW<DT>>* r) {
+    if constexpr (DT == F16) {
+        typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+        H2 top = {-__builtin_inff16(), -__builtin_inff16()};
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            H2 v[kW<DT> / 2];
+            __builtin_memcpy(v, &r[c], sizeof(v));
+#pragma unroll
+            for (int k = 0; k < kW<DT> / 2; ++k) top = __builtin_elementwise_max(top, v[k]);
+        }
+        return __builtin_fmaxf((float)top.x, (float)top.y);
+    } else {
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+#pragma unroll
+            for (int k = 0; k < kW<DT>; ++k) top = __builtin_fmaxf(top, to_f32<DT>(r[c].e[k]));
+        return top;
+    }
+}
+
 // Adds N runs; their maximum.
 template <int DT, int U, int N>
 __device__ __forceinline__ float add_runs(LaneSums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, const Heat& h) {
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-        for (int k = 0; k < kW<DT>; ++k) top = __builtin_fmaxf(top, to_f32<DT>(r[c].e[k]));
+    const float top = largest<DT, N>(r);
     a.rebase(top, h);
-    if (a.huge()) {
-        for (int c = 0; c < N; ++c)
-            for (int k = 0; k < kW<DT>; ++k) a.add_far(to_f32<DT>(r[c].e[k]), h);
-    } else {
+    const float s = a.s, u = a.u;
+    if (!a.huge()) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
 #pragma unroll
-            for (int k = 0; k < kW<DT>; ++k) a.add(to_f32<DT>(r[c].e[k]), h);
+            for (int k = 0; k < kW<DT>; ++k) a.template add<false>(to_f32<DT>(r[c].e[k]), h);
+    }
+    if (a.huge() || (U == kEntropy && a.u != a.u && a.s == a.s)) {  // again: among them were huge ones, or -inf
+        a.s = s;
+        a.u = u;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            // from the words anew: values kept for here would cost the pass its registers
+            u32x4 words;
+            __builtin_memcpy(&words, &r[c], sizeof(words));
+            asm volatile("" : "+v"(words));
+            Run<typename Elem<DT>::T, kW<DT>> v;
+            __builtin_memcpy(&v, &words, sizeof(v));
+#pragma unroll
+            for (int k = 0; k < kW<DT>; ++k) {
+                const float x = to_f32<DT>(v.e[k]);
+                if (a.huge()) a.add_far(x, h);
+                else a.template add<true>(x, h);
+            }
+        }
     }
     return top;
 }
@@ -358,18 +396,19 @@ __device__ __forceinline__ void ignored_row(const Statistics& out, int64_t r, in
     }
 }
 
-// A row's sums to its results, by one lane; log sum exp(x / tau).
 template <int DT>
+__device__ __forceinline__ float label_logit(const Rows& q, const typename Elem<DT>::T* x, int64_t label) {
+    return q.labels && (uint64_t)label < (uint64_t)q.vocab ? to_f32<DT>(*gbl(x + label)) : 0.0f;
+}
+
+// A row's sums and its label's logit x to its results, by one lane; log sum exp(x / tau).
 __device__ __forceinline__ double row_results(const Rows& q, const Heat& h, const Statistics& out, int64_t r, int64_t label,
-                                              const Sums<kEntropy>& a) {
-    using T = typename Elem<DT>::T;
+                                              float x, const Sums<kEntropy>& a) {
     const double log_sum = log((double)a.s);
     const float entropy = (float)(log_sum - (double)a.u / (double)a.s * h.inv64);
-    if (out.logps) {
-        const bool in = label >= 0 && label < q.vocab;
-        const float x = in ? to_f32<DT>(*gbl((const T*)q.x + row_offset(q, r) + label)) : 0.0f;
-        out.logps[r] = in ? (float)(((double)x - (double)a.m) * h.inv64 - log_sum) : __uint_as_float(0x7fc00000u);
-    }
+    if (out.logps)
+        out.logps[r] = (uint64_t)label < (uint64_t)q.vocab ? (float)(((double)x - (double)a.m) * h.inv64 - log_sum)
+                                                           : __uint_as_float(0x7fc00000u);
     out.entropy[r] = entropy;
     out.stats[r] = make_float4(a.m, a.s, (float)log_sum, entropy);
     return (double)a.m * h.inv64 + log_sum;
@@ -433,6 +472,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     const int64_t runs = (q.vocab + W - 1) / W, begin = split * q.split_runs;
     const int64_t end = begin + q.split_runs < runs ? begin + q.split_runs : runs;
     const T* x = (const T*)q.x + row_offset(q, r);
+    const float xl = alone ? label_logit<DT>(q, x, label) : 0.0f;  // on its way early
     const auto none = [](int64_t) { return false; };
     const int slots = TOP && begin < end ? (int)(((end - begin + kStep * TH - 1) / (kStep * TH) + steps_of_slot - 1) / steps_of_slot) : 0;
     uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1)) : 0);
@@ -458,14 +498,14 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     else a = group_join(a, h, waves);
     if constexpr (!TOP) {
         if (lane == 0) {
-            if (alone) row_results<DT>(q, h, out, r, label, a);
+            if (alone) row_results(q, h, out, r, label, xl, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
     } else {
         Hunt<TH>& hunt = hunts[wave];
         if (lane == 0) {
             hunt.n_suspects = hunt.n_candidates = 0;
-            if (alone) hunt.log_sum_exp = row_results<DT>(q, h, out, r, label, a);
+            if (alone) hunt.log_sum_exp = row_results(q, h, out, r, label, xl, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
         const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, hunt.orders));  // a barrier inside
@@ -566,6 +606,7 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
         if (threadIdx.x == 0) count = 0;
     }
     if (!TOP || threadIdx.x < 64) {
+        const float xl = label_logit<DT>(q, (const typename Elem<DT>::T*)q.x + row_offset(q, r), label);
         Sums<kEntropy> a;
         for (int i = lane; i < q.splits; i += TOP ? 64 : lanes) {
             const float4 p = part[r * q.splits + i];
@@ -573,7 +614,7 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
         }
         wave_join(a, h, TOP ? 64 : lanes);
         if (lane == 0) {
-            const double lse = row_results<DT>(q, h, out, r, label, a);
+            const double lse = row_results(q, h, out, r, label, xl, a);
             if (TOP) log_sum_exp = lse;
         }
     }
