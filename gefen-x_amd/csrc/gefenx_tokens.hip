@@ -353,25 +353,33 @@ __device__ __forceinline__ void select_keys(const typename Elem<DT>::T* x, int64
 }
 
 // The want-th largest (want <= TH) of the orders that a group's lanes bring, or 0, by bits from the highest that the
-// type's values tell apart; every wave looks through all of them, TH / 64 to a lane.
+// type's values tell apart.  A workgroup's first wave looks through all of them, four to a lane, the others wait.
 template <int DT, int TH>
 __device__ __forceinline__ uint32_t largest_of_lanes(uint32_t own, int want, uint32_t* all) {
     constexpr int kLast = DT == F32 ? 0 : DT == F16 ? 13 : 16, N = TH / 64;
-    uint32_t v[N] = {own};
+    uint32_t v[N] = {own}, found = 0;
     if constexpr (N > 1) {
         all[threadIdx.x] = own;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = all[i * 64 + (threadIdx.x & 63)];
     }
-    uint32_t found = 0;
-#pragma unroll 4
-    for (int bit = 31; bit >= kLast; --bit) {
-        const uint32_t next = found | 1u << bit;
-        int n = 0;
+    if (N == 1 || threadIdx.x < 64) {
+        if constexpr (N > 1) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) n += (int)__popcll(__ballot(v[i] >= next));
-        if (n >= want) found = next;
+            for (int i = 0; i < N; ++i) v[i] = all[i * 64 + threadIdx.x];
+        }
+#pragma unroll 4
+        for (int bit = 31; bit >= kLast; --bit) {
+            const uint32_t next = found | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) n += (int)__popcll(__ballot(v[i] >= next));
+            if (n >= want) found = next;
+        }
+    }
+    if constexpr (N > 1) {
+        if (threadIdx.x == 0) all[0] = found;
+        __syncthreads();
+        found = all[0];
     }
     // below, a value's order has zeros where it is positive and ones where it is negative
     return found | (found >> 31 || found == 0 ? 0 : (1u << kLast) - 1);
@@ -419,13 +427,21 @@ __device__ __forceinline__ void top_result(const Heat& h, const Statistics& out,
     out.top_logps[at] = (float)((double)value_of((uint32_t)(key >> 32)) * h.inv64 - log_sum_exp);
 }
 
-// The place of each of n keys (no two alike) among them: put(place, key) for the `top` largest.
+// The place of each of n keys (no two alike) among them: put(place, key) for the `top` largest.  keys: at a multiple of
+// 16 bytes, and room for one more.
 template <int TH, class Put>
-__device__ __forceinline__ void by_rank(const uint64_t* keys, int n, int top, Put&& put) {
+__device__ __forceinline__ void by_rank(uint64_t* keys, int n, int top, Put&& put) {
+    if (threadIdx.x % TH == 0) keys[n] = 0;
+    meet<TH>();
+    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(keys);
     for (int i = threadIdx.x % TH; i < n; i += TH) {
         const uint64_t key = keys[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += keys[j] > key ? 1 : 0;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 two = pairs[j / 2];
+            rank += (two.x > key ? 1 : 0) + (two.y > key ? 1 : 0);
+        }
         if (rank < top) put(rank, key);
     }
 }
@@ -435,7 +451,7 @@ __device__ __forceinline__ void by_rank(const uint64_t* keys, int n, int top, Pu
 constexpr int kSlots = 20, kWaveSlots = (int)kShortRuns / (64 * kStep);
 constexpr int kWaveTop = 32;  // likeliest tokens that a wave finds for a row of its own
 template <int TH> constexpr int kSuspects = TH == kT ? 384 : 128;
-template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 512 : 1024; }
+template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 512 : 1024; }  // and one more
 template <int TH> struct Hunt {
     uint32_t orders[TH == kT ? kT : TH / 64];
     uint16_t suspects[kSuspects<TH>];
@@ -458,7 +474,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     constexpr int TH = kT / PER, W = kW<DT>;
     __shared__ float4 waves[kT / 64];
     __shared__ std::conditional_t<TOP, Hunt<TH>, char> hunts[PER];
-    extern __shared__ uint64_t dynamic[];
+    extern __shared__ __align__(16) uint64_t dynamic[];
     const int lane = threadIdx.x % TH, wave = PER > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
     const int64_t at = (int64_t)blockIdx.x * PER + wave;
     const int64_t r = PER > 1 ? at : at / (uint32_t)q.splits, split = PER > 1 ? 0 : at % (uint32_t)q.splits;
@@ -475,7 +491,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     const float xl = alone ? label_logit<DT>(q, x, label) : 0.0f;  // on its way early
     const auto none = [](int64_t) { return false; };
     const int slots = TOP && begin < end ? (int)(((end - begin + kStep * TH - 1) / (kStep * TH) + steps_of_slot - 1) / steps_of_slot) : 0;
-    uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1)) : 0);
+    uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1) + 2) : 0);
     float* tops = reinterpret_cast<float*>(own_lds);
     float* slot = tops + lane;
     float held = -__builtin_inff();
@@ -584,7 +600,7 @@ template <int DT, bool TOP>
 __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat h, int top, const Statistics out,
                                                         const float4* __restrict__ part, const uint64_t* __restrict__ keys,
                                                         int lanes) {
-    __shared__ uint64_t candidates[TOP ? kMergeKeys : 1];
+    __shared__ __align__(16) uint64_t candidates[TOP ? kMergeKeys + 2 : 1];
     __shared__ uint32_t orders[TOP ? kT : 1];
     __shared__ uint32_t count;
     __shared__ double log_sum_exp;
@@ -687,27 +703,22 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
     if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
 }
 
-// From a row's sums to its loss and slope, a wave per row, in float64: the divergence is what is left of terms that
-// cancel.  BUCKET: the runs with tokens of the teacher are added up here, the others apart from the teacher's.
+// What a wave finds of a row's teacher: mass and sum of p (log p - z) over its tokens (one outside of the vocabulary
+// makes them NaN), and, BUCKET, the sums over its tokens and over what else is in their runs.
+template <int U> struct Known {
+    double mass = 0.0, cross = 0.0, log_mass = 0.0;
+    Sums<U> tokens, others;
+};
+
+// ids: room for the teacher's ids, of this wave alone.
 template <int DT, int U, bool BUCKET>
-__global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h, const Teacher t, const float4* __restrict__ part,
-                                                     double2* __restrict__ each, float* __restrict__ divergence,
-                                                     Slope* __restrict__ slopes) {
+__device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, const Teacher& t, int64_t r,
+                                               const typename Elem<DT>::T* x, int32_t* ids) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>;
-    __shared__ int32_t ids[kMaxTeacher];
-    const int64_t r = blockIdx.x, label = sload(q.labels + r);
-    const int lane = threadIdx.x;
-    if (label == q.ignore || (q.n_seq > 0 && seq_of(q, r) < 0)) {
-        if (lane == 0) {
-            each[r] = make_double2(0.0, 0.0);
-            divergence[r] = 0.0f;
-        }
-        return;
-    }
-    const T* x = (const T*)q.x + row_offset(q, r);
-    // mass and sum of p (log p - z) over the teacher's tokens; one outside of the vocabulary makes the row NaN
-    double mass = 0.0, cross = 0.0;
+    const int lane = threadIdx.x & 63;
+    Known<U> o;
+    Run<T, W> held_run;  // of the lane's first token
     for (int j = lane; j < t.top; j += 64) {
         const int64_t id = teacher_id(t, r * t.top + j);
         const float lp = *gbl(t.logps + r * t.top + j);
@@ -715,68 +726,82 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
         ids[j] = held && in ? (int32_t)id : -1;
         if (!held) continue;
         const double p = in ? exp((double)lp) : __longlong_as_double(0x7ff8000000000000ll);
-        mass += p;
-        if (p > 0.0) cross += p * ((double)lp - (in ? (double)to_f32<DT>(*gbl(x + id)) * h.inv64 : 0.0));
+        o.mass += p;
+        const float v = in ? to_f32<DT>(*gbl(x + id)) : 0.0f;
+        if (BUCKET && in && j == lane) held_run = load_logits<DT, false>(x + id / W * W, q.vocab - id / W * W);
+        if (p > 0.0) o.cross += p * ((double)lp - (double)v * h.inv64);
     }
-    __syncthreads();
-    mass = wave_allsum_d(mass);
-    cross = wave_allsum_d(cross);
-    double log_mass = 0.0;
+    meet<64>();
+    o.mass = wave_allsum_d(o.mass);
+    o.cross = wave_allsum_d(o.cross);
     if (t.rest == kNormalize) {
         // the same sum with p / mass: log p - log mass
-        const bool some = !(mass <= 0.0);
-        log_mass = some ? log(mass) : 0.0;
-        cross = some ? cross / mass - log_mass : 0.0;
-        mass = some ? mass / mass : 0.0;
+        const bool some = !(o.mass <= 0.0);
+        o.log_mass = some ? log(o.mass) : 0.0;
+        o.cross = some ? o.cross / o.mass - o.log_mass : 0.0;
+        o.mass = some ? o.mass / o.mass : 0.0;
     }
-    Sums<U> a;
-    for (int i = lane; i < q.splits; i += 64) {
-        const float4 p = part[r * q.splits + i];
-        a.join(p.x, p.y, p.z, h);
-    }
-    Sums<U> known;
     if constexpr (BUCKET) {
         for (int j = lane; j < t.top; j += 64) {
             const int32_t id = ids[j];
             if (id < 0) continue;
+            const int32_t start = id / W * W;
             bool first = true, first_run = true;
-            for (int i = 0; i < j; ++i) {
-                first &= ids[i] != id;
-                first_run &= ids[i] < 0 || ids[i] / W != id / W;
+            uint32_t named = 0;
+#pragma unroll 4
+            for (int i = 0; i < t.top; ++i) {
+                const int32_t other = ids[i];
+                const uint32_t off = (uint32_t)(other - start);  // of no token: far
+                if (off < (uint32_t)W) {
+                    named |= 1u << off;
+                    first_run &= i >= j;
+                    first &= i >= j || other != id;
+                }
+            }
+            if (!first_run && !first) continue;
+            const Run<T, W> run = j == lane ? held_run : load_logits<DT, false>(x + start, q.vocab - start);
+            float own = 0.0f, top = -__builtin_inff(), v[W];
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                const float f = to_f32<DT>(run.e[k]);
+                own = start + k == id ? f : own;
+                v[k] = named >> k & 1 ? -__builtin_inff() : f;  // beyond the row's end -inf too
+                top = __builtin_fmaxf(top, v[k]);
             }
             if (first) {
-                const float v = to_f32<DT>(*gbl(x + id));
-                known.rebase(v, h);
-                known.add(v, known.base(), h);
+                o.tokens.rebase(own, h);
+                o.tokens.add(own, o.tokens.base(), h);
             }
             if (!first_run) continue;
-            const int32_t start = id / W * W;
-            uint32_t taken = 0;
-            for (int i = 0; i < t.top; ++i) {
-                const uint32_t off = (uint32_t)(ids[i] - start);
-                if (ids[i] >= 0 && off < (uint32_t)W) taken |= 1u << off;
-            }
-            for (int k = 0; k < W; ++k) {
-                if (taken >> k & 1 || start + k >= q.vocab) continue;
-                const float v = to_f32<DT>(*gbl(x + start + k));
-                a.rebase(v, h);
-                a.add(v, a.base(), h);
-            }
+            o.others.rebase(top, h);
+            const float base = o.others.base();
+#pragma unroll
+            for (int k = 0; k < W; ++k) o.others.add(v[k], base, h);
         }
-        wave_join(known, h);
+        wave_join(o.tokens, h);
+        wave_join(o.others, h);
     }
-    wave_join(a, h);
+    return o;
+}
+
+// A row's loss and slope by the sums a over the logits outside of the teacher's runs (BUCKET, else over all) and the
+// teacher's part, in float64: the divergence is what is left of terms that cancel.
+template <int DT, int U, bool BUCKET>
+__device__ __forceinline__ Slope row_slope(const Rows& q, const Heat& h, const Teacher& t, int64_t label, float label_x, Sums<U> a,
+                                           const Known<U>& known, double2& each) {
     Sums<U> total = a;
-    if constexpr (BUCKET) total.join(known.m, known.s, known.u, h);
-    if (lane != 0) return;
-    const double sum = (double)total.s, log_sum = log(sum), m = (double)total.m;
-    double d = cross + mass * (m * h.inv64 + log_sum), rest = 0.0, other = 0.0;
-    Slope s = {};
+    if constexpr (BUCKET) {
+        a.join(known.others.m, known.others.s, known.others.u, h);
+        total = a;
+        total.join(known.tokens.m, known.tokens.s, known.tokens.u, h);
+    }
+    const double sum = (double)total.s, log_sum = log(sum), m = (double)total.m, mass = known.mass;
+    double d = known.cross + mass * (m * h.inv64 + log_sum), rest = 0.0, other = 0.0;
     if constexpr (BUCKET) {
         if (mass < 1.0 && a.s != 0.0f) {
             rest = 1.0 - mass;
             // the teacher's tokens against the others, the log of 1 / rho - 1
-            const double odds = log((double)known.s / (double)a.s) + ((double)known.m - (double)a.m) * h.inv64;
+            const double odds = log((double)known.tokens.s / (double)a.s) + ((double)known.tokens.m - (double)a.m) * h.inv64;
             d += rest * (log1p(-mass) + (odds > 50.0 ? odds : log1p(exp(odds))));
             other = rest / (double)a.s;
         }
@@ -787,8 +812,8 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
     double mine = t.soft * whole / sum, others = t.soft * (whole / sum * shift - other), plain = 0.0, nll = 0.0;
     if (t.hard > 0.0) {
         const double sum1 = U == kPlain ? (double)total.u : sum;
-        const bool in = label >= 0 && label < q.vocab;
-        nll = in ? log(sum1) - ((double)to_f32<DT>(*gbl(x + label)) - m) : __longlong_as_double(0x7ff8000000000000ll);
+        const bool in = (uint64_t)label < (uint64_t)q.vocab;
+        nll = in ? log(sum1) - ((double)label_x - m) : __longlong_as_double(0x7ff8000000000000ll);
         if (U == kPlain) {
             plain = t.hard / sum1;
         } else {
@@ -797,23 +822,69 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
         }
         if (!in) mine = others = nll;
     }
-    each[r] = make_double2(d, nll);
-    divergence[r] = (float)d;
+    each = make_double2(d, nll);
+    Slope s = {};
     s.m = total.m;
     s.other_m = apart ? a.m : total.m;
     s.mine = (float)mine;
     s.other = (float)others;
     s.plain = (float)plain;
-    s.log_mass = (float)log_mass;
-    slopes[r] = s;
+    s.log_mass = (float)known.log_mass;
+    return s;
+}
+
+// From the splits' sums of a row to its loss and slope, a wave per row: it waits for two dependent reads.
+template <int DT, int U, bool BUCKET>
+__global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h, const Teacher t, const float4* __restrict__ part,
+                                                     double2* __restrict__ each, float* __restrict__ divergence,
+                                                     Slope* __restrict__ slopes) {
+    using T = typename Elem<DT>::T;
+    __shared__ __align__(16) int32_t ids[kMaxTeacher];
+    const int64_t r = blockIdx.x, label = sload(q.labels + r);
+    if (label == q.ignore || (q.n_seq > 0 && seq_of(q, r) < 0)) {
+        if (threadIdx.x == 0) {
+            each[r] = make_double2(0.0, 0.0);
+            divergence[r] = 0.0f;
+        }
+        return;
+    }
+    const T* x = (const T*)q.x + row_offset(q, r);
+    const float label_x = label_logit<DT>(q, x, label);
+    Sums<U> a;
+    for (int i = threadIdx.x; i < q.splits; i += 64) {
+        const float4 p = part[r * q.splits + i];
+        a.join(p.x, p.y, p.z, h);
+    }
+    const Known<U> known = known_part<DT, U, BUCKET>(q, h, t, r, x, ids);
+    wave_join(a, h);
+    if (threadIdx.x != 0) return;
+    double2 e;
+    slopes[r] = row_slope<DT, U, BUCKET>(q, h, t, label, label_x, a, known, e);
+    each[r] = e;
+    divergence[r] = (float)e.x;
 }
 
 struct DistillSums {
     double divergence, nll, n;
 };
 
-// One workgroup per sequence, or one for all rows where there are none.
-__global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const double2* __restrict__ each, DistillSums* __restrict__ sums) {
+struct DistillTotals {
+    float *loss, *divergence, *nll, *weights;
+    double soft, hard;
+    int32_t n_seq, by_sequence;
+};
+
+__device__ __forceinline__ void distill_total(const DistillTotals& o, double divergence, double nll) {
+    // a part of weight 0 is not there, whatever it would be
+    *o.loss = (float)((o.soft != 0.0 ? o.soft * divergence : 0.0) + (o.hard != 0.0 ? o.hard * nll : 0.0));
+    *o.divergence = (float)divergence;
+    *o.nll = (float)nll;
+}
+
+// Sums over rows, one workgroup per sequence, or one for all rows where there are none; one alone gives the loss and
+// the weight too.  each: null where only the rows are counted.
+__global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const double2* __restrict__ each, DistillSums* __restrict__ sums,
+                                                        const DistillTotals out) {
     __shared__ DistillSums waves[kSeqT / 64];
     int64_t begin = 0, end = q.rows;
     if (q.n_seq > 0) {
@@ -823,57 +894,56 @@ __global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const doub
     begin = begin < 0 ? 0 : begin;
     end = end > q.rows ? q.rows : end;
     DistillSums own = {0.0, 0.0, 0.0};
+#pragma unroll 4
     for (int64_t r = begin + threadIdx.x; r < end; r += kSeqT) {
-        if (*gbl(q.labels + r) == q.ignore) continue;
-        const double2 e = each[r];
-        own.divergence += e.x;
-        own.nll += e.y;
-        own.n += 1.0;
+        const bool counts = *gbl(q.labels + r) != q.ignore;
+        const double2 e = each ? each[r] : make_double2(0.0, 0.0);  // of every row
+        own.divergence += counts ? e.x : 0.0;
+        own.nll += counts ? e.y : 0.0;
+        own.n += counts ? 1.0 : 0.0;
     }
     own.divergence = wave_sum_d(own.divergence);
     own.nll = wave_sum_d(own.nll);
     own.n = wave_sum_d(own.n);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = own;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kSeqT / 64; ++w) {
-            own.divergence += waves[w].divergence;
-            own.nll += waves[w].nll;
-            own.n += waves[w].n;
-        }
-        sums[blockIdx.x] = own;
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kSeqT / 64; ++w) {
+        own.divergence += waves[w].divergence;
+        own.nll += waves[w].nll;
+        own.n += waves[w].n;
     }
+    if (gridDim.x > 1) {
+        sums[blockIdx.x] = own;
+        return;
+    }
+    const double w = own.n > 0.0 ? 1.0 / own.n : 0.0;
+    out.weights[0] = (float)w;
+    distill_total(out, w > 0.0 ? own.divergence * w : 0.0, w > 0.0 ? own.nll * w : 0.0);
 }
 
-// Loss, means of both parts, weights per sequence.
-__global__ __launch_bounds__(kT) void k_distill_total(const DistillSums* __restrict__ sums, int n_seq, int by_sequence, const Teacher t,
-                                                      float* __restrict__ loss_out, float* __restrict__ divergence_out,
-                                                      float* __restrict__ nll_out, float* __restrict__ weights) {
+// Loss, means of both parts, weights per sequence, where there are several.
+__global__ __launch_bounds__(kT) void k_distill_total(const DistillSums* __restrict__ sums, const DistillTotals out) {
     __shared__ double waves[kT / 64];
     double n = 0.0, seqs = 0.0;
-    for (int i = threadIdx.x; i < n_seq; i += kT) {
+    for (int i = threadIdx.x; i < out.n_seq; i += kT) {
         n += sums[i].n;
         seqs += sums[i].n > 0.0 ? 1.0 : 0.0;
     }
     n = block_sum(n, waves);
     seqs = block_sum(seqs, waves);
     double divergence = 0.0, nll = 0.0;
-    for (int i = threadIdx.x; i < n_seq; i += kT) {
-        const double w = sums[i].n > 0.0 ? (by_sequence ? 1.0 / (sums[i].n * seqs) : 1.0 / n) : 0.0;
+    for (int i = threadIdx.x; i < out.n_seq; i += kT) {
+        const double w = sums[i].n > 0.0 ? (out.by_sequence ? 1.0 / (sums[i].n * seqs) : 1.0 / n) : 0.0;
         if (w > 0.0) {
             divergence += sums[i].divergence * w;
             nll += sums[i].nll * w;
         }
-        weights[i] = (float)w;
+        out.weights[i] = (float)w;
     }
     divergence = block_sum(divergence, waves);
     nll = block_sum(nll, waves);
-    if (threadIdx.x == 0) {
-        // a part of weight 0 is not there, whatever it would be
-        *loss_out = (float)((t.loss != 0.0 ? t.loss * divergence : 0.0) + (t.hard != 0.0 ? t.hard * nll : 0.0));
-        *divergence_out = (float)divergence;
-        *nll_out = (float)nll;
-    }
+    if (threadIdx.x == 0) distill_total(out, divergence, nll);
 }
 
 // ------------------------------------------------------------ gradients
@@ -1179,6 +1249,9 @@ struct Distill {
     float4* part;
     double2* each;
     DistillSums* sums;
+    float* token_divergence;
+    Slope* slopes;
+    DistillTotals out;
     size_t bytes;
     hipStream_t s;
 };
@@ -1209,10 +1282,18 @@ int make_distill(const char* what, const gefenx_logits* l, const gefenx_teacher*
     return GEFENX_OK;
 }
 
-int distill_forward(Distill& d, float* loss, float* divergence, float* nll, float* token_divergence, void* slopes, float* weights,
+// The loss and the weights by the rows' results, or (each null) the weights alone.
+int distill_totals(const Distill& d, const double2* each) {
+    const int n = std::max(d.q.n_seq, 1);
+    k_distill_sums<<<(uint32_t)n, kSeqT, 0, d.s>>>(d.q, each, d.sums, d.out);
+    if (n > 1) k_distill_total<<<1, kT, 0, d.s>>>(d.sums, d.out);
+    return launched(d.what);
+}
+
+int distill_outputs(Distill& d, float* loss, float* divergence, float* nll, float* token_divergence, void* slopes, float* weights,
                     void* workspace, size_t workspace_bytes, void* stream) {
     const char* what = d.what;
-    int rc = enough(what, workspace, workspace_bytes, d.bytes);
+    const int rc = enough(what, workspace, workspace_bytes, d.bytes);
     if (rc != GEFENX_OK) return rc;
     if (!loss || !divergence || !nll || !weights || (d.q.rows > 0 && (!token_divergence || !slopes)))
         return set_error(GEFENX_EINVAL, "%s: null pointer", what);
@@ -1221,6 +1302,15 @@ int distill_forward(Distill& d, float* loss, float* divergence, float* nll, floa
     d.each = reinterpret_cast<double2*>(ws + sums_bytes(d.q));
     d.sums = reinterpret_cast<DistillSums*>(d.each + d.q.rows);
     d.s = static_cast<hipStream_t>(stream);
+    d.token_divergence = token_divergence;
+    d.slopes = static_cast<Slope*>(slopes);
+    d.out = DistillTotals{loss, divergence, nll, weights, d.t.loss, d.t.hard, d.q.n_seq, d.by_sequence};
+    return GEFENX_OK;
+}
+
+int distill_forward(Distill& d) {
+    const char* what = d.what;
+    int rc = GEFENX_OK;
     const Rows& q = d.q;
     const bool plain = d.t.hard > 0.0 && d.h.inv64 != 1.0;
     if (q.rows > 0) {
@@ -1231,8 +1321,8 @@ int distill_forward(Distill& d, float* loss, float* divergence, float* nll, floa
                 constexpr bool B = decltype(bucket)::value;
                 if (q.per > 1) k_distill<DT, U, B, kT / 64><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, d.s>>>(q, d.h, d.t, d.part);
                 else k_distill<DT, U, B, 1><<<(uint32_t)(q.rows * q.splits), kT, 0, d.s>>>(q, d.h, d.t, d.part);
-                k_distill_rows<DT, U, B><<<(uint32_t)q.rows, 64, 0, d.s>>>(q, d.h, d.t, d.part, d.each, token_divergence,
-                                                                         static_cast<Slope*>(slopes));
+                k_distill_rows<DT, U, B><<<(uint32_t)q.rows, 64, 0, d.s>>>(q, d.h, d.t, d.part, d.each, d.token_divergence,
+                                                                         d.slopes);
             };
             using N = std::integral_constant<int, kNone>;
             using P = std::integral_constant<int, kPlain>;
@@ -1247,10 +1337,7 @@ int distill_forward(Distill& d, float* loss, float* divergence, float* nll, floa
         });
         if (rc != GEFENX_OK) return rc;
     }
-    const int n = std::max(q.n_seq, 1);
-    k_distill_sums<<<(uint32_t)n, kSeqT, 0, d.s>>>(q, d.each, d.sums);
-    k_distill_total<<<1, kT, 0, d.s>>>(d.sums, n, d.by_sequence, d.t, loss, divergence, nll, weights);
-    return launched(what);
+    return distill_totals(d, d.each);
 }
 
 int distill_grad(const char* what, const gefenx_logits* l, const gefenx_teacher* t, const void* slopes, const float* weights,
@@ -1297,13 +1384,13 @@ int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int
     return by_dtype(logits->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (top && q.per > 1) {
-            const size_t lds = kT / 64 * (sizeof(float) * 64 * kWaveSlots + sizeof(uint64_t) * room<64>(1));
+            const size_t lds = kT / 64 * (sizeof(float) * 64 * kWaveSlots + sizeof(uint64_t) * (room<64>(1) + 2));
             k_statistics<DT, kT / 64, true><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, lds, s>>>(q, h, top, 1, out, part, keys);
         } else if (top) {
             constexpr int W = kW<DT>;
             const int64_t runs = std::min(q.split_runs, (q.vocab + W - 1) / W), steps = (runs + kStep * kT - 1) / (kStep * kT);
             const int per = (int)((steps + kSlots - 1) / kSlots), slots = (int)((steps + per - 1) / per);
-            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * room<kT>(slots);
+            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * (room<kT>(slots) + 2);
             k_statistics<DT, 1, true><<<(uint32_t)(q.rows * q.splits), kT, lds, s>>>(q, h, top, per, out, part, keys);
             if (q.splits > 1) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
         } else if (q.per > 1) {
@@ -1346,9 +1433,10 @@ int gefenx_distillation_loss(const gefenx_logits* logits, const gefenx_teacher* 
                              float* nll, float* token_divergence, float* slopes, float* weights, void* workspace,
                              size_t workspace_bytes, void* stream) {
     Distill d;
-    const int rc = make_distill("gefenx_distillation_loss", logits, teacher, 0, d);
-    if (rc != GEFENX_OK) return rc;
-    return distill_forward(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    int rc = make_distill("gefenx_distillation_loss", logits, teacher, 0, d);
+    if (rc == GEFENX_OK)
+        rc = distill_outputs(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    return rc == GEFENX_OK ? distill_forward(d) : rc;
 }
 
 int gefenx_distillation_grad(const gefenx_logits* logits, const gefenx_teacher* teacher, const float* slopes,
@@ -1363,7 +1451,9 @@ int gefenx_distillation_loss_grad(const gefenx_logits* logits, const gefenx_teac
     Distill d;
     int rc = make_distill(what, logits, teacher, 0, d);
     if (rc == GEFENX_OK && d.q.rows > 0 && !grad) rc = set_error(GEFENX_EINVAL, "%s: null pointer", what);
-    if (rc == GEFENX_OK) rc = distill_forward(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    if (rc == GEFENX_OK)
+        rc = distill_outputs(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    if (rc == GEFENX_OK) rc = distill_forward(d);
     return rc == GEFENX_OK ? distill_grad(what, logits, teacher, slopes, weights, scale_dev, scale, grad, stream) : rc;
 }
 
