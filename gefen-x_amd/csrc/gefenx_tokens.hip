@@ -65,11 +65,19 @@ template <int U> struct Sums {
     }
 };
 
+// The sums of a group of lanes, in every one of them: to their maximum first, then plain sums.
 template <int U>
 __device__ __forceinline__ void wave_join(Sums<U>& a, const Heat& h, int lanes = 64) {
+    float top = a.m;
+    for (int off = lanes >> 1; off > 0; off >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, off, 64));
+    const float d = a.m - (top == -__builtin_inff() ? 0.0f : top), f = heat_exp(d, h);
+    if (U == kEntropy) a.u = f * __builtin_fmaf(a.s, __builtin_fmaxf(d, kFar), a.u);
+    if (U == kPlain) a.u *= exp_(d);
+    a.s *= f;
+    a.m = top;
     for (int off = lanes >> 1; off > 0; off >>= 1) {
-        const float m2 = __shfl_xor(a.m, off, 64), s2 = __shfl_xor(a.s, off, 64), u2 = __shfl_xor(a.u, off, 64);
-        a.join(m2, s2, u2, h);
+        a.s += __shfl_xor(a.s, off, 64);
+        if (U != kNone) a.u += __shfl_xor(a.u, off, 64);
     }
 }
 
@@ -785,35 +793,39 @@ __device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, con
 }
 
 // A row's loss and slope by the sums a over the logits outside of the teacher's runs (BUCKET, else over all) and the
-// teacher's part, in float64: the divergence is what is left of terms that cancel.
+// teacher's part, in float64: the divergence is what is left of terms that cancel.  By a whole wave: its lanes take the
+// logarithms and exponentials side by side, each of which is a hundred operations.
 template <int DT, int U, bool BUCKET>
 __device__ __forceinline__ Slope row_slope(const Rows& q, const Heat& h, const Teacher& t, int64_t label, float label_x, Sums<U> a,
                                            const Known<U>& known, double2& each) {
+    const int lane = threadIdx.x & 63;
     Sums<U> total = a;
     if constexpr (BUCKET) {
         a.join(known.others.m, known.others.s, known.others.u, h);
         total = a;
         total.join(known.tokens.m, known.tokens.s, known.tokens.u, h);
     }
-    const double sum = (double)total.s, log_sum = log(sum), m = (double)total.m, mass = known.mass;
-    double d = known.cross + mass * (m * h.inv64 + log_sum), rest = 0.0, other = 0.0;
-    if constexpr (BUCKET) {
-        if (mass < 1.0 && a.s != 0.0f) {
-            rest = 1.0 - mass;
-            // the teacher's tokens against the others, the log of 1 / rho - 1
-            const double odds = log((double)known.tokens.s / (double)a.s) + ((double)known.tokens.m - (double)a.m) * h.inv64;
-            d += rest * (log1p(-mass) + (odds > 50.0 ? odds : log1p(exp(odds))));
-            other = rest / (double)a.s;
-        }
-    }
-    const double whole = mass + rest;
+    const double sum = (double)total.s, m = (double)total.m, mass = known.mass;
     const bool apart = BUCKET && a.s != 0.0f;
-    const double shift = apart ? exp(((double)a.m - m) * h.inv64) : 1.0;
+    const double rest = apart && mass < 1.0 ? 1.0 - mass : 0.0;
+    // the teacher's tokens against the others is 1 / rho - 1; so far apart that 1 is lost: its log alone
+    const double gap = ((double)known.tokens.m - (double)a.m) * h.inv64;
+    double shift = 1.0, odds = 0.0;
+    if (apart) {
+        const double e = exp(lane == 0 ? ((double)a.m - m) * h.inv64 : fmin(gap, 600.0));
+        shift = __shfl(e, 0, 64);
+        odds = (double)known.tokens.s / (double)a.s * (gap > 600.0 ? 1.0 : __shfl(e, 1, 64));
+    }
+    const double sum1 = U == kPlain ? (double)total.u : sum;
+    const double log_of = log(lane == 0 ? sum : lane == 1 ? sum1 : lane == 2 ? rest : gap > 600.0 ? odds : 1.0 + odds);
+    const double log_sum = __shfl(log_of, 0, 64), log_sum1 = __shfl(log_of, 1, 64), log_rest = __shfl(log_of, 2, 64);
+    const double log_odds = __shfl(log_of, 3, 64) + (gap > 600.0 ? gap : 0.0);
+    const double d = known.cross + mass * (m * h.inv64 + log_sum) + (rest > 0.0 ? rest * (log_rest + log_odds) : 0.0);
+    const double whole = mass + rest, other = rest > 0.0 ? rest / (double)a.s : 0.0;
     double mine = t.soft * whole / sum, others = t.soft * (whole / sum * shift - other), plain = 0.0, nll = 0.0;
     if (t.hard > 0.0) {
-        const double sum1 = U == kPlain ? (double)total.u : sum;
         const bool in = (uint64_t)label < (uint64_t)q.vocab;
-        nll = in ? log(sum1) - ((double)label_x - m) : __longlong_as_double(0x7ff8000000000000ll);
+        nll = in ? log_sum1 - ((double)label_x - m) : __longlong_as_double(0x7ff8000000000000ll);
         if (U == kPlain) {
             plain = t.hard / sum1;
         } else {
@@ -857,9 +869,10 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
     }
     const Known<U> known = known_part<DT, U, BUCKET>(q, h, t, r, x, ids);
     wave_join(a, h);
-    if (threadIdx.x != 0) return;
     double2 e;
-    slopes[r] = row_slope<DT, U, BUCKET>(q, h, t, label, label_x, a, known, e);
+    const Slope s = row_slope<DT, U, BUCKET>(q, h, t, label, label_x, a, known, e);
+    if (threadIdx.x != 0) return;
+    slopes[r] = s;
     each[r] = e;
     divergence[r] = (float)e.x;
 }
