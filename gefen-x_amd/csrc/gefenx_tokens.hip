@@ -81,7 +81,7 @@ __device__ __forceinline__ void wave_join(Sums<U>& a, const Heat& h, int lanes =
     }
 }
 
-template <int U>
+template <int U, int TH = kT>
 __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* waves) {
     wave_join(a, h);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float4(a.m, a.s, a.u, 0.0f);
@@ -90,7 +90,7 @@ __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* 
     a.s = waves[0].y;
     a.u = waves[0].z;
 #pragma unroll
-    for (int w = 1; w < kT / 64; ++w) a.join(waves[w].x, waves[w].y, waves[w].z, h);
+    for (int w = 1; w < TH / 64; ++w) a.join(waves[w].x, waves[w].y, waves[w].z, h);
     return a;
 }
 
@@ -714,19 +714,32 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
 // What a wave finds of a row's teacher: mass and sum of p (log p - z) over its tokens (one outside of the vocabulary
 // makes them NaN), and, BUCKET, the sums over its tokens and over what else is in their runs.
 template <int U> struct Known {
-    double mass = 0.0, cross = 0.0, log_mass = 0.0;
+    double mass, cross, log_mass;
     Sums<U> tokens, others;
 };
 
-// ids: room for the teacher's ids, of this wave alone.
-template <int DT, int U, bool BUCKET>
+// Of one wave alone: the teacher's ids, and bits of the runs that some of them may share.
+constexpr int kSeen = 16384;
+template <int N> struct Named {
+    int32_t ids[N];
+    uint32_t seen[kSeen / 32];
+};
+
+template <int DT, int U, bool BUCKET, int N>
 __device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, const Teacher& t, int64_t r,
-                                               const typename Elem<DT>::T* x, int32_t* ids) {
+                                               const typename Elem<DT>::T* x, Named<N>& own_lds) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>;
     const int lane = threadIdx.x & 63;
     Known<U> o;
+    o.mass = o.cross = o.log_mass = 0.0;
     Run<T, W> held_run;  // of the lane's first token
+    int32_t* ids = own_lds.ids;
+    bool shared = false;  // whether another token may be in the run of one of this lane's
+    if constexpr (BUCKET) {
+        for (int i = lane; i < kSeen / 32; i += 64) own_lds.seen[i] = 0;
+        meet<64>();
+    }
     for (int j = lane; j < t.top; j += 64) {
         const int64_t id = teacher_id(t, r * t.top + j);
         const float lp = *gbl(t.logps + r * t.top + j);
@@ -736,6 +749,10 @@ __device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, con
         const double p = in ? exp((double)lp) : __longlong_as_double(0x7ff8000000000000ll);
         o.mass += p;
         const float v = in ? to_f32<DT>(*gbl(x + id)) : 0.0f;
+        if (BUCKET && in) {
+            const uint32_t bit = (uint32_t)(id / W) % kSeen;
+            shared |= atomicOr(&own_lds.seen[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
+        }
         if (BUCKET && in && j == lane) held_run = load_logits<DT, false>(x + id / W * W, q.vocab - id / W * W);
         if (p > 0.0) o.cross += p * ((double)lp - (double)v * h.inv64);
     }
@@ -750,14 +767,15 @@ __device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, con
         o.mass = some ? o.mass / o.mass : 0.0;
     }
     if constexpr (BUCKET) {
+        const int others = __ballot(shared) ? t.top : 0;
         for (int j = lane; j < t.top; j += 64) {
             const int32_t id = ids[j];
             if (id < 0) continue;
             const int32_t start = id / W * W;
             bool first = true, first_run = true;
-            uint32_t named = 0;
+            uint32_t named = 1u << (id - start);
 #pragma unroll 4
-            for (int i = 0; i < t.top; ++i) {
+            for (int i = 0; i < others; ++i) {
                 const int32_t other = ids[i];
                 const uint32_t off = (uint32_t)(other - start);  // of no token: far
                 if (off < (uint32_t)W) {
@@ -851,7 +869,7 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
                                                      double2* __restrict__ each, float* __restrict__ divergence,
                                                      Slope* __restrict__ slopes) {
     using T = typename Elem<DT>::T;
-    __shared__ __align__(16) int32_t ids[kMaxTeacher];
+    __shared__ Named<kMaxTeacher> named;
     const int64_t r = blockIdx.x, label = sload(q.labels + r);
     if (label == q.ignore || (q.n_seq > 0 && seq_of(q, r) < 0)) {
         if (threadIdx.x == 0) {
@@ -867,7 +885,7 @@ __global__ __launch_bounds__(64) void k_distill_rows(const Rows q, const Heat h,
         const float4 p = part[r * q.splits + i];
         a.join(p.x, p.y, p.z, h);
     }
-    const Known<U> known = known_part<DT, U, BUCKET>(q, h, t, r, x, ids);
+    const Known<U> known = known_part<DT, U, BUCKET>(q, h, t, r, x, named);
     wave_join(a, h);
     double2 e;
     const Slope s = row_slope<DT, U, BUCKET>(q, h, t, label, label_x, a, known, e);
@@ -1030,18 +1048,29 @@ struct DistillGrad {
         int64_t first;
         bool zero;
     };
-    __device__ __forceinline__ Row row(const Rows& q, const Heat&, int64_t r, int64_t, int) const {
-        Row o;
-        float w = g.scale_dev ? sload(g.scale_dev) * g.scale : g.scale;
+    __device__ __forceinline__ float weight(const Rows& q, int64_t r) const {
         const int s = q.n_seq > 0 ? seq_of(q, r) : 0;
-        w = s >= 0 ? w * sload(g.weights + s) : 0.0f;
+        return s >= 0 ? (g.scale_dev ? sload(g.scale_dev) * g.scale : g.scale) * sload(g.weights + s) : 0.0f;
+    }
+    __device__ __forceinline__ Row row(const Rows& q, const Heat&, int64_t r, int64_t, int) const {
         const Slope* p = g.slopes + r;
-        o.m = sload(&p->m);
-        o.other_m = sload(&p->other_m);
-        o.mine = sload(&p->mine) * w;
-        o.other = sload(&p->other) * w;
-        o.plain = sload(&p->plain) * w;
-        o.log_mass = sload(&p->log_mass);
+        Slope s;
+        s.m = sload(&p->m);
+        s.other_m = sload(&p->other_m);
+        s.mine = sload(&p->mine);
+        s.other = sload(&p->other);
+        s.plain = sload(&p->plain);
+        s.log_mass = sload(&p->log_mass);
+        return row(s, weight(q, r), r);
+    }
+    __device__ __forceinline__ Row row(const Slope& s, float w, int64_t r) const {
+        Row o;
+        o.m = s.m;
+        o.other_m = s.other_m;
+        o.mine = s.mine * w;
+        o.other = s.other * w;
+        o.plain = s.plain * w;
+        o.log_mass = s.log_mass;
         o.label_extra = g.t.hard > 0.0 ? -(float)g.t.hard * w : 0.0f;
         o.soft = g.t.soft * w;
         o.first = r * g.t.top;
@@ -1060,6 +1089,25 @@ struct DistillGrad {
         return lp != -__builtin_inff() && (uint64_t)id < (uint64_t)q.vocab;
     }
 };
+
+// An entry at column `off` of a run v whose gradient is y: the teacher's first there changes the element's slope, each
+// adds its extra.  named: the columns that have been changed.
+template <int DT, class G>
+__device__ __forceinline__ void take_entry(const G& g, const typename G::Row& o, const Heat& h,
+                                           const Run<typename Elem<DT>::T, kW<DT>>& v, float (&y)[kW<DT>], uint32_t off, float extra,
+                                           bool teacher, uint32_t& named) {
+    if (teacher && !(named >> off & 1)) {
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kW<DT>; ++k) x = (uint32_t)k == off ? to_f32<DT>(v.e[k]) : x;
+        const float mine = g.at(o, h, x, true);
+#pragma unroll
+        for (int k = 0; k < kW<DT>; ++k) y[k] = (uint32_t)k == off ? mine : y[k];
+        named |= 1u << off;
+    }
+#pragma unroll
+    for (int k = 0; k < kW<DT>; ++k) y[k] += (uint32_t)k == off ? extra : 0.0f;
+}
 
 // The gradient of a split of a row, in runs of 16 bytes from the ends of cache lines.  Runs that hold a label or one
 // of the entries are marked; the lanes that have them look through the split's list.
@@ -1148,20 +1196,10 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
 #pragma unroll
             for (int k = 0; k < W; ++k) y[k] = g.at(o, h, to_f32<DT>(v[i].e[k]), false);
             if (marks[wave][(run - first) >> 5] >> ((run - first) & 31) & 1) {
-                float extra[W] = {};
                 uint32_t named = 0;
                 for (int j = 0; j < n; ++j) {
                     const uint32_t id = ids[wave][j], off = (id & 0x7fffffffu) - (uint32_t)at;
-                    if (off >= (uint32_t)W) continue;
-                    const float e = extras[wave][j];
-#pragma unroll
-                    for (int k = 0; k < W; ++k) extra[k] += (uint32_t)k == off ? e : 0.0f;
-                    named |= (id >> 31 ^ 1u) << off;
-                }
-#pragma unroll
-                for (int k = 0; k < W; ++k) {
-                    if (named >> k & 1) y[k] = g.at(o, h, to_f32<DT>(v[i].e[k]), true);
-                    y[k] += extra[k];
+                    if (off < (uint32_t)W) take_entry<DT>(g, o, h, v[i], y, off, extras[wave][j], !(id >> 31), named);
                 }
             }
 #pragma unroll
@@ -1172,6 +1210,166 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
         if (c >= end) break;
         load();
     }
+}
+
+// ------------------------------------------------------------ loss and gradient of a row in one go
+constexpr int kRowT = 1024;                 // threads of a workgroup that keeps a row to itself
+constexpr int kKeptLds = 4, kKeptRegs = 2;  // steps of a row (16 KB) that it keeps on chip
+constexpr int kRowMarks = 32768;            // runs of such a row
+constexpr int kRowEntries = 2;              // of a lane: the teacher's tokens and the label
+
+// A row by one workgroup: its sums, its loss, its gradient, where its weight is known before (the labels alone give it).
+// Two workgroups a CU hold 512 rows, which the 256 MB cache still has when they are read again, last part first; the
+// last steps stay in LDS and registers between.  Rows of the gradient start at multiples of 16 bytes.  The first wave
+// reads the teacher's tokens while the others are at the sums; in the gradient every wave holds them, a few to a lane,
+// and asks by ballots which fall into its step.
+template <int DT, bool BUCKET>
+__global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const Heat h, const DistillGrad<false> g,
+                                                                          double2* __restrict__ each, float* __restrict__ divergence,
+                                                                          Slope* __restrict__ slopes, void* __restrict__ grad) {
+    using T = typename Elem<DT>::T;
+    constexpr int W = kW<DT>, U = kNone;
+    __shared__ float4 waves[kRowT / 64];
+    __shared__ Slope slope_of;
+    __shared__ uint32_t marks[BUCKET ? kRowMarks / 32 : 1];
+    __shared__ Named<kRowEntries * 64> named_of;
+    __shared__ Run<T, W> kept[kKeptLds * kRowT];
+    const Teacher& t = g.g.t;
+    const int64_t r = blockIdx.x, label = sload(q.labels + r);
+    const int lane = threadIdx.x & 63;
+    T* out = (T*)grad + r * q.vocab;
+    const int64_t n = q.vocab / W;
+    const bool counts = label != q.ignore && (q.n_seq == 0 || seq_of(q, r) >= 0);
+    Run<T, W> zeros;
+#pragma unroll
+    for (int i = 0; i < W; ++i) zeros.e[i] = T(0);
+    if (!counts) {
+        for (int64_t c = threadIdx.x; c < n; c += kRowT) store_run<T, W>(out + c * W, W, zeros);
+        if (threadIdx.x == 0) {
+            each[r] = make_double2(0.0, 0.0);
+            divergence[r] = 0.0f;
+        }
+        return;
+    }
+    const T* x = (const T*)q.x + row_offset(q, r);
+    // this lane's entries: columns (-1: none) and log-probabilities
+    int32_t id[kRowEntries];
+    float lp[kRowEntries];
+#pragma unroll
+    for (int e = 0; e < kRowEntries; ++e) {
+        const int j = e * 64 + lane;
+        id[e] = -1;
+        lp[e] = 0.0f;
+        if (j < t.top) {
+            const int64_t at = teacher_id(t, r * t.top + j);
+            lp[e] = *gbl(t.logps + r * t.top + j);
+            if (lp[e] != -__builtin_inff() && (uint64_t)at < (uint64_t)q.vocab) id[e] = (int32_t)at;
+        } else if (j == t.top && t.hard > 0.0 && (uint64_t)label < (uint64_t)q.vocab) {
+            id[e] = (int32_t)label;
+        }
+    }
+    if constexpr (BUCKET) {
+        for (int i = threadIdx.x; i < kRowMarks / 32; i += kRowT) marks[i] = 0;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+#pragma unroll
+            for (int e = 0; e < kRowEntries; ++e)
+                if (id[e] >= 0 && e * 64 + lane < t.top) atomicOr(&marks[id[e] / W >> 5], 1u << (id[e] / W & 31));
+        }
+        __syncthreads();
+    }
+    __shared__ uint64_t known_words[sizeof(Known<U>) / 8];  // not in registers meanwhile
+    Known<U>& known_of = *reinterpret_cast<Known<U>*>(known_words);
+    if (threadIdx.x < 64) {
+        const Known<U> known = known_part<DT, U, BUCKET>(q, h, t, r, x, named_of);
+        if (threadIdx.x == 0) known_of = known;
+    }
+    const auto skip = [&](int64_t run) { return BUCKET && (marks[run >> 5] >> (run & 31) & 1); };
+    const int64_t steps = (n + kRowT - 1) / kRowT;
+    constexpr int kKept = kKeptLds + kKeptRegs;
+    const int64_t first = steps > kKept ? steps - kKept : 0;
+    const auto number = [&](int i) { return (first + i) * kRowT + threadIdx.x; };  // of kept run i
+    Sums<U> a = row_sums<DT, U, kRowT, false>(x, q.vocab, 0, first * kRowT, threadIdx.x, h, skip, [](float) {});
+    Run<T, W> held[kKeptRegs];
+    {
+        LaneSums<U> end;
+        const auto add = [&](const Run<T, W>& raw, int i) {
+            Run<T, W> v[1] = {raw};
+            if (number(i) < n && skip(number(i))) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) v[0].e[k] = DT == F32 ? (T)-__builtin_inff() : (T)(DT == BF16 ? 0xff80 : 0xfc00);
+            }
+            add_runs<DT, U, 1>(end, v, h);
+        };
+        // what lies past the row's end reads as -inf
+#pragma unroll
+        for (int i = 0; i < kKeptLds; i += 2) {
+            Run<T, W> v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[j] = load_logits<DT>(x + number(i + j) * W, q.vocab - number(i + j) * W);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                add(v[j], i + j);
+                kept[(i + j) * kRowT + threadIdx.x] = v[j];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kKeptRegs; ++i)
+            held[i] = load_logits<DT>(x + number(kKeptLds + i) * W, q.vocab - number(kKeptLds + i) * W);
+#pragma unroll
+        for (int i = 0; i < kKeptRegs; ++i) add(held[i], kKeptLds + i);
+        const Sums<U> b = end.sums(h);
+        a.join(b.m, b.s, b.u, h);
+    }
+    a = group_join<U, kRowT>(a, h, waves);
+    if (threadIdx.x < 64) {
+        double2 e;
+        const Known<U> known = known_of;
+        const Slope s = row_slope<DT, U, BUCKET>(q, h, t, label, label_logit<DT>(q, x, label), a, known, e);
+        if (threadIdx.x == 0) {
+            slope_of = s;
+            slopes[r] = s;
+            each[r] = e;
+            divergence[r] = (float)e.x;
+        }
+    }
+    __syncthreads();
+    const DistillGrad<false>::Row o = g.row(slope_of, g.weight(q, r), r);
+    float extra_of[kRowEntries];
+#pragma unroll
+    for (int e = 0; e < kRowEntries; ++e) extra_of[e] = e * 64 + lane < t.top ? -o.soft * exp_(lp[e] - o.log_mass) : o.label_extra;
+    const auto put = [&](Run<T, W> v, int64_t c) {  // c: of a wave 64 runs in a row
+        if (o.zero) {
+            if (c < n) store_run<T, W>(out + c * W, W, zeros);
+            return;
+        }
+        float y[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) y[k] = g.at(o, h, to_f32<DT>(v.e[k]), false);
+        const int32_t start = (int32_t)(c * W), step = __builtin_amdgcn_readfirstlane(start);
+        uint32_t named = 0;
+#pragma unroll
+        for (int e = 0; e < kRowEntries; ++e) {
+            uint64_t who = __ballot(id[e] >= 0 && (uint32_t)(id[e] - step) < 64u * W);
+            while (who) {  // in the entries' order
+                const int j = __builtin_ctzll(who);
+                who &= who - 1;
+                const uint32_t off = (uint32_t)(__builtin_amdgcn_readlane(id[e], j) - start);
+                const float add = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(extra_of[e]), j));
+                if (off < (uint32_t)W) take_entry<DT>(g, o, h, v, y, off, add, e * 64 + j < t.top, named);
+            }
+        }
+        if (c >= n) return;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v.e[k] = from_f32<DT>(y[k]);
+        store_run<T, W>(out + c * W, W, v);
+    };
+#pragma unroll
+    for (int i = kKeptRegs - 1; i >= 0; --i) put(held[i], number(kKeptLds + i));
+#pragma unroll
+    for (int i = kKeptLds - 1; i >= 0; --i) put(kept[i * kRowT + threadIdx.x], number(i));
+    for (int64_t c = (first - 1) * kRowT + threadIdx.x; c >= 0; c -= kRowT)
+        put(o.zero ? zeros : load_logits<DT>(x + c * W), c);
 }
 
 // ------------------------------------------------------------ host side
@@ -1321,11 +1519,26 @@ int distill_outputs(Distill& d, float* loss, float* divergence, float* nll, floa
     return GEFENX_OK;
 }
 
+// go(kind of the sums, whether the teacher's other tokens count)
+template <class Go>
+int by_kind(const Distill& d, Go&& go) {
+    using N = std::integral_constant<int, kNone>;
+    using P = std::integral_constant<int, kPlain>;
+    const bool plain = d.t.hard > 0.0 && d.h.inv64 != 1.0;
+    if (d.t.rest == kBucket) {
+        if (plain) go(P(), std::true_type());
+        else go(N(), std::true_type());
+    } else {
+        if (plain) go(P(), std::false_type());
+        else go(N(), std::false_type());
+    }
+    return launched(d.what);
+}
+
 int distill_forward(Distill& d) {
     const char* what = d.what;
     int rc = GEFENX_OK;
     const Rows& q = d.q;
-    const bool plain = d.t.hard > 0.0 && d.h.inv64 != 1.0;
     if (q.rows > 0) {
         rc = by_dtype(d.dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
@@ -1337,20 +1550,35 @@ int distill_forward(Distill& d) {
                 k_distill_rows<DT, U, B><<<(uint32_t)q.rows, 64, 0, d.s>>>(q, d.h, d.t, d.part, d.each, d.token_divergence,
                                                                          d.slopes);
             };
-            using N = std::integral_constant<int, kNone>;
-            using P = std::integral_constant<int, kPlain>;
-            if (d.t.rest == kBucket) {
-                if (plain) go(P(), std::true_type());
-                else go(N(), std::true_type());
-            } else {
-                if (plain) go(P(), std::false_type());
-                else go(N(), std::false_type());
-            }
-            return launched(what);
+            return by_kind(d, go);
         });
         if (rc != GEFENX_OK) return rc;
     }
     return distill_totals(d, d.each);
+}
+
+// Whether loss and gradient go row by row.
+bool rows_alone(const gefenx_logits& l, const gefenx_teacher& t, const void* grad) {
+    const int64_t run = l.dtype == GEFENX_F32 ? 4 : 8, bytes = l.vocab * (16 / run);
+    return bytes >= (l.dtype == GEFENX_F32 ? 128 : 192) << 10 && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)400 << 20 &&
+           l.vocab % run == 0 && l.vocab / run <= kRowMarks && !(t.hard_weight > 0.0 && t.temperature != 1.0) && t.top < kRowEntries * 64 && ((uintptr_t)grad & 15) == 0;
+}
+
+int distill_alone(Distill& d, const float* scale_dev, double scale, void* grad) {
+    int rc = distill_totals(d, nullptr);  // the sequences' weights come from the labels alone
+    if (rc != GEFENX_OK) return rc;
+    const Downhill g = {d.slopes, d.out.weights, scale_dev, (float)scale, d.t};
+    rc = by_dtype(d.dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        const auto go = [&](auto bucket) {
+            k_distill_alone<DT, decltype(bucket)::value><<<(uint32_t)d.q.rows, kRowT, 0, d.s>>>(
+                d.q, d.h, DistillGrad<false>{g}, d.each, d.token_divergence, d.slopes, grad);
+        };
+        if (d.t.rest == kBucket) go(std::true_type());
+        else go(std::false_type());
+        return launched(d.what);
+    });
+    return rc == GEFENX_OK ? distill_totals(d, d.each) : rc;
 }
 
 int distill_grad(const char* what, const gefenx_logits* l, const gefenx_teacher* t, const void* slopes, const float* weights,
@@ -1466,6 +1694,7 @@ int gefenx_distillation_loss_grad(const gefenx_logits* logits, const gefenx_teac
     if (rc == GEFENX_OK && d.q.rows > 0 && !grad) rc = set_error(GEFENX_EINVAL, "%s: null pointer", what);
     if (rc == GEFENX_OK)
         rc = distill_outputs(d, loss, divergence, nll, token_divergence, slopes, weights, workspace, workspace_bytes, stream);
+    if (rc == GEFENX_OK && rows_alone(*logits, *teacher, grad)) return distill_alone(d, scale_dev, scale, grad);
     if (rc == GEFENX_OK) rc = distill_forward(d);
     return rc == GEFENX_OK ? distill_grad(what, logits, teacher, slopes, weights, scale_dev, scale, grad, stream) : rc;
 }

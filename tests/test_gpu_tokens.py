@@ -455,6 +455,57 @@ def test_distillation(dev, lengths, V, k, dtype, packed):
             assert abs(o.nll.item() - nll.item()) <= (sum_error(d.x64).max().item() + U * abs(nll.item()) if hard else 0.0)
 
 
+ALONE = [  # many long rows, whose loss and gradient one workgroup each finds: type, rows, vocabulary, teacher's tokens, column
+    (torch.bfloat16, 1050, 200000, 64, 0), (torch.bfloat16, 1700, 131072, 127, 3), (torch.float16, 1700, 131080, 5, 0),
+    (torch.float32, 1100, 100000, 100, 1), (torch.bfloat16, 1700, 131072, 128, 0), (torch.float16, 1700, 131079, 20, 0)]
+
+
+@pytest.mark.parametrize("dtype,T,V,k,column", ALONE)
+def test_many_long_rows(dev, dtype, T, V, k, column):
+    """Most rows masked; those that are not against the formulas, by both calls."""
+    g = torch.Generator(dev).manual_seed(k)
+    held = torch.randn(T, V + (8 if column else 0), device=dev, dtype=dtype, generator=g) * 2
+    x = held[:, column:column + V]
+    keep = torch.tensor([0, 1, 77, 1024, T - 2], device=dev)
+    labels = torch.full((T,), IGNORE, device=dev)
+    near = (x[keep].float() + torch.randn(5, V, device=dev, generator=g)).log_softmax(-1)
+    lp, ids = near.topk(k, -1)
+    ids[0, -1], lp[0, -2], ids[1, 0] = V - 1, -INF, ids[1, 1]  # the last column, no token, one twice
+    ids[3, :3] = torch.tensor([8, 9, 15], device=dev)  # of one run
+    labels[keep] = torch.tensor([0, V - 1, int(ids[2, 0]), 16, V // 2], device=dev)  # one of them the teacher's
+    all_ids, all_lp = torch.zeros(T, k, dtype=torch.long, device=dev), torch.zeros(T, k, device=dev)
+    all_ids[keep], all_lp[keep] = ids, lp
+    for rest, hard, temperature in (("bucket", 0.0, 1.0), ("bucket", 0.3, 2.0), ("drop", 0.2, 1.0), ("normalize", 0.5, 0.7)):
+        y, spans = labels[keep].cpu(), [(0, 5)]
+        x64 = x[keep].double().cpu().requires_grad_()
+        loss, _, _, each = distill64(x64, y, spans, ids.cpu(), lp.cpu(), temperature, rest, hard, "token")
+        loss.backward()
+        kw = dict(rest=rest, hard_weight=hard, temperature=temperature)
+        scale = torch.tensor(512.0, device=dev)
+        out, grad = gefen.distillation_loss_and_grad(x, labels, all_ids, all_lp, grad_scale=scale, **kw)
+        leaf = x.detach().clone().requires_grad_()
+        two = gefen.distillation_loss(leaf, labels, all_ids, all_lp, **kw)
+        (two.loss * 512.0).backward()
+        masked = torch.ones(T, dtype=torch.bool, device=dev)
+        masked[keep] = False
+        for o, d in ((out, grad), (two, leaf.grad)):
+            off = check_distill(x64.detach(), y, spans, ids.cpu(), lp.cpu(), temperature, rest, hard, "token", x64.grad, each.detach(),
+                                d[keep].cpu().double(), o.token_divergence.detach()[keep].cpu().double(), dtype, 512.0)
+            assert abs(o.loss.item() - loss.item()) <= off + 2 * U * abs(loss.item())
+            assert not d[masked].any() and not o.token_divergence[masked].any()
+    # a spoilt row is spoilt alone; a scale of 0 asks for no gradient
+    all_ids[1, 2] = V
+    out, grad = gefen.distillation_loss_and_grad(x, labels, all_ids, all_lp)
+    assert out.token_divergence.isnan().nonzero().view(-1).tolist() == [1] and grad.isnan().any(1).nonzero().view(-1).tolist() == [1]
+    out, grad = gefen.distillation_loss_and_grad(x, labels, all_ids, all_lp, grad_scale=0.0)
+    assert not grad.any()
+    cu = torch.tensor([1, 78, 1025], dtype=torch.int32, device=dev)  # rows 0 and T - 2 belong to none
+    all_ids[1, 2] = 0
+    one = gefen.distillation_loss_and_grad(x, labels, all_ids, all_lp, cu_seqlens=cu, reduction="sequence")
+    assert not one[1][0].any() and not one[1][-2].any() and one[1][1].any()
+    assert abs(one[0].loss.item() - (one[0].token_divergence[[1, 77]].mean() + one[0].token_divergence[1024]).item() / 2) <= 1e-6
+
+
 def test_distillation_gradients_against_differences(dev):
     """Central differences of the 64-bit loss, step 1e-5: third derivatives (below 10 here) leave 1e-9."""
     d = Data([3, 2], 6, 2, torch.float32, dev, False, scale=1.0)
