@@ -1214,7 +1214,7 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
 
 // ------------------------------------------------------------ loss and gradient of a row in one go
 constexpr int kRowT = 1024;                 // threads of a workgroup that keeps a row to itself
-constexpr int kKeptLds = 4, kKeptRegs = 2;  // steps of a row (16 KB) that it keeps on chip
+constexpr int kKeptLds = 4, kKeptRegs = 1;  // steps of a row (16 KB) that it keeps on chip
 constexpr int kRowMarks = 32768;            // runs of such a row
 constexpr int kRowEntries = 2;              // of a lane: the teacher's tokens and the label
 
