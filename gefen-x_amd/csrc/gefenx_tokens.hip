@@ -177,10 +177,9 @@ __device__ __forceinline__ float largest(const Run<typename Elem<DT>::T, kW<DT>>
     }
 }
 
-// Adds N runs; their maximum.
+// Adds N runs, the largest of which is top.
 template <int DT, int U, int N>
-__device__ __forceinline__ float add_runs(LaneSums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, const Heat& h) {
-    const float top = largest<DT, N>(r);
+__device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, float top, const Heat& h) {
     a.rebase(top, h);
     const float s = a.s, u = a.u;
     if (!a.huge()) {
@@ -208,13 +207,12 @@ __device__ __forceinline__ float add_runs(LaneSums<U>& a, const Run<typename Ele
             }
         }
     }
-    return top;
 }
 
 constexpr int kStep = 4;  // runs of a lane in flight
 
 // Runs begin .. end - 1 of a row, TH lanes at a time in steps of kStep runs each; each lane's sums.  skip(run): a
-// run that is left out; note(maximum): what a lane found in a step.  Which logits a lane adds up does not
+// run that is left out; note(a, b): the largest of the first and of the second half of a lane's step.  Which logits a lane adds up does not
 // depend on where the row starts in memory.
 template <int DT, int U, int TH, bool STREAM, class Skip, class Note>
 __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t begin, int64_t end, int lane,
@@ -238,7 +236,9 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
             for (int i = 0; i < kStep; ++i) v[i] = load(x + (c + lane + i * TH) * W);
 #pragma unroll
             for (int i = 0; i < kStep; ++i) put(v[i], c + lane + i * TH);
-            note(add_runs<DT, U, kStep>(a, v, h));
+            const float one = largest<DT, kStep / 2>(v), two = largest<DT, kStep / 2>(v + kStep / 2);
+            add_runs<DT, U, kStep>(a, v, __builtin_fmaxf(one, two), h);
+            note(one, two);
         }
     };
     if (DT != F32 && ((uintptr_t)x & 3)) add([](const T* p) { return load_odd<DT, STREAM>(p); });
@@ -250,14 +250,16 @@ __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64
             const int64_t at = (c + lane + i * TH) * W;
             v[i] = load_logits<DT, STREAM>(x + at, last - at);
         }
-        float top = -__builtin_inff();
+        float half[2] = {-__builtin_inff(), -__builtin_inff()};
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
             if (c + i * TH >= end) break;
             if (c + lane + i * TH < end) put(v[i], c + lane + i * TH);
-            top = __builtin_fmaxf(top, add_runs<DT, U, 1>(a, v + i, h));
+            const float top = largest<DT, 1>(v + i);
+            add_runs<DT, U, 1>(a, v + i, top, h);
+            half[i / (kStep / 2)] = __builtin_fmaxf(half[i / (kStep / 2)], top);
         }
-        note(top);
+        note(half[0], half[1]);
     }
     return a.sums(h);
 }
@@ -454,6 +456,19 @@ __device__ __forceinline__ void by_rank(uint64_t* keys, int n, int top, Put&& pu
     }
 }
 
+// The maxima of both halves of a lane's step in a word: of 2-byte logits each, of fp32 ones the larger.
+template <int DT> struct Maxima {
+    static constexpr int kParts = DT == F32 ? 1 : 2;
+    static __device__ __forceinline__ uint32_t put(float a, float b) {
+        if constexpr (DT == F32) return __float_as_uint(__builtin_fmaxf(a, b));
+        else return (uint32_t)from_f32<DT>(a) | (uint32_t)from_f32<DT>(b) << 16;
+    }
+    static __device__ __forceinline__ float get(uint32_t w, int part) {
+        if constexpr (DT == F32) return __uint_as_float(w);
+        else return to_f32<DT>((uint16_t)(w >> 16 * part));
+    }
+};
+
 // Maxima of a lane's steps that are kept; how many of them are looked through again, and candidates that there is room
 // for (short rows may have all of their logits among them).
 constexpr int kSlots = 20, kWaveSlots = (int)kShortRuns / (64 * kStep);
@@ -500,17 +515,18 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     const auto none = [](int64_t) { return false; };
     const int slots = TOP && begin < end ? (int)(((end - begin + kStep * TH - 1) / (kStep * TH) + steps_of_slot - 1) / steps_of_slot) : 0;
     uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1) + 2) : 0);
-    float* tops = reinterpret_cast<float*>(own_lds);
-    float* slot = tops + lane;
-    float held = -__builtin_inff();
+    uint32_t* tops = reinterpret_cast<uint32_t*>(own_lds);
+    uint32_t* slot = tops + lane;
+    float held[2] = {-__builtin_inff(), -__builtin_inff()};
     int to_go = steps_of_slot;
-    const auto note = [&](float m) {
+    const auto note = [&](float one, float two) {
         if constexpr (TOP) {
-            held = __builtin_fmaxf(held, m);
-            *slot = held;
+            held[0] = __builtin_fmaxf(held[0], one);
+            held[1] = __builtin_fmaxf(held[1], two);
+            *slot = Maxima<DT>::put(held[0], held[1]);
             if (--to_go == 0) {
                 to_go = steps_of_slot;
-                held = -__builtin_inff();
+                held[0] = held[1] = -__builtin_inff();
                 slot += TH;
             }
         }
@@ -534,7 +550,8 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
         }
         const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, hunt.orders));  // a barrier inside
         meet<TH>();
-        const int each = kStep * steps_of_slot;  // runs of a slot
+        constexpr int kParts = Maxima<DT>::kParts, kRuns = kStep / kParts;
+        const int each = kRuns * steps_of_slot;  // runs of a part of a slot
         const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
         uint64_t* mine = keys + at * top;
         uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
@@ -542,18 +559,23 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
         // those that reach the bound, or (above) that are over it; whether there was room for all
         const auto gather = [&](bool above) {
             for (int i = 0; i < slots; ++i) {
-                const float m = tops[i * TH + lane];
-                if (above ? m > bound : m >= bound) {
-                    const uint32_t n = atomicAdd(&hunt.n_suspects, 1u);
-                    if (n < kSuspects<TH>) hunt.suspects[n] = (uint16_t)(i * TH + lane);
+                const uint32_t both = tops[i * TH + lane];
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    const float m = Maxima<DT>::get(both, part);
+                    if (above ? m > bound : m >= bound) {
+                        const uint32_t n = atomicAdd(&hunt.n_suspects, 1u);
+                        if (n < kSuspects<TH>) hunt.suspects[n] = (uint16_t)((i * TH + lane) * kParts + part);
+                    }
                 }
             }
             meet<TH>();
             const uint32_t suspects = hunt.n_suspects;
             if (suspects > kSuspects<TH>) return false;
             for (int i = lane; i < (int)suspects * each; i += TH) {
-                const int s = hunt.suspects[i / each], place = s / TH, who = s % TH;
-                const int64_t run = begin + who + ((int64_t)place * each + i % each) * TH, col = run * W;
+                const int s = hunt.suspects[i / each], part = s % kParts, place = s / kParts / TH, who = s / kParts % TH;
+                const int step = place * steps_of_slot + i % each / kRuns, of = part * kRuns + i % kRuns;
+                const int64_t run = begin + who + ((int64_t)step * kStep + of) * TH, col = run * W;
                 if (run >= end) continue;
                 const Run<T, W> v = load_logits<DT, false>(x + col, last - col);
 #pragma unroll
@@ -703,7 +725,7 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
     if (!counts) return;
     const T* x = (const T*)q.x + row_offset(q, r);
     const auto skip = [&](int64_t run) { return BUCKET && (mine[(run - begin) >> 5] >> ((run - begin) & 31) & 1); };
-    const auto note = [](float) {};
+    const auto note = [](float, float) {};
     Sums<U> a = q.cached ? row_sums<DT, U, TH, false>(x, q.vocab, begin, end, lane, h, skip, note)
                          : row_sums<DT, U, TH, true>(x, q.vocab, begin, end, lane, h, skip, note);
     if constexpr (PER > 1) wave_join(a, h);
@@ -1289,7 +1311,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
     constexpr int kKept = kKeptLds + kKeptRegs;
     const int64_t first = steps > kKept ? steps - kKept : 0;
     const auto number = [&](int i) { return (first + i) * kRowT + threadIdx.x; };  // of kept run i
-    Sums<U> a = row_sums<DT, U, kRowT, false>(x, q.vocab, 0, first * kRowT, threadIdx.x, h, skip, [](float) {});
+    Sums<U> a = row_sums<DT, U, kRowT, false>(x, q.vocab, 0, first * kRowT, threadIdx.x, h, skip, [](float, float) {});
     Run<T, W> held[kKeptRegs];
     {
         LaneSums<U> end;
@@ -1299,7 +1321,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
 #pragma unroll
                 for (int k = 0; k < W; ++k) v[0].e[k] = DT == F32 ? (T)-__builtin_inff() : (T)(DT == BF16 ? 0xff80 : 0xfc00);
             }
-            add_runs<DT, U, 1>(end, v, h);
+            add_runs<DT, U, 1>(end, v, largest<DT, 1>(v), h);
         };
         // what lies past the row's end reads as -inf
 #pragma unroll

@@ -44,19 +44,29 @@ class DistillationLoss(NamedTuple):
 
 # ------------------------------------------------------------ token statistics
 
-def _statistics_forward(call, top, temperature):
+def _scratch(call, kept, n, keep):
+    """`kept` fp32 values that the gradient needs (None unless it does) and a workspace of n bytes: tensors, and the
+    pointers of both."""
+    saved = call.empty(kept) if keep else None
+    end = (n + 15) // 16 * 16
+    ws = torch.empty(end + (16 if keep else 4 * kept + 16), dtype=torch.uint8, device=call.device)
+    at = ws.data_ptr()
+    return saved, ws, saved.data_ptr() if keep else at + end, at
+
+
+def _statistics_forward(call, top, temperature, keep=False):
+    """The statistics, and where asked to keep it, what their gradient needs."""
     top, lead = operator.index(top), call.lead
     lib = _native.load()
     logps = None if call.labels is None else call.empty(*lead)
     entropy, top_logps = call.empty(*lead), call.empty(*lead, max(top, 0))
     top_ids = torch.empty(top_logps.shape, dtype=torch.int64, device=call.device)
-    saved = call.empty(call.rows, 4)
     n = int(lib.gefenx_token_statistics_workspace_bytes(call.ref, top))
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=call.device)
+    saved, ws, saved_ptr, ws_ptr = _scratch(call, 4 * call.rows, n, keep)
     with _on_device(call.device):
         _native.check(lib.gefenx_token_statistics(
             call.ref, temperature, top, _ptr(logps), entropy.data_ptr(), top_ids.data_ptr(), top_logps.data_ptr(),
-            saved.data_ptr(), ws.data_ptr(), n, call.stream), "token_statistics")
+            saved_ptr, ws_ptr, n, call.stream), "token_statistics")
     return (logps, entropy, top_ids, top_logps), saved
 
 
@@ -64,7 +74,7 @@ class _TokenStatistics(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, top, temperature, ignore_index):
         call = _Call(logits, labels, ignore_index, sequences=False, labelled=False)
-        out, saved = _statistics_forward(call, top, temperature)
+        out, saved = _statistics_forward(call, top, temperature, keep=True)
         ctx.top, ctx.temperature, ctx.ignore_index, ctx.desc = operator.index(top), temperature, ignore_index, call.desc
         ctx.save_for_backward(logits, labels, out[2], saved)
         ctx.mark_non_differentiable(out[2])
@@ -134,27 +144,26 @@ def _distillation_call(logits, labels, ignore_index, cu_seqlens, ids, logps, tem
     return call, _Teacher(call, ids, logps, temperature, rest, hard_weight, reduction)
 
 
-def _distillation_saved(call, saved):
-    """Pointers of the rows' slopes [rows, 8] and the sequences' weights in what the gradient needs."""
-    return saved.data_ptr(), saved.data_ptr() + 32 * call.desc.rows
+def _distillation_saved(call, at):
+    """Pointers of the rows' slopes [rows, 8] and the sequences' weights in what the gradient needs, at `at`."""
+    return at, at + 32 * call.desc.rows
 
 
 def _distillation_forward(call, teacher, grad_scale=None):
     """The loss and what its gradient needs; with a grad_scale the gradient too."""
     lib = _native.load()
     loss, divergence, nll, each = call.empty(), call.empty(), call.empty(), call.empty(*call.lead)
-    saved = call.empty(8 * call.rows + max(call.n_seq, 1))
     n = int(lib.gefenx_distillation_workspace_bytes(call.ref, teacher.ref))
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=call.device)
+    saved, ws, saved_ptr, ws_ptr = _scratch(call, 8 * call.rows + max(call.n_seq, 1), n, grad_scale is None)
     args = [call.ref, teacher.ref, loss.data_ptr(), divergence.data_ptr(), nll.data_ptr(), each.data_ptr(),
-            *_distillation_saved(call, saved)]
+            *_distillation_saved(call, saved_ptr)]
     entry, grad = lib.gefenx_distillation_loss, None
     if grad_scale is not None:
         (scale_dev, factor), grad = call.scale(grad_scale), call.empty_grad()
         entry = lib.gefenx_distillation_loss_grad
         args += [_ptr(scale_dev), factor, grad.data_ptr()]
     with _on_device(call.device):
-        _native.check(entry(*args, ws.data_ptr(), n, call.stream), "distillation_loss")
+        _native.check(entry(*args, ws_ptr, n, call.stream), "distillation_loss")
     return DistillationLoss(loss, divergence, nll, each), saved, grad
 
 
@@ -180,7 +189,7 @@ class _Distillation(torch.autograd.Function):
         (scale_dev, factor), out = call.scale(grad), call.empty_grad()
         with _on_device(call.device):
             _native.check(_native.load().gefenx_distillation_grad(
-                call.ref, teacher.ref, *_distillation_saved(call, saved), _ptr(scale_dev), factor, out.data_ptr(), call.stream),
+                call.ref, teacher.ref, *_distillation_saved(call, saved.data_ptr()), _ptr(scale_dev), factor, out.data_ptr(), call.stream),
                 "distillation gradient")
         return (out,) + (None,) * 6
 
