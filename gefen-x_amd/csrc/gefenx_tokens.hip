@@ -181,7 +181,8 @@ __device__ __forceinline__ float largest(const Run<typename Elem<DT>::T, kW<DT>>
 template <int DT, int U, int N>
 __device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem<DT>::T, kW<DT>>* r, float top, const Heat& h) {
     a.rebase(top, h);
-    const float s = a.s, u = a.u;
+    const float s = a.s, u = a.u;  // N runs are added up by themselves: a long row's sum keeps more of them
+    a.s = a.u = 0.0f;
     if (!a.huge()) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
@@ -189,8 +190,7 @@ __device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem
             for (int k = 0; k < kW<DT>; ++k) a.template add<false>(to_f32<DT>(r[c].e[k]), h);
     }
     if (a.huge() || (U == kEntropy && a.u != a.u && a.s == a.s)) {  // again: among them were huge ones, or -inf
-        a.s = s;
-        a.u = u;
+        a.s = a.u = 0.0f;
 #pragma unroll
         for (int c = 0; c < N; ++c) {
             // from the words anew: values kept for here would cost the pass its registers
@@ -207,6 +207,8 @@ __device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem
             }
         }
     }
+    a.s += s;
+    a.u += u;
 }
 
 constexpr int kStep = 4;  // runs of a lane in flight
@@ -474,11 +476,10 @@ template <int DT> struct Maxima {
 constexpr int kSlots = 20, kWaveSlots = (int)kShortRuns / (64 * kStep);
 constexpr int kWaveTop = 32;  // likeliest tokens that a wave finds for a row of its own
 template <int TH> constexpr int kSuspects = TH == kT ? 384 : 128;
-template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 512 : 1024; }  // and one more
+template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 384 : 1024; }  // and one more
 template <int TH> struct Hunt {
-    uint32_t orders[TH == kT ? kT : TH / 64];
     uint16_t suspects[kSuspects<TH>];
-    uint32_t n_suspects, n_candidates;
+    uint32_t n_suspects, n_candidates, waves[TH / 64];
     double log_sum_exp;
 };
 
@@ -548,13 +549,14 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
             if (alone) hunt.log_sum_exp = row_results(q, h, out, r, label, xl, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
-        const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, hunt.orders));  // a barrier inside
+        uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
+        uint32_t* orders = reinterpret_cast<uint32_t*>(candidates);  // before them
+        const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, orders));  // a barrier inside
         meet<TH>();
         constexpr int kParts = Maxima<DT>::kParts, kRuns = kStep / kParts;
         const int each = kRuns * steps_of_slot;  // runs of a part of a slot
         const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
         uint64_t* mine = keys + at * top;
-        uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
         const uint32_t most = room<TH>(slots);
         // those that reach the bound, or (above) that are over it; whether there was room for all
         const auto gather = [&](bool above) {
@@ -598,7 +600,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
             found = gather(true);
             const uint32_t over = hunt.n_candidates;
             if (found && over < (uint32_t)top) {
-                first_equal<DT, TH>(x, first, last, order_of(bound), (uint32_t)top - over, hunt.orders, candidates + over);
+                first_equal<DT, TH>(x, first, last, order_of(bound), (uint32_t)top - over, hunt.waves, candidates + over);
                 meet<TH>();
                 if (lane == 0) hunt.n_candidates = (uint32_t)(last - first < top ? last - first : top);
                 meet<TH>();
