@@ -98,16 +98,20 @@ __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* 
 // 2^((x - m) (hi + lo)) is three (the statistics of 4096 x 128256 bf16 are bound by such operations as much as by
 // memory).  What M's rounding and hi's make of the sums is known and put right in sums(): 2^(m hi - M) for all of
 // them, and by hi alone s grows by (hi / (hi + lo) - 1) sum z exp(z), which u gives; without u the product with lo is
-// taken too.  Beyond kHuge, where x hi may overflow (rows of the type's lowest value), the difference is taken first.
-constexpr float kHuge = 1e30f;
+// taken too.  Where M is beyond kHuge its rounding would be more than half a power of two, or x hi overflow (rows that
+// a mask of -1e10 or the type's lowest value leaves nothing): there the difference is taken first.
+constexpr float kHuge = 16777216.0f;
 template <int U> struct LaneSums {
     float m = -__builtin_inff(), s = 0.0f, u = 0.0f, minus = 0.0f, minus1 = 0.0f;  // -M, and that of exp(x)
-    __device__ __forceinline__ bool huge() const { return __builtin_fabsf(m) > kHuge && m != -__builtin_inff(); }
+    static __device__ __forceinline__ bool huge(float of, float of1) {
+        return __builtin_fabsf(of) > kHuge || (U == kPlain && __builtin_fabsf(of1) > kHuge);
+    }
+    __device__ __forceinline__ bool huge() const { return huge(minus, minus1); }
     __device__ __forceinline__ void rebase(float m2, const Heat& h) {
         if (!(m2 > m)) return;
         const float next = -(m2 * h.hi), next1 = -(m2 * kLog2e);
         if (m != -__builtin_inff()) {
-            const bool apart = huge() || __builtin_fabsf(m2) > kHuge;
+            const bool apart = huge() || huge(next, next1);
             const float d = apart ? (m - m2) * h.hi : next - minus, f = __builtin_amdgcn_exp2f(d);
             if (U == kEntropy) u = f * __builtin_fmaf(s, __builtin_fmaxf(d, kFar), u);
             if (U == kPlain) u *= __builtin_amdgcn_exp2f(apart ? (m - m2) * kLog2e : next1 - minus1);
@@ -130,7 +134,7 @@ template <int U> struct LaneSums {
     }
     __device__ __forceinline__ void add_far(float x, const Heat& h) {
         const float d = x - m;
-        exponent<true>(d * h.hi);
+        exponent<true>(U == kEntropy ? d * h.hi : __builtin_fmaf(d, h.lo, d * h.hi));
         if (U == kPlain) u += exp_(d);
     }
     __device__ __forceinline__ Sums<U> sums(const Heat& h) const {
@@ -214,8 +218,8 @@ __device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem
 constexpr int kStep = 4;  // runs of a lane in flight
 
 // Runs begin .. end - 1 of a row, TH lanes at a time in steps of kStep runs each; each lane's sums.  skip(run): a
-// run that is left out; note(a, b): the largest of the first and of the second half of a lane's step.  Which logits a lane adds up does not
-// depend on where the row starts in memory.
+// run that is left out; note(a, b): the largest of the first and of the second half of a lane's step.  Which logits a
+// lane adds up does not depend on where the row starts in memory.
 template <int DT, int U, int TH, bool STREAM, class Skip, class Note>
 __device__ __forceinline__ Sums<U> row_sums(const typename Elem<DT>::T* x, int64_t vocab, int64_t begin, int64_t end, int lane,
                                             const Heat& h, Skip&& skip, Note&& note) {
@@ -421,8 +425,13 @@ __device__ __forceinline__ float label_logit(const Rows& q, const typename Elem<
     return q.labels && (uint64_t)label < (uint64_t)q.vocab ? to_f32<DT>(*gbl(x + label)) : 0.0f;
 }
 
-// A row's sums and its label's logit x to its results, by one lane; log sum exp(x / tau).
-__device__ __forceinline__ double row_results(const Rows& q, const Heat& h, const Statistics& out, int64_t r, int64_t label,
+// A row's maximum and the log of its sum: a log-probability is (x - max) / tau - log_sum.
+struct Level {
+    double max, log_sum;
+};
+
+// A row's sums and its label's logit x to its results, by one lane.
+__device__ __forceinline__ Level row_results(const Rows& q, const Heat& h, const Statistics& out, int64_t r, int64_t label,
                                               float x, const Sums<kEntropy>& a) {
     const double log_sum = log((double)a.s);
     const float entropy = (float)(log_sum - (double)a.u / (double)a.s * h.inv64);
@@ -431,12 +440,12 @@ __device__ __forceinline__ double row_results(const Rows& q, const Heat& h, cons
                                                            : __uint_as_float(0x7fc00000u);
     out.entropy[r] = entropy;
     out.stats[r] = make_float4(a.m, a.s, (float)log_sum, entropy);
-    return (double)a.m * h.inv64 + log_sum;
+    return {(double)a.m, log_sum};
 }
 
-__device__ __forceinline__ void top_result(const Heat& h, const Statistics& out, int64_t at, uint64_t key, double log_sum_exp) {
+__device__ __forceinline__ void top_result(const Heat& h, const Statistics& out, int64_t at, uint64_t key, const Level& level) {
     out.top_ids[at] = (int64_t)(uint32_t)~(uint32_t)key;
-    out.top_logps[at] = (float)((double)value_of((uint32_t)(key >> 32)) * h.inv64 - log_sum_exp);
+    out.top_logps[at] = (float)(((double)value_of((uint32_t)(key >> 32)) - level.max) * h.inv64 - level.log_sum);
 }
 
 // The place of each of n keys (no two alike) among them: put(place, key) for the `top` largest.  keys: at a multiple of
@@ -480,7 +489,7 @@ template <int TH> __host__ __device__ constexpr int room(int slots) { return TH 
 template <int TH> struct Hunt {
     uint16_t suspects[kSuspects<TH>];
     uint32_t n_suspects, n_candidates, waves[TH / 64];
-    double log_sum_exp;
+    Level level;
 };
 
 // part[row][split] = the sums of a split of a row, keys[row][split][top] its largest, 0 where there are fewer; a whole
@@ -546,7 +555,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
         Hunt<TH>& hunt = hunts[wave];
         if (lane == 0) {
             hunt.n_suspects = hunt.n_candidates = 0;
-            if (alone) hunt.log_sum_exp = row_results(q, h, out, r, label, xl, a);
+            if (alone) hunt.level = row_results(q, h, out, r, label, xl, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
         uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
@@ -614,12 +623,12 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
             meet<TH>();
             for (int i = lane; i < top; i += TH) own_lds[i] = mine[i];
             meet<TH>();
-            by_rank<TH>(own_lds, top, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+            by_rank<TH>(own_lds, top, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.level); });
             return;
         }
         const int n = (int)hunt.n_candidates;
         if (alone) {
-            by_rank<TH>(candidates, n, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.log_sum_exp); });
+            by_rank<TH>(candidates, n, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, hunt.level); });
         } else {
             for (int i = n + lane; i < top; i += TH) mine[i] = 0;
             by_rank<TH>(candidates, n, top, [&](int rank, uint64_t key) { mine[rank] = key; });
@@ -635,7 +644,7 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
     __shared__ __align__(16) uint64_t candidates[TOP ? kMergeKeys + 2 : 1];
     __shared__ uint32_t orders[TOP ? kT : 1];
     __shared__ uint32_t count;
-    __shared__ double log_sum_exp;
+    __shared__ Level level_of;
     const int lane = TOP ? threadIdx.x : threadIdx.x % lanes;
     const int64_t r = TOP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (kT / lanes) + threadIdx.x / lanes;
     if (r >= q.rows) return;
@@ -662,8 +671,8 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
         }
         wave_join(a, h, TOP ? 64 : lanes);
         if (lane == 0) {
-            const double lse = row_results(q, h, out, r, label, xl, a);
-            if (TOP) log_sum_exp = lse;
+            const Level level = row_results(q, h, out, r, label, xl, a);
+            if (TOP) level_of = level;
         }
     }
     if constexpr (TOP) {
@@ -672,7 +681,7 @@ __global__ __launch_bounds__(kT) void k_statistics_rows(const Rows q, const Heat
         for (int i = 0; i < kMergeKeys / kT; ++i)
             if (own[i] != 0 && (uint32_t)(own[i] >> 32) >= bound) candidates[atomicAdd(&count, 1u)] = own[i];
         __syncthreads();
-        by_rank<kT>(candidates, (int)count, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, log_sum_exp); });
+        by_rank<kT>(candidates, (int)count, top, [&](int rank, uint64_t key) { top_result(h, out, r * top + rank, key, level_of); });
     }
 }
 
@@ -735,10 +744,10 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
     if (lane == 0) part[at] = make_float4(a.m, a.s, a.u, 0.0f);
 }
 
-// What a wave finds of a row's teacher: mass and sum of p (log p - z) over its tokens (one outside of the vocabulary
-// makes them NaN), and, BUCKET, the sums over its tokens and over what else is in their runs.
+// What a wave finds of a row's teacher: mass and sum of p (log p - (x - ref) / tau) over its tokens (one outside of the
+// vocabulary makes them NaN), ref a logit of one of them, so that large ones lose nothing, and, BUCKET, the sums over its tokens and over what else is in their runs.
 template <int U> struct Known {
-    double mass, cross, log_mass;
+    double mass, cross, log_mass, ref;
     Sums<U> tokens, others;
 };
 
@@ -764,22 +773,31 @@ __device__ __forceinline__ Known<U> known_part(const Rows& q, const Heat& h, con
         for (int i = lane; i < kSeen / 32; i += 64) own_lds.seen[i] = 0;
         meet<64>();
     }
-    for (int j = lane; j < t.top; j += 64) {
-        const int64_t id = teacher_id(t, r * t.top + j);
-        const float lp = *gbl(t.logps + r * t.top + j);
+    float ref = 0.0f;
+    for (int j0 = 0; j0 < t.top; j0 += 64) {  // every lane: the first 64 agree on ref
+        const int j = j0 + lane;
+        const bool there = j < t.top;
+        const int64_t id = there ? teacher_id(t, r * t.top + j) : -1;
+        const float lp = there ? *gbl(t.logps + r * t.top + j) : -__builtin_inff();
         const bool held = lp != -__builtin_inff(), in = id >= 0 && id < q.vocab;
-        ids[j] = held && in ? (int32_t)id : -1;
+        const float v = held && in ? to_f32<DT>(*gbl(x + id)) : -__builtin_inff();
+        if (j0 == 0) {
+            ref = v;
+            for (int off = 32; off > 0; off >>= 1) ref = __builtin_fmaxf(ref, __shfl_xor(ref, off, 64));
+            if (__builtin_fabsf(ref) == __builtin_inff()) ref = 0.0f;
+        }
+        if (there) ids[j] = held && in ? (int32_t)id : -1;
         if (!held) continue;
         const double p = in ? exp((double)lp) : __longlong_as_double(0x7ff8000000000000ll);
         o.mass += p;
-        const float v = in ? to_f32<DT>(*gbl(x + id)) : 0.0f;
         if (BUCKET && in) {
             const uint32_t bit = (uint32_t)(id / W) % kSeen;
             shared |= atomicOr(&own_lds.seen[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
         }
         if (BUCKET && in && j == lane) held_run = load_logits<DT, false>(x + id / W * W, q.vocab - id / W * W);
-        if (p > 0.0) o.cross += p * ((double)lp - (double)v * h.inv64);
+        if (p > 0.0) o.cross += p * ((double)lp - ((double)v - (double)ref) * h.inv64);
     }
+    o.ref = (double)ref;
     meet<64>();
     o.mass = wave_allsum_d(o.mass);
     o.cross = wave_allsum_d(o.cross);
@@ -862,7 +880,7 @@ __device__ __forceinline__ Slope row_slope(const Rows& q, const Heat& h, const T
     const double log_of = log(lane == 0 ? sum : lane == 1 ? sum1 : lane == 2 ? rest : gap > 600.0 ? odds : 1.0 + odds);
     const double log_sum = __shfl(log_of, 0, 64), log_sum1 = __shfl(log_of, 1, 64), log_rest = __shfl(log_of, 2, 64);
     const double log_odds = __shfl(log_of, 3, 64) + (gap > 600.0 ? gap : 0.0);
-    const double d = known.cross + mass * (m * h.inv64 + log_sum) + (rest > 0.0 ? rest * (log_rest + log_odds) : 0.0);
+    const double d = known.cross + mass * ((m - known.ref) * h.inv64 + log_sum) + (rest > 0.0 ? rest * (log_rest + log_odds) : 0.0);
     const double whole = mass + rest, other = rest > 0.0 ? rest / (double)a.s : 0.0;
     double mine = t.soft * whole / sum, others = t.soft * (whole / sum * shift - other), plain = 0.0, nll = 0.0;
     if (t.hard > 0.0) {
@@ -926,7 +944,7 @@ struct DistillSums {
 struct DistillTotals {
     float *loss, *divergence, *nll, *weights;
     double soft, hard;
-    int32_t n_seq, by_sequence;
+    int32_t n_seq, parts, by_sequence;  // parts: sums to add up
 };
 
 __device__ __forceinline__ void distill_total(const DistillTotals& o, double divergence, double nll) {
@@ -936,12 +954,12 @@ __device__ __forceinline__ void distill_total(const DistillTotals& o, double div
     *o.nll = (float)nll;
 }
 
-// Sums over rows, one workgroup per sequence, or one for all rows where there are none; one alone gives the loss and
-// the weight too.  each: null where only the rows are counted.
+// Sums over rows, one workgroup per sequence, or for every span of rows where there are none; one alone gives the loss
+// and the weight too.  each: null where only the rows are counted.
 __global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const double2* __restrict__ each, DistillSums* __restrict__ sums,
-                                                        const DistillTotals out) {
+                                                        int64_t span, const DistillTotals out) {
     __shared__ DistillSums waves[kSeqT / 64];
-    int64_t begin = 0, end = q.rows;
+    int64_t begin = blockIdx.x * span, end = begin + span;
     if (q.n_seq > 0) {
         begin = q.cu ? (int64_t)sload(q.cu + blockIdx.x) : (int64_t)blockIdx.x * q.per_batch;
         end = q.cu ? (int64_t)sload(q.cu + blockIdx.x + 1) : begin + q.per_batch;
@@ -981,24 +999,26 @@ __global__ __launch_bounds__(kSeqT) void k_distill_sums(const Rows q, const doub
 __global__ __launch_bounds__(kT) void k_distill_total(const DistillSums* __restrict__ sums, const DistillTotals out) {
     __shared__ double waves[kT / 64];
     double n = 0.0, seqs = 0.0;
-    for (int i = threadIdx.x; i < out.n_seq; i += kT) {
+    for (int i = threadIdx.x; i < out.parts; i += kT) {
         n += sums[i].n;
         seqs += sums[i].n > 0.0 ? 1.0 : 0.0;
     }
     n = block_sum(n, waves);
     seqs = block_sum(seqs, waves);
     double divergence = 0.0, nll = 0.0;
-    for (int i = threadIdx.x; i < out.n_seq; i += kT) {
+    for (int i = threadIdx.x; i < out.parts; i += kT) {
         const double w = sums[i].n > 0.0 ? (out.by_sequence ? 1.0 / (sums[i].n * seqs) : 1.0 / n) : 0.0;
         if (w > 0.0) {
             divergence += sums[i].divergence * w;
             nll += sums[i].nll * w;
         }
-        out.weights[i] = (float)w;
+        if (out.n_seq > 0) out.weights[i] = (float)w;
     }
     divergence = block_sum(divergence, waves);
     nll = block_sum(nll, waves);
-    if (threadIdx.x == 0) distill_total(out, divergence, nll);
+    if (threadIdx.x != 0) return;
+    if (out.n_seq == 0) out.weights[0] = n > 0.0 ? (float)(1.0 / n) : 0.0f;
+    distill_total(out, divergence, nll);
 }
 
 // ------------------------------------------------------------ gradients
@@ -1052,7 +1072,7 @@ struct StatisticsGrad {
     }
     __device__ __forceinline__ float at(const Row& o, const Heat& h, float x, bool) const {
         const float d = x - o.m, p = heat_exp(d, h) * o.inv_sum;
-        const float logq = __builtin_fmaxf(d, kFar) * h.inv - o.log_sum;
+        const float logq = __builtin_fmaxf(d * h.inv - o.log_sum, -1e3f);  // p is 0 long before
         return p * __builtin_fmaf(o.slope, logq + o.entropy, o.all);
     }
     __device__ __forceinline__ bool entry(const Row& o, const Rows& q, const Heat& h, int j, int64_t& id, float& extra) const {
@@ -1440,7 +1460,7 @@ int statistics_rows(const char* what, const gefenx_logits* l, int top, Rows& q) 
     if (top > kWaveTop) q.per = 1;
     split_sums(*l, q);
     if (top && q.splits * top > kMergeKeys) set_splits(*l, q, kMergeKeys / top);
-    if (q.rows * q.splits > kMaxThreads / kT)
+    if ((q.rows * q.splits + q.per - 1) / q.per > kMaxThreads / kT)
         return set_error(GEFENX_EINVAL, "%s: too many rows (%lld)", what, (long long)l->rows);
     return GEFENX_OK;
 }
@@ -1451,7 +1471,7 @@ int marked_rows(const char* what, const gefenx_logits* l, bool sequences, bool l
     if (rc != GEFENX_OK) return rc;
     if (!most) split_sums(*l, q);
     if (q.split_runs > kBits) set_splits(*l, q, q.splits * ((q.split_runs + kBits - 1) / kBits) + 1);
-    if (q.split_runs > kBits || q.rows * q.splits > kMaxThreads / kT)
+    if (q.split_runs > kBits || (q.rows * q.splits + q.per - 1) / q.per > kMaxThreads / kT)
         return set_error(GEFENX_EINVAL, "%s: too many logits (%lld x %lld)", what, (long long)l->rows, (long long)l->vocab);
     return GEFENX_OK;
 }
@@ -1473,6 +1493,9 @@ int run_tokens_grad(const char* what, const Rows& q, int dtype, const Heat& h, c
         return launched(what);
     });
 }
+
+// Workgroups that add up the rows: one per sequence; without sequences one alone as long as it is quick about it.
+int sum_parts(const Rows& q) { return q.n_seq > 0 ? q.n_seq : (int)std::min<int64_t>(64, std::max<int64_t>(1, q.rows / 16384)); }
 
 // A checked call of the distillation.
 struct Distill {
@@ -1513,15 +1536,15 @@ int make_distill(const char* what, const gefenx_logits* l, const gefenx_teacher*
     d.by_sequence = t->by_sequence;
     d.t = Teacher{t->ids, t->logps, t->top, t->ids64, t->rest, (float)((1.0 - t->hard_weight) * t->temperature),
                   (1.0 - t->hard_weight) * t->temperature * t->temperature, t->hard_weight};
-    d.bytes = sums_bytes(d.q) + sizeof(double2) * (size_t)d.q.rows + sizeof(DistillSums) * (size_t)std::max(d.q.n_seq, 1);
+    d.bytes = sums_bytes(d.q) + sizeof(double2) * (size_t)d.q.rows + sizeof(DistillSums) * (size_t)sum_parts(d.q);
     return GEFENX_OK;
 }
 
 // The loss and the weights by the rows' results, or (each null) the weights alone.
 int distill_totals(const Distill& d, const double2* each) {
-    const int n = std::max(d.q.n_seq, 1);
-    k_distill_sums<<<(uint32_t)n, kSeqT, 0, d.s>>>(d.q, each, d.sums, d.out);
-    if (n > 1) k_distill_total<<<1, kT, 0, d.s>>>(d.sums, d.out);
+    const int64_t span = (d.q.rows + d.out.parts - 1) / d.out.parts;
+    k_distill_sums<<<(uint32_t)d.out.parts, kSeqT, 0, d.s>>>(d.q, each, d.sums, span, d.out);
+    if (d.out.parts > 1) k_distill_total<<<1, kT, 0, d.s>>>(d.sums, d.out);
     return launched(d.what);
 }
 
@@ -1539,7 +1562,7 @@ int distill_outputs(Distill& d, float* loss, float* divergence, float* nll, floa
     d.s = static_cast<hipStream_t>(stream);
     d.token_divergence = token_divergence;
     d.slopes = static_cast<Slope*>(slopes);
-    d.out = DistillTotals{loss, divergence, nll, weights, d.t.loss, d.t.hard, d.q.n_seq, d.by_sequence};
+    d.out = DistillTotals{loss, divergence, nll, weights, d.t.loss, d.t.hard, d.q.n_seq, sum_parts(d.q), d.by_sequence};
     return GEFENX_OK;
 }
 

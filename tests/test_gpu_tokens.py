@@ -243,6 +243,68 @@ def test_masked_logits(dev, V, dtype):
         assert math.isnan(got.logps[r].item()) and math.isnan(got.entropy[r].item())
 
 
+FILLS = {torch.float32: [-1e7, -3e7, -1e9, -1e10, -1e12, 1e10, 2e30, -1e38], torch.float16: [-1e4, -65504.0, 6e4],
+         torch.bfloat16: [-1e9, -1e10, 1e12, -1e38]}
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.01, 50.0])
+@pytest.mark.parametrize("V", [24, 3001, 9000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_logits(dev, dtype, V, temperature):
+    """Rows that a large mask value leaves nothing, or one step above it, or some ordinary logits."""
+    rows = []
+    for fill in FILLS[dtype]:
+        row = torch.full((V,), fill).to(dtype)
+        next_ = row.clone()
+        # one representable step towards 0, for every third
+        step = torch.nextafter(row.float() if dtype is torch.float32 else row, torch.zeros_like(row))
+        next_[::3] = step[::3].to(dtype)
+        some = row.clone()
+        some[5:15] = torch.linspace(-2, 2, 10).to(dtype)
+        rows += [row, next_, some]
+    x = torch.stack(rows)
+    T = x.shape[0]
+    labels = torch.arange(T) % V
+    z = x.double() / temperature
+    ids = statistics64(z, 7)[2]
+    logits = x.to(dev).requires_grad_()
+    got = gefen.token_statistics(logits, labels.to(dev), top=7, temperature=temperature)
+    (got.logps.sum() + got.entropy.sum()).backward()
+    err = sum_error(z)
+    assert torch.equal(got.top_ids.cpu(), ids)
+    for r in range(T):
+        # relative to the maximum: a logsumexp of numbers like these rounds at their scale
+        exact = ((z[r, labels[r]] - z[r].amax()) - torch.log(torch.exp(z[r] - z[r].amax()).sum())).item()
+        if exact < -3.5e38:  # beyond fp32
+            assert got.logps[r].item() == -INF
+        else:
+            assert abs(got.logps[r].item() - exact) <= err[r] + U * (2 * abs(exact) + 4), r
+        p = torch.softmax(z[r] - z[r].amax(), 0)
+        ent = -(p * torch.where(p > 0, p.log(), torch.zeros_like(p))).sum()
+        assert abs(got.entropy[r].item() - ent.item()) <= entropy_error(z[r:r + 1] - z[r].amax(), ent[None]).item(), r
+        assert torch.all(logits.grad[r].isfinite())
+    # a student like that, held to its own top tokens: nothing to learn, and nothing lost
+    own = gefen.token_statistics(x.to(dev), top=7, temperature=temperature)
+    for rest in ("bucket", "drop", "normalize"):
+        out, grad = gefen.distillation_loss_and_grad(x.to(dev), labels.to(dev), own.top_ids, own.top_logps, rest=rest,
+                                                     temperature=temperature, hard_weight=0.25)
+        if rest != "normalize":
+            # of the difference of p log p and p log q the roundings of log p (up to 10) and the sums' errors are left
+            assert torch.all(out.token_divergence.abs().cpu().double() <= 1e-5 + 2 * err), rest
+        assert out.token_divergence.isfinite().all() and grad.isfinite().all()
+
+
+def test_statistics_without_labels(dev):
+    x, _, g = rows_of(6, 700, torch.float32)
+    a, b = x.to(dev).requires_grad_(), x.to(dev).requires_grad_()
+    one = gefen.token_statistics(a, top=3)
+    two = gefen.token_statistics(b, torch.zeros(6, dtype=torch.long, device=dev), top=3)
+    assert one.logps is None and torch.equal(one.entropy, two.entropy) and torch.equal(one.top_logps, two.top_logps)
+    for o in (one, two):
+        (o.entropy.sum() * 2 + o.top_logps[:, 1].sum()).backward()
+    assert torch.equal(a.grad, b.grad)
+
+
 def test_labels_outside_of_the_vocabulary(dev):
     x, _, _ = rows_of(4, 30, torch.float32)
     labels = torch.tensor([3, 30, -1, IGNORE])
@@ -598,6 +660,27 @@ def test_rows_outside_of_the_sequences(dev):
         assert torch.equal(out.loss, inside.loss) and torch.equal(grad[2:8], g2)
         assert not grad[:2].any() and not grad[8:].any()
         assert not out.token_divergence[:2].any() and not out.token_divergence[8:].any()
+
+
+def test_many_short_rows(dev):
+    """More rows than one workgroup adds up, without sequences and with them."""
+    T, V, k = 70000, 24, 3
+    g = torch.Generator(dev).manual_seed(9)
+    x = torch.randn(T, V, device=dev, generator=g)
+    lp, ids = (x + torch.randn(T, V, device=dev, generator=g)).log_softmax(-1).topk(k, -1)
+    labels = torch.randint(0, V, (T,), device=dev, generator=g)
+    labels[torch.rand(T, device=dev, generator=g) < 0.5] = IGNORE
+    valid = labels != IGNORE
+    out, grad = gefen.distillation_loss_and_grad(x, labels, ids, lp, hard_weight=0.5)
+    n = int(valid.sum())
+    each = out.token_divergence.double()
+    assert abs(out.divergence.item() - each[valid].mean().item()) <= 2 * U * abs(out.divergence.item()) + 1e-9
+    nll = -x.double().log_softmax(-1).gather(1, labels.clamp(min=0)[:, None])[:, 0][valid].mean().item()
+    assert abs(out.nll.item() - nll) <= 70 * U + U * nll
+    cu = torch.tensor([0, 30000, T], dtype=torch.int32, device=dev)
+    two, g2 = gefen.distillation_loss_and_grad(x, labels, ids, lp, hard_weight=0.5, cu_seqlens=cu)
+    assert torch.equal(out.token_divergence, two.token_divergence) and abs(out.loss.item() - two.loss.item()) <= 2 * U * out.loss.item()
+    assert (grad - g2).abs().max().item() <= 4 * U / n
 
 
 def test_nothing_to_learn_from(dev):
