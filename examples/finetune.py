@@ -1,11 +1,12 @@
-"""A fine-tuning loop on one MI355X: preference loss, then policy loss, stepped by AdamW.
+"""A fine-tuning loop on one MI355X: preference loss, then policy loss, then distillation, stepped by AdamW.
 
     python examples/finetune.py [--steps N]
 
 A small random language model learns to prefer answers that use one half of the
 vocabulary (pairs of answers, a frozen copy of the model as the reference, 8-bit
 moments), then to emit tokens of one residue class (sampled answers, advantages
-within the group, 32-bit moments).  Synthetic data; prints the losses.
+within the group, 32-bit moments); a fresh student learns from its likeliest tokens.
+Synthetic data; prints the losses.
 """
 import argparse
 import copy
@@ -97,6 +98,25 @@ def reinforce(model, steps, group=64):
     return torch.stack(rewards).tolist()
 
 
+def distill(teacher, student, steps, batch=16, temperature=2.0):
+    """The student learns from the teacher's 32 likeliest tokens along answers that the teacher sampled."""
+    opt = gefen.AdamW(student.named_parameters(), lr=2e-3, weight_decay=0.0, max_grad_norm=1.0)
+    divergences = []
+    for _ in range(steps):
+        tokens = sample(teacher, torch.randint(0, VOCAB, (batch, PROMPT), device=teacher.head.weight.device))
+        labels = shifted(tokens)
+        with torch.no_grad():
+            top = gefen.token_statistics(teacher(tokens), labels, top=32, temperature=temperature)
+        logits = student(tokens)
+        out, grad = gefen.distillation_loss_and_grad(logits, labels, top.top_ids, top.top_logps, temperature=temperature,
+                                                     hard_weight=0.1)
+        opt.zero_grad()
+        logits.backward(grad)
+        opt.step()
+        divergences.append(out.divergence)
+    return torch.stack(divergences).tolist()
+
+
 def main(steps=60, dtype=torch.bfloat16):
     torch.manual_seed(0)
     model = Model().to("cuda", dtype)
@@ -104,6 +124,8 @@ def main(steps=60, dtype=torch.bfloat16):
     print("preference loss: first {:.4f}, last {:.4f}".format(losses[0], losses[-1]))
     rewards = reinforce(model, steps)
     print("mean reward: first {:.4f}, last {:.4f}".format(rewards[0], rewards[-1]))
+    divergences = distill(model, Model().to("cuda", dtype), steps)
+    print("divergence from the teacher: first {:.4f}, last {:.4f}".format(divergences[0], divergences[-1]))
     return losses, rewards
 
 

@@ -209,7 +209,7 @@ def test_ties_and_orders(dev, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [40, 3001])
+@pytest.mark.parametrize("V", [40, 3001, 70001])
 def test_masked_logits(dev, V, dtype):
     """-inf and the type's lowest value in masked places, rows that they leave nothing, NaN and +inf."""
     g = torch.Generator().manual_seed(1)
@@ -402,6 +402,60 @@ def test_long_rows(dev):
         assert torch.all((x.grad[keep].cpu().double() - want).abs() <= tol)
         assert not x.grad[2:1000].any()
         x.grad = None
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 logits, of which a few rows count; and a row of 20 million."""
+    T, V = 17000, 131072
+    x = torch.zeros(T, V, device=dev, dtype=torch.bfloat16)
+    keep = torch.tensor([3, T - 2, T - 1], device=dev)
+    x[keep] = (torch.randn(3, V, device=dev, generator=torch.Generator(dev).manual_seed(2)) * 2).bfloat16()
+    labels = torch.full((T,), IGNORE, device=dev)
+    labels[keep] = torch.tensor([0, 70000, V - 1], device=dev)
+    z, y = x[keep].double().cpu(), labels[keep].cpu()
+    got = gefen.token_statistics(x.requires_grad_(), labels, top=16)
+    lq, h, ids = statistics64(z, 16)
+    assert torch.equal(got.top_ids[keep].cpu(), ids)
+    lp = lq.gather(1, y[:, None])[:, 0]
+    assert torch.all((got.logps[keep].detach().cpu().double() - lp).abs() <= sum_error(z) + U * (2 * lp.abs() + 4))
+    got.logps.sum().backward()
+    p = lq.exp()
+    hot = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+    far = z.amax(1, keepdim=True) - z
+    tol = UNIT[x.dtype] * (hot - p).abs() * 1.01 + p * (sum_error(z)[:, None] + U * (4 * far + 32)) + LEAST[x.dtype]
+    assert torch.all((x.grad[keep].cpu().double() - (hot - p)).abs() <= tol)
+    assert not x.grad[4:T - 2].any()
+    x.grad = None
+    x.requires_grad_(False)
+    lps = torch.zeros(T, 16, device=dev)
+    lps[keep] = got.top_logps.detach()[keep] - 0.125
+    x64 = z.clone().requires_grad_()
+    loss, _, _, each = distill64(x64, y, [(0, 3)], ids, lps[keep].cpu(), 1.0, "bucket", 0.0, "token")
+    loss.backward()
+    for hard in (0.0, 0.3):  # rows of their own, and two passes
+        t = 1.0 if hard == 0.0 else 2.0
+        x64 = z.clone().requires_grad_()
+        loss, _, _, each = distill64(x64, y, [(0, 3)], ids, lps[keep].cpu(), t, "bucket", hard, "token")
+        loss.backward()
+        out, grad = gefen.distillation_loss_and_grad(x, labels, got.top_ids, lps, hard_weight=hard, temperature=t)
+        check_distill(z, y, [(0, 3)], ids, lps[keep].cpu(), t, "bucket", hard, "token", x64.grad, each.detach(),
+                      grad[keep].cpu().double(), out.token_divergence[keep].cpu().double(), x.dtype)
+        del grad
+    del x
+    V = 20000003
+    x = torch.randn(2, V, device=dev, generator=torch.Generator(dev).manual_seed(3)).half()
+    got = gefen.token_statistics(x, top=128)
+    ids = torch.sort(x.double(), dim=-1, descending=True, stable=True)[1][:, :128]
+    assert torch.equal(got.top_ids, ids)
+    lq = torch.log_softmax(x.double(), -1)
+    assert (got.top_logps.double() - lq.gather(1, ids)).abs().max().item() <= U * (V / 256 + 100)
+    out, grad = gefen.distillation_loss_and_grad(x, torch.zeros(2, dtype=torch.long, device=dev), ids, got.top_logps - 1.0, rest="drop",
+                                                 grad_scale=1e5)
+    q, p = lq.exp(), (got.top_logps - 1.0).double().exp()
+    want = (q * p.sum(1, keepdim=True)).scatter_add_(1, ids, -p) * 5e4
+    # the bound of a sum's error, V / 256 units, is 5e-3 here
+    assert torch.all((grad.double() - want).abs() <= UNIT[x.dtype] * want.abs() * 1.01 + 5e4 * q * 1e-2 * p.sum(1, keepdim=True) + 5e4 * p.max() * 1e-5
+                     + LEAST[x.dtype])
 
 
 # ------------------------------------------------ distillation
@@ -786,6 +840,49 @@ def test_teacher_to_student(dev):
     out, grad = gefen.distillation_loss_and_grad(same, labels.to(dev), own.top_ids, own.top_logps, temperature=temperature)
     # of a divergence of 0 the terms' errors are left: the log-probabilities' roundings (2^-24 of up to 10) on both sides
     assert abs(out.loss.item()) <= 1e-5 and grad.abs().max().item() <= 1e-6
+
+
+def test_example_distills(dev):
+    """The example's distillation runs, and its student's gradients are those of plain torch in float64."""
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("finetune", os.path.join(root, "examples", "finetune.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    torch.manual_seed(0)
+    teacher, student = m.Model().to(dev), m.Model().to(dev)
+    twin = m.Model().to(dev)
+    twin.load_state_dict(student.state_dict())
+    seen = {}
+    real = gefen.distillation_loss_and_grad
+
+    def watched(logits, labels, ids, logps, **kw):
+        if not seen:
+            seen.update(labels=labels, ids=ids, logps=logps, kw=kw)
+        return real(logits, labels, ids, logps, **kw)
+
+    class Watch:
+        token_statistics, distillation_loss_and_grad = staticmethod(gefen.token_statistics), staticmethod(watched)
+
+        class AdamW(gefen.AdamW):
+            def step(self, closure=None):
+                seen.setdefault("grads", [p.grad.clone() for g in self.param_groups for p in g["params"]])
+                return super().step(closure)
+
+    tokens = []
+    sample, m.sample, m.gefen = m.sample, lambda *a: tokens.append(sample(*a)) or tokens[-1], Watch
+    divergences = m.distill(teacher, student, 3)
+    assert len(divergences) == 3 and all(math.isfinite(d) and d > 0 for d in divergences)
+    twin = twin.double().cpu()
+    logits = twin(tokens[0].cpu()).view(-1, m.VOCAB)
+    labels, k = seen["labels"].cpu().view(-1), seen["ids"].shape[-1]
+    loss = distill64(logits, labels, [(0, labels.numel())], seen["ids"].cpu().view(-1, k), seen["logps"].cpu().view(-1, k),
+                     seen["kw"]["temperature"], "bucket", seen["kw"]["hard_weight"], "token")[0]
+    loss.backward()
+    for got, want in zip(seen["grads"], twin.parameters()):
+        # an fp32 model against a float64 one: sums of hundreds of terms either way
+        assert (got.cpu().double() - want.grad).abs().max().item() <= 1e-4 * want.grad.abs().max().item() + 1e-9
 
 
 def test_repeats_are_equal(dev):
