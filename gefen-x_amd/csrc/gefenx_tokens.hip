@@ -1412,8 +1412,21 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
     for (int i = kKeptRegs - 1; i >= 0; --i) put(held[i], number(kKeptLds + i));
 #pragma unroll
     for (int i = kKeptLds - 1; i >= 0; --i) put(kept[i * kRowT + threadIdx.x], number(i));
-    for (int64_t c = (first - 1) * kRowT + threadIdx.x; c >= 0; c -= kRowT)
+    // the others in pairs, one on its way while the other is written
+    int64_t c = (first - 1) * kRowT + threadIdx.x;
+    if (first & 1) {
         put(o.zero ? zeros : load_logits<DT>(x + c * W), c);
+        c -= kRowT;
+    }
+    for (; c >= 0; c -= 2 * kRowT) {
+        Run<T, W> v[2] = {zeros, zeros};
+        if (!o.zero) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[i] = load_logits<DT>(x + (c - i * kRowT) * W);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) put(v[i], c - i * kRowT);
+    }
 }
 
 // ------------------------------------------------------------ host side
