@@ -1258,13 +1258,14 @@ __global__ __launch_bounds__(kT) void k_tokens_grad(const Rows q, const Heat h, 
 
 // ------------------------------------------------------------ loss and gradient of a row in one go
 constexpr int kRowT = 1024;                 // threads of a workgroup that keeps a row to itself
-constexpr int kKeptLds = 4, kKeptRegs = 1;  // steps of a row (16 KB) that it keeps on chip
+constexpr int kKept = 4;                    // steps of a row (16 KB) that it keeps in LDS
 constexpr int kRowMarks = 32768;            // runs of such a row
 constexpr int kRowEntries = 2;              // of a lane: the teacher's tokens and the label
 
 // A row by one workgroup: its sums, its loss, its gradient, where its weight is known before (the labels alone give it).
 // Two workgroups a CU hold 512 rows, which the 256 MB cache still has when they are read again, last part first; the
-// last steps stay in LDS and registers between.  Rows of the gradient start at multiples of 16 bytes.  The first wave
+// last steps stay in LDS between (a step in registers too spills: 8192 x 128256 bf16 all labelled, without the others'
+// sum, 0 / 1 / 2 steps 844 / 895 / 976 us).  Rows of the gradient start at multiples of 16 bytes.  The first wave
 // reads the teacher's tokens while the others are at the sums; in the gradient every wave holds them, a few to a lane,
 // and asks by ballots which fall into its step.
 template <int DT, bool BUCKET>
@@ -1277,7 +1278,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
     __shared__ Slope slope_of;
     __shared__ uint32_t marks[BUCKET ? kRowMarks / 32 : 1];
     __shared__ Named<kRowEntries * 64> named_of;
-    __shared__ Run<T, W> kept[kKeptLds * kRowT];
+    __shared__ Run<T, W> kept[kKept * kRowT];
     const Teacher& t = g.g.t;
     const int64_t r = blockIdx.x, label = sload(q.labels + r);
     const int lane = threadIdx.x & 63;
@@ -1330,11 +1331,9 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
     }
     const auto skip = [&](int64_t run) { return BUCKET && (marks[run >> 5] >> (run & 31) & 1); };
     const int64_t steps = (n + kRowT - 1) / kRowT;
-    constexpr int kKept = kKeptLds + kKeptRegs;
     const int64_t first = steps > kKept ? steps - kKept : 0;
     const auto number = [&](int i) { return (first + i) * kRowT + threadIdx.x; };  // of kept run i
     Sums<U> a = row_sums<DT, U, kRowT, false>(x, q.vocab, 0, first * kRowT, threadIdx.x, h, skip, [](float, float) {});
-    Run<T, W> held[kKeptRegs];
     {
         LaneSums<U> end;
         const auto add = [&](const Run<T, W>& raw, int i) {
@@ -1347,7 +1346,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
         };
         // what lies past the row's end reads as -inf
 #pragma unroll
-        for (int i = 0; i < kKeptLds; i += 2) {
+        for (int i = 0; i < kKept; i += 2) {
             Run<T, W> v[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) v[j] = load_logits<DT>(x + number(i + j) * W, q.vocab - number(i + j) * W);
@@ -1357,11 +1356,6 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
                 kept[(i + j) * kRowT + threadIdx.x] = v[j];
             }
         }
-#pragma unroll
-        for (int i = 0; i < kKeptRegs; ++i)
-            held[i] = load_logits<DT>(x + number(kKeptLds + i) * W, q.vocab - number(kKeptLds + i) * W);
-#pragma unroll
-        for (int i = 0; i < kKeptRegs; ++i) add(held[i], kKeptLds + i);
         const Sums<U> b = end.sums(h);
         a.join(b.m, b.s, b.u, h);
     }
@@ -1409,9 +1403,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
         store_run<T, W>(out + c * W, W, v);
     };
 #pragma unroll
-    for (int i = kKeptRegs - 1; i >= 0; --i) put(held[i], number(kKeptLds + i));
-#pragma unroll
-    for (int i = kKeptLds - 1; i >= 0; --i) put(kept[i * kRowT + threadIdx.x], number(i));
+    for (int i = kKept - 1; i >= 0; --i) put(kept[i * kRowT + threadIdx.x], number(i));
     // the others in pairs, one on its way while the other is written
     int64_t c = (first - 1) * kRowT + threadIdx.x;
     if (first & 1) {
