@@ -1609,11 +1609,16 @@ int distill_forward(Distill& d) {
     return distill_totals(d, d.each);
 }
 
-// Whether loss and gradient go row by row.
+// Whether loss and gradient go row by row: rows of 96 KB or more, in rounds of two workgroups a CU that are full enough
+// (32 tokens of the teacher, a fifth masked, us against two passes: bf16 256 x 128256 43 / 53, 768 x 128256 108 / 103,
+// 1536 x 128256 173 / 219, 4096 x 49152 191 / 194, 8192 x 65536 436 / 464, fp32 8192 x 16384 249 / 247, 8192 x 32768
+// 386 / 462).  The second exponential, where labels count at a temperature, would spill.  All rows count: how many are
+// masked only the device knows.
 bool rows_alone(const gefenx_logits& l, const gefenx_teacher& t, const void* grad) {
     const int64_t run = l.dtype == GEFENX_F32 ? 4 : 8, bytes = l.vocab * (16 / run);
-    return bytes >= (l.dtype == GEFENX_F32 ? 128 : 192) << 10 && l.rows >= 1024 && l.rows <= kMaxThreads / kRowT && l.rows * bytes > (int64_t)400 << 20 &&
-           l.vocab % run == 0 && l.vocab / run <= kRowMarks && !(t.hard_weight > 0.0 && t.temperature != 1.0) && t.top < kRowEntries * 64 && ((uintptr_t)grad & 15) == 0;
+    const bool full = l.rows >= 4 * kCus || (l.rows >= kCus && l.rows <= 2 * kCus);
+    return bytes >= (96 << 10) && full && l.rows <= kMaxThreads / kRowT && l.vocab % run == 0 && l.vocab / run <= kRowMarks &&
+           ((uintptr_t)grad & 15) == 0 && t.top < kRowEntries * 64 && !(t.hard_weight > 0.0 && t.temperature != 1.0);
 }
 
 int distill_alone(Distill& d, const float* scale_dev, double scale, void* grad) {

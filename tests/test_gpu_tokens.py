@@ -573,7 +573,8 @@ def test_distillation(dev, lengths, V, k, dtype, packed):
 
 ALONE = [  # many long rows, whose loss and gradient one workgroup each finds: type, rows, vocabulary, teacher's tokens, column
     (torch.bfloat16, 1050, 200000, 64, 0), (torch.bfloat16, 1700, 131072, 127, 3), (torch.float16, 1700, 131080, 5, 0),
-    (torch.float32, 1100, 100000, 100, 1), (torch.bfloat16, 1700, 131072, 128, 0), (torch.float16, 1700, 131079, 20, 0)]
+    (torch.float32, 1100, 100000, 100, 1), (torch.bfloat16, 1700, 131072, 128, 0), (torch.float16, 1700, 131079, 20, 0),
+    (torch.bfloat16, 1030, 49160, 33, 5), (torch.float32, 1030, 24576, 4, 0)]
 
 
 @pytest.mark.parametrize("dtype,T,V,k,column", ALONE)
