@@ -885,7 +885,8 @@ __device__ __forceinline__ Slope row_slope(const Rows& q, const Heat& h, const T
     const double log_sum = __shfl(log_of, 0, 64), log_sum1 = __shfl(log_of, 1, 64), log_rest = __shfl(log_of, 2, 64);
     const double log_odds = __shfl(log_of, 3, 64) + (gap > 600.0 ? gap : 0.0);
     const double d = known.cross + mass * ((m - known.ref) * h.inv64 + log_sum) + (rest > 0.0 ? rest * (log_rest + log_odds) : 0.0);
-    const double whole = mass + rest, other = rest > 0.0 ? rest / (double)a.s : 0.0;
+    // of weight 0 the teacher's part is not there, whatever it would be
+    const double whole = t.soft > 0.0f ? mass + rest : 0.0, other = t.soft > 0.0f && rest > 0.0 ? rest / (double)a.s : 0.0;
     double mine = t.soft * whole / sum, others = t.soft * (whole / sum * shift - other), plain = 0.0, nll = 0.0;
     if (t.hard > 0.0) {
         const bool in = (uint64_t)label < (uint64_t)q.vocab;
@@ -1131,10 +1132,11 @@ struct DistillGrad {
         if (PLAIN) y = __builtin_fmaf(exp_(x - o.m), o.plain, y);
         return y;
     }
-    __device__ __forceinline__ bool entry(const Row& o, const Rows& q, const Heat&, int j, int64_t& id, float& extra) const {
+    __device__ __forceinline__ float extra(const Row& o, float lp) const { return g.t.soft > 0.0f ? -o.soft * exp_(lp - o.log_mass) : 0.0f; }
+    __device__ __forceinline__ bool entry(const Row& o, const Rows& q, const Heat&, int j, int64_t& id, float& more) const {
         id = teacher_id(g.t, o.first + j);
         const float lp = *gbl(g.t.logps + o.first + j);
-        extra = -o.soft * exp_(lp - o.log_mass);
+        more = extra(o, lp);
         return lp != -__builtin_inff() && (uint64_t)id < (uint64_t)q.vocab;
     }
 };
@@ -1382,7 +1384,7 @@ __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const 
     const DistillGrad<false>::Row o = g.row(slope_of, g.weight(q, r), r);
     float extra_of[kRowEntries];
 #pragma unroll
-    for (int e = 0; e < kRowEntries; ++e) extra_of[e] = e * 64 + lane < t.top ? -o.soft * exp_(lp[e] - o.log_mass) : o.label_extra;
+    for (int e = 0; e < kRowEntries; ++e) extra_of[e] = e * 64 + lane < t.top ? g.extra(o, lp[e]) : o.label_extra;
     const auto put = [&](Run<T, W> v, int64_t c) {  // c: of a wave 64 runs in a row
         if (o.zero) {
             if (c < n) store_run<T, W>(out + c * W, W, zeros);

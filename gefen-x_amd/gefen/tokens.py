@@ -208,7 +208,8 @@ def distillation_loss(logits, labels, teacher_ids, teacher_logps, *, cu_seqlens=
 
     and loss = mean of (1 - hard_weight) temperature^2 D - hard_weight log softmax(logits)[label] over the labelled
     rows, or (reduction "sequence") the mean over the sequences that have any of their mean; 0 without any.  An entry of
-    log-probability -inf names no token, whatever its id.  With hard_weight 0 labels only say which rows count."""
+    log-probability -inf names no token, whatever its id.  With hard_weight 0 labels only say which rows count, with 1
+    the teacher gives the divergence alone, whatever it holds."""
     how = (temperature, rest, hard_weight, reduction)
     return DistillationLoss(*_Distillation.apply(logits, labels, cu_seqlens, ignore_index, teacher_ids, teacher_logps, how))
 

@@ -703,6 +703,33 @@ def test_bad_ids_spoil_their_rows_alone(dev):
     assert out.loss.isfinite() and grad.isfinite().all()
 
 
+@pytest.mark.parametrize("T,V", [(6, 40), (2304, 40), (256, 24576)])  # a workgroup, a wave, rows of their own
+@pytest.mark.parametrize("rest", ["bucket", "drop", "normalize"])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_labels_alone_leave_the_teacher_out(dev, T, V, rest, temperature):
+    """hard_weight 1: a teacher that cannot be told spoils its divergence, neither the loss nor the gradient."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(T, V, generator=g)
+    labels = torch.randint(V, (T,), generator=g)
+    ids = torch.arange(4).repeat(T, 1)
+    logps = torch.full((T, 4), -2.0)
+    ids[1, 2], ids[4, 0] = V, -1
+    logps[3, 1], logps[5, 0] = math.nan, INF
+    out, grad = gefen.distillation_loss_and_grad(x.to(dev), labels.to(dev), ids.to(dev), logps.to(dev), rest=rest, hard_weight=1.0,
+                                                 temperature=temperature, grad_scale=T)
+    assert out.token_divergence[[1, 3, 4]].isnan().all() and out.token_divergence.isfinite().sum() == T - 4
+    x64 = x.double()
+    q = torch.softmax(x64, -1)
+    nll = -torch.log_softmax(x64, -1).gather(1, labels[:, None])[:, 0]
+    err = sum_error(x64)
+    # each row's in float64 from sums in fp32, the loss rounded once
+    assert abs(out.loss.item() - nll.mean().item()) <= err.max().item() + 2 * U * nll.mean().item()
+    want = q.scatter_add(1, labels[:, None], -torch.ones(T, 1, dtype=torch.float64))
+    # an exponent's units over distances up to 10 (32), six products and sums of values up to 1
+    limit = (err[:, None] + 32 * U) * q + 8 * U
+    assert torch.all((grad.cpu().double() - want).abs() <= limit)
+
+
 def test_rows_outside_of_the_sequences(dev):
     d = Data([10], 50, 5, torch.float32, dev, True)
     labels, ids, logps = d.args()
@@ -963,6 +990,37 @@ def test_captured_calls(dev):
             torch.cuda.synchronize()
             assert torch.equal(bits(grad), bits(g)) and all(torch.equal(bits(a), bits(b)) for a, b in zip(out, want))
             assert all(torch.equal(bits(a), bits(b)) for a, b in zip(stats, st))
+
+
+def test_captured_backward(dev):
+    """Forward and backward of fresh leaves in a graph, replayed with new data and eager calls between."""
+    d = [Data([12, 9], 3001, 20, torch.bfloat16, dev, False, seed=s) for s in range(3)]
+
+    def step(x, args):
+        x.grad = None
+        stats = gefen.token_statistics(x, args[0], top=5)
+        out = gefen.distillation_loss(x, *args, hard_weight=0.2)
+        (out.loss + stats.entropy.mean() + stats.top_logps[..., 0].mean()).backward()
+        return out.loss.detach(), stats.entropy.detach(), x.grad
+
+    x, args = d[0].logits(True), d[0].args()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, args)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, args)
+    for new in (d[1], d[2], d[0]):
+        with torch.no_grad():
+            x.copy_(new.logits())
+        for a, b in zip(args, new.args()):
+            a.copy_(b)
+        graph.replay()
+        want = step(new.logits(True), new.args())
+        torch.cuda.synchronize()
+        assert all(torch.equal(bits(a), bits(b)) for a, b in zip(got, want))
 
 
 def test_compiled_callers(dev):
