@@ -501,8 +501,8 @@ template <int TH> struct Hunt {
 // (equal logits) are those over the bound and the first of the equal ones; NaN, +inf and what is left go through
 // select_keys.
 //
-// 4096 x 128256 bf16: 163 us, 6.4 TB/s, the vector units busy 78% of it (7.1 instructions a logit: convert, the
-// maximum, fma, exp, the two sums); with 64 tokens ~215 us, 7% read again for them.  16384 x 1000 fp32 14 us.
+// 4096 x 128256 bf16: 163-175 us, 6.0-6.4 TB/s, the vector units busy 78% of it (7.1 instructions a logit: convert,
+// the maximum, fma, exp, the two sums); with 64 tokens 186 us, 7% read again for them.  16384 x 1000 fp32 14 us.
 template <int DT, int PER, bool TOP>
 __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, const Statistics out,
                                                    float4* __restrict__ part, uint64_t* __restrict__ keys) {
