@@ -9,6 +9,7 @@
 //     d D / d z_v = (P + r) q_v - p_v for the teacher's tokens, q_v (P + r - r / rho) elsewhere
 //     loss = mean over rows of (1 - w) tau^2 D - w log softmax(x)[y]
 // A pass over the logits for the sums, a few numbers per row, and a pass that writes the gradient.
+#include "gefenx_hunt.h"
 #include "gefenx_logits.h"
 
 namespace gx {
@@ -214,8 +215,6 @@ __device__ __forceinline__ void add_runs(LaneSums<U>& a, const Run<typename Elem
     a.s += s;
     a.u += u;
 }
-
-constexpr int kStep = 4;  // runs of a lane in flight
 
 // Runs begin .. end - 1 of a row, TH lanes at a time in steps of kStep runs each; each lane's sums.  skip(run): a
 // run that is left out; note(a, b): the largest of the first and of the second half of a lane's step.  Which logits a
@@ -480,12 +479,10 @@ template <int DT> struct Maxima {
     }
 };
 
-// Maxima of a lane's steps that are kept; how many of them are looked through again, and candidates that there is room
-// for (short rows may have all of their logits among them).
-constexpr int kSlots = 20, kWaveSlots = (int)kShortRuns / (64 * kStep);
+// Maxima of a lane of a wave that has a row of its own; how many maxima are looked through again.
+constexpr int kWaveSlots = (int)kShortRuns / (64 * kStep);
 constexpr int kWaveTop = 32;  // likeliest tokens that a wave finds for a row of its own
 template <int TH> constexpr int kSuspects = TH == kT ? 384 : 128;
-template <int TH> __host__ __device__ constexpr int room(int slots) { return TH < kT ? 256 : slots > 4 ? 384 : 1024; }  // and one more
 template <int TH> struct Hunt {
     uint16_t suspects[kSuspects<TH>];
     uint32_t n_suspects, n_candidates, waves[TH / 64];
@@ -504,7 +501,7 @@ template <int TH> struct Hunt {
 // 4096 x 128256 bf16: 163-175 us, 6.0-6.4 TB/s, the vector units busy 78% of it (7.1 instructions a logit: convert,
 // the maximum, fma, exp, the two sums); with 64 tokens 186 us, 7% read again for them.  16384 x 1000 fp32 14 us.
 template <int DT, int PER, bool TOP>
-__global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, const Statistics out,
+__global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, int room, const Statistics out,
                                                    float4* __restrict__ part, uint64_t* __restrict__ keys) {
     using T = typename Elem<DT>::T;
     constexpr int TH = kT / PER, W = kW<DT>;
@@ -526,8 +523,8 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
     const T* x = (const T*)q.x + row_offset(q, r);
     const float xl = alone ? label_logit<DT>(q, x, label) : 0.0f;  // on its way early
     const auto none = [](int64_t) { return false; };
-    const int slots = TOP && begin < end ? (int)(((end - begin + kStep * TH - 1) / (kStep * TH) + steps_of_slot - 1) / steps_of_slot) : 0;
-    uint64_t* own_lds = dynamic + (PER > 1 ? wave * (TH / 2 * kWaveSlots + room<TH>(1) + 2) : 0);
+    const int slots = TOP && begin < end ? slots_of(end - begin, TH, steps_of_slot) : 0;  // no more than a whole split's
+    uint64_t* own_lds = dynamic + (PER > 1 ? wave * hunt_words(TH, kWaveSlots) : 0);
     uint32_t* tops = reinterpret_cast<uint32_t*>(own_lds);
     uint32_t* slot = tops + lane;
     float held[2] = {-__builtin_inff(), -__builtin_inff()};
@@ -561,7 +558,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
             if (alone) hunt.level = row_results(q, h, out, r, label, xl, a);
             else part[at] = make_float4(a.m, a.s, a.u, 0.0f);
         }
-        uint64_t* candidates = own_lds + TH / 2 * (PER > 1 ? kWaveSlots : slots);  // behind the maxima
+        uint64_t* candidates = own_lds + maxima_words(TH, PER > 1 ? kWaveSlots : slots);  // behind the maxima
         uint32_t* orders = reinterpret_cast<uint32_t*>(candidates);  // before them
         const float bound = value_of(largest_of_lanes<DT, TH>(order_of(own), top, orders));  // a barrier inside
         meet<TH>();
@@ -569,7 +566,7 @@ __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, i
         const int each = kRuns * steps_of_slot;  // runs of a part of a slot
         const int64_t first = begin * W < q.vocab ? begin * W : q.vocab, last = end * W < q.vocab ? end * W : q.vocab;
         uint64_t* mine = keys + at * top;
-        const uint32_t most = room<TH>(slots);
+        const uint32_t most = room;
         // those that reach the bound, or (above) that are over it; whether there was room for all
         const auto gather = [&](bool above) {
             for (int i = 0; i < slots; ++i) {
@@ -1691,19 +1688,19 @@ int gefenx_token_statistics(const gefenx_logits* logits, double temperature, int
     return by_dtype(logits->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         if (top && q.per > 1) {
-            const size_t lds = kT / 64 * (sizeof(float) * 64 * kWaveSlots + sizeof(uint64_t) * (room<64>(1) + 2));
-            k_statistics<DT, kT / 64, true><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, lds, s>>>(q, h, top, 1, out, part, keys);
+            const size_t lds = kT / 64 * sizeof(uint64_t) * hunt_words(64, kWaveSlots);
+            k_statistics<DT, kT / 64, true><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, lds, s>>>(
+                q, h, top, 1, candidates_room(64, kWaveSlots), out, part, keys);
         } else if (top) {
             constexpr int W = kW<DT>;
-            const int64_t runs = std::min(q.split_runs, (q.vocab + W - 1) / W), steps = (runs + kStep * kT - 1) / (kStep * kT);
-            const int per = (int)((steps + kSlots - 1) / kSlots), slots = (int)((steps + per - 1) / per);
-            const size_t lds = sizeof(float) * kT * (size_t)slots + sizeof(uint64_t) * (room<kT>(slots) + 2);
-            k_statistics<DT, 1, true><<<(uint32_t)(q.rows * q.splits), kT, lds, s>>>(q, h, top, per, out, part, keys);
+            const HuntPlan plan = plan_hunt(std::min(q.split_runs, (q.vocab + W - 1) / W), kT);
+            k_statistics<DT, 1, true><<<(uint32_t)(q.rows * q.splits), kT, plan.bytes, s>>>(
+                q, h, top, plan.steps_of_slot, plan.room, out, part, keys);
             if (q.splits > 1) k_statistics_rows<DT, true><<<(uint32_t)q.rows, kT, 0, s>>>(q, h, top, out, part, keys, 64);
         } else if (q.per > 1) {
-            k_statistics<DT, kT / 64, false><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, 0, 1, out, part, keys);
+            k_statistics<DT, kT / 64, false><<<(uint32_t)((q.rows + q.per - 1) / q.per), kT, 0, s>>>(q, h, 0, 1, 0, out, part, keys);
         } else {
-            k_statistics<DT, 1, false><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, 0, 1, out, part, keys);
+            k_statistics<DT, 1, false><<<(uint32_t)(q.rows * q.splits), kT, 0, s>>>(q, h, 0, 1, 0, out, part, keys);
             int lanes = 1;
             while (lanes < q.splits && lanes < 64) lanes *= 2;
             if (q.splits > 1)

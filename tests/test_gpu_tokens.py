@@ -208,6 +208,30 @@ def test_ties_and_orders(dev, V, dtype):
             assert got.logps is None and torch.equal(got.top_ids.cpu(), want)
 
 
+# 2 or 4 splits of 5 steps of 1024 runs, the last of 4
+UNEVEN = [(torch.bfloat16, 131072, 128), (torch.float16, 65536, 256), (torch.float32, 32768, 256)]
+
+
+@pytest.mark.parametrize("dtype,V,T", UNEVEN)
+@pytest.mark.parametrize("equal", [300, 600, 1000])
+def test_ties_in_a_shorter_last_split(dev, dtype, V, T, equal):
+    """The row's highest values in its last split alone, many of them equal, neighbours or a few apart."""
+    g = torch.Generator().manual_seed(equal)
+    x = torch.randn(T, V, generator=g).clamp(max=4.0)
+    x[::2, V - 50 - equal:V - 50] = 9.0
+    x[1::2, V - 50 - 3 * equal:V - 50:3] = 9.0
+    x[:, V - 60] = 10.0
+    x[:, V - 20] = 11.0
+    x = x.to(dtype).to(dev)
+    want = torch.sort(x.float(), dim=-1, descending=True, stable=True)[1][:, :128]
+    lq = torch.log_softmax(x.double(), -1).gather(1, want)
+    tol = sum_error(x.double())[:, None] + U * (2 * lq.abs() + 4)
+    for top in (1, 20, 128):
+        got = gefen.token_statistics(x, top=top)
+        assert torch.equal(got.top_ids, want[:, :top])
+        assert torch.all((got.top_logps.double() - lq[:, :top]).abs() <= tol[:, :top])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V", [40, 3001, 70001])
 def test_masked_logits(dev, V, dtype):

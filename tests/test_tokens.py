@@ -1,5 +1,7 @@
 """Argument checks of token statistics and distillation that need no GPU."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 import torch
@@ -7,6 +9,7 @@ import torch
 import gefen
 from gefen.kernels import _native
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 GOOD = dict(logits=64, labels=64, rows=4, rows_per_batch=2, batch_stride=10, row_stride=5, vocab=5, dtype=0, n_seq=2)
 BAD = [({"dtype": 3}, -2), ({"vocab": 0}, -1), ({"rows": -1}, -1), ({"rows_per_batch": 0}, -1), ({"logits": None}, -1),
        ({"rows": 1 << 31}, -1), ({"rows": 1 << 30}, -1), ({"n_seq": -1}, -1), ({"n_seq": 1 << 30}, -1)]
@@ -109,3 +112,13 @@ def test_small_workspaces_and_missing_outputs():
     t = teacher()
     for slopes, weights, out in ((None, 64, 64), (64, None, 64), (64, 64, None)):
         assert lib.gefenx_distillation_grad(ctypes.byref(logits()), ctypes.byref(t), slopes, weights, None, 1.0, out, None) == -1
+
+
+def test_last_splits_stay_within_shared_memory(tmp_path):
+    """The launch's shared memory, sized by whole splits, holds what a shorter last split addresses."""
+    exe = tmp_path / "hunt_layout"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "gefen-x_amd", "csrc"), "-o", str(exe),
+                    os.path.join(ROOT, "tests", "c", "hunt_layout.cpp")], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, check=True)
+    bad, checked = map(int, out.stdout.split())
+    assert checked > 10000 and bad == 0, out.stderr
