@@ -100,7 +100,8 @@ __device__ __forceinline__ Sums<U> group_join(Sums<U> a, const Heat& h, float4* 
 // memory).  What M's rounding and hi's make of the sums is known and put right in sums(): 2^(m hi - M) for all of
 // them, and by hi alone s grows by (hi / (hi + lo) - 1) sum z exp(z), which u gives; without u the product with lo is
 // taken too.  Where M is beyond kHuge its rounding would be more than half a power of two, or x hi overflow (rows that
-// a mask of -1e10 or the type's lowest value leaves nothing): there the difference is taken first.
+// a mask of -1e10 or the type's lowest value leaves nothing): there the difference is taken first, and a maximum that
+// passes kHuge takes what the lane has so far from one scale to the other.
 constexpr float kHuge = 16777216.0f;
 template <int U> struct LaneSums {
     float m = -__builtin_inff(), s = 0.0f, u = 0.0f, minus = 0.0f, minus1 = 0.0f;  // -M, and that of exp(x)
@@ -108,14 +109,30 @@ template <int U> struct LaneSums {
         return __builtin_fabsf(of) > kHuge || (U == kPlain && __builtin_fabsf(of1) > kHuge);
     }
     __device__ __forceinline__ bool huge() const { return huge(minus, minus1); }
+    // the exponents that a term of x = m has in s, and in kPlain's u: what the roundings leave of 0
+    static __device__ __forceinline__ void offsets(float m, float of, float of1, const Heat& h, float& off, float& off1) {
+        off = off1 = 0.0f;
+        if (huge(of, of1)) return;
+        off = __builtin_fmaf(m, h.hi, of);
+        if (U != kEntropy) off = __builtin_fmaf(m, h.lo, off);
+        off1 = __builtin_fmaf(m, kLog2eRest, __builtin_fmaf(m, kLog2e, of1));
+    }
     __device__ __forceinline__ void rebase(float m2, const Heat& h) {
         if (!(m2 > m)) return;
         const float next = -(m2 * h.hi), next1 = -(m2 * kLog2e);
         if (m != -__builtin_inff()) {
-            const bool apart = huge() || huge(next, next1);
-            const float d = apart ? (m - m2) * h.hi : next - minus, f = __builtin_amdgcn_exp2f(d);
+            float d = next - minus, d1 = next1 - minus1;
+            if (huge() || huge(next, next1)) {
+                const float by = m - m2;
+                float from, from1, to, to1;
+                offsets(m, minus, minus1, h, from, from1);
+                offsets(m2, next, next1, h, to, to1);
+                d = (U == kEntropy ? by * h.hi : __builtin_fmaf(by, h.lo, by * h.hi)) + (to - from);
+                d1 = __builtin_fmaf(by, kLog2eRest, by * kLog2e) + (to1 - from1);
+            }
+            const float f = __builtin_amdgcn_exp2f(d);
             if (U == kEntropy) u = f * __builtin_fmaf(s, __builtin_fmaxf(d, kFar), u);
-            if (U == kPlain) u *= __builtin_amdgcn_exp2f(apart ? (m - m2) * kLog2e : next1 - minus1);
+            if (U == kPlain) u *= __builtin_amdgcn_exp2f(d1);
             s *= f;
         }
         m = m2;
@@ -142,11 +159,7 @@ template <int U> struct LaneSums {
         Sums<U> a;
         a.m = m;
         float off = 0.0f, off1 = 0.0f;
-        if (m != -__builtin_inff() && !huge()) {
-            off = __builtin_fmaf(m, h.hi, minus);
-            if (U != kEntropy) off = __builtin_fmaf(m, h.lo, off);
-            off1 = __builtin_fmaf(m, kLog2eRest, __builtin_fmaf(m, kLog2e, minus1));
-        }
+        if (m != -__builtin_inff()) offsets(m, minus, minus1, h, off, off1);
         const float f = __builtin_amdgcn_exp2f(-off);
         a.s = s * f;
         if (U == kEntropy) {

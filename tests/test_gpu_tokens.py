@@ -318,6 +318,67 @@ def test_large_logits(dev, dtype, V, temperature):
         assert out.token_divergence.isfinite().all() and grad.isfinite().all()
 
 
+LIMIT = 2.0 ** 24 / 1.4426950408889634  # of logits over their temperature that a lane takes by one fused operation
+EDGES = [(1.0, LIMIT), (0.001, 0.001 * LIMIT), (1e-4, 1e-4 * LIMIT), (100.0, 100.0 * LIMIT), (2.0, LIMIT), (0.5, LIMIT)]
+
+
+@pytest.mark.parametrize("T,V", [(4, 9000), (2304, 2800), (300, 40960)])  # a workgroup, a wave, splits and rows of their own
+@pytest.mark.parametrize("temperature,edge", EDGES)
+def test_rows_across_the_limit_of_fused_exponents(dev, temperature, edge, T, V):
+    """Rows that rise by steps of fp32 from below 2^24 temperature / log2(e) to above it, and from -above to -below; where
+    labels count at a temperature, the same of the logits themselves.  Formulas of the differences from the maximum, which
+    are exact in 64 bits."""
+    g = torch.Generator().manual_seed(V)
+    step = 2.0 ** (math.floor(math.log2(edge)) - 23)
+    rise = torch.arange(V) * 9 // V - 4 + torch.randint(-1, 2, (4, V), generator=g)
+    rows = torch.tensor([1.0, -1.0, 1.0, -1.0], dtype=torch.float64)[:, None] * (round(edge / step) * step) + rise * step
+    x = rows.float()
+    assert torch.equal(x.double(), rows)
+    keep = torch.tensor([0, 1, T // 2, T - 1])
+    labels, y = torch.full((T,), IGNORE), torch.randint(0, V, (4,), generator=g)
+    labels[keep] = y
+    held = torch.zeros(T, V, device=dev)
+    held[keep] = x.to(dev)
+    labels = labels.to(dev)
+    x64 = rows - rows.amax(1, keepdim=True)
+    z = x64 / temperature
+    lq, h, ids = statistics64(z, 5)
+    leaf = held.clone().requires_grad_()
+    got = gefen.token_statistics(leaf, labels, top=5, temperature=temperature)
+    (got.logps.sum() + got.entropy.sum()).backward()
+    of = lambda t: t.detach()[keep].cpu().double()  # noqa: E731
+    err, lp, tl = sum_error(z), lq.gather(1, y[:, None])[:, 0], lq.gather(1, ids)
+    assert torch.equal(got.top_ids[keep].cpu(), ids)
+    assert torch.all((of(got.logps) - lp).abs() <= err + U * (2 * lp.abs() + 4))
+    assert torch.all((of(got.top_logps) - tl).abs() <= err[:, None] + U * (2 * tl.abs() + 4))
+    assert torch.all((of(got.entropy) - h).abs() <= entropy_error(z, h))
+    p, far = lq.exp(), -z
+    hot = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+    want = (hot - p * (1 + lq + h[:, None])) / temperature
+    size = 1 + lq.abs() + h[:, None]
+    tol = (p * size * (err[:, None] + U * (4 * far + 32)) + p * (entropy_error(z, h) + err)[:, None] + 8 * U * hot) / temperature
+    assert torch.all((of(leaf.grad) - want).abs() <= tol + U * want.abs() * 1.01 + LEAST[torch.float32])
+    # the same rows as a student's
+    teacher = torch.stack([torch.randperm(V, generator=g)[:6] for _ in range(4)])
+    logps = torch.full((4, 6), math.log(0.1))
+    all_ids, all_lp = torch.zeros(T, 6, dtype=torch.long), torch.zeros(T, 6)
+    all_ids[keep], all_lp[keep] = teacher, logps
+    all_ids, all_lp = all_ids.to(dev), all_lp.to(dev)
+    for rest, hard in (("bucket", 0.0), ("drop", 0.3)):
+        at = x64.clone().requires_grad_()
+        loss, _, _, each = distill64(at, y, [(0, 4)], teacher, logps, temperature, rest, hard, "token")
+        loss.backward()
+        kw = dict(rest=rest, hard_weight=hard, temperature=temperature)
+        leaf = held.clone().requires_grad_()
+        two = gefen.distillation_loss(leaf, labels, all_ids, all_lp, **kw)
+        two.loss.backward()
+        out, grad = gefen.distillation_loss_and_grad(held, labels, all_ids, all_lp, **kw)
+        for o, d in ((two, leaf.grad), (out, grad)):
+            off = check_distill(x64, y, [(0, 4)], teacher, logps, temperature, rest, hard, "token", at.grad, each.detach(), of(d),
+                                of(o.token_divergence), torch.float32)
+            assert abs(o.loss.item() - loss.item()) <= off + 2 * U * abs(loss.item())
+
+
 def test_statistics_without_labels(dev):
     x, _, g = rows_of(6, 700, torch.float32)
     a, b = x.to(dev).requires_grad_(), x.to(dev).requires_grad_()
