@@ -15,6 +15,7 @@ import operator
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from gefen.gefen import _on_device, _outside_graphs
@@ -104,7 +105,9 @@ def token_statistics(logits, labels=None, *, top=0, temperature=1.0, ignore_inde
     labels every row counts and logps is None.  Differentiable in the logits through the log-probabilities, the
     entropy and the top log-probabilities."""
     temperature = float(temperature)
-    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
+    # a tangent goes there too: the function refuses forward mode
+    if isinstance(logits, torch.Tensor) and ((logits.requires_grad and torch.is_grad_enabled())
+                                             or forward_ad.unpack_dual(logits).tangent is not None):
         return TokenStatistics(*_TokenStatistics.apply(logits, labels, top, temperature, ignore_index))
     call = _Call(logits, labels, ignore_index, sequences=False, labelled=False)
     return TokenStatistics(*_statistics_forward(call, top, temperature)[0])

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import gefen
 
@@ -388,6 +389,22 @@ def test_statistics_without_labels(dev):
     for o in (one, two):
         (o.entropy.sum() * 2 + o.top_logps[:, 1].sum()).backward()
     assert torch.equal(a.grad, b.grad)
+
+
+def test_forward_mode_is_refused(dev):
+    """Logits with a tangent, which none of the results would carry."""
+    x = torch.randn(3, 50, device=dev)
+    y = torch.zeros(3, dtype=torch.long, device=dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.randn_like(x))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for call in (lambda: gefen.token_statistics(dual, y, top=3), lambda: gefen.token_statistics(dual),
+                             lambda: gefen.token_logps(dual, y)):
+                    with pytest.raises(NotImplementedError, match="jvp"):
+                        call()
+        inside = gefen.token_statistics(x, y, top=3)
+    assert all(torch.equal(a, b) for a, b in zip(inside, gefen.token_statistics(x, y, top=3)))
 
 
 def test_labels_outside_of_the_vocabulary(dev):
