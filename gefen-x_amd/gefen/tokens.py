@@ -23,6 +23,7 @@ from gefen.kernels import _native
 from gefen.losses import _Call, _ptr
 
 _REST = {"bucket": 0, "drop": 1, "normalize": 2}
+_MOST_TOP = 128  # likeliest tokens of a row
 
 
 class TokenStatistics(NamedTuple):
@@ -58,9 +59,11 @@ def _scratch(call, kept, n, keep):
 def _statistics_forward(call, top, temperature, keep=False):
     """The statistics, and where asked to keep it, what their gradient needs."""
     top, lead = operator.index(top), call.lead
+    if not 0 <= top <= min(_MOST_TOP, call.vocab):  # before anything of that size is allocated
+        raise ValueError("top must be in [0, {}] but is: {!r}".format(min(_MOST_TOP, call.vocab), top))
     lib = _native.load()
     logps = None if call.labels is None else call.empty(*lead)
-    entropy, top_logps = call.empty(*lead), call.empty(*lead, max(top, 0))
+    entropy, top_logps = call.empty(*lead), call.empty(*lead, top)
     top_ids = torch.empty(top_logps.shape, dtype=torch.int64, device=call.device)
     n = int(lib.gefenx_token_statistics_workspace_bytes(call.ref, top))
     saved, ws, saved_ptr, ws_ptr = _scratch(call, 4 * call.rows, n, keep)

@@ -407,6 +407,18 @@ def test_forward_mode_is_refused(dev):
     assert all(torch.equal(a, b) for a, b in zip(inside, gefen.token_statistics(x, y, top=3)))
 
 
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("top", [129, 1 << 20, -1])
+def test_bad_counts_of_tokens_take_no_memory(dev, top, grad):
+    x = torch.zeros(64, 200, device=dev, requires_grad=grad)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(dev)
+    before = torch.cuda.memory_allocated(dev)
+    with pytest.raises(ValueError, match="top"):
+        gefen.token_statistics(x, top=top)
+    assert torch.cuda.max_memory_allocated(dev) == before
+
+
 def test_labels_outside_of_the_vocabulary(dev):
     x, _, _ = rows_of(4, 30, torch.float32)
     labels = torch.tensor([3, 30, -1, IGNORE])
