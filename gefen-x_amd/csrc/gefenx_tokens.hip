@@ -1555,6 +1555,7 @@ int make_distill(const char* what, const gefenx_logits* l, const gefenx_teacher*
     if (d.q.per > 1 && t->top > kMaxTop) {
         d.q.per = 1;
         set_splits(*l, d.q, 1);
+        if (d.q.rows > kMaxThreads / kT) return set_error(GEFENX_EINVAL, "%s: too many rows (%lld)", what, (long long)l->rows);
     }
     d.dtype = l->dtype;
     d.by_sequence = t->by_sequence;

@@ -87,6 +87,20 @@ def test_bad_teachers(change):
     assert _native.load().gefenx_distillation_workspace_bytes(ctypes.byref(logits()), ctypes.byref(teacher(**change))) == 0
 
 
+@pytest.mark.parametrize("top,rows,fits", [(128, 1 << 24, True), (128, (1 << 26) - 4, True), (129, (1 << 24) - 1, True),
+                                          (129, 1 << 24, False), (512, (1 << 26) - 4, False)])
+def test_rows_of_a_launch(top, rows, fits):
+    """Short rows go to a wave each, with more than 128 tokens of the teacher to a workgroup each: a launch has 2^32 - 1
+    threads at most."""
+    desc, t = logits(rows=rows, rows_per_batch=rows, batch_stride=0, row_stride=600, vocab=600), teacher(top=top)
+    assert (_native.load().gefenx_distillation_workspace_bytes(ctypes.byref(desc), ctypes.byref(t)) > 0) == fits
+    if not fits:
+        assert distill(desc, t, n=1 << 40) == -1 and "too many rows" in _native.last_error()
+        grad = _native.load().gefenx_distillation_grad
+        assert grad(ctypes.byref(desc), ctypes.byref(t), None, 64, None, 1.0, 64, None) == -1
+        assert "too many rows" in _native.last_error()
+
+
 def test_sequences_have_to_cover_the_rows():
     assert distill(logits(n_seq=3), teacher(by_sequence=1)) == -1
     assert distill(logits(n_seq=0), teacher(by_sequence=1)) == -1
