@@ -511,7 +511,7 @@ template <int TH> struct Hunt {
 // (equal logits) are those over the bound and the first of the equal ones; NaN, +inf and what is left go through
 // select_keys.
 //
-// 4096 x 128256 bf16: 163-175 us, 6.0-6.4 TB/s, the vector units busy 78% of it (7.1 instructions a logit: convert,
+// 4096 x 128256 bf16: 163-175 us, 6.0-6.4 TB/s, the vector units busy 79% of it (7.2 instructions a logit: convert,
 // the maximum, fma, exp, the two sums); with 64 tokens 186 us, 7% read again for them.  16384 x 1000 fp32 14 us.
 template <int DT, int PER, bool TOP>
 __global__ __launch_bounds__(kT) void k_statistics(const Rows q, const Heat h, int top, int steps_of_slot, int room, const Statistics out,
@@ -759,7 +759,8 @@ __global__ __launch_bounds__(kT) void k_distill(const Rows q, const Heat h, cons
 }
 
 // What a wave finds of a row's teacher: mass and sum of p (log p - (x - ref) / tau) over its tokens (one outside of the
-// vocabulary makes them NaN), ref a logit of one of them, so that large ones lose nothing, and, BUCKET, the sums over its tokens and over what else is in their runs.
+// vocabulary makes them NaN), ref a logit of one of them, so that large ones lose nothing, and, BUCKET, the sums over its
+// tokens (each once, however many entries name it) and over what else is in their runs.
 template <int U> struct Known {
     double mass, cross, log_mass, ref;
     Sums<U> tokens, others;
@@ -1289,8 +1290,8 @@ constexpr int kRowEntries = 2;              // of a lane: the teacher's tokens a
 // and a write take 584, the vector units busy 65% of the time; 2406 x 32000 fp32 92 us, 5.4 TB/s.
 template <int DT, bool BUCKET>
 __global__ __launch_bounds__(kRowT, 8) void k_distill_alone(const Rows q, const Heat h, const DistillGrad<false> g,
-                                                                          double2* __restrict__ each, float* __restrict__ divergence,
-                                                                          Slope* __restrict__ slopes, void* __restrict__ grad) {
+                                                            double2* __restrict__ each, float* __restrict__ divergence,
+                                                            Slope* __restrict__ slopes, void* __restrict__ grad) {
     using T = typename Elem<DT>::T;
     constexpr int W = kW<DT>, U = kNone;
     __shared__ float4 waves[kRowT / 64];
@@ -1464,10 +1465,14 @@ void set_splits(const gefenx_logits& l, Rows& q, int64_t splits) {
 }
 
 // How a row is split for its sums.  A split is a round of dependent reads and joins of its own, and its results go through
-// a second kernel, so rows are split only where there are fewer than two workgroups a CU, and into no less than 4 passes
-// (statistics with 20 tokens, us, whole / 2 / 4 / 8 / 16 splits: 1 x 128256 bf16 20 / 18 / 15 / 13 / 12, 64 x 151936
-// 23 / 21 / 17 / 16 / 18, 400 x 50257, 25 passes, 19 / 24 / 25 / 29 / 40, 400 x 151936 fp32 58 / 51 / 55 / 57 / 63;
-// 4096 x 128256 with 64 tokens 197 / 232 / 265 in 4).
+// a second kernel, so rows are split only where there are fewer than two workgroups a CU and 32 passes or more, and into
+// no less than 4 passes (statistics with 20 tokens, us, whole / 2 / 4 / 8 / 16 splits: 1 x 128256 bf16 20 / 18 / 15 / 13 /
+// 12, 64 x 151936 23 / 21 / 17 / 16 / 18, 400 x 151936 fp32 58 / 51 / 55 / 57 / 63; 4096 x 128256 with 64 tokens 197 / 232
+// / 265 in 4).  Below 32 passes the second kernel costs what the splits give (as parts of a replayed graph, whole / 2 / 4 /
+// 8: 1 x 32000 bf16, 16 passes, 10.9 / 13.4 / 12.3 / 12.6, 1 x 50257, 25 passes, 12.8 / 14.9 / 13.4 / 13.0, 64 x 50257
+// 14.7 / 16.3 / 14.4 / 14.3, 256 x 50257 14.8 / 19.1 / 18.4 / 22.2; 1 x 64000, 32 passes, 14.0 / 15.4 / 13.6 / 12.8).  The
+// distillation has that kernel either way and takes 2-4 us longer whole there (64 x 50257 24.9 / 22.9 / 21.4 / 21.0), of
+// which an eager call, 33 us of host work, shows nothing.
 void split_sums(const gefenx_logits& l, Rows& q) {
     if (q.per > 1) return;
     const int64_t passes = (l.vocab * (l.dtype == GEFENX_F32 ? 4 : 2) + 16 * kT - 1) / (16 * kT);

@@ -106,7 +106,7 @@ def token_statistics(logits, labels=None, *, top=0, temperature=1.0, ignore_inde
     entropy, and the `top` (up to 128) likeliest tokens with their log-probabilities, ties by the lowest id, NaN
     before all.  Rows whose label is ignore_index are not read: 0, 0, and ids 0 with log-probability -inf.  Without
     labels every row counts and logps is None.  Differentiable in the logits through the log-probabilities, the
-    entropy and the top log-probabilities."""
+    entropy and the top log-probabilities, in reverse mode."""
     temperature = float(temperature)
     # a tangent goes there too: the function refuses forward mode
     if isinstance(logits, torch.Tensor) and ((logits.requires_grad and torch.is_grad_enabled())
@@ -214,7 +214,8 @@ def distillation_loss(logits, labels, teacher_ids, teacher_logps, *, cu_seqlens=
 
     and loss = mean of (1 - hard_weight) temperature^2 D - hard_weight log softmax(logits)[label] over the labelled
     rows, or (reduction "sequence") the mean over the sequences that have any of their mean; 0 without any.  An entry of
-    log-probability -inf names no token, whatever its id.  With hard_weight 0 labels only say which rows count, with 1
+    log-probability -inf names no token, whatever its id; a token that several entries name is in P and the sum of D with
+    each of them, in s once.  With hard_weight 0 labels only say which rows count, with 1
     the teacher gives the divergence alone, whatever it holds."""
     how = (temperature, rest, hard_weight, reduction)
     return DistillationLoss(*_Distillation.apply(logits, labels, cu_seqlens, ignore_index, teacher_ids, teacher_logps, how))
